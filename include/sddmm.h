@@ -506,6 +506,84 @@ int sddmm_csr_noalloc(int64_t n_rows, int64_t n_cols, int64_t nnz, const int32_t
                       const int32_t *d_col_ind, const float *d_val, int32_t K, const float *d_W,
                       const float *d_H, float *d_out, void *stream);
 
+/* Dense attention: the same forms where the pattern follows from positions -- no
+ * index array, scores that never reach memory, heads, 16-bit operands.  No
+ * counterpart in the reference.
+ *
+ * Row i of a sequence with n_q rows and n_k keys has the position n_k - n_q + i
+ * (the last row the last key's), key j the position j.  A row at p sees the keys
+ *     max(0, p - window_left) <= j < min(n_k, max(p + window_right + 1, prefix))
+ * where a window of -1 has no bound on that side: window_right = 0 is the causal
+ * mask, `prefix` the number of first keys of the sequence that all of its rows see
+ * to their right.  Documents that must not see each other are sequences of their
+ * own (q_ptr, k_ptr).  With q, k, v the rows of a head,
+ *     t_ij = scale * dot(q_i, k_j);     s_ij = cap > 0 ? cap * tanh(t_ij / cap) : t_ij
+ *     s_ij -= slopes[head] * |p_i - j|                              (slopes not NULL)
+ *     lse_i = log sum_j exp(s_ij);      out_i = sum_j exp(s_ij - lse_i) v_j
+ * over the keys that row i sees; a row that sees none gets 0 and an lse of
+ * -infinity.  Query head h reads key head h / (n_heads / n_kv_heads).
+ *
+ * A call is described by this structure (start from sddmm_attention_desc_init).
+ * Rows: without q_ptr every sequence has max_q rows (or q_len[s] of them), and row i
+ * of sequence s and head h begins at element s * q_seq + i * q_row + h * q_head; with
+ * q_ptr[n_seq + 1] sequence s has the rows q_ptr[s] .. q_ptr[s + 1] - 1 of one
+ * packed array, which begin at r * q_row + h * q_head.  Keys and values the same
+ * with k_ptr, k_len, max_k (a cache: k_ptr NULL, max_k its longest sequence, k_len the
+ * lengths so far).  What lies behind the end of a sequence is neither read nor
+ * written.  lse: fp32, n_heads to a row, rows in the order of q_ptr or s * max_q + i.
+ *
+ * Operands: n_heads a multiple of n_kv_heads; head_dim a multiple of 8 up to 128;
+ * every pointer and stride a multiple of 16 bytes; a row's stride at least its
+ * length and below 2^23 bytes; scale finite and above 0, cap finite.  Products are
+ * summed in fp32, statistics kept in fp32; 16-bit operands: the probabilities (and,
+ * backwards, their gradients) are rounded to the operands' type before they are
+ * multiplied, as results are; fp32 operands: no rounding below fp32.  Infinities and
+ * NaNs in keys that a row does not see do not reach it; in values (backwards, in rows
+ * of q, out and d_out) they may where a row of the same 64 keys or 128 rows meets them.
+ * Lengths and pointers of sequences live on the device and are not validated: q_ptr
+ * and k_ptr must rise from 0 and end at q_rows and k_rows at most; q_len and k_len
+ * are taken as 0 .. max_q and 0 .. max_k.
+ *
+ * Calls allocate nothing, launch on `stream` only and may be captured into a graph.
+ * d_workspace: sddmm_attention_workspace_bytes of device memory, 256-byte aligned, for
+ * the time of the call; calls that overlap in time need one each, and a graph keeps
+ * using the one that it was captured with.                                       */
+enum { SDDMM_TYPE_F32 = 0, SDDMM_TYPE_BF16 = 1, SDDMM_TYPE_F16 = 2 };
+
+typedef struct sddmm_attention_desc {
+    int32_t type;                        /* SDDMM_TYPE_*, of q, k, v, out and their gradients */
+    int32_t head_dim, n_heads, n_kv_heads;
+    int32_t n_seq, max_q, max_k;         /* sequences; no sequence has more rows / keys */
+    int32_t window_left, window_right;   /* -1: no bound */
+    int32_t shared_len;                  /* sddmm_attention_shared: keys that all sequences begin with; else 0 */
+    float scale, cap;                    /* cap 0: scores are not bent */
+    int64_t q_rows, k_rows;              /* with q_ptr / k_ptr: rows of the packed arrays */
+    int64_t q_seq, q_row, q_head;        /* strides in elements */
+    int64_t k_seq, k_row, k_head;
+    int64_t v_seq, v_row, v_head;
+    int64_t o_seq, o_row, o_head;
+    const int32_t *q_ptr, *k_ptr;        /* device, [n_seq + 1], or NULL */
+    const int32_t *q_len, *k_len;        /* device, [n_seq], or NULL; not beside q_ptr / k_ptr */
+    const int32_t *prefix;               /* device, [n_seq], or NULL */
+    const float *slopes;                 /* device, [n_heads], or NULL */
+} sddmm_attention_desc;
+void sddmm_attention_desc_init(sddmm_attention_desc *desc);   /* zeros, windows of -1 */
+
+/* Bytes that sddmm_attention_forward (or _shared, where shared_len > 0) and
+ * sddmm_attention_backward need (0: none); either pointer may be NULL.  They depend
+ * on the structure's numbers only, not on what its pointers point to. */
+int sddmm_attention_workspace_bytes(const sddmm_attention_desc *desc, int64_t *forward, int64_t *backward);
+/* lse may be NULL. */
+int sddmm_attention_forward(const sddmm_attention_desc *desc, const void *d_q, const void *d_k, const void *d_v,
+                            void *d_out, float *d_lse, void *d_workspace, int64_t workspace_bytes, void *stream);
+/* Sequences that begin with the same shared_len keys, which exist once (d_shared_k, d_shared_v: rows of k_row, k_head and v_row,
+ * v_head) and are read once for all of them; d_k and d_v hold what follows, so that position, window and prefix count
+ * from the first shared key: key j of a sequence's own has the position shared_len + j, its last row
+ * shared_len + n_k - 1.  Without q_ptr; n_seq * max_q * n_heads below 2^31. */
+int sddmm_attention_shared(const sddmm_attention_desc *desc, const void *d_q, const void *d_shared_k, const void *d_shared_v,
+                           const void *d_k, const void *d_v, void *d_out, float *d_lse, void *d_workspace,
+                           int64_t workspace_bytes, void *stream);
+
 /* Measurement aid: copies n_bytes (a multiple of 16, both pointers 16-byte
  * aligned device memory) with a plain streaming kernel, sddmm_copy_probe_kernel,
  * on `stream`.  A profile of a run that also calls this holds a kernel of known

@@ -19,6 +19,7 @@ OK, ERR_ARG, ERR_IO, ERR_FORMAT, ERR_RANGE, ERR_UNSORTED, ERR_HIP, ERR_NOMEM = r
 KERNEL_AUTO, KERNEL_ROW_GATHER, KERNEL_LDS_TILE, KERNEL_PANEL, KERNEL_HYBRID, KERNEL_DENSE_BLOCK = 0, 1, 2, 3, 4, 5
 EPILOGUE_SCALE, EPILOGUE_RESIDUAL = 0, 1
 FORM_SOFTMAX = 0x100
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 SPMM_CSR, SPMM_TILES, SPMM_WALK, SPMM_BLOCKS = 0, 1, 2, 3
 
 
@@ -62,6 +63,33 @@ class PlanOptions(C.Structure):
 
     def as_dict(self):
         return {f: getattr(self, f) for f, _ in self._fields_}
+
+
+class AttentionDesc(C.Structure):
+    """sddmm_attention_desc; AttentionDesc.defaults(**fields) starts from sddmm_attention_desc_init (pointers as integers)."""
+    _fields_ = [(n, c_int32) for n in ("type", "head_dim", "n_heads", "n_kv_heads", "n_seq", "max_q", "max_k", "window_left", "window_right",
+                                       "shared_len")] + [("scale", c_float), ("cap", c_float)] + [(n, c_int64) for n in (
+        "q_rows", "k_rows", "q_seq", "q_row", "q_head", "k_seq", "k_row", "k_head", "v_seq", "v_row", "v_head", "o_seq", "o_row", "o_head")] + [
+        (n, c_void_p) for n in ("q_ptr", "k_ptr", "q_len", "k_len", "prefix", "slopes")]
+
+    @classmethod
+    def defaults(cls, **kw):
+        d = cls()
+        lib().sddmm_attention_desc_init(byref(d))
+        for k, v in kw.items():
+            if k not in dict(cls._fields_):
+                raise KeyError(k)
+            setattr(d, k, (v or None) if k in ("q_ptr", "k_ptr", "q_len", "k_len", "prefix", "slopes") else v)
+        return d
+
+    @classmethod
+    def packed(cls, type, n_seq, n_heads, n_kv_heads, head_dim, **kw):
+        """The strides of contiguous arrays: q and out [sequence, max_q, n_heads, head_dim], k and v [sequence, max_k, n_kv_heads,
+        head_dim] (with q_ptr / k_ptr: [rows, ...]); scale = head_dim ** -0.5 unless given."""
+        d = dict(scale=max(head_dim, 1) ** -0.5)
+        for n, heads, most in (("q", n_heads, "max_q"), ("o", n_heads, "max_q"), ("k", n_kv_heads, "max_k"), ("v", n_kv_heads, "max_k")):
+            d[n + "_head"], d[n + "_row"], d[n + "_seq"] = head_dim, heads * head_dim, kw.get(most, 0) * heads * head_dim
+        return cls.defaults(type=type, n_seq=n_seq, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, **{**d, **kw})
 
 
 class LaunchProfile(C.Structure):
@@ -128,6 +156,10 @@ SIGNATURES = {
     "sddmm_gpu": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, POINTER(c_float)]),
     "sddmm_csr_noalloc": (c_int, [c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p,
                                   c_void_p, c_void_p]),
+    "sddmm_attention_desc_init": (None, [POINTER(AttentionDesc)]),
+    "sddmm_attention_workspace_bytes": (c_int, [POINTER(AttentionDesc), POINTER(c_int64), POINTER(c_int64)]),
+    "sddmm_attention_forward": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 6 + [c_int64, c_void_p]),
+    "sddmm_attention_shared": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 8 + [c_int64, c_void_p]),
     "sddmm_copy_probe": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "sddmm_device_info": (c_int, [POINTER(c_int), c_char_p, c_int]),
 }
@@ -373,7 +405,8 @@ class Plan:
             check(rc)
 
     def spmm_form(self):
-        """SPMM_CSR, SPMM_TILES or SPMM_WALK: what spmm does behind this plan."""
+        """TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+SPMM_CSR, SPMM_TILES or SPMM_WALK: what spmm does behind this plan."""
         f = c_int32()
         check(lib().sddmm_plan_spmm_form(self.h, byref(f)))
         return f.value
@@ -440,6 +473,29 @@ def row_softmax(n_rows, d_row_ptr, d_x, d_out, stream=0):
 
 def spmm_csr(n_rows, n_cols, nnz, d_row_ptr, d_col_ind, d_x, K, d_H, d_Y, stream=0):
     rc = lib().sddmm_spmm_csr(n_rows, n_cols, nnz, d_row_ptr, d_col_ind or None, d_x or None, K, d_H or None, d_Y, stream or None)
+    if rc:
+        check(rc)
+
+
+def attention_workspace_bytes(desc):
+    """(bytes for attention_forward or attention_shared, bytes for attention_backward)."""
+    f, b = c_int64(), c_int64()
+    check(lib().sddmm_attention_workspace_bytes(byref(desc), byref(f), byref(b)))
+    return f.value, b.value
+
+
+def attention_forward(desc, d_q, d_k, d_v, d_out, d_lse=0, d_workspace=0, workspace_bytes=0, stream=0):
+    """sddmm_attention_forward: softmax attention under masks that follow from positions (desc: AttentionDesc)."""
+    rc = lib().sddmm_attention_forward(byref(desc), d_q or None, d_k or None, d_v or None, d_out or None, d_lse or None, d_workspace or None,
+                                       workspace_bytes, stream or None)
+    if rc:
+        check(rc)
+
+
+def attention_shared(desc, d_q, d_shared_k, d_shared_v, d_k, d_v, d_out, d_lse=0, d_workspace=0, workspace_bytes=0, stream=0):
+    """sddmm_attention_shared: sequences that begin with the same desc.shared_len keys."""
+    rc = lib().sddmm_attention_shared(byref(desc), d_q or None, d_shared_k or None, d_shared_v or None, d_k or None, d_v or None, d_out or None,
+                                      d_lse or None, d_workspace or None, workspace_bytes, stream or None)
     if rc:
         check(rc)
 

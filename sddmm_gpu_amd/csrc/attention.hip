@@ -1,0 +1,197 @@
+// Entry points of the dense attention: what they check, which kernels they launch, and how large a workspace is.
+#include <hip/hip_runtime.h>
+#include <cmath>
+#include <cstring>
+#include "internal.hpp"
+#include "attention.hpp"
+#include "attention_launch.hpp"
+
+using namespace sddmm;
+
+namespace {
+
+constexpr int64_t kMostRows = INT32_MAX;
+
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+int element(int type) { return type == SDDMM_TYPE_F32 ? 4 : 2; }
+
+bool strides_fit(const sddmm_attention_desc &d, int64_t seq, int64_t row, int64_t head, bool packed)
+{
+    const int64_t e = element(d.type), piece = 16 / e;
+    return row >= d.head_dim && row * e < ((int64_t)1 << 23) && row % piece == 0 && head % piece == 0 && (packed || seq % piece == 0) &&
+           head >= 0 && (packed || seq >= 0);
+}
+
+int check_desc(const char *who, const sddmm_attention_desc *p)
+{
+    if (!p) return fail(SDDMM_ERR_ARG, "%s: NULL description", who);
+    const sddmm_attention_desc &d = *p;
+    if (d.type != SDDMM_TYPE_F32 && d.type != SDDMM_TYPE_BF16 && d.type != SDDMM_TYPE_F16) return fail(SDDMM_ERR_ARG, "%s: unknown type %d", who, d.type);
+    if (d.head_dim < 8 || d.head_dim > 128 || d.head_dim % 8)
+        return fail(SDDMM_ERR_ARG, "%s: head_dim = %d is no multiple of 8 up to 128", who, d.head_dim);
+    if (d.n_heads < 1 || d.n_kv_heads < 1 || d.n_heads % d.n_kv_heads || d.n_heads > 65536)
+        return fail(SDDMM_ERR_ARG, "%s: %d query heads do not share %d key heads", who, d.n_heads, d.n_kv_heads);
+    if (d.n_seq < 0 || d.max_q < 0 || d.max_k < 0 || d.shared_len < 0 || d.q_rows < 0 || d.k_rows < 0) return fail(SDDMM_ERR_ARG, "%s: negative size", who);
+    if (d.window_left < -1 || d.window_right < -1) return fail(SDDMM_ERR_ARG, "%s: a window below -1", who);
+    if (!std::isfinite(d.scale) || !(d.scale > 0.f)) return fail(SDDMM_ERR_ARG, "%s: scale must be finite and above 0", who);
+    if (!std::isfinite(d.cap) || d.cap < 0.f) return fail(SDDMM_ERR_ARG, "%s: cap must be finite and not negative", who);
+    if ((d.q_ptr && d.q_len) || (d.k_ptr && d.k_len)) return fail(SDDMM_ERR_ARG, "%s: lengths beside the pointers of packed sequences", who);
+    if (!strides_fit(d, d.q_seq, d.q_row, d.q_head, d.q_ptr) || !strides_fit(d, d.k_seq, d.k_row, d.k_head, d.k_ptr) ||
+        !strides_fit(d, d.v_seq, d.v_row, d.v_head, d.k_ptr) || !strides_fit(d, d.o_seq, d.o_row, d.o_head, d.q_ptr))
+        return fail(SDDMM_ERR_ARG, "%s: strides must be multiples of 16 bytes, a row's from head_dim to 2^23 bytes", who);
+    const int64_t rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
+    if (rows > kMostRows || d.k_rows > kMostRows || (int64_t)d.shared_len + d.max_k > kMostRows / 2 || d.max_q > kMostRows / 2)
+        return fail(SDDMM_ERR_RANGE, "%s: sizes beyond 32-bit positions", who);
+    return SDDMM_OK;
+}
+
+// How a call's rows are dealt out.
+struct Deal {
+    int64_t rows = 0;          // of all sequences
+    bool token = false;        // the kernel for few rows
+    int mapping = kRowsOfHead;
+    int64_t slots = 0, grid = 0, splits = 1;
+    int64_t shared_slots = 0, shared_grid = 0, shared_splits = 0;
+    int64_t parts = 1, part_bytes = 0, bytes = 0;
+};
+
+// Pieces that the keys are cut into: so many that the grid fills the card (256 compute units, two workgroups each), each of
+// `least` keys at least.
+int64_t pieces(int64_t workgroups, int64_t keys, int64_t least)
+{
+    const int64_t fill = 512;
+    return std::max<int64_t>(1, std::min(std::min(div_up(fill, std::max<int64_t>(workgroups, 1)), div_up(keys, least)), (int64_t)256));
+}
+
+Deal deal(const sddmm_attention_desc &d)
+{
+    Deal r;
+    const int64_t group = d.n_heads / d.n_kv_heads, tile = attention_forward_rows();
+    r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
+    // keys that a tile's rows can see
+    const int64_t span = d.window_left >= 0 && d.window_right >= 0 && !d.prefix ? (int64_t)d.window_left + d.window_right + std::min<int64_t>(d.max_q, tile) : d.max_k;
+    const int64_t keys = std::min<int64_t>(d.max_k, span);
+    const int64_t packed = d.max_q * group;
+    r.token = packed <= attention_token_rows();
+    if (r.token) {
+        r.slots = 1;
+        const int64_t units = (int64_t)d.n_seq * d.n_kv_heads;
+        r.splits = pieces(units, keys, 256);
+        r.grid = units * r.splits;
+    } else {
+        r.mapping = group > 1 && d.max_q < tile ? kRowsPacked : kRowsOfHead;
+        const int64_t share = r.mapping == kRowsPacked ? group : 1, tiles = div_up(d.max_q * share, tile);
+        // (packed sequences: a slot for each tile there can be, see slot_sequence; pairs of tokens and heads are not packed there)
+        if (d.q_ptr && r.mapping == kRowsPacked) r.mapping = kRowsOfHead;
+        if (d.q_ptr) r.slots = r.rows / tile + d.n_seq;
+        else r.slots = r.mapping == kRowsPacked ? tiles : div_up(d.max_q, tile);
+        const int64_t units = (d.q_ptr ? 1 : (int64_t)d.n_seq) * d.n_kv_heads * (r.mapping == kRowsPacked ? 1 : group);
+        r.splits = pieces(units * r.slots, keys, 512);
+        r.grid = units * r.slots * r.splits;
+    }
+    r.parts = r.splits;
+    if (d.shared_len > 0) {
+        r.shared_slots = div_up(r.rows * group, tile);
+        r.shared_splits = pieces(r.shared_slots * d.n_kv_heads, d.shared_len, 256);
+        r.shared_grid = r.shared_slots * d.n_kv_heads * r.shared_splits;
+        r.parts += r.shared_splits;
+    }
+    if (r.parts > 1) {
+        r.part_bytes = padded(r.parts * r.rows * d.n_heads * d.head_dim * (int64_t)sizeof(float));
+        r.bytes = r.part_bytes + padded(r.parts * r.rows * d.n_heads * (int64_t)sizeof(float2));
+    }
+    return r;
+}
+
+AttnArgs arguments(const sddmm_attention_desc &d)
+{
+    AttnArgs a{};
+    a.q_seq = d.q_seq, a.q_row = d.q_row, a.q_head = d.q_head, a.k_seq = d.k_seq, a.k_row = d.k_row, a.k_head = d.k_head;
+    a.v_seq = d.v_seq, a.v_row = d.v_row, a.v_head = d.v_head, a.o_seq = d.o_seq, a.o_row = d.o_row, a.o_head = d.o_head;
+    a.q_ptr = d.q_ptr, a.k_ptr = d.k_ptr, a.q_len = d.q_len, a.k_len = d.k_len, a.prefix = d.prefix, a.slopes = d.slopes;
+    a.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
+    a.head_dim = d.head_dim, a.n_heads = d.n_heads, a.n_kv_heads = d.n_kv_heads, a.group = d.n_heads / d.n_kv_heads;
+    a.n_seq = d.n_seq, a.max_q = d.max_q, a.max_k = d.max_k, a.left = d.window_left, a.right = d.window_right, a.shared_len = d.shared_len;
+    a.scale = d.scale, a.cap = d.cap;
+    return a;
+}
+
+bool aligned(std::initializer_list<const void *> pointers)
+{
+    for (const void *p : pointers)
+        if ((uintptr_t)p & 15u) return false;
+    return true;
+}
+
+int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d_q, const void *d_shared_k, const void *d_shared_v, const void *d_k,
+                const void *d_v, void *d_out, float *d_lse, void *d_workspace, int64_t workspace_bytes, void *stream)
+{
+    const sddmm_attention_desc &d = *desc;
+    const Deal r = deal(d);
+    if (r.rows == 0 || d.n_seq == 0) return SDDMM_OK;
+    const bool keys = d.k_ptr ? d.k_rows > 0 : d.max_k > 0;
+    if (!d_q || !d_out || (keys && (!d_k || !d_v)) || (d.shared_len && (!d_shared_k || !d_shared_v))) return fail(SDDMM_ERR_ARG, "%s: NULL device pointer", who);
+    if (!aligned({d_q, d_k, d_v, d_out, d_shared_k, d_shared_v})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
+    if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
+        return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
+    if (r.grid > INT32_MAX || r.shared_grid > INT32_MAX || (r.parts > 1 && r.rows * d.n_heads > INT32_MAX))
+        return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
+
+    AttnArgs a = arguments(d);
+    a.q = d_q, a.k = d_k, a.v = d_v, a.out = d_out, a.lse = d_lse, a.shared_k = d_shared_k, a.shared_v = d_shared_v;
+    a.part_o = (float *)d_workspace, a.part_ml = (float2 *)((char *)d_workspace + r.part_bytes);
+    a.n_slots = (int)r.slots, a.n_split = (int)r.splits, a.part0 = 0, a.n_part = (int)r.parts;
+    const hipStream_t st = (hipStream_t)stream;
+    hipError_t e = hipSuccess;
+    if (d.shared_len > 0) {
+        AttnArgs b = a;
+        b.n_slots = (int)r.shared_slots, b.n_split = (int)r.shared_splits, b.part0 = (int)r.splits;
+        e = launch_attention_forward(b, d.type, kRowsShared, (unsigned)r.shared_grid, st);
+    }
+    if (e == hipSuccess) e = r.token ? launch_attention_token(a, d.type, (unsigned)r.grid, st) : launch_attention_forward(a, d.type, r.mapping, (unsigned)r.grid, st);
+    if (e == hipSuccess && r.parts > 1) e = launch_attention_join(a, d.type, st);
+    if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
+    return SDDMM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+void sddmm_attention_desc_init(sddmm_attention_desc *desc)
+{
+    if (!desc) return;
+    memset(desc, 0, sizeof *desc);
+    desc->window_left = desc->window_right = -1;
+}
+
+int sddmm_attention_workspace_bytes(const sddmm_attention_desc *desc, int64_t *forward, int64_t *backward)
+{
+    if (int rc = check_desc("sddmm_attention_workspace_bytes", desc)) return rc;
+    if (forward) *forward = deal(*desc).bytes;
+    if (backward) *backward = 0;
+    return SDDMM_OK;
+}
+
+int sddmm_attention_forward(const sddmm_attention_desc *desc, const void *d_q, const void *d_k, const void *d_v, void *d_out, float *d_lse,
+                            void *d_workspace, int64_t workspace_bytes, void *stream)
+{
+    const char *who = "sddmm_attention_forward";
+    if (int rc = check_desc(who, desc)) return rc;
+    if (desc->shared_len) return fail(SDDMM_ERR_ARG, "%s: shared_len is for sddmm_attention_shared", who);
+    return run_forward(who, desc, d_q, nullptr, nullptr, d_k, d_v, d_out, d_lse, d_workspace, workspace_bytes, stream);
+}
+
+int sddmm_attention_shared(const sddmm_attention_desc *desc, const void *d_q, const void *d_shared_k, const void *d_shared_v, const void *d_k,
+                           const void *d_v, void *d_out, float *d_lse, void *d_workspace, int64_t workspace_bytes, void *stream)
+{
+    const char *who = "sddmm_attention_shared";
+    if (int rc = check_desc(who, desc)) return rc;
+    if (desc->q_ptr) return fail(SDDMM_ERR_ARG, "%s: rows of packed sequences are not taken", who);
+    if ((int64_t)desc->n_seq * desc->max_q * desc->n_heads > INT32_MAX) return fail(SDDMM_ERR_RANGE, "%s: too many rows", who);
+    return run_forward(who, desc, d_q, d_shared_k, d_shared_v, d_k, d_v, d_out, d_lse, d_workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

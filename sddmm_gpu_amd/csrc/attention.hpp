@@ -1,0 +1,277 @@
+// Dense attention (gfx950): arguments of the kernels, and the pieces that they share -- fragments of the matrix
+// instructions, tiles of rows in LDS, masks and scores.
+//
+// Every product is made of 32 x 32 x 16 matrix instructions (fp32: eight of 32 x 32 x 2).  A lane l of a wave holds, with
+// n = l % 32 and h = l / 32:
+//   operands   row (or column) n, elements 8 h + j of the 16 that are summed over, j = 0 .. 7
+//   results    column n, rows 8 (i / 4) + 4 h + i % 4, i = 0 .. 15
+// The order of summation is free as long as both operands agree, so the eight results i = 8 c .. 8 c + 7 of a lane, rounded to
+// the element type, are an operand of the next product as they are: its sum then runs over 16 c + 8 (j / 4) + 4 h + j % 4,
+// which is how `column_operand` reads the other operand.  Probabilities and their gradients never leave the registers.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <cstdint>
+#include "../../include/sddmm.h"
+#include "bf16_parts.hpp"
+
+namespace sddmm {
+
+// One call, as the kernels see it (strides in elements).
+struct AttnArgs {
+    const void *q, *k, *v;
+    void *out;                  // forward: written; backward: read
+    float *lse;                 // [rows][n_heads] or null; backward: read
+    const void *shared_k, *shared_v;
+    const void *dout;
+    void *dq, *dk, *dv;
+    float *part_o;              // partial results of split keys: [part][row of all heads][head_dim]
+    float2 *part_ml;            // [part][row of all heads]: maximum (in powers of two) and sum
+    float2 *stats;              // backward: [n_heads][all rows] (log-sum-exp in powers of two, sum of dout * out)
+    float *slope_part;          // backward: [n_heads][workgroups of a head] parts of the slopes' gradients
+    int64_t q_seq, q_row, q_head, k_seq, k_row, k_head, v_seq, v_row, v_head, o_seq, o_row, o_head;
+    const int32_t *q_ptr, *k_ptr, *q_len, *k_len, *prefix;
+    const float *slopes;
+    int64_t rows;               // rows of all sequences (of q_ptr: at most)
+    int32_t head_dim, n_heads, n_kv_heads, group, n_seq, max_q, max_k, left, right, shared_len;
+    int32_t n_slots;            // tiles of rows (or keys) that the grid holds
+    int32_t n_split;            // pieces that the keys of a tile of rows are cut into
+    int32_t part0, n_part;      // first piece of this launch, pieces in all
+    float scale, cap;
+};
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float floatx8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+
+template <class T> struct Elem;
+template <> struct Elem<__bf16> {
+    typedef bf16x8 Vec8;
+    typedef bf16x4 Vec4;
+    static __device__ __forceinline__ floatx16 mma(Vec8 a, Vec8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Elem<_Float16> {
+    typedef half8 Vec8;
+    typedef half4 Vec4;
+    static __device__ __forceinline__ floatx16 mma(Vec8 a, Vec8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Elem<float> {
+    typedef floatx8 Vec8;
+    typedef floatx4 Vec4;
+    static __device__ __forceinline__ floatx16 mma(Vec8 a, Vec8 b, floatx16 c)
+    {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+__device__ __forceinline__ floatx16 zero16()
+{
+    return floatx16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+}
+
+// results 8 c .. 8 c + 7 as an operand, rounded to the element type
+template <class T>
+__device__ __forceinline__ typename Elem<T>::Vec8 operand(const floatx16 &r, int c)
+{
+    floatx8 x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = r[8 * c + j];
+    return __builtin_convertvector(x, typename Elem<T>::Vec8);
+}
+
+// the two halves of a wave hold parts of the same column: both get the maximum / the sum
+__device__ __forceinline__ float halves_max(float x)
+{
+    const uint2v r = __builtin_bit_cast(uint2v, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ __forceinline__ float halves_sum(float x)
+{
+    const uint2v r = __builtin_bit_cast(uint2v, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+
+// A tile of R rows of DP elements in LDS.  A row's 16-byte pieces are exchanged among themselves by its number so that both
+// ways of reading are free of bank conflicts: 16 rows at one piece (`row_operand`), and 4 rows at 64 consecutive bytes (`column_operand`).
+template <class T, int DP, int R>
+struct Tile {
+    static constexpr int kRowBytes = DP * (int)sizeof(T);
+    static constexpr int kBytes = R * kRowBytes;
+    static constexpr int kPieces = kRowBytes / 16;
+    static_assert(kRowBytes == 128 || kRowBytes == 256 || kRowBytes == 512);
+
+    static __device__ __forceinline__ int turn(int row)
+    {
+        return kRowBytes == 128 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+    }
+
+    // Requests the tile: rows 0 .. R - 1 at `base`, `stride` bytes apart, of which `valid` exist and have `bytes` bytes; all
+    // else becomes 0.  NW waves share the work; what arrives goes straight to LDS.
+    template <int NW>
+    static __device__ __forceinline__ void request(char *lds, const char *base, uint32_t stride, int valid, int bytes, int wave, int lane)
+    {
+        const uint32_t range = valid > 0 ? (uint32_t)(min(valid, R) - 1) * stride + (uint32_t)bytes : 0u;
+        uint4v src = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)base),
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)((uintptr_t)base >> 32) & 0xffffu)),
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)range), 0x00020000u};
+        uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds);
+        asm volatile("s_nop 4" : "+s"(src), "+s"(to));  // (scalars that a vector instruction wrote, before a load reads them)
+        constexpr int kSteps = kBytes / 1024 / NW;
+        static_assert(kSteps * NW * 1024 == kBytes);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int at = (i * NW + wave) * 1024;
+            const int pos = at + lane * 16, row = pos / kRowBytes, piece = (pos % kRowBytes / 16) ^ turn(row);
+            const uint32_t off = piece * 16 < bytes ? (uint32_t)row * stride + (uint32_t)piece * 16 : 0x7ffffff0u;
+            // (not the builtin: behind it the compiler waits for all loads before it reads LDS in the transposing way.  It keeps
+            // nothing in m0 by itself, and nothing else in these kernels needs that register.)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to + at), "v"(off), "s"(src) : "memory");
+        }
+    }
+
+    // elements 16 c + 8 h + j of row block + n
+    static __device__ __forceinline__ typename Elem<T>::Vec8 row_operand(const char *lds, int block, int c, int lane)
+    {
+        const int row = block + (lane & 31), h = lane >> 5;
+        const char *p = lds + row * kRowBytes;
+        if constexpr (sizeof(T) == 2) {
+            return *(const typename Elem<T>::Vec8 *)(p + (((2 * c + h) ^ turn(row)) << 4));
+        } else {
+            const floatx4 a = *(const floatx4 *)(p + (((4 * c + 2 * h) ^ turn(row)) << 4));
+            const floatx4 b = *(const floatx4 *)(p + (((4 * c + 2 * h + 1) ^ turn(row)) << 4));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+
+    // element 32 d + n of the rows 16 c + 8 (j / 4) + 4 h + j % 4 (a transposing read: 16 lanes take 4 rows of 16 elements)
+    static __device__ __forceinline__ typename Elem<T>::Vec8 column_operand(const char *lds, int d, int c, int lane)
+    {
+        const int h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            const int i = lane & 15, piece = 4 * d + ((lane >> 3) & 2) + ((i >> 1) & 1);
+            short4v r[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int row = 16 * c + 8 * k + 4 * h + (i >> 2);
+                r[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) short4v *)(lds + row * kRowBytes + ((piece ^ turn(row)) << 4) + (i & 1) * 8));
+            }
+            typedef short short8 __attribute__((ext_vector_type(8)));
+            const short8 s = __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(typename Elem<T>::Vec8, s);
+        } else {
+            floatx8 x;
+            const int col = 32 * d + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = 16 * c + 8 * (j >> 2) + 4 * h + (j & 3);
+                x[j] = *(const float *)(lds + row * kRowBytes + (((col >> 2) ^ turn(row)) << 4) + (col & 3) * 4);
+            }
+            return x;
+        }
+    }
+};
+
+// All requested tiles have arrived, for every wave, and no wave reads the other buffer any more.
+__device__ __forceinline__ void tiles_arrived()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0), in a form that the compiler counts
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Eight elements of a row in global memory, 0 behind its end.
+template <class T>
+__device__ __forceinline__ typename Elem<T>::Vec8 global_operand(const T *row, bool there, int at, int dim)
+{
+    typename Elem<T>::Vec8 x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (T)0.f;
+    if (there && at < dim) x = *(const typename Elem<T>::Vec8 *)(row + at);
+    return x;
+}
+
+// A sequence: where its rows and keys begin and how many there are.  Lengths from the device are held to their bounds.
+struct Seq {
+    int64_t q0, k0;  // first row and key, in rows of q_row and k_row (0 where sequences have strides of their own)
+    int64_t lse0;    // first row in lse
+    int32_t nq, nk;
+};
+__device__ __forceinline__ Seq sequence(const AttnArgs &a, int s)
+{
+    Seq r;
+    if (a.q_ptr) {
+        r.q0 = r.lse0 = a.q_ptr[s];
+        r.nq = max(0, a.q_ptr[s + 1] - a.q_ptr[s]);
+    } else {
+        r.q0 = 0;
+        r.lse0 = (int64_t)s * a.max_q;
+        r.nq = a.q_len ? min(max(0, a.q_len[s]), a.max_q) : a.max_q;
+    }
+    if (a.k_ptr) {
+        r.k0 = a.k_ptr[s];
+        r.nk = max(0, a.k_ptr[s + 1] - a.k_ptr[s]);
+    } else {
+        r.k0 = 0;
+        r.nk = a.k_len ? min(max(0, a.k_len[s]), a.max_k) : a.max_k;
+    }
+    return r;
+}
+template <class T> __device__ __forceinline__ const T *q_base(const AttnArgs &a, const void *q, const Seq &e, int s, int head)
+{
+    return (const T *)q + (a.q_ptr ? e.q0 * a.q_row : s * a.q_seq) + head * a.q_head;
+}
+template <class T> __device__ __forceinline__ const T *o_base(const AttnArgs &a, const void *o, const Seq &e, int s, int head)
+{
+    return (const T *)o + (a.q_ptr ? e.q0 * a.o_row : s * a.o_seq) + head * a.o_head;
+}
+template <class T> __device__ __forceinline__ const T *k_base(const AttnArgs &a, const void *k, const Seq &e, int s, int kv)
+{
+    return (const T *)k + (a.k_ptr ? e.k0 * a.k_row : s * a.k_seq) + kv * a.k_head;
+}
+template <class T> __device__ __forceinline__ const T *v_base(const AttnArgs &a, const void *v, const Seq &e, int s, int kv)
+{
+    return (const T *)v + (a.k_ptr ? e.k0 * a.v_row : s * a.v_seq) + kv * a.v_head;
+}
+
+// Tiles of `size` rows of packed sequences: sequence s takes the slots from ptr[s] / size + s on, which is at least as many as it
+// needs, so that no count of all tiles has to be known beforehand.
+__device__ __forceinline__ int slot_sequence(const int32_t *ptr, int n_seq, int size, int slot, int &tile)
+{
+    int lo = 0, hi = n_seq;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (ptr[mid] / size + mid <= slot) lo = mid; else hi = mid;
+    }
+    tile = slot - (ptr[lo] / size + lo);
+    return lo;
+}
+
+// The keys that a row at position pos sees: [lo, hi).
+__device__ __forceinline__ int first_key(const AttnArgs &a, int pos) { return a.left < 0 ? 0 : max(0, pos - a.left); }
+__device__ __forceinline__ int end_key(const AttnArgs &a, int pos, int prefix, int n_keys)
+{
+    return a.right < 0 ? n_keys : min(n_keys, max(min(pos, INT32_MAX - 1 - a.right) + a.right + 1, prefix));
+}
+
+// tanh(x) / x by powers of x^2 where |x| <= 0.25 (the next term is 1e-8 of it), and the whole function elsewhere: 1 - 2 / (1 + e^2x)
+// loses 24 bits below the difference's last place for small x.
+__device__ __forceinline__ float tanh_any(float x)
+{
+    const float s = x * x;
+    const float near = x * fmaf(s, fmaf(s, fmaf(s, fmaf(s, 0.021869489f, -0.053968254f), 0.13333334f), -0.33333334f), 1.f);
+    const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e));
+    const float away = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f);
+    return s <= 0.0625f ? near : away;
+}
+
+}  // namespace sddmm

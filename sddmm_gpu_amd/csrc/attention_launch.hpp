@@ -1,0 +1,17 @@
+// Launches of the dense attention kernels, for the entry points.
+#pragma once
+#include <hip/hip_runtime.h>
+
+namespace sddmm {
+
+struct AttnArgs;
+
+enum { kRowsOfHead = 0, kRowsPacked = 1, kRowsShared = 2 };  // what the rows of a forward workgroup are (attention_forward.hip)
+
+int attention_forward_rows();  // rows of a workgroup
+int attention_token_rows();
+hipError_t launch_attention_forward(const AttnArgs &a, int type, int rows, unsigned grid, hipStream_t st);
+hipError_t launch_attention_token(const AttnArgs &a, int type, unsigned grid, hipStream_t st);
+hipError_t launch_attention_join(const AttnArgs &a, int type, hipStream_t st);
+
+}  // namespace sddmm
