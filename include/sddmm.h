@@ -584,6 +584,14 @@ int sddmm_attention_shared(const sddmm_attention_desc *desc, const void *d_q, co
                            const void *d_k, const void *d_v, void *d_out, float *d_lse, void *d_workspace,
                            int64_t workspace_bytes, void *stream);
 
+/* Gradients of sum(out * d_out) by q, k and v (each laid out as its operand, d_dout as out), and by the slopes (d_dslopes, [n_heads] fp32;
+ * NULL: not wanted).  d_out and d_lse are what sddmm_attention_forward left for the same description and operands.  They are
+ * overwritten, not added to; a key head's are the sums over the query heads that share it, keys that no row sees get 0.
+ * No atomics: the same bits on every call.  No gradient may lie in an operand's place.  */
+int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, const void *d_k, const void *d_v, const void *d_out,
+                             const float *d_lse, const void *d_dout, void *d_dq, void *d_dk, void *d_dv, float *d_dslopes,
+                             void *d_workspace, int64_t workspace_bytes, void *stream);
+
 /* Measurement aid: copies n_bytes (a multiple of 16, both pointers 16-byte
  * aligned device memory) with a plain streaming kernel, sddmm_copy_probe_kernel,
  * on `stream`.  A profile of a run that also calls this holds a kernel of known

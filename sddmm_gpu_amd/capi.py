@@ -160,6 +160,7 @@ SIGNATURES = {
     "sddmm_attention_workspace_bytes": (c_int, [POINTER(AttentionDesc), POINTER(c_int64), POINTER(c_int64)]),
     "sddmm_attention_forward": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 6 + [c_int64, c_void_p]),
     "sddmm_attention_shared": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 8 + [c_int64, c_void_p]),
+    "sddmm_attention_backward": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 11 + [c_int64, c_void_p]),
     "sddmm_copy_probe": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "sddmm_device_info": (c_int, [POINTER(c_int), c_char_p, c_int]),
 }
@@ -496,6 +497,14 @@ def attention_shared(desc, d_q, d_shared_k, d_shared_v, d_k, d_v, d_out, d_lse=0
     """sddmm_attention_shared: sequences that begin with the same desc.shared_len keys."""
     rc = lib().sddmm_attention_shared(byref(desc), d_q or None, d_shared_k or None, d_shared_v or None, d_k or None, d_v or None, d_out or None,
                                       d_lse or None, d_workspace or None, workspace_bytes, stream or None)
+    if rc:
+        check(rc)
+
+
+def attention_backward(desc, d_q, d_k, d_v, d_out, d_lse, d_dout, d_dq, d_dk, d_dv, d_dslopes=0, d_workspace=0, workspace_bytes=0, stream=0):
+    """sddmm_attention_backward: the gradients of attention_forward's operands (and of the slopes)."""
+    rc = lib().sddmm_attention_backward(byref(desc), d_q or None, d_k or None, d_v or None, d_out or None, d_lse or None, d_dout or None, d_dq or None,
+                                        d_dk or None, d_dv or None, d_dslopes or None, d_workspace or None, workspace_bytes, stream or None)
     if rc:
         check(rc)
 

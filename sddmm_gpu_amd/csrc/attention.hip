@@ -105,6 +105,36 @@ Deal deal(const sddmm_attention_desc &d)
     return r;
 }
 
+// The same for the backward pass.
+struct DealBack {
+    int64_t rows = 0, key_rows = 0, q_slots = 0, kv_slots = 0, q_grid = 0, kv_grid = 0, splits = 1, slope_parts = 0;
+    int64_t lse_at = 0, delta_at = 0, parts_at = 0, slopes_at = 0, bytes = 0;  // places in the workspace
+};
+
+DealBack deal_back(const sddmm_attention_desc &d)
+{
+    DealBack r;
+    const int64_t tile = attention_backward_rows(), group = d.n_heads / d.n_kv_heads;
+    r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
+    r.key_rows = d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k;
+    if (r.rows > 0) {
+        r.q_slots = d.q_ptr ? r.rows / tile + d.n_seq : div_up(d.max_q, tile);
+        r.slope_parts = r.q_slots * (d.q_ptr ? 1 : d.n_seq);
+        r.q_grid = r.slope_parts * d.n_heads;
+    }
+    if (r.key_rows > 0) {
+        r.kv_slots = d.k_ptr ? r.key_rows / tile + d.n_seq : div_up(d.max_k, tile);
+        const int64_t workgroups = r.kv_slots * (d.k_ptr ? 1 : d.n_seq) * d.n_kv_heads;
+        r.splits = std::min<int64_t>(pieces(workgroups, group * d.max_q, 256), 16);
+        r.kv_grid = workgroups * r.splits;
+    }
+    r.delta_at = padded(r.rows * d.n_heads * 4);
+    r.parts_at = 2 * r.delta_at;
+    r.slopes_at = r.parts_at + (r.splits > 1 ? padded(2 * r.splits * r.key_rows * d.n_kv_heads * d.head_dim * 4) : 0);
+    r.bytes = r.slopes_at + (d.slopes ? padded(r.slope_parts * d.n_heads * 8) : 0);
+    return r;
+}
+
 AttnArgs arguments(const sddmm_attention_desc &d)
 {
     AttnArgs a{};
@@ -112,6 +142,7 @@ AttnArgs arguments(const sddmm_attention_desc &d)
     a.v_seq = d.v_seq, a.v_row = d.v_row, a.v_head = d.v_head, a.o_seq = d.o_seq, a.o_row = d.o_row, a.o_head = d.o_head;
     a.q_ptr = d.q_ptr, a.k_ptr = d.k_ptr, a.q_len = d.q_len, a.k_len = d.k_len, a.prefix = d.prefix, a.slopes = d.slopes;
     a.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
+    a.key_rows = d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k;
     a.head_dim = d.head_dim, a.n_heads = d.n_heads, a.n_kv_heads = d.n_kv_heads, a.group = d.n_heads / d.n_kv_heads;
     a.n_seq = d.n_seq, a.max_q = d.max_q, a.max_k = d.max_k, a.left = d.window_left, a.right = d.window_right, a.shared_len = d.shared_len;
     a.scale = d.scale, a.cap = d.cap;
@@ -171,7 +202,7 @@ int sddmm_attention_workspace_bytes(const sddmm_attention_desc *desc, int64_t *f
 {
     if (int rc = check_desc("sddmm_attention_workspace_bytes", desc)) return rc;
     if (forward) *forward = deal(*desc).bytes;
-    if (backward) *backward = 0;
+    if (backward) *backward = deal_back(*desc).bytes;
     return SDDMM_OK;
 }
 
@@ -192,6 +223,36 @@ int sddmm_attention_shared(const sddmm_attention_desc *desc, const void *d_q, co
     if (desc->q_ptr) return fail(SDDMM_ERR_ARG, "%s: rows of packed sequences are not taken", who);
     if ((int64_t)desc->n_seq * desc->max_q * desc->n_heads > INT32_MAX) return fail(SDDMM_ERR_RANGE, "%s: too many rows", who);
     return run_forward(who, desc, d_q, d_shared_k, d_shared_v, d_k, d_v, d_out, d_lse, d_workspace, workspace_bytes, stream);
+}
+
+int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, const void *d_k, const void *d_v, const void *d_out,
+                             const float *d_lse, const void *d_dout, void *d_dq, void *d_dk, void *d_dv, float *d_dslopes, void *d_workspace,
+                             int64_t workspace_bytes, void *stream)
+{
+    const char *who = "sddmm_attention_backward";
+    if (int rc = check_desc(who, desc)) return rc;
+    const sddmm_attention_desc &d = *desc;
+    if (d.shared_len) return fail(SDDMM_ERR_ARG, "%s: shared_len is for sddmm_attention_shared", who);
+    if (d_dslopes && !d.slopes) return fail(SDDMM_ERR_ARG, "%s: gradients of slopes that are not there", who);
+    const DealBack r = deal_back(d);
+    if (d.n_seq == 0 || (r.rows == 0 && r.key_rows == 0 && !d_dslopes)) return SDDMM_OK;
+    if ((r.rows > 0 && (!d_q || !d_out || !d_lse || !d_dout || !d_dq)) || (r.key_rows > 0 && (!d_k || !d_v || !d_dk || !d_dv)))
+        return fail(SDDMM_ERR_ARG, "%s: NULL device pointer", who);
+    if (!aligned({d_q, d_k, d_v, d_out, d_dout, d_dq, d_dk, d_dv})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
+    if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
+        return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
+    if (r.q_grid > INT32_MAX || r.kv_grid > INT32_MAX || r.rows * d.n_heads / 16 > INT32_MAX || r.key_rows * d.n_kv_heads > INT32_MAX)
+        return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
+
+    AttnArgs a = arguments(d);
+    char *ws = (char *)d_workspace;
+    a.q = d_q, a.k = d_k, a.v = d_v, a.out = (void *)d_out, a.lse = (float *)d_lse, a.dout = d_dout, a.dq = d_dq, a.dk = d_dk, a.dv = d_dv;
+    a.stat_lse = (float *)(ws + r.lse_at), a.stat_delta = (float *)(ws + r.delta_at), a.part_o = (float *)(ws + r.parts_at);
+    a.dslopes = d_dslopes, a.slope_part = d_dslopes ? (double *)(ws + r.slopes_at) : nullptr, a.slope_parts = (int)r.slope_parts;
+    a.n_slots = (int)r.kv_slots, a.n_split = (int)r.splits;
+    const hipError_t e = launch_attention_backward(a, d.type, (unsigned)r.kv_grid, (unsigned)r.q_grid, (int)r.q_slots, (hipStream_t)stream);
+    if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
+    return SDDMM_OK;
 }
 
 }  // extern "C"

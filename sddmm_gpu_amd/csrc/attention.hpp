@@ -26,16 +26,18 @@ struct AttnArgs {
     void *dq, *dk, *dv;
     float *part_o;              // partial results of split keys: [part][row of all heads][head_dim]
     float2 *part_ml;            // [part][row of all heads]: maximum (in powers of two) and sum
-    float2 *stats;              // backward: [n_heads][all rows] (log-sum-exp in powers of two, sum of dout * out)
-    float *slope_part;          // backward: [n_heads][workgroups of a head] parts of the slopes' gradients
+    float *stat_lse, *stat_delta;  // backward: [n_heads][all rows] log-sum-exp in powers of two, sum of dout * out
+    double *slope_part;         // backward: [n_heads][slope_parts] parts of the slopes' gradients, or null
+    float *dslopes;
     int64_t q_seq, q_row, q_head, k_seq, k_row, k_head, v_seq, v_row, v_head, o_seq, o_row, o_head;
     const int32_t *q_ptr, *k_ptr, *q_len, *k_len, *prefix;
     const float *slopes;
-    int64_t rows;               // rows of all sequences (of q_ptr: at most)
+    int64_t rows, key_rows;     // rows and keys of all sequences (of q_ptr, k_ptr: at most)
     int32_t head_dim, n_heads, n_kv_heads, group, n_seq, max_q, max_k, left, right, shared_len;
     int32_t n_slots;            // tiles of rows (or keys) that the grid holds
     int32_t n_split;            // pieces that the keys of a tile of rows are cut into
     int32_t part0, n_part;      // first piece of this launch, pieces in all
+    int32_t slope_parts;
     float scale, cap;
 };
 
@@ -179,6 +181,20 @@ struct Tile {
         }
     }
 };
+
+// Requests R floats at `base`, of which `valid` exist (all else becomes 0), by one wave.
+template <int R>
+__device__ __forceinline__ void request_floats(float *lds, const float *base, int valid, int lane)
+{
+    static_assert(R <= 64);
+    uint4v src = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)base),
+                  (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)((uintptr_t)base >> 32) & 0xffffu)),
+                  (uint32_t)__builtin_amdgcn_readfirstlane(max(0, min(valid, R)) * 4), 0x00020000u};
+    uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)(char *)lds);
+    const uint32_t off = lane * 4;
+    asm volatile("s_nop 4" : "+s"(src), "+s"(to));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(src) : "memory");
+}
 
 // All requested tiles have arrived, for every wave, and no wave reads the other buffer any more.
 __device__ __forceinline__ void tiles_arrived()

@@ -12,6 +12,8 @@ int attention_forward_rows();  // rows of a workgroup
 int attention_token_rows();
 hipError_t launch_attention_forward(const AttnArgs &a, int type, int rows, unsigned grid, hipStream_t st);
 hipError_t launch_attention_token(const AttnArgs &a, int type, unsigned grid, hipStream_t st);
+int attention_backward_rows();
+hipError_t launch_attention_backward(const AttnArgs &a, int type, unsigned kv_grid, unsigned q_grid, int q_slots, hipStream_t st);
 hipError_t launch_attention_join(const AttnArgs &a, int type, hipStream_t st);
 
 }  // namespace sddmm

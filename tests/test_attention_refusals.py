@@ -86,3 +86,31 @@ def test_nothing_to_do():
     forward(desc(n_seq=0), q=0, k=0, v=0, out=0)
     forward(desc(max_q=0), q=0, k=0, v=0, out=0)
     forward(desc(q_ptr=A, q_rows=0), q=0, k=0, v=0, out=0)
+
+
+def backward(d, q=A, k=A, v=A, out=A, lse=A, dout=A, dq=A, dk=A, dv=A, dslopes=0, ws=A, n=1 << 40):
+    capi.attention_backward(d, q, k, v, out, lse, dout, dq, dk, dv, dslopes, ws, n)
+
+
+def test_backward():
+    for kw, says in BAD:
+        with pytest.raises(capi.SddmmError, match=says):
+            backward(desc(**kw))
+    for name in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv"):
+        with pytest.raises(capi.SddmmError, match="NULL device pointer"):
+            backward(desc(), **{name: 0})
+        if name != "lse":
+            with pytest.raises(capi.SddmmError, match="16-byte aligned"):
+                backward(desc(), **{name: A + 8})
+    with pytest.raises(capi.SddmmError, match="slopes that are not there"):
+        backward(desc(), dslopes=A)
+    with pytest.raises(capi.SddmmError, match="sddmm_attention_shared"):
+        backward(desc(shared_len=5))
+    need = capi.attention_workspace_bytes(desc())[1]
+    for kw in (dict(ws=0), dict(n=need - 1), dict(ws=A + 128)):
+        with pytest.raises(capi.SddmmError, match="workspace"):
+            backward(desc(), **kw)
+    with pytest.raises(capi.SddmmError, match="one launch"):
+        backward(desc(n_seq=1 << 18, max_q=1 << 12, n_heads=65536, n_kv_heads=1, q_seq=64, o_seq=64, q_row=64, o_row=64))
+    backward(desc(n_seq=0), *[0] * 9)
+    backward(desc(max_q=0, max_k=0), *[0] * 9)
