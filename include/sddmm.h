@@ -592,6 +592,38 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
                              const float *d_lse, const void *d_dout, void *d_dq, void *d_dk, void *d_dv, float *d_dslopes,
                              void *d_workspace, int64_t workspace_bytes, void *stream);
 
+/* Rotary positions: the rows of queries and keys (or of W and H) turned by angles that grow with their position, so that
+ * products depend on distances.  Of a head's first rot_dim elements pair e = 0 .. rot_dim / 2 - 1 becomes
+ *     (x, y) -> amplitude * (x cos - y sin, x sin + y cos),   angle = position * freq[e] radians
+ * the pair being elements (e, e + rot_dim / 2) (SDDMM_ROTARY_HALF) or (2 e, 2 e + 1) (_INTERLEAVED); the rest of a head is
+ * copied.  inverse: with -angle, which is the gradient.  Angles are taken in 64 bits, results of any type rounded once.  Row r
+ * of q and k has the position d_positions[r] (device, int32), or first_position + r where d_positions is NULL; d_freq is a
+ * device array of rot_dim / 2 doubles, from sddmm_rotary_frequencies or the caller's own.  Strides in elements; d_q_out may
+ * be d_q with the same strides (in place), or for instance the rows of a cache; no n_kv_heads: d_k is not looked at.
+ * Any sizes and alignment (the elements' own); pieces of 16 bytes are the fast way.  No counterpart in the reference.  */
+enum { SDDMM_ROTARY_HALF = 0, SDDMM_ROTARY_INTERLEAVED = 1 };
+typedef struct sddmm_rotary_desc {
+    int32_t type;                          /* SDDMM_TYPE_*, of q and k */
+    int32_t head_dim, n_heads, n_kv_heads;
+    int32_t rot_dim;                       /* even, 2 .. head_dim */
+    int32_t layout, inverse;
+    float amplitude;
+    int64_t n_rows, first_position;
+    int64_t q_row, q_head, q_out_row, q_out_head;
+    int64_t k_row, k_head, k_out_row, k_out_head;
+} sddmm_rotary_desc;
+void sddmm_rotary_desc_init(sddmm_rotary_desc *desc);   /* zeros, amplitude 1 */
+int sddmm_rotary(const sddmm_rotary_desc *desc, const int32_t *d_positions, const double *d_freq, const void *d_q, void *d_q_out,
+                 const void *d_k, void *d_k_out, void *stream);
+/* The frequencies of rot_dim / 2 pairs, base^(-2 e / rot_dim), and what longer contexts than the known_len positions that a model was
+ * made for do to them (factor: how many times longer; host memory; *amplitude is 1 where not said otherwise):
+ *   PLAIN   nothing          LINEAR  all divided by factor      BASE  the base times factor^(rot_dim / (rot_dim - 2))
+ *   BANDS   pairs of more than `high` turns in known_len kept, of fewer than `low` divided, a mixture between
+ *   PARTS   a ramp over the pairs' numbers, from those of `high` turns (kept) to those of `low` (divided); amplitude 0.1 ln(factor) + 1 */
+enum { SDDMM_ROTARY_PLAIN = 0, SDDMM_ROTARY_LINEAR = 1, SDDMM_ROTARY_BASE = 2, SDDMM_ROTARY_BANDS = 3, SDDMM_ROTARY_PARTS = 4 };
+int sddmm_rotary_frequencies(int32_t rot_dim, double base, int32_t scaling, double factor, int64_t known_len, double low, double high,
+                             double *freq, double *amplitude);
+
 /* Measurement aid: copies n_bytes (a multiple of 16, both pointers 16-byte
  * aligned device memory) with a plain streaming kernel, sddmm_copy_probe_kernel,
  * on `stream`.  A profile of a run that also calls this holds a kernel of known

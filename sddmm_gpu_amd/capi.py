@@ -20,6 +20,8 @@ KERNEL_AUTO, KERNEL_ROW_GATHER, KERNEL_LDS_TILE, KERNEL_PANEL, KERNEL_HYBRID, KE
 EPILOGUE_SCALE, EPILOGUE_RESIDUAL = 0, 1
 FORM_SOFTMAX = 0x100
 TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BANDS, ROTARY_PARTS = range(5)
 SPMM_CSR, SPMM_TILES, SPMM_WALK, SPMM_BLOCKS = 0, 1, 2, 3
 
 
@@ -92,6 +94,32 @@ class AttentionDesc(C.Structure):
         return cls.defaults(type=type, n_seq=n_seq, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, **{**d, **kw})
 
 
+class RotaryDesc(C.Structure):
+    """sddmm_rotary_desc; RotaryDesc.defaults(**fields) starts from sddmm_rotary_desc_init."""
+    _fields_ = [(n, c_int32) for n in ("type", "head_dim", "n_heads", "n_kv_heads", "rot_dim", "layout", "inverse")] + [("amplitude", c_float)] + [
+        (n, c_int64) for n in ("n_rows", "first_position", "q_row", "q_head", "q_out_row", "q_out_head", "k_row", "k_head", "k_out_row", "k_out_head")]
+
+    @classmethod
+    def defaults(cls, **kw):
+        d = cls()
+        lib().sddmm_rotary_desc_init(byref(d))
+        for k, v in kw.items():
+            if k not in dict(cls._fields_):
+                raise KeyError(k)
+            setattr(d, k, v)
+        return d
+
+    @classmethod
+    def packed(cls, type, n_rows, n_heads, n_kv_heads, head_dim, rot_dim, layout, **kw):
+        """The strides of contiguous arrays [rows, heads, head_dim], of the results too."""
+        d = {}
+        for n, heads in (("q", n_heads), ("k", n_kv_heads)):
+            for out in ("", "_out"):
+                d[n + out + "_row"], d[n + out + "_head"] = heads * head_dim, head_dim
+        return cls.defaults(type=type, n_rows=n_rows, n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim, rot_dim=rot_dim, layout=layout,
+                            **{**d, **kw})
+
+
 class LaunchProfile(C.Structure):
     _fields_ = [("kernel", c_int32), ("lanes_per_nnz", c_int32), ("k_slice", c_int32), ("n_kernel_launches", c_int32),
                 ("nnz", c_int64), ("rows", c_int64), ("stream_positions", c_int64), ("ms", c_float)]
@@ -161,6 +189,9 @@ SIGNATURES = {
     "sddmm_attention_forward": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 6 + [c_int64, c_void_p]),
     "sddmm_attention_shared": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 8 + [c_int64, c_void_p]),
     "sddmm_attention_backward": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 11 + [c_int64, c_void_p]),
+    "sddmm_rotary_desc_init": (None, [POINTER(RotaryDesc)]),
+    "sddmm_rotary": (c_int, [POINTER(RotaryDesc)] + [c_void_p] * 7),
+    "sddmm_rotary_frequencies": (c_int, [c_int32, c_double, c_int32, c_double, c_int64, c_double, c_double, c_void_p, POINTER(c_double)]),
     "sddmm_copy_probe": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "sddmm_device_info": (c_int, [POINTER(c_int), c_char_p, c_int]),
 }
@@ -407,6 +438,8 @@ class Plan:
 
     def spmm_form(self):
         """TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BANDS, ROTARY_PARTS = range(5)
 SPMM_CSR, SPMM_TILES or SPMM_WALK: what spmm does behind this plan."""
         f = c_int32()
         check(lib().sddmm_plan_spmm_form(self.h, byref(f)))
@@ -507,6 +540,21 @@ def attention_backward(desc, d_q, d_k, d_v, d_out, d_lse, d_dout, d_dq, d_dk, d_
                                         d_dk or None, d_dv or None, d_dslopes or None, d_workspace or None, workspace_bytes, stream or None)
     if rc:
         check(rc)
+
+
+def rotary(desc, d_positions, d_freq, d_q, d_q_out, d_k=0, d_k_out=0, stream=0):
+    """sddmm_rotary: rotary positions of queries and keys (desc: RotaryDesc; d_positions 0: first_position on)."""
+    rc = lib().sddmm_rotary(byref(desc), d_positions or None, d_freq or None, d_q or None, d_q_out or None, d_k or None, d_k_out or None, stream or None)
+    if rc:
+        check(rc)
+
+
+def rotary_frequencies(rot_dim, base=10000.0, scaling=ROTARY_PLAIN, factor=1.0, known_len=1, low=0.0, high=0.0):
+    """(float64 array of rot_dim / 2 radians a position, amplitude): sddmm_rotary_frequencies."""
+    freq = np.empty(max(rot_dim // 2, 0), np.float64)
+    amplitude = c_double()
+    check(lib().sddmm_rotary_frequencies(rot_dim, base, scaling, factor, known_len, low, high, _np_ptr(freq), byref(amplitude)))
+    return freq, amplitude.value
 
 
 def copy_probe(d_src, d_dst, n_bytes, stream=0):

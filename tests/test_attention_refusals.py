@@ -111,6 +111,6 @@ def test_backward():
         with pytest.raises(capi.SddmmError, match="workspace"):
             backward(desc(), **kw)
     with pytest.raises(capi.SddmmError, match="one launch"):
-        backward(desc(n_seq=1 << 18, max_q=1 << 12, n_heads=65536, n_kv_heads=1, q_seq=64, o_seq=64, q_row=64, o_row=64))
+        backward(desc(n_seq=1 << 18, max_q=1 << 12, n_heads=65536, n_kv_heads=1, q_seq=64, o_seq=64, q_row=64, o_row=64), n=1 << 62)
     backward(desc(n_seq=0), *[0] * 9)
     backward(desc(max_q=0, max_k=0), *[0] * 9)
