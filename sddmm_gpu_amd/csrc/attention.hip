@@ -52,44 +52,40 @@ struct Deal {
     int64_t rows = 0;          // of all sequences
     bool token = false;        // the kernel for few rows
     int mapping = kRowsOfHead;
-    int64_t slots = 0, grid = 0, splits = 1;
+    int64_t slots = 0, max_tiles = 0, grid = 0, splits = 1;
     int64_t shared_slots = 0, shared_grid = 0, shared_splits = 0;
     int64_t parts = 1, part_bytes = 0, bytes = 0;
 };
 
-// Pieces that the keys are cut into: so many that the grid fills the card (256 compute units, two workgroups each), each of
-// `least` keys at least.
+constexpr int64_t kFill = 512;  // workgroups that fill the card: 256 compute units, two each
+
+// Pieces that the keys are cut into: so many that the grid fills the card, each of `least` keys at least.
 int64_t pieces(int64_t workgroups, int64_t keys, int64_t least)
 {
-    const int64_t fill = 512;
-    return std::max<int64_t>(1, std::min(std::min(div_up(fill, std::max<int64_t>(workgroups, 1)), div_up(keys, least)), (int64_t)256));
+    return std::max<int64_t>(1, std::min(std::min(div_up(kFill, std::max<int64_t>(workgroups, 1)), div_up(keys, least)), (int64_t)256));
 }
 
 Deal deal(const sddmm_attention_desc &d)
 {
     Deal r;
-    const int64_t group = d.n_heads / d.n_kv_heads, tile = attention_forward_rows();
+    const int64_t group = d.n_heads / d.n_kv_heads, tile = attention_forward_rows(), few = attention_token_rows();
     r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
     // keys that a tile's rows can see
     const int64_t span = d.window_left >= 0 && d.window_right >= 0 && !d.prefix ? (int64_t)d.window_left + d.window_right + std::min<int64_t>(d.max_q, tile) : d.max_k;
-    const int64_t keys = std::min<int64_t>(d.max_k, span);
-    const int64_t packed = d.max_q * group;
-    r.token = packed <= attention_token_rows();
+    const int64_t keys = std::min<int64_t>(d.max_k, span), seqs = d.q_ptr ? 1 : d.n_seq, packed = d.max_q * group;
+    // tiles of 128 rows, of one head or of pairs of few tokens and the heads that share a key head (not in packed sequences)
+    r.mapping = group > 1 && d.max_q < tile && !d.q_ptr ? kRowsPacked : kRowsOfHead;
+    r.max_tiles = div_up(r.mapping == kRowsPacked ? packed : d.max_q, tile);
+    r.slots = d.q_ptr ? r.rows / tile + d.n_seq : r.max_tiles;
+    r.grid = r.slots * seqs * d.n_kv_heads * (r.mapping == kRowsPacked ? 1 : group);
+    // or tiles of 32 pairs, each wave on keys of its own, where pairs are few or the others would leave compute units without work
+    r.token = packed <= few || r.grid < kFill / 2;
     if (r.token) {
-        r.slots = 1;
-        const int64_t units = (int64_t)d.n_seq * d.n_kv_heads;
-        r.splits = pieces(units, keys, 256);
-        r.grid = units * r.splits;
-    } else {
-        r.mapping = group > 1 && d.max_q < tile ? kRowsPacked : kRowsOfHead;
-        const int64_t share = r.mapping == kRowsPacked ? group : 1, tiles = div_up(d.max_q * share, tile);
-        // (packed sequences: a slot for each tile there can be, see slot_sequence; pairs of tokens and heads are not packed there)
-        if (d.q_ptr && r.mapping == kRowsPacked) r.mapping = kRowsOfHead;
-        if (d.q_ptr) r.slots = r.rows / tile + d.n_seq;
-        else r.slots = r.mapping == kRowsPacked ? tiles : div_up(d.max_q, tile);
-        const int64_t units = (d.q_ptr ? 1 : (int64_t)d.n_seq) * d.n_kv_heads * (r.mapping == kRowsPacked ? 1 : group);
-        r.splits = pieces(units * r.slots, keys, 512);
-        r.grid = units * r.slots * r.splits;
+        r.max_tiles = div_up(packed, few);
+        r.slots = r.max_tiles == 1 ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
+        r.grid = r.slots * d.n_kv_heads;
+        r.splits = pieces(r.grid, keys, 256);
+        r.grid *= r.splits;
     }
     r.parts = r.splits;
     if (d.shared_len > 0) {
@@ -107,7 +103,8 @@ Deal deal(const sddmm_attention_desc &d)
 
 // The same for the backward pass.
 struct DealBack {
-    int64_t rows = 0, key_rows = 0, q_slots = 0, kv_slots = 0, q_grid = 0, kv_grid = 0, splits = 1, slope_parts = 0;
+    int64_t rows = 0, key_rows = 0, q_slots = 0, q_tiles = 0, kv_slots = 0, kv_tiles = 0, q_grid = 0, kv_grid = 0, splits = 1, chunk = 1, slope_parts = 0;
+    bool few = false;
     int64_t lse_at = 0, delta_at = 0, parts_at = 0, slopes_at = 0, bytes = 0;  // places in the workspace
 };
 
@@ -118,14 +115,35 @@ DealBack deal_back(const sddmm_attention_desc &d)
     r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
     r.key_rows = d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k;
     if (r.rows > 0) {
-        r.q_slots = d.q_ptr ? r.rows / tile + d.n_seq : div_up(d.max_q, tile);
-        r.slope_parts = r.q_slots * (d.q_ptr ? 1 : d.n_seq);
-        r.q_grid = r.slope_parts * d.n_heads;
+        for (int64_t rows : {tile, (int64_t)attention_backward_few_rows()}) {
+            r.few = rows != tile;
+            r.q_tiles = div_up(d.max_q, rows);
+            r.q_slots = d.q_ptr ? r.rows / rows + d.n_seq : r.q_tiles;
+            r.slope_parts = r.q_slots * (d.q_ptr ? 1 : d.n_seq);
+            r.q_grid = r.slope_parts * d.n_heads;
+            if (r.q_grid >= kFill / 2) break;
+        }
     }
     if (r.key_rows > 0) {
-        r.kv_slots = d.k_ptr ? r.key_rows / tile + d.n_seq : div_up(d.max_k, tile);
+        r.kv_tiles = div_up(d.max_k, tile);
+        r.kv_slots = d.k_ptr ? r.key_rows / tile + d.n_seq : r.kv_tiles;
         const int64_t workgroups = r.kv_slots * (d.k_ptr ? 1 : d.n_seq) * d.n_kv_heads;
-        r.splits = std::min<int64_t>(pieces(workgroups, group * d.max_q, 256), 16);
+        const bool window = d.window_left >= 0 && d.window_right >= 0 && !d.prefix;
+        const int64_t most = group * (window ? std::min<int64_t>(d.max_q, (int64_t)d.window_left + d.window_right + tile) : d.max_q);
+        // A tile of keys that most rows see is cut where it would take more than 2.5 equal shares of all work.  The work of uneven sequences is
+        // not known here: between the mean and the longest length.  A piece costs the time of some 650 rows, written and read, so
+        // pieces of c rows cost 650 work / c and save half of c at the end: c = sqrt(1300 share).  us of the backward pass, bf16, causal, with
+        // this and whole tiles: 8192 tokens, 16 heads over 4 of 128 1150 and 1853, 13 documents of 22 to 2281 tokens in all 8192 386 and
+        // 590; 4096, 16 over 2 390 and 1537; 2048, 16 over 4 of 64 104 and 300; where whole tiles stay: 8192, 16 over 16 1020, in pieces of 3600 1076.
+        const double mean = d.k_ptr ? (double)r.key_rows / d.n_seq : d.max_k;
+        const double rows = most * std::min(1., std::sqrt(mean / std::max(d.max_k, 1))) * (d.window_right == 0 && !window ? 0.5 : 1.);
+        const int64_t places = d.type == SDDMM_TYPE_F32 && d.head_dim > 64 ? kFill / 2 : kFill, tiles = div_up(r.key_rows, tile) * d.n_kv_heads;
+        const double share = rows * tiles / places;
+        if (most > 2.5 * share) {
+            r.chunk = std::max<int64_t>((int64_t)std::sqrt(1300. * share), 256);
+            r.splits = std::max<int64_t>(1, std::min<int64_t>(div_up(most, r.chunk), 32));
+        }
+        r.chunk = std::max(r.chunk, div_up(most, r.splits));
         r.kv_grid = workgroups * r.splits;
     }
     r.delta_at = padded(r.rows * d.n_heads * 4);
@@ -173,7 +191,7 @@ int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d
     AttnArgs a = arguments(d);
     a.q = d_q, a.k = d_k, a.v = d_v, a.out = d_out, a.lse = d_lse, a.shared_k = d_shared_k, a.shared_v = d_shared_v;
     a.part_o = (float *)d_workspace, a.part_ml = (float2 *)((char *)d_workspace + r.part_bytes);
-    a.n_slots = (int)r.slots, a.n_split = (int)r.splits, a.part0 = 0, a.n_part = (int)r.parts;
+    a.n_slots = (int)r.slots, a.max_tiles = (int)r.max_tiles, a.n_split = (int)r.splits, a.part0 = 0, a.n_part = (int)r.parts;
     const hipStream_t st = (hipStream_t)stream;
     hipError_t e = hipSuccess;
     if (d.shared_len > 0) {
@@ -249,8 +267,10 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
     a.q = d_q, a.k = d_k, a.v = d_v, a.out = (void *)d_out, a.lse = (float *)d_lse, a.dout = d_dout, a.dq = d_dq, a.dk = d_dk, a.dv = d_dv;
     a.stat_lse = (float *)(ws + r.lse_at), a.stat_delta = (float *)(ws + r.delta_at), a.part_o = (float *)(ws + r.parts_at);
     a.dslopes = d_dslopes, a.slope_part = d_dslopes ? (double *)(ws + r.slopes_at) : nullptr, a.slope_parts = (int)r.slope_parts;
-    a.n_slots = (int)r.kv_slots, a.n_split = (int)r.splits;
-    const hipError_t e = launch_attention_backward(a, d.type, (unsigned)r.kv_grid, (unsigned)r.q_grid, (int)r.q_slots, (hipStream_t)stream);
+    AttnArgs b = a;
+    a.n_slots = (int)r.kv_slots, a.max_tiles = (int)r.kv_tiles, a.n_split = (int)r.splits, a.chunk = (int)std::min<int64_t>(r.chunk, INT32_MAX);
+    b.n_slots = (int)r.q_slots, b.max_tiles = (int)r.q_tiles, b.n_split = 1;
+    const hipError_t e = launch_attention_backward(a, b, d.type, (unsigned)r.kv_grid, (unsigned)r.q_grid, r.few, (hipStream_t)stream);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;
 }

@@ -35,9 +35,11 @@ struct AttnArgs {
     int64_t rows, key_rows;     // rows and keys of all sequences (of q_ptr, k_ptr: at most)
     int32_t head_dim, n_heads, n_kv_heads, group, n_seq, max_q, max_k, left, right, shared_len;
     int32_t n_slots;            // tiles of rows (or keys) that the grid holds
+    int32_t max_tiles;          // tiles of a sequence at most
     int32_t n_split;            // pieces that the keys of a tile of rows are cut into
     int32_t part0, n_part;      // first piece of this launch, pieces in all
     int32_t slope_parts;
+    int32_t chunk;              // backward: rows (of all query heads) that a workgroup of keys walks, more being cut into pieces
     float scale, cap;
 };
 
@@ -259,16 +261,39 @@ template <class T> __device__ __forceinline__ const T *v_base(const AttnArgs &a,
     return (const T *)v + (a.k_ptr ? e.k0 * a.v_row : s * a.v_seq) + kv * a.v_head;
 }
 
-// Tiles of `size` rows of packed sequences: sequence s takes the slots from ptr[s] / size + s on, which is at least as many as it
-// needs, so that no count of all tiles has to be known beforehand.
-__device__ __forceinline__ int slot_sequence(const int32_t *ptr, int n_seq, int size, int slot, int &tile)
+// Tiles of `size` rows of packed sequences (of `per` pairs for each row): sequence s takes the slots from ptr[s] * per / size + s on, which
+// is at least as many as it needs, so that no count of all tiles has to be known beforehand.
+//
+// Up to 64 sequences of up to 64 tiles: the slots go to the tiles of all sequences in the order of their distance from their sequence's
+// first one, the farthest first (LAST: from the last one).  Under a causal mask that is the order of their work, so that no long tile starts when
+// the others are done (13 documents, 8192 tokens, 16 heads of 128: @@).  Returns -1 for a slot that is none.
+template <bool LAST>
+__device__ __forceinline__ int slot_sequence(const int32_t *ptr, int n_seq, int per, int size, int max_tiles, int n_slots, int slot, int &tile)
 {
+    if (n_seq <= 64 && max_tiles <= 64) {
+        const int lane = threadIdx.x & 63;
+        int tiles = 0;
+        if (lane < n_seq) tiles = (max(0, ptr[lane + 1] - ptr[lane]) * per + size - 1) / size;
+        for (int r = max_tiles - 1; r >= 0; --r) {
+            uint64_t some = __ballot(tiles > r);
+            const int n = __builtin_popcountll(some);
+            if (slot < n) {
+                for (; slot > 0; --slot) some &= some - 1;
+                const int s = __builtin_ctzll(some);
+                tile = LAST ? __builtin_amdgcn_readlane(tiles, s) - 1 - r : r;
+                return s;
+            }
+            slot -= n;
+        }
+        return -1;
+    }
+    if (!LAST) slot = n_slots - 1 - slot;
     int lo = 0, hi = n_seq;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (ptr[mid] / size + mid <= slot) lo = mid; else hi = mid;
+        if ((int64_t)ptr[mid] * per / size + mid <= slot) lo = mid; else hi = mid;
     }
-    tile = slot - (ptr[lo] / size + lo);
+    tile = slot - (int)((int64_t)ptr[lo] * per / size + lo);
     return lo;
 }
 
@@ -279,15 +304,53 @@ __device__ __forceinline__ int end_key(const AttnArgs &a, int pos, int prefix, i
     return a.right < 0 ? n_keys : min(n_keys, max(min(pos, INT32_MAX - 1 - a.right) + a.right + 1, prefix));
 }
 
-// tanh(x) / x by powers of x^2 where |x| <= 0.25 (the next term is 1e-8 of it), and the whole function elsewhere: 1 - 2 / (1 + e^2x)
-// loses 24 bits below the difference's last place for small x.
-__device__ __forceinline__ float tanh_any(float x)
-{
-    const float s = x * x;
-    const float near = x * fmaf(s, fmaf(s, fmaf(s, fmaf(s, 0.021869489f, -0.053968254f), 0.13333334f), -0.33333334f), 1.f);
-    const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e));
-    const float away = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f);
-    return s <= 0.0625f ? near : away;
-}
+// The bound of scores: cap tanh(t / cap), t = scale * product, of N results in registers, in powers of two (BACK: and 1 - tanh^2 of each).
+// Where all of the wave's |t / cap| are 0.25 at most, which they mostly are, by powers: x (C0 + C1 x^2 + ...), six instructions where 1 - 2 / (1 + e^2y) takes
+// two of the slow kind and as many others, and to the last place, since that difference loses 24 bits below 1 (the next term is 1e-8 of the result).
+struct Bend {
+    float limit, c0, c1, c2, c3, c4, twice, to, cap;
+    __device__ __forceinline__ void init(float scale, float cap_)
+    {
+        cap = cap_;
+        const float by = cap > 0.f ? scale / cap : 0.f, s = by * by;
+        to = cap * kLog2e, twice = by * (2.f * kLog2e), limit = cap > 0.f ? 0.25f / by : 0.f;
+        c0 = by, c1 = c0 * s * -0.33333334f, c2 = c0 * s * s * 0.13333334f, c3 = c0 * s * s * s * -0.053968254f, c4 = c0 * s * s * s * s * 0.021869489f;
+    }
+    __device__ __forceinline__ float near(float x) const
+    {
+        const float s = x * x;
+        return x * fmaf(s, fmaf(s, fmaf(s, fmaf(s, c4, c3), c2), c1), c0);
+    }
+    template <int N, bool BACK>
+    __device__ __forceinline__ void apply(floatx16 (&x)[N], floatx16 (&back)[N]) const
+    {
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(x[i][r]));
+        if (__any(!(most <= limit))) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float away = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[i][r] * twice)), 1.f);
+                    x[i][r] = fabsf(x[i][r]) <= limit ? near(x[i][r]) : away;
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[i][r] = near(x[i][r]);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                if constexpr (BACK) back[i][r] = fmaf(-x[i][r], x[i][r], 1.f);
+                x[i][r] *= to;
+            }
+    }
+};
 
 }  // namespace sddmm

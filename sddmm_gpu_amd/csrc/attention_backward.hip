@@ -51,22 +51,18 @@ void sddmm_attention_stats_kernel(const AttnArgs a)
     }
 }
 
-// scores in powers of two from products, and what they have to be multiplied by on the way back
+// scores in powers of two from products, and what their gradients have to be multiplied by on the way back
 template <bool MOD>
-__device__ __forceinline__ void bend(floatx16 &x, floatx16 &back, float scale, float cap, float cap_inv, bool bias, float slope, float at, float step)
+__device__ __forceinline__ void scores(floatx16 &x, floatx16 &back, const Bend &bend, float unit, bool bias, float slope, float at, float step)
 {
     if constexpr (MOD) {
-        if (cap > 0.f) {
-            const float to = cap * kLog2e;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float y = tanh_any(x[r] * cap_inv);
-                back[r] = fmaf(-y, y, 1.f);
-                x[r] = to * y;
-            }
+        if (bend.cap > 0.f) {
+            floatx16 y[1] = {x}, z[1];
+            bend.apply<1, true>(y, z);
+            x = y[0], back = z[0];
         } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) back[r] = 1.f, x[r] *= scale * kLog2e;
+            for (int r = 0; r < 16; ++r) back[r] = 1.f, x[r] *= unit;
         }
         if (bias) {
 #pragma unroll
@@ -74,7 +70,7 @@ __device__ __forceinline__ void bend(floatx16 &x, floatx16 &back, float scale, f
         }
     } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] *= scale * kLog2e;
+        for (int r = 0; r < 16; ++r) x[r] *= unit;
     }
 }
 
@@ -86,6 +82,32 @@ __device__ __forceinline__ int first_row(const AttnArgs &a, int j, int prefix, i
 __device__ __forceinline__ int end_row(const AttnArgs &a, int j, int shift, int n_rows)
 {
     return a.left < 0 ? n_rows : min(n_rows, max(0, min(j, INT32_MAX / 2) + min(a.left, INT32_MAX / 2) + 1 - shift));
+}
+
+// The keys of a workgroup, and how the rows that see them are cut into pieces (a.n_split at most, of about a.chunk rows of all heads): a
+// key tile early in a long sequence has many times the rows of others.
+struct KeyTile {
+    Seq e;
+    int s, kv, tile, shift, prefix, any_lo, any_hi, pieces;
+};
+__device__ __forceinline__ bool key_tile(const AttnArgs &a, int b, KeyTile &k)
+{
+    k.kv = b % a.n_kv_heads;
+    b /= a.n_kv_heads;
+    if (a.k_ptr) {
+        k.s = slot_sequence<true>(a.k_ptr, a.n_seq, 1, kRows, a.max_tiles, a.n_slots, b, k.tile);
+        if (k.s < 0) return false;
+    } else {
+        k.s = b % a.n_seq, k.tile = b / a.n_seq;
+    }
+    k.e = sequence(a, k.s);
+    if (k.tile * kRows >= k.e.nk) return false;
+    k.shift = k.e.nk - k.e.nq, k.prefix = a.prefix ? a.prefix[k.s] : 0;
+    k.any_lo = first_row(a, k.tile * kRows, k.prefix, k.shift);
+    k.any_hi = end_row(a, min(k.e.nk, k.tile * kRows + kRows) - 1, k.shift, k.e.nq);
+    const int64_t rows = (int64_t)max(0, k.any_hi - k.any_lo) * a.group;
+    k.pieces = (int)max((int64_t)1, min((int64_t)a.n_split, (rows + a.chunk - 1) / a.chunk));
+    return true;
 }
 
 // dk and dv.  A wave holds 32 keys: k and v as operands, the sums of dk and dv turned (element of the head by key).  Per tile of rows, q and
@@ -107,20 +129,15 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
     __shared__ __align__(16) float stat[2][2][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
 
-    int b = blockIdx.x, s, tile, split = 0;
-    const int kv = b % a.n_kv_heads;
-    b /= a.n_kv_heads;
-    if (!a.k_ptr) { s = b % a.n_seq; b /= a.n_seq; }
-    if (a.n_split > 1) { split = b % a.n_split; b /= a.n_split; }
-    if (a.k_ptr) s = slot_sequence(a.k_ptr, a.n_seq, kRows, b, tile); else tile = b;
-    const Seq e = sequence(a, s);
-    if (tile * kRows >= e.nk) return;
-    const int shift = e.nk - e.nq, prefix = a.prefix ? a.prefix[s] : 0;
+    KeyTile at_keys;
+    // (pieces outermost: next to each other they would go to different dies, the later ones, of which there are fewer, always to the same)
+    const int groups = gridDim.x / a.n_split, split = blockIdx.x / groups;
+    if (!key_tile(a, blockIdx.x - split * groups, at_keys) || split >= at_keys.pieces) return;
+    const auto [e, s, kv, tile, shift, prefix, any_lo, any_hi, pieces] = at_keys;
     const int key = tile * kRows + wave * 32 + n;
     const bool there = key < e.nk;
     const int lo = first_row(a, key, prefix, shift), hi = there ? end_row(a, key, shift, e.nq) : 0;
-    const int k0 = tile * kRows, k1 = min(e.nk, k0 + kRows) - 1, w0 = k0 + wave * 32, w1 = min(e.nk, w0 + 32) - 1;
-    const int any_lo = first_row(a, k0, prefix, shift), any_hi = end_row(a, k1, shift, e.nq);
+    const int k0 = tile * kRows, w0 = k0 + wave * 32, w1 = min(e.nk, w0 + 32) - 1;
     const int wave_lo = first_row(a, w0, prefix, shift), wave_hi = w1 < w0 ? 0 : end_row(a, w1, shift, e.nq);
     const int full_lo = first_row(a, max(w1, 0), prefix, shift), full_hi = w1 < w0 + 31 ? 0 : end_row(a, w0, shift, e.nq);
 
@@ -141,9 +158,11 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
 #pragma unroll
     for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
 
-    const float scale = a.scale, cap = a.cap, cap_inv = MOD && cap > 0.f ? scale / cap : 0.f;
+    const float scale = a.scale, unit = scale * kLog2e;
+    Bend bend;
+    if constexpr (MOD) bend.init(scale, a.cap);
     const int tiles = any_hi > any_lo ? (any_hi - any_lo + QT - 1) / QT : 0, all = tiles * a.group;
-    const int each = (all + a.n_split - 1) / a.n_split, first = split * each, last = min(all, first + each);
+    const int each = (all + pieces - 1) / pieces, first = split * each, last = min(all, first + each);
     const uint32_t q_stride = (uint32_t)(a.q_row * sizeof(T)), o_stride = (uint32_t)(a.o_row * sizeof(T));
     auto request = [&](int t) {
         const int head = kv * a.group + t / tiles, row = any_lo + t % tiles * QT;
@@ -169,7 +188,7 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
             for (int c = 0; c < DP / 16; ++c) x = Elem<T>::mma(Rows::row_operand(qt, 32 * u, c, l), kf[c], x);
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) y = Elem<T>::mma(Rows::row_operand(dot, 32 * u, c, l), kKeepV ? vf[kKeepV ? c : 0] : Values::row_operand(values, 32 * wave, c, l), y);
-            bend<MOD>(x, back, scale, cap, cap_inv, a.slopes != nullptr, slope, (float)(row + 4 * h + shift - key), 1.f);
+            scores<MOD>(x, back, bend, unit, a.slopes != nullptr, slope, (float)(row + 4 * h + shift - key), 1.f);
             const bool masked = row < full_lo || row + 32 > full_hi;
             const int at = row + 4 * h - lo;
             const uint32_t span = hi > lo ? hi - lo : 0;
@@ -210,7 +229,7 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
     if (!there) return;
 #pragma unroll
     for (int d = 0; d < DB; ++d) dk[d] *= scale;
-    if (a.n_split > 1) {
+    if (pieces > 1) {
         // parts of dk, then of dv: [part][key][key head][head_dim]
         const int64_t place = ((e.k0 + (a.k_ptr ? 0 : (int64_t)s * a.max_k) + key) * a.n_kv_heads + kv) * a.head_dim, part = a.key_rows * a.n_kv_heads * a.head_dim;
         float *to = a.part_o + split * part + place, *to_v = to + a.n_split * part;
@@ -238,49 +257,147 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
         }
 }
 
-// The sum of the parts of dk and dv, four elements a thread.
+// The sum of the parts of dk and dv of the keys whose rows were cut, 16 keys to a workgroup.
+constexpr int kSumKeys = 16;
 template <class T>
 __global__ __launch_bounds__(256)
 void sddmm_attention_dkv_sum_kernel(const AttnArgs a)
 {
-    const int64_t per = a.n_kv_heads * (a.head_dim / 4), at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= a.key_rows * per) return;
-    const int64_t row = at / per;
-    const int rest = (int)(at % per), kv = rest / (a.head_dim / 4), col = rest % (a.head_dim / 4) * 4;
-    int64_t k_off, v_off;
-    if (a.k_ptr) {
-        if (row < a.k_ptr[0] || row >= a.k_ptr[a.n_seq]) return;
-        k_off = row * a.k_row, v_off = row * a.v_row;
-    } else {
-        const int s = (int)(row / a.max_k), i = (int)(row % a.max_k);
-        if (a.k_len && i >= min(a.k_len[s], a.max_k)) return;
-        k_off = s * a.k_seq + i * a.k_row, v_off = s * a.v_seq + i * a.v_row;
+    KeyTile at;
+    if (!key_tile(a, blockIdx.x / (kRows / kSumKeys), at) || at.pieces == 1) return;
+    const int per = a.head_dim / 4, k0 = at.tile * kRows + blockIdx.x % (kRows / kSumKeys) * kSumKeys, n = min(kSumKeys, at.e.nk - k0) * per;
+    const int64_t part = a.key_rows * a.n_kv_heads * a.head_dim, first = at.e.k0 + (a.k_ptr ? 0 : (int64_t)at.s * a.max_k);
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int key = k0 + i / per, col = i % per * 4;
+        const float *from = a.part_o + ((first + key) * a.n_kv_heads + at.kv) * a.head_dim + col, *from_v = from + a.n_split * part;
+        floatx4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll 4
+        for (int p = 0; p < at.pieces; ++p) {
+            x += *(const floatx4 *)(from + p * part);
+            y += *(const floatx4 *)(from_v + p * part);
+        }
+        typedef typename Elem<T>::Vec4 Vec4;
+        *(Vec4 *)((T *)k_base<T>(a, a.dk, at.e, at.s, at.kv) + key * a.k_row + col) = __builtin_convertvector(x, Vec4);
+        *(Vec4 *)((T *)v_base<T>(a, a.dv, at.e, at.s, at.kv) + key * a.v_row + col) = __builtin_convertvector(y, Vec4);
     }
-    const int64_t part = a.key_rows * a.n_kv_heads * a.head_dim;
-    const float *from = a.part_o + at * 4, *from_v = from + a.n_split * part;
-    floatx4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-    for (int p = 0; p < a.n_split; ++p) {
-        x += *(const floatx4 *)(from + p * part);
-        y += *(const floatx4 *)(from_v + p * part);
-    }
-    typedef typename Elem<T>::Vec4 Vec4;
-    *(Vec4 *)((T *)a.dk + k_off + kv * a.k_head + col) = __builtin_convertvector(x, Vec4);
-    *(Vec4 *)((T *)a.dv + v_off + kv * a.v_head + col) = __builtin_convertvector(y, Vec4);
 }
 
-// dq.  A wave holds 32 rows: q and do as operands, the sums of dq turned.  Per tile of keys in LDS: S^T = K Q^T, dP^T = V dO^T, then
+// dq.  A wave holds 32 rows: q and do as operands, the sums of dq turned.  Per tile of 32 keys in LDS: S^T = K Q^T, dP^T = V dO^T, then
 // dQ^T += K^T dS^T.
 //
 // The gradient of a head's slope, - sum ds |p_i - j|, is asked to fp32 whatever the operands' type, and delta, which comes from the rounded
 // output, would put an error of every row times its mean distance into it.  So it is made of sums that need no delta:
 // with far = |p_i - j|, - sum_i (sum_j p dp far - (sum_j p dp) (sum_j p far) / sum_j p).
 template <class T, int DP, bool MOD>
+struct DqRows {
+    static constexpr int DB = DP / 32;
+    typedef typename Elem<T>::Vec8 Vec8;
+    Vec8 qf[DP / 16], of[DP / 16];
+    floatx16 dq[DB];
+    float lse, delta, unit, slope;
+    Bend bend;
+    bool bias, slopes_too, there;
+    int pos, lo, hi, h;
+    double far_ds, far_p, sum_ds, sum_p;
+
+    __device__ __forceinline__ void init(const AttnArgs &a, const Seq &e, int s, int head, int row, int prefix, bool want_slopes, int lane)
+    {
+        h = lane >> 5;
+        there = row < e.nq;
+        pos = row + e.nk - e.nq, lo = first_key(a, pos), hi = there ? end_key(a, pos, prefix, e.nk) : 0;
+        const T *q = q_base<T>(a, a.q, e, s, head) + row * a.q_row, *dout = o_base<T>(a, a.dout, e, s, head) + row * a.o_row;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) qf[c] = global_operand<T>(q, there, 16 * c + 8 * h, a.head_dim);
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) of[c] = global_operand<T>(dout, there, 16 * c + 8 * h, a.head_dim);
+        const int64_t at = (int64_t)head * a.rows + e.lse0 + row;
+        lse = there ? a.stat_lse[at] : INFINITY, delta = there ? a.stat_delta[at] : 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) dq[d] = zero16();
+        unit = a.scale * kLog2e;
+        if constexpr (MOD) bend.init(a.scale, a.cap);
+        bias = MOD && a.slopes, slope = bias ? a.slopes[head] * kLog2e : 0.f;
+        slopes_too = MOD && want_slopes;
+        far_ds = far_p = sum_ds = sum_p = 0.;
+    }
+    template <class Keys> __device__ __forceinline__ floatx16 product(const char *tile, int block, const Vec8 (&f)[DP / 16], int lane) const
+    {
+        floatx16 x = zero16();
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) x = Elem<T>::mma(Keys::row_operand(tile, block, c, lane), f[c], x);
+        return x;
+    }
+    // from the products with k and v of the 32 keys from `key` on to the gradients of their scores, in y
+    __device__ __forceinline__ void gradients(floatx16 &x, floatx16 &y, int key, bool masked)
+    {
+        floatx16 back;
+        const float away = (float)(pos - key - 4 * h);
+        scores<MOD>(x, back, bend, unit, bias, slope, away, -1.f);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r] - lse);
+        if (masked) {
+            const int at = key + 4 * h - lo;
+            const uint32_t span = hi > lo ? hi - lo : 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool seen = (uint32_t)(at + 8 * (r >> 2) + (r & 3)) < span;
+                x[r] = seen ? x[r] : 0.f;
+                y[r] = seen ? y[r] : 0.f;
+            }
+        }
+        if constexpr (MOD) {
+            if (slopes_too) {
+                float w0 = 0.f, w1 = 0.f, w2 = 0.f, w3 = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float far = fabsf(away - (float)(8 * (r >> 2) + (r & 3))), z = x[r] * y[r];
+                    w0 = fmaf(z, far, w0), w1 = fmaf(x[r], far, w1), w2 += z, w3 += x[r];
+                }
+                far_ds += w0, far_p += w1, sum_ds += w2, sum_p += w3;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            y[r] = x[r] * (y[r] - delta);
+            if constexpr (MOD) y[r] *= back[r];
+        }
+    }
+    template <class Keys> __device__ __forceinline__ void add(const char *kt, int block, const floatx16 &y, int lane)
+    {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const Vec8 ds = operand<T>(y, c);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) dq[d] = Elem<T>::mma(Keys::column_operand(kt, d, block / 16 + c, lane), ds, dq[d]);
+        }
+    }
+    // both halves of the wave hold parts of the rows' sums
+    __device__ __forceinline__ void join_halves()
+    {
+        far_ds += __shfl_xor(far_ds, 32), far_p += __shfl_xor(far_p, 32), sum_ds += __shfl_xor(sum_ds, 32), sum_p += __shfl_xor(sum_p, 32);
+    }
+    static __device__ __forceinline__ double of_slope(double far_ds, double far_p, double sum_ds, double sum_p)
+    {
+        double g = sum_p > 0. || sum_p != sum_p ? sum_ds * far_p / sum_p - far_ds : 0.;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) g += __shfl_xor(g, d);
+        return g;
+    }
+};
+
+template <class T>
+__device__ __forceinline__ void store_dq(const AttnArgs &a, T *to, int col, floatx4 y)
+{
+    typedef typename Elem<T>::Vec4 Vec4;
+    if (col < a.head_dim) *(Vec4 *)(to + col) = __builtin_convertvector(y * a.scale, Vec4);
+}
+
+template <class T, int DP, bool MOD>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : 2)
 void sddmm_attention_dq_kernel(const AttnArgs a)
 {
     constexpr int KT = sizeof(T) == 2 ? 64 : 32, DB = DP / 32;
     typedef Tile<T, DP, KT> Keys;
-    typedef typename Elem<T>::Vec8 Vec8;
     __shared__ __align__(1024) char lds[2][2][Keys::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
 
@@ -290,37 +407,24 @@ void sddmm_attention_dq_kernel(const AttnArgs a)
     if (!a.q_ptr) { s = b % a.n_seq; b /= a.n_seq; }
     const int head = kv * a.group + b % a.group;
     b /= a.group;
-    const int slot = a.n_slots - 1 - b;
-    double *slope_part = MOD && a.slope_part ? a.slope_part + (int64_t)head * a.slope_parts + (a.q_ptr ? slot : slot * a.n_seq + s) : nullptr;
+    double *slope_part = MOD && a.slope_part ? a.slope_part + (int64_t)head * a.slope_parts + (a.q_ptr ? b : (int64_t)b * a.n_seq + s) : nullptr;
     if (slope_part && threadIdx.x == 0) *slope_part = 0.;
-    if (a.q_ptr) s = slot_sequence(a.q_ptr, a.n_seq, kRows, slot, tile); else tile = slot;
+    if (a.q_ptr) {
+        s = slot_sequence<false>(a.q_ptr, a.n_seq, 1, kRows, a.max_tiles, a.n_slots, b, tile);
+        if (s < 0) return;
+    } else {
+        tile = a.n_slots - 1 - b;
+    }
     const Seq e = sequence(a, s);
     if (tile * kRows >= e.nq) return;
-    const int row = tile * kRows + wave * 32 + n, shift = e.nk - e.nq, prefix = a.prefix ? a.prefix[s] : 0, pos = row + shift;
-    const bool there = row < e.nq;
-    const int lo = first_key(a, pos), hi = there ? end_key(a, pos, prefix, e.nk) : 0;
+    const int row = tile * kRows + wave * 32 + n, shift = e.nk - e.nq, prefix = a.prefix ? a.prefix[s] : 0;
     const int r1 = min(e.nq, tile * kRows + kRows) - 1, w0 = tile * kRows + wave * 32, w1 = min(e.nq, w0 + 32) - 1;
     const int any_lo = first_key(a, tile * kRows + shift), any_hi = end_key(a, r1 + shift, prefix, e.nk);
     const int wave_lo = first_key(a, w0 + shift), wave_hi = w1 < w0 ? 0 : end_key(a, w1 + shift, prefix, e.nk);
     const int full_lo = first_key(a, w1 + shift), full_hi = w1 < w0 + 31 ? 0 : end_key(a, w0 + shift, prefix, e.nk);
-
-    Vec8 qf[DP / 16], of[DP / 16];
-    {
-        const T *q = q_base<T>(a, a.q, e, s, head) + row * a.q_row, *dout = o_base<T>(a, a.dout, e, s, head) + row * a.o_row;
-#pragma unroll
-        for (int c = 0; c < DP / 16; ++c) qf[c] = global_operand<T>(q, there, 16 * c + 8 * h, a.head_dim);
-#pragma unroll
-        for (int c = 0; c < DP / 16; ++c) of[c] = global_operand<T>(dout, there, 16 * c + 8 * h, a.head_dim);
-    }
-    const int64_t at_stat = (int64_t)head * a.rows + e.lse0 + row;
-    const float lse = there ? a.stat_lse[at_stat] : INFINITY, delta = there ? a.stat_delta[at_stat] : 0.f;
+    DqRows<T, DP, MOD> rows;
+    rows.init(a, e, s, head, row, prefix, slope_part != nullptr, lane);
     const T *k = k_base<T>(a, a.k, e, s, kv), *v = v_base<T>(a, a.v, e, s, kv);
-    floatx16 dq[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) dq[d] = zero16();
-    const float scale = a.scale, cap = a.cap, cap_inv = MOD && cap > 0.f ? scale / cap : 0.f;
-    const float slope = MOD && a.slopes ? a.slopes[head] * kLog2e : 0.f;
-    double far_ds = 0., far_p = 0., sum_ds = 0., sum_p = 0.;
 
     const int last = any_hi > any_lo ? (any_hi - any_lo + KT - 1) / KT : 0;
     const int row_bytes = a.head_dim * (int)sizeof(T);
@@ -342,70 +446,122 @@ void sddmm_attention_dq_kernel(const AttnArgs a)
             if (key + 32 <= wave_lo || key >= wave_hi) continue;
             int l = lane;  // (places in LDS made anew in every tile: kept, they would not fit the registers)
             asm volatile("" : "+v"(l));
-            floatx16 x = zero16(), y = zero16(), back;
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) x = Elem<T>::mma(Keys::row_operand(kt, 32 * u, c, l), qf[c], x);
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) y = Elem<T>::mma(Keys::row_operand(vt, 32 * u, c, l), of[c], y);
-            const float away = (float)(pos - key - 4 * h);
-            bend<MOD>(x, back, scale, cap, cap_inv, a.slopes != nullptr, slope, away, -1.f);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r] - lse);
-            if (key < full_lo || key + 32 > full_hi) {
-                const int at = key + 4 * h - lo;
-                const uint32_t span = hi > lo ? hi - lo : 0;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool seen = (uint32_t)(at + 8 * (r >> 2) + (r & 3)) < span;
-                    x[r] = seen ? x[r] : 0.f;
-                    y[r] = seen ? y[r] : 0.f;
-                }
-            }
-            if constexpr (MOD) {
-                if (slope_part) {
-                    float w0 = 0.f, w1 = 0.f, w2 = 0.f, w3 = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float far = fabsf(away - (float)(8 * (r >> 2) + (r & 3))), z = x[r] * y[r];
-                        w0 = fmaf(z, far, w0), w1 = fmaf(x[r], far, w1), w2 += z, w3 += x[r];
-                    }
-                    far_ds += w0, far_p += w1, sum_ds += w2, sum_p += w3;
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                y[r] = x[r] * (y[r] - delta);
-                if constexpr (MOD) y[r] *= back[r];
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const Vec8 ds = operand<T>(y, c);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) dq[d] = Elem<T>::mma(Keys::column_operand(kt, d, 2 * u + c, l), ds, dq[d]);
-            }
+            floatx16 x = rows.template product<Keys>(kt, 32 * u, rows.qf, l), y = rows.template product<Keys>(vt, 32 * u, rows.of, l);
+            rows.gradients(x, y, key, key < full_lo || key + 32 > full_hi);
+            rows.template add<Keys>(kt, 32 * u, y, l);
         }
     }
     if (MOD && slope_part) {
         __shared__ double parts[kWaves];
-        far_ds += __shfl_xor(far_ds, 32), far_p += __shfl_xor(far_p, 32), sum_ds += __shfl_xor(sum_ds, 32), sum_p += __shfl_xor(sum_p, 32);
-        double g = sum_p > 0. || sum_p != sum_p ? sum_ds * far_p / sum_p - far_ds : 0.;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) g += __shfl_xor(g, d);
+        rows.join_halves();
+        const double g = rows.of_slope(rows.far_ds, rows.far_p, rows.sum_ds, rows.sum_p);
         if (lane == 0) parts[wave] = g;
         __syncthreads();
         if (threadIdx.x == 0) *slope_part = parts[0] + parts[1] + parts[2] + parts[3];
     }
-    if (!there) return;
-    typedef typename Elem<T>::Vec4 Vec4;
+    if (!rows.there) return;
     T *to = (T *)q_base<T>(a, a.dq, e, s, head) + row * a.q_row;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int col = 32 * d + 8 * i + 4 * h;
-            if (col < a.head_dim)
-                *(Vec4 *)(to + col) = __builtin_convertvector((floatx4{dq[d][4 * i], dq[d][4 * i + 1], dq[d][4 * i + 2], dq[d][4 * i + 3]} * scale), Vec4);
+        for (int i = 0; i < 4; ++i)
+            store_dq(a, to, 32 * d + 8 * i + 4 * h, floatx4{rows.dq[d][4 * i], rows.dq[d][4 * i + 1], rows.dq[d][4 * i + 2], rows.dq[d][4 * i + 3]});
+}
+
+// dq where workgroups of 128 rows would leave compute units without work: 32 rows to a workgroup, each wave on every NW-th tile of keys, in LDS of its
+// own (keys twice, since they are needed to the end of a tile's work) and without a barrier; sums are joined at the end.
+constexpr int kFewRows = 32;
+template <class T, int DP, bool MOD, int NW>
+__global__ __launch_bounds__(64 * NW, 1)
+void sddmm_attention_dq_few_kernel(const AttnArgs a)
+{
+    constexpr int KT = 32, DB = DP / 32;
+    typedef Tile<T, DP, KT> Keys;
+    constexpr int kLoads = Keys::kBytes / 1024;
+    __shared__ __align__(1024) char lds[NW][3][Keys::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+    int b = blockIdx.x, s = 0, tile;
+    const int head = b % a.n_heads, kv = head / a.group;
+    b /= a.n_heads;
+    if (!a.q_ptr) { s = b % a.n_seq; b /= a.n_seq; }
+    double *slope_part = MOD && a.slope_part ? a.slope_part + (int64_t)head * a.slope_parts + (a.q_ptr ? b : (int64_t)b * a.n_seq + s) : nullptr;
+    if (slope_part && threadIdx.x == 0) *slope_part = 0.;
+    if (a.q_ptr) {
+        s = slot_sequence<false>(a.q_ptr, a.n_seq, 1, kFewRows, a.max_tiles, a.n_slots, b, tile);
+        if (s < 0) return;
+    } else {
+        tile = a.n_slots - 1 - b;
+    }
+    const Seq e = sequence(a, s);
+    if (tile * kFewRows >= e.nq) return;
+    const int row = tile * kFewRows + n, shift = e.nk - e.nq, prefix = a.prefix ? a.prefix[s] : 0;
+    const int w0 = tile * kFewRows, w1 = min(e.nq, w0 + kFewRows) - 1;
+    const int any_lo = first_key(a, w0 + shift), any_hi = end_key(a, w1 + shift, prefix, e.nk);
+    const int full_lo = first_key(a, w1 + shift), full_hi = w1 < w0 + 31 ? 0 : end_key(a, w0 + shift, prefix, e.nk);
+    DqRows<T, DP, MOD> rows;
+    rows.init(a, e, s, head, row, prefix, slope_part != nullptr, lane);
+    const T *k = k_base<T>(a, a.k, e, s, kv), *v = v_base<T>(a, a.v, e, s, kv);
+
+    const int last = any_hi > any_lo ? (any_hi - any_lo + KT - 1) / KT : 0;
+    const int row_bytes = a.head_dim * (int)sizeof(T);
+    const uint32_t k_stride = (uint32_t)(a.k_row * sizeof(T)), v_stride = (uint32_t)(a.v_row * sizeof(T));
+    // (behind the last tile nothing is read, but the requests are made, so that the waits count the same)
+    auto request = [&](char *to, const T *base, int64_t step, uint32_t stride, int t) {
+        const int key = any_lo + t * KT;
+        const bool more = t < last;
+        Keys::template request<1>(to, (const char *)(base + (more ? key : 0) * step), stride, more ? e.nk - key : 0, row_bytes, 0, lane);
+    };
+    char *vt = lds[wave][2];
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // the rows: from here on only tiles are under way
+    request(lds[wave][0], k, a.k_row, k_stride, wave);
+    request(vt, v, a.v_row, v_stride, wave);
+    for (int t = wave, turn = 0; t < last; t += NW, turn ^= 1) {
+        const int key = any_lo + t * KT;
+        const char *kt = lds[wave][turn];
+        request(lds[wave][turn ^ 1], k, a.k_row, k_stride, t + NW);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
+        floatx16 x = rows.template product<Keys>(kt, 0, rows.qf, lane);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+        floatx16 y = rows.template product<Keys>(vt, 0, rows.of, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x), "+v"(y) :: "memory");  // (all of the values have been read)
+        request(vt, v, a.v_row, v_stride, t + NW);
+        rows.gradients(x, y, key, key < full_lo || key + 32 > full_hi);
+        rows.template add<Keys>(kt, 0, y, lane);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(rows.dq[d]) :: "memory");
+    }
+    // join the waves: [element of the lane / 4][lane] of 16 bytes for each wave
+    static_assert(3 * Keys::kBytes >= 128 * DP);
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    floatx4 *mine = (floatx4 *)lds[wave][0];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine[(4 * d + i) * 64 + lane] = floatx4{rows.dq[d][4 * i], rows.dq[d][4 * i + 1], rows.dq[d][4 * i + 2], rows.dq[d][4 * i + 3]};
+    if (MOD && slope_part) {
+        __shared__ double sums[NW][32][4];
+        rows.join_halves();
+        if (h == 0) sums[wave][n][0] = rows.far_ds, sums[wave][n][1] = rows.far_p, sums[wave][n][2] = rows.sum_ds, sums[wave][n][3] = rows.sum_p;
+        __syncthreads();
+        if (wave == 0) {
+            double y[4] = {0., 0., 0., 0.};
+            for (int w = 0; w < NW; ++w)
+                for (int i = 0; i < 4; ++i) y[i] += sums[w][n][i];
+            const double g = rows.of_slope(y[0], y[1], y[2], y[3]);
+            if (lane == 0) *slope_part = g;
         }
+    }
+    __syncthreads();
+    if (!rows.there) return;
+    T *to = (T *)q_base<T>(a, a.dq, e, s, head) + row * a.q_row;
+#pragma unroll
+    for (int j = 0; j < 4 * DB / NW; ++j) {
+        const int piece = wave * (4 * DB / NW) + j;
+        floatx4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NW; ++i) y += ((const floatx4 *)lds[i][0])[piece * 64 + lane];
+        store_dq(a, to, 8 * piece + 4 * h, y);
+    }
 }
 
 // The slopes' gradients: a head's parts in a fixed order.
@@ -425,36 +581,38 @@ void sddmm_attention_dslopes_kernel(const AttnArgs a)
 }
 
 template <class T, int DP>
-hipError_t launch_typed(const AttnArgs &a, unsigned kv_grid, unsigned q_grid, int q_slots, hipStream_t st)
+hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, unsigned q_grid, bool few, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
-    constexpr int kPer = 256 / (DP / 8);
+    constexpr int kPer = 256 / (DP / 8), NW = sizeof(T) == 4 && DP == 128 ? 2 : 4;
+    const auto dkv = mod ? sddmm_attention_dkv_kernel<T, DP, true> : sddmm_attention_dkv_kernel<T, DP, false>;
+    const auto dq = mod ? sddmm_attention_dq_kernel<T, DP, true> : sddmm_attention_dq_kernel<T, DP, false>;
+    const auto dq_few = mod ? sddmm_attention_dq_few_kernel<T, DP, true, NW> : sddmm_attention_dq_few_kernel<T, DP, false, NW>;
     hipError_t e = hipSuccess;
     if (q_grid) e = launch(sddmm_attention_stats_kernel<T, DP>, dim3((unsigned)((a.rows * a.n_heads + kPer - 1) / kPer)), dim3(256), 0, st, a);
-    if (e == hipSuccess && kv_grid) e = launch(mod ? sddmm_attention_dkv_kernel<T, DP, true> : sddmm_attention_dkv_kernel<T, DP, false>, dim3(kv_grid), dim3(64 * kWaves), 0, st, a);
+    if (e == hipSuccess && kv_grid) e = launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a);
     if (e == hipSuccess && kv_grid && a.n_split > 1)
-        e = launch(sddmm_attention_dkv_sum_kernel<T>, dim3((unsigned)((a.key_rows * a.n_kv_heads * (a.head_dim / 4) + 255) / 256)), dim3(256), 0, st, a);
-    AttnArgs b = a;
-    b.n_slots = q_slots;
-    if (e == hipSuccess && q_grid) e = launch(mod ? sddmm_attention_dq_kernel<T, DP, true> : sddmm_attention_dq_kernel<T, DP, false>, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
-    if (e == hipSuccess && a.dslopes) e = launch(sddmm_attention_dslopes_kernel, dim3((unsigned)a.n_heads), dim3(256), 0, st, a);
+        e = launch(sddmm_attention_dkv_sum_kernel<T>, dim3(kv_grid / a.n_split * (kRows / kSumKeys)), dim3(256), 0, st, a);
+    if (e == hipSuccess && q_grid) e = few ? launch(dq_few, dim3(q_grid), dim3(64 * NW), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
+    if (e == hipSuccess && a.dslopes) e = launch(sddmm_attention_dslopes_kernel, dim3((unsigned)a.n_heads), dim3(256), 0, st, b);
     return e;
 }
 
 template <class T>
-hipError_t launch_dims(const AttnArgs &a, unsigned kv_grid, unsigned q_grid, int q_slots, hipStream_t st)
+hipError_t launch_dims(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, unsigned q_grid, bool few, hipStream_t st)
 {
-    return a.head_dim <= 64 ? launch_typed<T, 64>(a, kv_grid, q_grid, q_slots, st) : launch_typed<T, 128>(a, kv_grid, q_grid, q_slots, st);
+    return a.head_dim <= 64 ? launch_typed<T, 64>(a, b, kv_grid, q_grid, few, st) : launch_typed<T, 128>(a, b, kv_grid, q_grid, few, st);
 }
 
 }  // namespace
 
 int attention_backward_rows() { return kRows; }
+int attention_backward_few_rows() { return kFewRows; }
 
-hipError_t launch_attention_backward(const AttnArgs &a, int type, unsigned kv_grid, unsigned q_grid, int q_slots, hipStream_t st)
+hipError_t launch_attention_backward(const AttnArgs &a, const AttnArgs &b, int type, unsigned kv_grid, unsigned q_grid, bool few, hipStream_t st)
 {
-    return type == SDDMM_TYPE_F32 ? launch_dims<float>(a, kv_grid, q_grid, q_slots, st)
-         : type == SDDMM_TYPE_F16 ? launch_dims<_Float16>(a, kv_grid, q_grid, q_slots, st) : launch_dims<__bf16>(a, kv_grid, q_grid, q_slots, st);
+    return type == SDDMM_TYPE_F32 ? launch_dims<float>(a, b, kv_grid, q_grid, few, st)
+         : type == SDDMM_TYPE_F16 ? launch_dims<_Float16>(a, b, kv_grid, q_grid, few, st) : launch_dims<__bf16>(a, b, kv_grid, q_grid, few, st);
 }
 
 }  // namespace sddmm

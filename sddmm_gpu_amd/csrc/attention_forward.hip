@@ -42,8 +42,12 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
         b /= a.group;
     }
     if (a.n_split > 1) { split = b % a.n_split; b /= a.n_split; }
-    const int slot = a.n_slots - 1 - b;
-    if (ROWS != kRowsShared && a.q_ptr) s = slot_sequence(a.q_ptr, a.n_seq, kRows, slot, tile); else tile = slot;
+    if (ROWS != kRowsShared && a.q_ptr) {
+        s = slot_sequence<false>(a.q_ptr, a.n_seq, 1, kRows, a.max_tiles, a.n_slots, b, tile);
+        if (s < 0) return;
+    } else {
+        tile = a.n_slots - 1 - b;
+    }
 
     // this lane's row: its token and head, and the keys [lo, hi) that it sees; and what any / all rows of the workgroup and of the wave see
     const int row = tile * kRows + wave * 32 + n;
@@ -107,7 +111,9 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
     floatx16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
-    const float scale = a.scale, cap = a.cap, cap_inv = MOD && cap > 0.f ? scale / cap : 0.f;
+    const float scale = a.scale;
+    Bend bend;
+    if constexpr (MOD) bend.init(scale, a.cap);
     const float unit = MOD ? 1.f : scale * kLog2e;  // scores in registers to powers of two
     const float raise = 8.f / unit;
     const float slope = MOD && a.slopes && there ? a.slopes[my_head] * kLog2e : 0.f;
@@ -141,12 +147,8 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
             for (int i = 0; i < KB; ++i) x[i] = Elem<T>::mma(Keys::row_operand(kt, 32 * i, c, lane), qf[c], x[i]);
 
         if constexpr (MOD) {
-            if (cap > 0.f) {
-                const float to = cap * kLog2e;
-#pragma unroll
-                for (int i = 0; i < KB; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[i][r] = to * tanh_any(x[i][r] * cap_inv);
+            if (bend.cap > 0.f) {
+                bend.apply<KB, false>(x, x);
             } else {
 #pragma unroll
                 for (int i = 0; i < KB; ++i)

@@ -33,7 +33,13 @@ void sddmm_attention_token_kernel(const AttnArgs a)
     b /= a.n_kv_heads;
     const int split = b % a.n_split;
     b /= a.n_split;
-    const int s = b % a.n_seq, tile = b / a.n_seq;
+    int s, tile;
+    if (a.q_ptr && a.max_tiles > 1) {
+        s = slot_sequence<false>(a.q_ptr, a.n_seq, a.group, kTokenRows, a.max_tiles, a.n_slots, b, tile);
+        if (s < 0) return;
+    } else {
+        s = b % a.n_seq, tile = a.max_tiles - 1 - b / a.n_seq;
+    }
     const Seq e = sequence(a, s);
     const int n_rows = e.nq * a.group, n_keys = e.nk;
     if (tile * kTokenRows >= n_rows) return;
@@ -54,7 +60,9 @@ void sddmm_attention_token_kernel(const AttnArgs a)
     floatx16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
-    const float scale = a.scale, cap = a.cap, cap_inv = MOD && cap > 0.f ? scale / cap : 0.f;
+    const float scale = a.scale;
+    Bend bend;
+    if constexpr (MOD) bend.init(scale, a.cap);
     const float unit = MOD ? 1.f : scale * kLog2e;
     const float slope = MOD && a.slopes && there ? a.slopes[head] * kLog2e : 0.f;
     float m = -INFINITY, sum = 0.f;
@@ -85,10 +93,10 @@ void sddmm_attention_token_kernel(const AttnArgs a)
         request(kt, k, a.k_row, k_stride, t + NW);
 
         if constexpr (MOD) {
-            if (cap > 0.f) {
-                const float to = cap * kLog2e;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = to * tanh_any(x[r] * cap_inv);
+            if (bend.cap > 0.f) {
+                floatx16 y[1] = {x};
+                bend.apply<1, false>(y, y);
+                x = y[0];
             } else {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[r] *= scale * kLog2e;
@@ -176,49 +184,56 @@ void sddmm_attention_token_kernel(const AttnArgs a)
     }
 }
 
-// The partial results of a row: weights 2^(m - largest m), sums of both.  One workgroup a row: groups of head_dim / 4 lanes take
-// every so many parts, all requests under way together, and meet in LDS.
+// The partial results of a row: weights 2^(m - largest m), sums of both.  Groups of head_dim / 4 lanes take the parts of a row in turn,
+// as many groups to a row as it has parts (up to the workgroup's), with all requests under way together, and meet in LDS.
 constexpr int kJoinBlock = 256;
 template <class T, int DP>
 __global__ __launch_bounds__(kJoinBlock)
-void sddmm_attention_join_kernel(const AttnArgs a)
+void sddmm_attention_join_kernel(const AttnArgs a, const int per_row)
 {
     constexpr int kLanes = DP / 4, kGroups = kJoinBlock / kLanes;
     __shared__ floatx4 sums[kGroups][kLanes];
     __shared__ float totals[kGroups];
-    const int head = blockIdx.x % a.n_heads;
-    const int64_t row = blockIdx.x / a.n_heads;
-    int64_t to_row;
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, mine = group % per_row, col = lane * 4;
+    const int64_t all = a.rows * a.n_heads, at = (int64_t)blockIdx.x * (kGroups / per_row) + group / per_row;
+    const int head = (int)(at % a.n_heads);
+    const int64_t row = at / a.n_heads;
+    int64_t to_row = 0;
+    bool there = at < all;
     if (a.q_ptr) {
-        if (row < a.q_ptr[0] || row >= a.q_ptr[a.n_seq]) return;
+        there = there && row >= a.q_ptr[0] && row < a.q_ptr[a.n_seq];
         to_row = row * a.o_row;
-    } else {
+    } else if (there) {
         const int s = (int)(row / a.max_q), i = (int)(row % a.max_q);
-        if (a.q_len && i >= min(a.q_len[s], a.max_q)) return;
+        there = !a.q_len || i < min(a.q_len[s], a.max_q);
         to_row = s * a.o_seq + i * a.o_row;
     }
-    const int64_t at = row * a.n_heads + head, all = a.rows * a.n_heads;
-    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, col = lane * 4;
-    float top = -INFINITY;
-    for (int p = 0; p < a.n_part; ++p) top = fmaxf(top, a.part_ml[p * all + at].x);
+    float top = -INFINITY, total = 0.f;
     floatx4 y = {0.f, 0.f, 0.f, 0.f};
-    float total = 0.f;
+    if (there) {
+        for (int p = lane; p < a.n_part; p += kLanes) top = fmaxf(top, a.part_ml[p * all + at].x);
+#pragma unroll
+        for (int d = 1; d < kLanes; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
 #pragma unroll 4
-    for (int p = group; p < a.n_part; p += kGroups) {
-        const float2 ml = a.part_ml[p * all + at];
-        const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
-        const floatx4 x = col < a.head_dim && ml.x != -INFINITY ? *(const floatx4 *)(a.part_o + (p * all + at) * a.head_dim + col) : floatx4{0.f, 0.f, 0.f, 0.f};
-        y += x * w;
-        total = fmaf(w, ml.y, total);
+        for (int p = mine; p < a.n_part; p += per_row) {
+            const float2 ml = a.part_ml[p * all + at];
+            const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+            const floatx4 x = col < a.head_dim && ml.x != -INFINITY ? *(const floatx4 *)(a.part_o + (p * all + at) * a.head_dim + col) : floatx4{0.f, 0.f, 0.f, 0.f};
+            y += x * w;
+            total = fmaf(w, ml.y, total);
+        }
     }
-    sums[group][lane] = y;
-    if (lane == 0) totals[group] = total;
-    __syncthreads();
-    if (group) return;
-    for (int g = 1; g < kGroups; ++g) {
-        y += sums[g][lane];
-        total += totals[g];
+    if (per_row > 1) {
+        sums[group][lane] = y;
+        if (lane == 0) totals[group] = total;
+        __syncthreads();
+        if (mine) return;
+        for (int g = 1; g < per_row; ++g) {
+            y += sums[group + g][lane];
+            total += totals[group + g];
+        }
     }
+    if (!there) return;
     const float by = total > 0.f || total != total ? 1.f / total : 0.f;
     T *to = (T *)a.out + to_row + head * a.o_head;
     if (col < a.head_dim) *(typename Elem<T>::Vec4 *)(to + col) = __builtin_convertvector(y * by, typename Elem<T>::Vec4);
@@ -232,12 +247,19 @@ hipError_t launch_typed(const AttnArgs &a, bool mod, unsigned grid, hipStream_t 
     return launch(mod ? sddmm_attention_token_kernel<T, DP, true, NW> : sddmm_attention_token_kernel<T, DP, false, NW>, dim3(grid), dim3(64 * NW), 0, st, a);
 }
 
-template <class T>
+template <class T, int DP>
 hipError_t join_typed(const AttnArgs &a, hipStream_t st)
 {
-    const dim3 grid((unsigned)(a.rows * a.n_heads));
-    return a.head_dim <= 64 ? launch(sddmm_attention_join_kernel<T, 64>, grid, dim3(kJoinBlock), 0, st, a)
-                            : launch(sddmm_attention_join_kernel<T, 128>, grid, dim3(kJoinBlock), 0, st, a);
+    constexpr int kGroups = kJoinBlock / (DP / 4);
+    int per_row = 1;
+    while (per_row < kGroups && per_row < a.n_part) per_row *= 2;
+    const int64_t rows = kGroups / per_row, grid = (a.rows * a.n_heads + rows - 1) / rows;
+    return launch(sddmm_attention_join_kernel<T, DP>, dim3((unsigned)grid), dim3(kJoinBlock), 0, st, a, per_row);
+}
+template <class T>
+hipError_t join_dims(const AttnArgs &a, hipStream_t st)
+{
+    return a.head_dim <= 64 ? join_typed<T, 64>(a, st) : join_typed<T, 128>(a, st);
 }
 
 }  // namespace
@@ -256,7 +278,7 @@ hipError_t launch_attention_token(const AttnArgs &a, int type, unsigned grid, hi
 
 hipError_t launch_attention_join(const AttnArgs &a, int type, hipStream_t st)
 {
-    return type == SDDMM_TYPE_F32 ? join_typed<float>(a, st) : type == SDDMM_TYPE_F16 ? join_typed<_Float16>(a, st) : join_typed<__bf16>(a, st);
+    return type == SDDMM_TYPE_F32 ? join_dims<float>(a, st) : type == SDDMM_TYPE_F16 ? join_dims<_Float16>(a, st) : join_dims<__bf16>(a, st);
 }
 
 }  // namespace sddmm
