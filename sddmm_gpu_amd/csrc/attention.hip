@@ -51,7 +51,7 @@ int check_desc(const char *who, const sddmm_attention_desc *p)
 struct Deal {
     int64_t rows = 0;          // of all sequences
     bool token = false;        // the kernel for few rows
-    int mapping = kRowsOfHead;
+    int mapping = kRowsOfHead, tile = 128;
     int64_t slots = 0, max_tiles = 0, grid = 0, splits = 1;
     int64_t shared_slots = 0, shared_grid = 0, shared_splits = 0;
     int64_t parts = 1, part_bytes = 0, bytes = 0;
@@ -68,18 +68,24 @@ int64_t pieces(int64_t workgroups, int64_t keys, int64_t least)
 Deal deal(const sddmm_attention_desc &d)
 {
     Deal r;
-    const int64_t group = d.n_heads / d.n_kv_heads, tile = attention_forward_rows(), few = attention_token_rows();
+    const int64_t group = d.n_heads / d.n_kv_heads, tile = 128, few = attention_token_rows();
     r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
     // keys that a tile's rows can see
     const int64_t span = d.window_left >= 0 && d.window_right >= 0 && !d.prefix ? (int64_t)d.window_left + d.window_right + std::min<int64_t>(d.max_q, tile) : d.max_k;
     const int64_t keys = std::min<int64_t>(d.max_k, span), seqs = d.q_ptr ? 1 : d.n_seq, packed = d.max_q * group;
-    // tiles of 128 rows, of one head or of pairs of few tokens and the heads that share a key head (not in packed sequences)
-    r.mapping = group > 1 && d.max_q < tile && !d.q_ptr ? kRowsPacked : kRowsOfHead;
-    r.max_tiles = div_up(r.mapping == kRowsPacked ? packed : d.max_q, tile);
-    r.slots = d.q_ptr ? r.rows / tile + d.n_seq : r.max_tiles;
-    r.grid = r.slots * seqs * d.n_kv_heads * (r.mapping == kRowsPacked ? 1 : group);
-    // or tiles of 32 pairs, each wave on keys of its own, where pairs are few or the others would leave compute units without work
-    r.token = packed <= few || r.grid < kFill / 2;
+    // Tiles of 128 rows where that makes 1024 workgroups, else of 64 (us of the forward pass, causal, with 128, 64 and 32: 4096 tokens, 16 heads of 128,
+    // bf16 98 / 93 / 114; 16 sequences of 512 44 / 57 / 88; 2048 tokens, 16 heads of 64 34 / 26 / 21, fp32 155 / 108 / 88; 2048, 4 of 128 43 / 30 / 23),
+    // of one head or of pairs of few tokens and the heads that share a key head (not in packed sequences);
+    for (int64_t tile : {128, 64}) {
+        r.tile = (int)tile;
+        r.mapping = group > 1 && d.max_q < tile && !d.q_ptr ? kRowsPacked : kRowsOfHead;
+        r.max_tiles = div_up(r.mapping == kRowsPacked ? packed : d.max_q, tile);
+        r.slots = d.q_ptr ? r.rows / tile + d.n_seq : r.max_tiles;
+        r.grid = r.slots * seqs * d.n_kv_heads * (r.mapping == kRowsPacked ? 1 : group);
+        if (r.grid >= 2 * kFill) break;
+    }
+    // or tiles of 32 pairs, each wave on keys of its own, where pairs are few or there would be less than 768 of 64 rows
+    r.token = packed <= few || r.grid < kFill * 3 / 2;
     if (r.token) {
         r.max_tiles = div_up(packed, few);
         r.slots = r.max_tiles == 1 ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
@@ -104,24 +110,26 @@ Deal deal(const sddmm_attention_desc &d)
 // The same for the backward pass.
 struct DealBack {
     int64_t rows = 0, key_rows = 0, q_slots = 0, q_tiles = 0, kv_slots = 0, kv_tiles = 0, q_grid = 0, kv_grid = 0, splits = 1, chunk = 1, slope_parts = 0;
-    bool few = false;
+    int q_rows = 128;  // of a dq workgroup
     int64_t lse_at = 0, delta_at = 0, parts_at = 0, slopes_at = 0, bytes = 0;  // places in the workspace
 };
 
 DealBack deal_back(const sddmm_attention_desc &d)
 {
     DealBack r;
-    const int64_t tile = attention_backward_rows(), group = d.n_heads / d.n_kv_heads;
+    const int64_t tile = attention_backward_keys(), group = d.n_heads / d.n_kv_heads;
     r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
     r.key_rows = d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k;
     if (r.rows > 0) {
-        for (int64_t rows : {tile, (int64_t)attention_backward_few_rows()}) {
-            r.few = rows != tile;
+        // (dq: us of the backward pass with 128, 64 and 32 rows: 4096 tokens, 16 heads of 128 358 / 343 / 411; 16 sequences of 512 163 / 174 / 175;
+        // 2048 tokens, 4 heads 107 / 83 / 72)
+        for (int64_t rows : {128, 64, 32}) {
+            r.q_rows = (int)rows;
             r.q_tiles = div_up(d.max_q, rows);
             r.q_slots = d.q_ptr ? r.rows / rows + d.n_seq : r.q_tiles;
             r.slope_parts = r.q_slots * (d.q_ptr ? 1 : d.n_seq);
             r.q_grid = r.slope_parts * d.n_heads;
-            if (r.q_grid >= kFill / 2) break;
+            if (r.q_grid >= (rows == 128 ? 2 * kFill : kFill)) break;
         }
     }
     if (r.key_rows > 0) {
@@ -148,7 +156,7 @@ DealBack deal_back(const sddmm_attention_desc &d)
     }
     r.delta_at = padded(r.rows * d.n_heads * 4);
     r.parts_at = 2 * r.delta_at;
-    r.slopes_at = r.parts_at + (r.splits > 1 ? padded(2 * r.splits * r.key_rows * d.n_kv_heads * d.head_dim * 4) : 0);
+    r.slopes_at = r.parts_at + (r.splits > 1 ? r.kv_grid * tile * (d.head_dim <= 64 ? 64 : 128) * 8 : 0);
     r.bytes = r.slopes_at + (d.slopes ? padded(r.slope_parts * d.n_heads * 8) : 0);
     return r;
 }
@@ -197,9 +205,9 @@ int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d
     if (d.shared_len > 0) {
         AttnArgs b = a;
         b.n_slots = (int)r.shared_slots, b.n_split = (int)r.shared_splits, b.part0 = (int)r.splits;
-        e = launch_attention_forward(b, d.type, kRowsShared, (unsigned)r.shared_grid, st);
+        e = launch_attention_forward(b, d.type, kRowsShared, 128, (unsigned)r.shared_grid, st);
     }
-    if (e == hipSuccess) e = r.token ? launch_attention_token(a, d.type, (unsigned)r.grid, st) : launch_attention_forward(a, d.type, r.mapping, (unsigned)r.grid, st);
+    if (e == hipSuccess) e = r.token ? launch_attention_token(a, d.type, (unsigned)r.grid, st) : launch_attention_forward(a, d.type, r.mapping, r.tile, (unsigned)r.grid, st);
     if (e == hipSuccess && r.parts > 1) e = launch_attention_join(a, d.type, st);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;
@@ -259,7 +267,7 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
     if (!aligned({d_q, d_k, d_v, d_out, d_dout, d_dq, d_dk, d_dv})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (r.q_grid > INT32_MAX || r.kv_grid > INT32_MAX || r.rows * d.n_heads / 16 > INT32_MAX || r.key_rows * d.n_kv_heads > INT32_MAX)
+    if (r.q_grid > INT32_MAX || r.kv_grid > INT32_MAX / 4 || r.rows * d.n_heads / 16 > INT32_MAX || r.key_rows * d.n_kv_heads > INT32_MAX)
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
 
     AttnArgs a = arguments(d);
@@ -270,7 +278,7 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
     AttnArgs b = a;
     a.n_slots = (int)r.kv_slots, a.max_tiles = (int)r.kv_tiles, a.n_split = (int)r.splits, a.chunk = (int)std::min<int64_t>(r.chunk, INT32_MAX);
     b.n_slots = (int)r.q_slots, b.max_tiles = (int)r.q_tiles, b.n_split = 1;
-    const hipError_t e = launch_attention_backward(a, b, d.type, (unsigned)r.kv_grid, (unsigned)r.q_grid, r.few, (hipStream_t)stream);
+    const hipError_t e = launch_attention_backward(a, b, d.type, (unsigned)r.kv_grid, (unsigned)r.q_grid, r.q_rows, (hipStream_t)stream);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;
 }

@@ -14,7 +14,7 @@ namespace sddmm {
 
 namespace {
 
-constexpr int kRows = 128, kWaves = 4;  // rows (or keys) of a workgroup, 32 to a wave
+constexpr int kKeys = 128, kWaves = 4;  // keys of a workgroup of the dk, dv kernel, 32 to a wave
 
 // stats[head][row] = (lse in powers of two, dout . out).  A row that saw nothing gets +infinity, so that 2^(s - lse) is 0.
 template <class T, int DP>
@@ -95,16 +95,16 @@ __device__ __forceinline__ bool key_tile(const AttnArgs &a, int b, KeyTile &k)
     k.kv = b % a.n_kv_heads;
     b /= a.n_kv_heads;
     if (a.k_ptr) {
-        k.s = slot_sequence<true>(a.k_ptr, a.n_seq, 1, kRows, a.max_tiles, a.n_slots, b, k.tile);
+        k.s = slot_sequence<true>(a.k_ptr, a.n_seq, 1, kKeys, a.max_tiles, a.n_slots, b, k.tile);
         if (k.s < 0) return false;
     } else {
         k.s = b % a.n_seq, k.tile = b / a.n_seq;
     }
     k.e = sequence(a, k.s);
-    if (k.tile * kRows >= k.e.nk) return false;
+    if (k.tile * kKeys >= k.e.nk) return false;
     k.shift = k.e.nk - k.e.nq, k.prefix = a.prefix ? a.prefix[k.s] : 0;
-    k.any_lo = first_row(a, k.tile * kRows, k.prefix, k.shift);
-    k.any_hi = end_row(a, min(k.e.nk, k.tile * kRows + kRows) - 1, k.shift, k.e.nq);
+    k.any_lo = first_row(a, k.tile * kKeys, k.prefix, k.shift);
+    k.any_hi = end_row(a, min(k.e.nk, k.tile * kKeys + kKeys) - 1, k.shift, k.e.nq);
     const int64_t rows = (int64_t)max(0, k.any_hi - k.any_lo) * a.group;
     k.pieces = (int)max((int64_t)1, min((int64_t)a.n_split, (rows + a.chunk - 1) / a.chunk));
     return true;
@@ -120,7 +120,7 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
 {
     constexpr int QT = 32, DB = DP / 32;
     typedef Tile<T, DP, QT> Rows;
-    typedef Tile<T, DP, kRows> Values;
+    typedef Tile<T, DP, kKeys> Values;
     typedef typename Elem<T>::Vec8 Vec8;
     // (registers: 128 for the sums, 32 for k, 32 for a tile's scores; v would be 32 more than two waves to a SIMD leave)
     constexpr bool kKeepV = sizeof(T) == 4 || DP == 64;
@@ -134,10 +134,10 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
     const int groups = gridDim.x / a.n_split, split = blockIdx.x / groups;
     if (!key_tile(a, blockIdx.x - split * groups, at_keys) || split >= at_keys.pieces) return;
     const auto [e, s, kv, tile, shift, prefix, any_lo, any_hi, pieces] = at_keys;
-    const int key = tile * kRows + wave * 32 + n;
+    const int key = tile * kKeys + wave * 32 + n;
     const bool there = key < e.nk;
     const int lo = first_row(a, key, prefix, shift), hi = there ? end_row(a, key, shift, e.nq) : 0;
-    const int k0 = tile * kRows, w0 = k0 + wave * 32, w1 = min(e.nk, w0 + 32) - 1;
+    const int k0 = tile * kKeys, w0 = k0 + wave * 32, w1 = min(e.nk, w0 + 32) - 1;
     const int wave_lo = first_row(a, w0, prefix, shift), wave_hi = w1 < w0 ? 0 : end_row(a, w1, shift, e.nq);
     const int full_lo = first_row(a, max(w1, 0), prefix, shift), full_hi = w1 < w0 + 31 ? 0 : end_row(a, w0, shift, e.nq);
 
@@ -226,24 +226,21 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
             }
         }
     }
-    if (!there) return;
 #pragma unroll
     for (int d = 0; d < DB; ++d) dk[d] *= scale;
     if (pieces > 1) {
-        // parts of dk, then of dv: [part][key][key head][head_dim]
-        const int64_t place = ((e.k0 + (a.k_ptr ? 0 : (int64_t)s * a.max_k) + key) * a.n_kv_heads + kv) * a.head_dim, part = a.key_rows * a.n_kv_heads * a.head_dim;
-        float *to = a.part_o + split * part + place, *to_v = to + a.n_split * part;
+        // parts of dk and dv as they lie in the registers: [part][workgroup][wave][element of the lane / 4][lane] of 16 bytes
+        floatx4 *to = (floatx4 *)a.part_o + ((int64_t)blockIdx.x * kWaves + wave) * (8 * DB * 64) + lane;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int col = 32 * d + 8 * i + 4 * h;
-                if (col >= a.head_dim) continue;
-                *(floatx4 *)(to + col) = floatx4{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
-                *(floatx4 *)(to_v + col) = floatx4{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
+                to[(4 * d + i) * 64] = floatx4{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
+                to[(4 * (DB + d) + i) * 64] = floatx4{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
             }
         return;
     }
+    if (!there) return;
     typedef typename Elem<T>::Vec4 Vec4;
     T *to = (T *)k_base<T>(a, a.dk, e, s, kv) + key * a.k_row, *to_v = (T *)v_base<T>(a, a.dv, e, s, kv) + key * a.v_row;
 #pragma unroll
@@ -257,28 +254,27 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
         }
 }
 
-// The sum of the parts of dk and dv of the keys whose rows were cut, 16 keys to a workgroup.
-constexpr int kSumKeys = 16;
-template <class T>
+// The sum of the parts of dk and dv of the keys whose rows were cut: a workgroup for the keys of a wave.
+template <class T, int DP>
 __global__ __launch_bounds__(256)
 void sddmm_attention_dkv_sum_kernel(const AttnArgs a)
 {
+    constexpr int DB = DP / 32;
     KeyTile at;
-    if (!key_tile(a, blockIdx.x / (kRows / kSumKeys), at) || at.pieces == 1) return;
-    const int per = a.head_dim / 4, k0 = at.tile * kRows + blockIdx.x % (kRows / kSumKeys) * kSumKeys, n = min(kSumKeys, at.e.nk - k0) * per;
-    const int64_t part = a.key_rows * a.n_kv_heads * a.head_dim, first = at.e.k0 + (a.k_ptr ? 0 : (int64_t)at.s * a.max_k);
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int key = k0 + i / per, col = i % per * 4;
-        const float *from = a.part_o + ((first + key) * a.n_kv_heads + at.kv) * a.head_dim + col, *from_v = from + a.n_split * part;
-        floatx4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+    if (!key_tile(a, blockIdx.x / kWaves, at) || at.pieces == 1) return;
+    const int wave = blockIdx.x % kWaves, lane = threadIdx.x & 63, key = at.tile * kKeys + wave * 32 + (lane & 31);
+    if (key >= at.e.nk) return;
+    const int64_t part = (int64_t)gridDim.x * (8 * DB * 64);
+    T *to = (T *)k_base<T>(a, a.dk, at.e, at.s, at.kv) + key * a.k_row, *to_v = (T *)v_base<T>(a, a.dv, at.e, at.s, at.kv) + key * a.v_row;
+#pragma unroll
+    for (int j = 0; j < 2 * DB; ++j) {
+        const int i = j * 4 + (threadIdx.x >> 6), col = 8 * (i % (4 * DB)) + 4 * (lane >> 5);
+        const floatx4 *from = (const floatx4 *)a.part_o + ((int64_t)blockIdx.x * (8 * DB) + i) * 64 + lane;
+        floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int p = 0; p < at.pieces; ++p) {
-            x += *(const floatx4 *)(from + p * part);
-            y += *(const floatx4 *)(from_v + p * part);
-        }
+        for (int p = 0; p < at.pieces; ++p) x += from[p * part];
         typedef typename Elem<T>::Vec4 Vec4;
-        *(Vec4 *)((T *)k_base<T>(a, a.dk, at.e, at.s, at.kv) + key * a.k_row + col) = __builtin_convertvector(x, Vec4);
-        *(Vec4 *)((T *)v_base<T>(a, a.dv, at.e, at.s, at.kv) + key * a.v_row + col) = __builtin_convertvector(y, Vec4);
+        if (col < a.head_dim) *(Vec4 *)((i < 4 * DB ? to : to_v) + col) = __builtin_convertvector(x, Vec4);
     }
 }
 
@@ -374,6 +370,7 @@ struct DqRows {
     // both halves of the wave hold parts of the rows' sums
     __device__ __forceinline__ void join_halves()
     {
+        if constexpr (!MOD) return;
         far_ds += __shfl_xor(far_ds, 32), far_p += __shfl_xor(far_p, 32), sum_ds += __shfl_xor(sum_ds, 32), sum_p += __shfl_xor(sum_p, 32);
     }
     static __device__ __forceinline__ double of_slope(double far_ds, double far_p, double sum_ds, double sum_p)
@@ -392,14 +389,16 @@ __device__ __forceinline__ void store_dq(const AttnArgs &a, T *to, int col, floa
     if (col < a.head_dim) *(Vec4 *)(to + col) = __builtin_convertvector(y * a.scale, Vec4);
 }
 
-template <class T, int DP, bool MOD>
+// RW: as in the forward kernel.
+template <class T, int DP, bool MOD, int RW>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : 2)
 void sddmm_attention_dq_kernel(const AttnArgs a)
 {
-    constexpr int KT = sizeof(T) == 2 ? 64 : 32, DB = DP / 32;
+    constexpr int KT = sizeof(T) == 2 || RW == 2 ? 64 : 32, KB = KT / 32 / (kWaves / RW), DB = DP / 32, kRows = 32 * RW;
     typedef Tile<T, DP, KT> Keys;
     __shared__ __align__(1024) char lds[2][2][Keys::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+    const int row_wave = wave % RW, half = wave / RW;
 
     int b = blockIdx.x, s = 0, tile;  // (as in the forward kernel)
     const int kv = b % a.n_kv_heads;
@@ -417,8 +416,8 @@ void sddmm_attention_dq_kernel(const AttnArgs a)
     }
     const Seq e = sequence(a, s);
     if (tile * kRows >= e.nq) return;
-    const int row = tile * kRows + wave * 32 + n, shift = e.nk - e.nq, prefix = a.prefix ? a.prefix[s] : 0;
-    const int r1 = min(e.nq, tile * kRows + kRows) - 1, w0 = tile * kRows + wave * 32, w1 = min(e.nq, w0 + 32) - 1;
+    const int row = tile * kRows + row_wave * 32 + n, shift = e.nk - e.nq, prefix = a.prefix ? a.prefix[s] : 0;
+    const int r1 = min(e.nq, tile * kRows + kRows) - 1, w0 = tile * kRows + row_wave * 32, w1 = min(e.nq, w0 + 32) - 1;
     const int any_lo = first_key(a, tile * kRows + shift), any_hi = end_key(a, r1 + shift, prefix, e.nk);
     const int wave_lo = first_key(a, w0 + shift), wave_hi = w1 < w0 ? 0 : end_key(a, w1 + shift, prefix, e.nk);
     const int full_lo = first_key(a, w1 + shift), full_hi = w1 < w0 + 31 ? 0 : end_key(a, w0 + shift, prefix, e.nk);
@@ -441,7 +440,7 @@ void sddmm_attention_dq_kernel(const AttnArgs a)
         if (t + 1 < last) request(t + 1);
         const char *kt = lds[t & 1][0], *vt = lds[t & 1][1];
 #pragma unroll 1
-        for (int u = 0; u < KT / 32; ++u) {
+        for (int u = half * KB; u < half * KB + KB; ++u) {
             const int key = any_lo + t * KT + 32 * u;
             if (key + 32 <= wave_lo || key >= wave_hi) continue;
             int l = lane;  // (places in LDS made anew in every tile: kept, they would not fit the registers)
@@ -451,15 +450,42 @@ void sddmm_attention_dq_kernel(const AttnArgs a)
             rows.template add<Keys>(kt, 32 * u, y, l);
         }
     }
+    if constexpr (RW < kWaves) {  // the halves of the keys
+        static_assert(RW * 128 * DP + RW * 1024 <= (int)sizeof lds);
+        __syncthreads();
+        floatx4 *other = (floatx4 *)((char *)lds + row_wave * 128 * DP);
+        double *other_sums = (double *)((char *)lds + RW * 128 * DP) + row_wave * 128 + n * 4;
+        rows.join_halves();
+        if (half) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) other[(4 * d + i) * 64 + lane] = floatx4{rows.dq[d][4 * i], rows.dq[d][4 * i + 1], rows.dq[d][4 * i + 2], rows.dq[d][4 * i + 3]};
+            if (MOD && h == 0) other_sums[0] = rows.far_ds, other_sums[1] = rows.far_p, other_sums[2] = rows.sum_ds, other_sums[3] = rows.sum_p;
+        }
+        __syncthreads();
+        if (!half) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const floatx4 y = other[(4 * d + i) * 64 + lane];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) rows.dq[d][4 * i + j] += y[j];
+                }
+            if constexpr (MOD) rows.far_ds += other_sums[0], rows.far_p += other_sums[1], rows.sum_ds += other_sums[2], rows.sum_p += other_sums[3];
+        }
+    } else {
+        rows.join_halves();
+    }
     if (MOD && slope_part) {
         __shared__ double parts[kWaves];
-        rows.join_halves();
-        const double g = rows.of_slope(rows.far_ds, rows.far_p, rows.sum_ds, rows.sum_p);
+        const double g = half ? 0. : rows.of_slope(rows.far_ds, rows.far_p, rows.sum_ds, rows.sum_p);
         if (lane == 0) parts[wave] = g;
         __syncthreads();
         if (threadIdx.x == 0) *slope_part = parts[0] + parts[1] + parts[2] + parts[3];
     }
-    if (!rows.there) return;
+    if (half || !rows.there) return;
     T *to = (T *)q_base<T>(a, a.dq, e, s, head) + row * a.q_row;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -581,38 +607,38 @@ void sddmm_attention_dslopes_kernel(const AttnArgs a)
 }
 
 template <class T, int DP>
-hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, unsigned q_grid, bool few, hipStream_t st)
+hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, unsigned q_grid, int q_rows, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
     constexpr int kPer = 256 / (DP / 8), NW = sizeof(T) == 4 && DP == 128 ? 2 : 4;
     const auto dkv = mod ? sddmm_attention_dkv_kernel<T, DP, true> : sddmm_attention_dkv_kernel<T, DP, false>;
-    const auto dq = mod ? sddmm_attention_dq_kernel<T, DP, true> : sddmm_attention_dq_kernel<T, DP, false>;
+    const auto dq = q_rows == 64 ? (mod ? sddmm_attention_dq_kernel<T, DP, true, 2> : sddmm_attention_dq_kernel<T, DP, false, 2>)
+                                 : (mod ? sddmm_attention_dq_kernel<T, DP, true, 4> : sddmm_attention_dq_kernel<T, DP, false, 4>);
     const auto dq_few = mod ? sddmm_attention_dq_few_kernel<T, DP, true, NW> : sddmm_attention_dq_few_kernel<T, DP, false, NW>;
     hipError_t e = hipSuccess;
     if (q_grid) e = launch(sddmm_attention_stats_kernel<T, DP>, dim3((unsigned)((a.rows * a.n_heads + kPer - 1) / kPer)), dim3(256), 0, st, a);
     if (e == hipSuccess && kv_grid) e = launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a);
     if (e == hipSuccess && kv_grid && a.n_split > 1)
-        e = launch(sddmm_attention_dkv_sum_kernel<T>, dim3(kv_grid / a.n_split * (kRows / kSumKeys)), dim3(256), 0, st, a);
-    if (e == hipSuccess && q_grid) e = few ? launch(dq_few, dim3(q_grid), dim3(64 * NW), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
+        e = launch(sddmm_attention_dkv_sum_kernel<T, DP>, dim3(kv_grid / a.n_split * kWaves), dim3(256), 0, st, a);
+    if (e == hipSuccess && q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * NW), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
     if (e == hipSuccess && a.dslopes) e = launch(sddmm_attention_dslopes_kernel, dim3((unsigned)a.n_heads), dim3(256), 0, st, b);
     return e;
 }
 
 template <class T>
-hipError_t launch_dims(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, unsigned q_grid, bool few, hipStream_t st)
+hipError_t launch_dims(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, unsigned q_grid, int q_rows, hipStream_t st)
 {
-    return a.head_dim <= 64 ? launch_typed<T, 64>(a, b, kv_grid, q_grid, few, st) : launch_typed<T, 128>(a, b, kv_grid, q_grid, few, st);
+    return a.head_dim <= 64 ? launch_typed<T, 64>(a, b, kv_grid, q_grid, q_rows, st) : launch_typed<T, 128>(a, b, kv_grid, q_grid, q_rows, st);
 }
 
 }  // namespace
 
-int attention_backward_rows() { return kRows; }
-int attention_backward_few_rows() { return kFewRows; }
+int attention_backward_keys() { return kKeys; }
 
-hipError_t launch_attention_backward(const AttnArgs &a, const AttnArgs &b, int type, unsigned kv_grid, unsigned q_grid, bool few, hipStream_t st)
+hipError_t launch_attention_backward(const AttnArgs &a, const AttnArgs &b, int type, unsigned kv_grid, unsigned q_grid, int q_rows, hipStream_t st)
 {
-    return type == SDDMM_TYPE_F32 ? launch_dims<float>(a, b, kv_grid, q_grid, few, st)
-         : type == SDDMM_TYPE_F16 ? launch_dims<_Float16>(a, b, kv_grid, q_grid, few, st) : launch_dims<__bf16>(a, b, kv_grid, q_grid, few, st);
+    return type == SDDMM_TYPE_F32 ? launch_dims<float>(a, b, kv_grid, q_grid, q_rows, st)
+         : type == SDDMM_TYPE_F16 ? launch_dims<_Float16>(a, b, kv_grid, q_grid, q_rows, st) : launch_dims<__bf16>(a, b, kv_grid, q_grid, q_rows, st);
 }
 
 }  // namespace sddmm

@@ -7,7 +7,7 @@ namespace sddmm {
 
 namespace {
 
-constexpr int kRows = 128, kWaves = 4;  // rows of a workgroup, 32 to a wave
+constexpr int kWaves = 4;  // of a workgroup, 32 rows to each
 
 // o_i = sum_j p_ij v_j / sum_j p_ij with p_ij = exp(s_ij - m_i), in one pass over the keys with a running maximum m_i.  A wave
 // holds 32 rows: their q as operands, the sums of o turned (element of the head by row).  Per tile of keys, which the four
@@ -19,15 +19,19 @@ constexpr int kRows = 128, kWaves = 4;  // rows of a workgroup, 32 to a wave
 // What the rows of a workgroup are: the rows of one query head (kRowsOfHead); the (token, head) pairs of the query heads that share
 // a key head, for few tokens (kRowsPacked); the same pairs of all sequences, against the keys that all of them begin with
 // (kRowsShared: each sequence's rows have positions, and so masks, of their own).
-template <class T, int DP, bool MOD, int ROWS>
+//
+// RW: waves on rows of their own.  With 2 the others take the second half of every tile of keys for the same 64 rows, and the halves
+// are joined at the end: twice the workgroups, where those of 128 rows are so few that the longest keeps the others waiting.
+template <class T, int DP, bool MOD, int ROWS, int RW>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : 2)
 void sddmm_attention_forward_kernel(const AttnArgs a)
 {
-    constexpr int KT = sizeof(T) == 2 ? 64 : 32, KB = KT / 32, DB = DP / 32;
+    constexpr int KT = sizeof(T) == 2 || RW == 2 ? 64 : 32, KB = KT / 32 / (kWaves / RW), DB = DP / 32, kRows = 32 * RW;
     typedef Tile<T, DP, KT> Keys;
     typedef typename Elem<T>::Vec8 Vec8;
     __shared__ __align__(1024) char lds[2][2][Keys::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+    const int row_wave = wave % RW, half = wave / RW;
 
     // Workgroups that read the same keys lie n_kv_heads (and n_seq) apart: with a multiple of 8 they are on one die, whose L2 then
     // holds them.  Tiles of rows in descending order, since under a causal mask the last rows see most keys.
@@ -50,7 +54,7 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
     }
 
     // this lane's row: its token and head, and the keys [lo, hi) that it sees; and what any / all rows of the workgroup and of the wave see
-    const int row = tile * kRows + wave * 32 + n;
+    const int row = tile * kRows + row_wave * 32 + n;
     Seq e;
     int n_keys, token, my_head = head, pos, lo, hi, any_lo, any_hi, wave_lo, wave_hi, full_lo, full_hi;
     bool there;
@@ -79,6 +83,7 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
         full_lo = __builtin_amdgcn_readfirstlane(full_lo), full_hi = __builtin_amdgcn_readfirstlane(full_hi);
         if (lane == 0) ends[wave][0] = wave_lo, ends[wave][1] = wave_hi;
         __syncthreads();
+        static_assert(ROWS != kRowsShared || RW == kWaves);
         any_lo = min(min(ends[0][0], ends[1][0]), min(ends[2][0], ends[3][0]));
         any_hi = max(max(ends[0][1], ends[1][1]), max(ends[2][1], ends[3][1]));
         any_lo = __builtin_amdgcn_readfirstlane(any_lo), any_hi = __builtin_amdgcn_readfirstlane(any_hi);
@@ -94,7 +99,7 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
         const int shift = e.nk - e.nq, prefix = a.prefix ? max(0, a.prefix[s] - a.shared_len) : 0;
         pos = token + shift;
         lo = first_key(a, pos), hi = end_key(a, pos, prefix, n_keys);
-        const int last = min(n_rows, tile * kRows + kRows) - 1, w0 = tile * kRows + wave * 32, w1 = min(n_rows, w0 + 32) - 1;
+        const int last = min(n_rows, tile * kRows + kRows) - 1, w0 = tile * kRows + row_wave * 32, w1 = min(n_rows, w0 + 32) - 1;
         auto of = [&](int r) { return (PACK ? r / a.group : r) + shift; };
         any_lo = first_key(a, of(tile * kRows)), any_hi = end_key(a, of(last), prefix, n_keys);
         wave_lo = first_key(a, of(w0)), wave_hi = w1 < w0 ? 0 : end_key(a, of(w1), prefix, n_keys);
@@ -134,17 +139,19 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
     for (int t = first; t < last; ++t) {
         tiles_arrived();
         if (t + 1 < last) request(t + 1);
-        const int key = any_lo + t * KT;
-        if (key + KT <= wave_lo || key >= wave_hi) continue;
+        const int key = any_lo + t * KT + half * 32 * KB;
+        if (key + 32 * KB <= wave_lo || key >= wave_hi) continue;
         const char *kt = lds[t & 1][0], *vt = lds[t & 1][1];
 
+        int l = lane;
+        if constexpr (MOD) asm volatile("" : "+v"(l));  // (places in LDS made anew in every tile: kept, they would not fit the registers)
         floatx16 x[KB];
 #pragma unroll
         for (int i = 0; i < KB; ++i) x[i] = zero16();
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
-            for (int i = 0; i < KB; ++i) x[i] = Elem<T>::mma(Keys::row_operand(kt, 32 * i, c, lane), qf[c], x[i]);
+            for (int i = 0; i < KB; ++i) x[i] = Elem<T>::mma(Keys::row_operand(kt, 32 * (half * KB + i), c, l), qf[c], x[i]);
 
         if constexpr (MOD) {
             if (bend.cap > 0.f) {
@@ -163,7 +170,7 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
                     for (int r = 0; r < 16; ++r) x[i][r] = fmaf(-slope, fabsf(at - (float)(32 * i + 8 * (r >> 2) + (r & 3))), x[i][r]);
             }
         }
-        if (key < full_lo || key + KT > full_hi) {
+        if (key < full_lo || key + 32 * KB > full_hi) {
             const int at = key + 4 * h - lo;
             const uint32_t span = there && hi > lo ? hi - lo : 0;
 #pragma unroll
@@ -199,14 +206,41 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
             for (int c = 0; c < 2; ++c) {
                 const Vec8 p = operand<T>(x[i], c);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = Elem<T>::mma(Keys::column_operand(vt, d, 2 * i + c, lane), p, o[d]);
+                for (int d = 0; d < DB; ++d) o[d] = Elem<T>::mma(Keys::column_operand(vt, d, 2 * (half * KB + i) + c, l), p, o[d]);
             }
     }
 
     sum = halves_sum(sum);
+    m = m == -INFINITY ? m : m * unit;
+    if constexpr (RW < kWaves) {
+        // the halves of the keys: [element of the lane / 4][lane] of 16 bytes, maximum and sum
+        static_assert(RW * 128 * DP + RW * 256 <= (int)sizeof lds);
+        __syncthreads();
+        floatx4 *other = (floatx4 *)((char *)lds + row_wave * 128 * DP);
+        float2 *other_ml = (float2 *)((char *)lds + RW * 128 * DP) + row_wave * 32;
+        if (half) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) other[(4 * d + i) * 64 + lane] = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+            if (h == 0) other_ml[n] = make_float2(m, sum);
+        }
+        __syncthreads();
+        if (half) return;
+        const float2 ml = other_ml[n];
+        const float top = fmaxf(m, ml.x), w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), u = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+        m = top, sum = sum * w + ml.y * u;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const floatx4 y = other[(4 * d + i) * 64 + lane];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[d][4 * i + j] = o[d][4 * i + j] * w + y[j] * u;
+            }
+    }
     if (!there) return;
     const int64_t at = (e.lse0 + token) * a.n_heads + my_head;
-    m = m == -INFINITY ? m : m * unit;
     if (a.n_part > 1) {
         const int64_t all = a.rows * a.n_heads, part = a.part0 + split;
         float *to = a.part_o + (part * all + at) * a.head_dim;
@@ -234,29 +268,28 @@ void sddmm_attention_forward_kernel(const AttnArgs a)
 }
 
 template <class T, int DP, bool MOD>
-hipError_t launch_rows(const AttnArgs &a, int rows, unsigned grid, hipStream_t st)
+hipError_t launch_rows(const AttnArgs &a, int rows, int tile, unsigned grid, hipStream_t st)
 {
-    return launch(rows == kRowsShared ? sddmm_attention_forward_kernel<T, DP, MOD, kRowsShared>
-                  : rows == kRowsPacked ? sddmm_attention_forward_kernel<T, DP, MOD, kRowsPacked> : sddmm_attention_forward_kernel<T, DP, MOD, kRowsOfHead>,
-                  dim3(grid), dim3(64 * kWaves), 0, st, a);
+    void (*fn)(AttnArgs) = rows == kRowsShared ? sddmm_attention_forward_kernel<T, DP, MOD, kRowsShared, 4>
+        : rows == kRowsPacked ? (tile == 64 ? sddmm_attention_forward_kernel<T, DP, MOD, kRowsPacked, 2> : sddmm_attention_forward_kernel<T, DP, MOD, kRowsPacked, 4>)
+                              : (tile == 64 ? sddmm_attention_forward_kernel<T, DP, MOD, kRowsOfHead, 2> : sddmm_attention_forward_kernel<T, DP, MOD, kRowsOfHead, 4>);
+    return launch(fn, dim3(grid), dim3(64 * kWaves), 0, st, a);
 }
 
 template <class T>
-hipError_t launch_typed(const AttnArgs &a, int rows, unsigned grid, hipStream_t st)
+hipError_t launch_typed(const AttnArgs &a, int rows, int tile, unsigned grid, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
-    if (a.head_dim <= 64) return mod ? launch_rows<T, 64, true>(a, rows, grid, st) : launch_rows<T, 64, false>(a, rows, grid, st);
-    return mod ? launch_rows<T, 128, true>(a, rows, grid, st) : launch_rows<T, 128, false>(a, rows, grid, st);
+    if (a.head_dim <= 64) return mod ? launch_rows<T, 64, true>(a, rows, tile, grid, st) : launch_rows<T, 64, false>(a, rows, tile, grid, st);
+    return mod ? launch_rows<T, 128, true>(a, rows, tile, grid, st) : launch_rows<T, 128, false>(a, rows, tile, grid, st);
 }
 
 }  // namespace
 
-int attention_forward_rows() { return kRows; }
-
-hipError_t launch_attention_forward(const AttnArgs &a, int type, int rows, unsigned grid, hipStream_t st)
+hipError_t launch_attention_forward(const AttnArgs &a, int type, int rows, int tile, unsigned grid, hipStream_t st)
 {
-    return type == SDDMM_TYPE_F32 ? launch_typed<float>(a, rows, grid, st)
-         : type == SDDMM_TYPE_F16 ? launch_typed<_Float16>(a, rows, grid, st) : launch_typed<__bf16>(a, rows, grid, st);
+    return type == SDDMM_TYPE_F32 ? launch_typed<float>(a, rows, tile, grid, st)
+         : type == SDDMM_TYPE_F16 ? launch_typed<_Float16>(a, rows, tile, grid, st) : launch_typed<__bf16>(a, rows, tile, grid, st);
 }
 
 }  // namespace sddmm

@@ -8,14 +8,14 @@ struct AttnArgs;
 
 enum { kRowsOfHead = 0, kRowsPacked = 1, kRowsShared = 2 };  // what the rows of a forward workgroup are (attention_forward.hip)
 
-int attention_forward_rows();  // rows of a workgroup
 int attention_token_rows();
-hipError_t launch_attention_forward(const AttnArgs &a, int type, int rows, unsigned grid, hipStream_t st);
+// tile: rows of a workgroup, 128, or 64 (not of kRowsShared)
+hipError_t launch_attention_forward(const AttnArgs &a, int type, int rows, int tile, unsigned grid, hipStream_t st);
 hipError_t launch_attention_token(const AttnArgs &a, int type, unsigned grid, hipStream_t st);
-int attention_backward_rows();
-int attention_backward_few_rows();  // of a workgroup of the dq kernel for few rows
+int attention_backward_keys();  // of a workgroup of the dk, dv kernel
 // a: the dealing out of keys (dk, dv); b: of rows (dq)
-hipError_t launch_attention_backward(const AttnArgs &a, const AttnArgs &b, int type, unsigned kv_grid, unsigned q_grid, bool few, hipStream_t st);
+// q_rows: rows of a dq workgroup, 128, 64 or 32
+hipError_t launch_attention_backward(const AttnArgs &a, const AttnArgs &b, int type, unsigned kv_grid, unsigned q_grid, int q_rows, hipStream_t st);
 hipError_t launch_attention_join(const AttnArgs &a, int type, hipStream_t st);
 
 }  // namespace sddmm
