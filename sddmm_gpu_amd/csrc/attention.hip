@@ -54,21 +54,22 @@ struct Deal {
     int mapping = kRowsOfHead, tile = 128;
     int64_t slots = 0, max_tiles = 0, grid = 0, splits = 1;
     int64_t shared_slots = 0, shared_grid = 0, shared_splits = 0;
+    int shared_tile = 128;
     int64_t parts = 1, part_bytes = 0, bytes = 0;
 };
 
 constexpr int64_t kFill = 512;  // workgroups that fill the card: 256 compute units, two each
 
-// Pieces that the keys are cut into: so many that the grid fills the card, each of `least` keys at least.
-int64_t pieces(int64_t workgroups, int64_t keys, int64_t least)
+// Pieces that the keys are cut into: so many that there are `fill` workgroups, each of `least` keys at least.
+int64_t pieces(int64_t workgroups, int64_t keys, int64_t least, int64_t fill)
 {
-    return std::max<int64_t>(1, std::min(std::min(div_up(kFill, std::max<int64_t>(workgroups, 1)), div_up(keys, least)), (int64_t)256));
+    return std::max<int64_t>(1, std::min(std::min(div_up(fill, std::max<int64_t>(workgroups, 1)), div_up(keys, least)), (int64_t)256));
 }
 
 Deal deal(const sddmm_attention_desc &d)
 {
     Deal r;
-    const int64_t group = d.n_heads / d.n_kv_heads, tile = 128, few = attention_token_rows();
+    const int64_t group = d.n_heads / d.n_kv_heads, tile = 128, few = kTokenRows;
     r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
     // keys that a tile's rows can see
     const int64_t span = d.window_left >= 0 && d.window_right >= 0 && !d.prefix ? (int64_t)d.window_left + d.window_right + std::min<int64_t>(d.max_q, tile) : d.max_k;
@@ -85,18 +86,24 @@ Deal deal(const sddmm_attention_desc &d)
         if (r.grid >= 2 * kFill) break;
     }
     // or tiles of 32 pairs, each wave on keys of its own, where pairs are few or there would be less than 768 of 64 rows
-    r.token = packed <= few || r.grid < kFill * 3 / 2;
+    r.token = d.shared_len > 0 || packed <= few || r.grid < kFill * 3 / 2;
     if (r.token) {
         r.max_tiles = div_up(packed, few);
         r.slots = r.max_tiles == 1 ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
         r.grid = r.slots * d.n_kv_heads;
-        r.splits = pieces(r.grid, keys, 256);
+        // Few workgroups: pieces of 256 keys, two for each wave (one user, 1501 keys, 32 heads over 8: with 64 / 128 / 256 / 512 12.1 / 11.4 / 11.7 / 13.1 us).
+        // Where each workgroup has a cache of its own four times as many even out their lengths (64 users of 284 to 8192 keys: 512 / 1024 / 2048 / 4096
+        // workgroups 232 / 221 / 210 / 214 us), which short ones do not pay for with a second launch.
+        r.splits = r.max_tiles == 1 && r.grid >= kFill ? pieces(r.grid, keys, 1024, 4 * kFill) : pieces(r.grid, keys, 256, kFill);
         r.grid *= r.splits;
     }
     r.parts = r.splits;
     if (d.shared_len > 0) {
-        r.shared_slots = div_up(r.rows * group, tile);
-        r.shared_splits = pieces(r.shared_slots * d.n_kv_heads, d.shared_len, 256);
+        // Tiles of 64 rows up to 256 rows of a key head, and one workgroup of them for each compute unit beside the others' (48 users behind 16,000 keys: 128, 256, 512
+        // of them 50, 43 and 47 us).
+        r.shared_tile = r.rows * group <= 256 ? 64 : 128;
+        r.shared_slots = div_up(r.rows * group, r.shared_tile);
+        r.shared_splits = pieces(r.shared_slots * d.n_kv_heads, d.shared_len, 256, kFill / 2);
         r.shared_grid = r.shared_slots * d.n_kv_heads * r.shared_splits;
         r.parts += r.shared_splits;
     }
@@ -193,7 +200,7 @@ int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d
     if (!aligned({d_q, d_k, d_v, d_out, d_shared_k, d_shared_v})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (r.grid > INT32_MAX || r.shared_grid > INT32_MAX || (r.parts > 1 && r.rows * d.n_heads > INT32_MAX))
+    if (r.grid + r.shared_grid > INT32_MAX || (r.parts > 1 && r.rows * d.n_heads > INT32_MAX))
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
 
     AttnArgs a = arguments(d);
@@ -205,9 +212,10 @@ int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d
     if (d.shared_len > 0) {
         AttnArgs b = a;
         b.n_slots = (int)r.shared_slots, b.n_split = (int)r.shared_splits, b.part0 = (int)r.splits;
-        e = launch_attention_forward(b, d.type, kRowsShared, 128, (unsigned)r.shared_grid, st);
+        e = launch_attention_shared(b, a, d.type, r.shared_tile, (unsigned)r.shared_grid, (unsigned)r.grid, st);
+    } else {
+        e = r.token ? launch_attention_token(a, d.type, (unsigned)r.grid, st) : launch_attention_forward(a, d.type, r.mapping, r.tile, (unsigned)r.grid, st);
     }
-    if (e == hipSuccess) e = r.token ? launch_attention_token(a, d.type, (unsigned)r.grid, st) : launch_attention_forward(a, d.type, r.mapping, r.tile, (unsigned)r.grid, st);
     if (e == hipSuccess && r.parts > 1) e = launch_attention_join(a, d.type, st);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;

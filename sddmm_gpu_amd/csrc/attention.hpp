@@ -266,7 +266,7 @@ template <class T> __device__ __forceinline__ const T *v_base(const AttnArgs &a,
 //
 // Up to 64 sequences of up to 64 tiles: the slots go to the tiles of all sequences in the order of their distance from their sequence's
 // first one, the farthest first (LAST: from the last one).  Under a causal mask that is the order of their work, so that no long tile starts when
-// the others are done (13 documents, 8192 tokens, 16 heads of 128: @@).  Returns -1 for a slot that is none.
+// the others are done (13 documents, 8192 tokens, 16 heads of 128: forward 82 and 73, dq 132 and 112 us).  Returns -1 for a slot that is none.
 template <bool LAST>
 __device__ __forceinline__ int slot_sequence(const int32_t *ptr, int n_seq, int per, int size, int max_tiles, int n_slots, int slot, int &tile)
 {

@@ -1,277 +1,24 @@
-// Dense attention, forward (gfx950): tiles of rows against tiles of keys.
-#include "attention.hpp"
-#include "attention_launch.hpp"
+// Dense attention, forward (gfx950): the kernels of one tile of rows to a workgroup.
+#include "attention_tile.hpp"
 #include "launch.hpp"
 
 namespace sddmm {
 
 namespace {
 
-constexpr int kWaves = 4;  // of a workgroup, 32 rows to each
-
-// o_i = sum_j p_ij v_j / sum_j p_ij with p_ij = exp(s_ij - m_i), in one pass over the keys with a running maximum m_i.  A wave
-// holds 32 rows: their q as operands, the sums of o turned (element of the head by row).  Per tile of keys, which the four
-// waves share in LDS: S^T = K Q^T, so that a lane holds scores of one row only and the statistics need one exchange between the
-// two halves of the wave; the probabilities are the second operand of O^T += V^T P^T as they lie.  The maximum is raised only
-// when a row's exceeds it by more than 2^8: the sums stay far inside fp32, and the sums of o are rarely scaled.
-// P is rounded to the element type (bf16: 2^-9 relative at most, as the output itself), its sum is not.
-//
-// What the rows of a workgroup are: the rows of one query head (kRowsOfHead); the (token, head) pairs of the query heads that share
-// a key head, for few tokens (kRowsPacked); the same pairs of all sequences, against the keys that all of them begin with
-// (kRowsShared: each sequence's rows have positions, and so masks, of their own).
-//
-// RW: waves on rows of their own.  With 2 the others take the second half of every tile of keys for the same 64 rows, and the halves
-// are joined at the end: twice the workgroups, where those of 128 rows are so few that the longest keeps the others waiting.
 template <class T, int DP, bool MOD, int ROWS, int RW>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : 2)
 void sddmm_attention_forward_kernel(const AttnArgs a)
 {
-    constexpr int KT = sizeof(T) == 2 || RW == 2 ? 64 : 32, KB = KT / 32 / (kWaves / RW), DB = DP / 32, kRows = 32 * RW;
-    typedef Tile<T, DP, KT> Keys;
-    typedef typename Elem<T>::Vec8 Vec8;
-    __shared__ __align__(1024) char lds[2][2][Keys::kBytes];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
-    const int row_wave = wave % RW, half = wave / RW;
-
-    // Workgroups that read the same keys lie n_kv_heads (and n_seq) apart: with a multiple of 8 they are on one die, whose L2 then
-    // holds them.  Tiles of rows in descending order, since under a causal mask the last rows see most keys.
-    int b = blockIdx.x, s = 0, tile, head, split = 0;
-    const int kv = b % a.n_kv_heads;
-    b /= a.n_kv_heads;
-    if (ROWS != kRowsShared && !a.q_ptr) { s = b % a.n_seq; b /= a.n_seq; }
-    if constexpr (ROWS != kRowsOfHead) {
-        head = kv * a.group;
-    } else {
-        head = kv * a.group + b % a.group;
-        b /= a.group;
-    }
-    if (a.n_split > 1) { split = b % a.n_split; b /= a.n_split; }
-    if (ROWS != kRowsShared && a.q_ptr) {
-        s = slot_sequence<false>(a.q_ptr, a.n_seq, 1, kRows, a.max_tiles, a.n_slots, b, tile);
-        if (s < 0) return;
-    } else {
-        tile = a.n_slots - 1 - b;
-    }
-
-    // this lane's row: its token and head, and the keys [lo, hi) that it sees; and what any / all rows of the workgroup and of the wave see
-    const int row = tile * kRows + row_wave * 32 + n;
-    Seq e;
-    int n_keys, token, my_head = head, pos, lo, hi, any_lo, any_hi, wave_lo, wave_hi, full_lo, full_hi;
-    bool there;
-    if constexpr (ROWS == kRowsShared) {
-        __shared__ int ends[kWaves][2];
-        n_keys = a.shared_len;
-        there = row < a.n_seq * a.max_q * a.group;
-        const int t = row / a.group;
-        my_head = head + row % a.group;
-        s = there ? t / a.max_q : 0;
-        token = t - s * a.max_q;
-        e = sequence(a, s);
-        there = there && token < e.nq;
-        pos = n_keys + e.nk - e.nq + token;
-        lo = first_key(a, pos);
-        hi = there ? min(n_keys, end_key(a, pos, a.prefix ? a.prefix[s] : 0, n_keys + e.nk)) : 0;
-        wave_lo = there ? lo : INT32_MAX, wave_hi = hi, full_lo = there ? lo : 0, full_hi = there ? hi : INT32_MAX;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            wave_lo = min(wave_lo, __shfl_xor(wave_lo, d));
-            wave_hi = max(wave_hi, __shfl_xor(wave_hi, d));
-            full_lo = max(full_lo, __shfl_xor(full_lo, d));
-            full_hi = min(full_hi, __shfl_xor(full_hi, d));
-        }
-        wave_lo = __builtin_amdgcn_readfirstlane(wave_lo), wave_hi = __builtin_amdgcn_readfirstlane(wave_hi);
-        full_lo = __builtin_amdgcn_readfirstlane(full_lo), full_hi = __builtin_amdgcn_readfirstlane(full_hi);
-        if (lane == 0) ends[wave][0] = wave_lo, ends[wave][1] = wave_hi;
-        __syncthreads();
-        static_assert(ROWS != kRowsShared || RW == kWaves);
-        any_lo = min(min(ends[0][0], ends[1][0]), min(ends[2][0], ends[3][0]));
-        any_hi = max(max(ends[0][1], ends[1][1]), max(ends[2][1], ends[3][1]));
-        any_lo = __builtin_amdgcn_readfirstlane(any_lo), any_hi = __builtin_amdgcn_readfirstlane(any_hi);
-    } else {
-        constexpr bool PACK = ROWS == kRowsPacked;
-        e = sequence(a, s);
-        n_keys = e.nk;
-        const int n_rows = PACK ? e.nq * a.group : e.nq;
-        if (tile * kRows >= n_rows) return;
-        there = row < n_rows;
-        token = PACK ? row / a.group : row;
-        if constexpr (PACK) my_head = head + row % a.group;
-        const int shift = e.nk - e.nq, prefix = a.prefix ? max(0, a.prefix[s] - a.shared_len) : 0;
-        pos = token + shift;
-        lo = first_key(a, pos), hi = end_key(a, pos, prefix, n_keys);
-        const int last = min(n_rows, tile * kRows + kRows) - 1, w0 = tile * kRows + row_wave * 32, w1 = min(n_rows, w0 + 32) - 1;
-        auto of = [&](int r) { return (PACK ? r / a.group : r) + shift; };
-        any_lo = first_key(a, of(tile * kRows)), any_hi = end_key(a, of(last), prefix, n_keys);
-        wave_lo = first_key(a, of(w0)), wave_hi = w1 < w0 ? 0 : end_key(a, of(w1), prefix, n_keys);
-        full_lo = first_key(a, of(max(w1, 0))), full_hi = end_key(a, of(w0), prefix, n_keys);
-    }
-
-    const T *q = q_base<T>(a, a.q, e, s, my_head) + (int64_t)token * a.q_row;
-    const T *k = ROWS == kRowsShared ? (const T *)a.shared_k + kv * a.k_head : k_base<T>(a, a.k, e, s, kv);
-    const T *v = ROWS == kRowsShared ? (const T *)a.shared_v + kv * a.v_head : v_base<T>(a, a.v, e, s, kv);
-    Vec8 qf[DP / 16];
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) qf[c] = global_operand<T>(q, there, 16 * c + 8 * h, a.head_dim);
-
-    floatx16 o[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = zero16();
-    const float scale = a.scale;
-    Bend bend;
-    if constexpr (MOD) bend.init(scale, a.cap);
-    const float unit = MOD ? 1.f : scale * kLog2e;  // scores in registers to powers of two
-    const float raise = 8.f / unit;
-    const float slope = MOD && a.slopes && there ? a.slopes[my_head] * kLog2e : 0.f;
-    float m = -INFINITY, sum = 0.f;
-
-    const int n_tiles = any_hi > any_lo ? (any_hi - any_lo + KT - 1) / KT : 0;
-    const int each = (n_tiles + a.n_split - 1) / a.n_split;
-    const int first = split * each, last = min(n_tiles, first + each);
-    const int row_bytes = a.head_dim * (int)sizeof(T);
-    const uint32_t k_stride = (uint32_t)(a.k_row * sizeof(T)), v_stride = (uint32_t)(a.v_row * sizeof(T));
-    auto request = [&](int t) {
-        const int key = any_lo + t * KT;
-        char *to = lds[t & 1][0];
-        Keys::template request<kWaves>(to, (const char *)(k + key * a.k_row), k_stride, n_keys - key, row_bytes, wave, lane);
-        Keys::template request<kWaves>(to + Keys::kBytes, (const char *)(v + key * a.v_row), v_stride, n_keys - key, row_bytes, wave, lane);
-    };
-    if (first < last) request(first);
-    for (int t = first; t < last; ++t) {
-        tiles_arrived();
-        if (t + 1 < last) request(t + 1);
-        const int key = any_lo + t * KT + half * 32 * KB;
-        if (key + 32 * KB <= wave_lo || key >= wave_hi) continue;
-        const char *kt = lds[t & 1][0], *vt = lds[t & 1][1];
-
-        int l = lane;
-        if constexpr (MOD) asm volatile("" : "+v"(l));  // (places in LDS made anew in every tile: kept, they would not fit the registers)
-        floatx16 x[KB];
-#pragma unroll
-        for (int i = 0; i < KB; ++i) x[i] = zero16();
-#pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
-#pragma unroll
-            for (int i = 0; i < KB; ++i) x[i] = Elem<T>::mma(Keys::row_operand(kt, 32 * (half * KB + i), c, l), qf[c], x[i]);
-
-        if constexpr (MOD) {
-            if (bend.cap > 0.f) {
-                bend.apply<KB, false>(x, x);
-            } else {
-#pragma unroll
-                for (int i = 0; i < KB; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[i][r] *= scale * kLog2e;
-            }
-            if (a.slopes) {
-                const float at = (float)(pos - key - 4 * h);
-#pragma unroll
-                for (int i = 0; i < KB; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[i][r] = fmaf(-slope, fabsf(at - (float)(32 * i + 8 * (r >> 2) + (r & 3))), x[i][r]);
-            }
-        }
-        if (key < full_lo || key + 32 * KB > full_hi) {
-            const int at = key + 4 * h - lo;
-            const uint32_t span = there && hi > lo ? hi - lo : 0;
-#pragma unroll
-            for (int i = 0; i < KB; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    x[i][r] = (uint32_t)(at + 32 * i + 8 * (r >> 2) + (r & 3)) < span ? x[i][r] : -INFINITY;
-        }
-        float top = x[0][0];
-#pragma unroll
-        for (int i = 0; i < KB; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, x[i][r]);
-        top = halves_max(top);
-        if (__any(top > m + raise || (m == -INFINITY && top > m))) {
-            const float raised = fmaxf(m, top), by = raised == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - raised) * unit);
-            m = raised;
-            sum *= by;
-#pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] *= by;
-        }
-        const float base = m == -INFINITY ? 0.f : m * unit;
-#pragma unroll
-        for (int i = 0; i < KB; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                x[i][r] = __builtin_amdgcn_exp2f(fmaf(x[i][r], unit, -base));
-                sum += x[i][r];
-            }
-#pragma unroll
-        for (int i = 0; i < KB; ++i)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const Vec8 p = operand<T>(x[i], c);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = Elem<T>::mma(Keys::column_operand(vt, d, 2 * (half * KB + i) + c, l), p, o[d]);
-            }
-    }
-
-    sum = halves_sum(sum);
-    m = m == -INFINITY ? m : m * unit;
-    if constexpr (RW < kWaves) {
-        // the halves of the keys: [element of the lane / 4][lane] of 16 bytes, maximum and sum
-        static_assert(RW * 128 * DP + RW * 256 <= (int)sizeof lds);
-        __syncthreads();
-        floatx4 *other = (floatx4 *)((char *)lds + row_wave * 128 * DP);
-        float2 *other_ml = (float2 *)((char *)lds + RW * 128 * DP) + row_wave * 32;
-        if (half) {
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) other[(4 * d + i) * 64 + lane] = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-            if (h == 0) other_ml[n] = make_float2(m, sum);
-        }
-        __syncthreads();
-        if (half) return;
-        const float2 ml = other_ml[n];
-        const float top = fmaxf(m, ml.x), w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), u = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
-        m = top, sum = sum * w + ml.y * u;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const floatx4 y = other[(4 * d + i) * 64 + lane];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[d][4 * i + j] = o[d][4 * i + j] * w + y[j] * u;
-            }
-    }
-    if (!there) return;
-    const int64_t at = (e.lse0 + token) * a.n_heads + my_head;
-    if (a.n_part > 1) {
-        const int64_t all = a.rows * a.n_heads, part = a.part0 + split;
-        float *to = a.part_o + (part * all + at) * a.head_dim;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int col = 32 * d + 8 * i + 4 * h;
-                if (col < a.head_dim) *(floatx4 *)(to + col) = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-            }
-        if (h == 0) a.part_ml[part * all + at] = make_float2(m, sum);
-        return;
-    }
-    const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    T *to = (T *)o_base<T>(a, a.out, e, s, my_head) + (int64_t)token * a.o_row;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int col = 32 * d + 8 * i + 4 * h;
-            const floatx4 y = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * by;
-            if (col < a.head_dim) *(typename Elem<T>::Vec4 *)(to + col) = __builtin_convertvector(y, typename Elem<T>::Vec4);
-        }
-    if (a.lse && h == 0) a.lse[at] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+    typedef ForwardTile<T, DP, MOD, ROWS, RW> Body;
+    __shared__ __align__(1024) char lds[Body::kLds];
+    Body::run(a, blockIdx.x, lds);
 }
 
 template <class T, int DP, bool MOD>
 hipError_t launch_rows(const AttnArgs &a, int rows, int tile, unsigned grid, hipStream_t st)
 {
-    void (*fn)(AttnArgs) = rows == kRowsShared ? sddmm_attention_forward_kernel<T, DP, MOD, kRowsShared, 4>
-        : rows == kRowsPacked ? (tile == 64 ? sddmm_attention_forward_kernel<T, DP, MOD, kRowsPacked, 2> : sddmm_attention_forward_kernel<T, DP, MOD, kRowsPacked, 4>)
+    void (*fn)(AttnArgs) = rows == kRowsPacked ? (tile == 64 ? sddmm_attention_forward_kernel<T, DP, MOD, kRowsPacked, 2> : sddmm_attention_forward_kernel<T, DP, MOD, kRowsPacked, 4>)
                               : (tile == 64 ? sddmm_attention_forward_kernel<T, DP, MOD, kRowsOfHead, 2> : sddmm_attention_forward_kernel<T, DP, MOD, kRowsOfHead, 4>);
     return launch(fn, dim3(grid), dim3(64 * kWaves), 0, st, a);
 }

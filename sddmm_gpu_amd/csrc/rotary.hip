@@ -48,7 +48,7 @@ void sddmm_rotary_kernel(const RotaryArgs a)
     const int pairs = a.rot_dim / 2;
     const int64_t row0 = (int64_t)blockIdx.x * a.per_row;
     const int rows = (int)min((int64_t)a.per_row, a.n_rows - row0);
-    // pairs beyond the table are turned in further rounds
+    // Pairs beyond the table are turned in further rounds; the last one also copies the rest of the heads, whose lines the pairs' pieces lie in.
     for (int p0 = 0; p0 < pairs; p0 += kTable) {
         const int some = min(pairs - p0, kTable);
         if (p0) __syncthreads();
@@ -65,11 +65,9 @@ void sddmm_rotary_kernel(const RotaryArgs a)
             table[i] = make_float2(cosine * a.amplitude, sine * a.amplitude * a.sign);
         }
         __syncthreads();
-        const int pieces = some / (HALF ? V : kPairs);
-        const float by_pieces = 1.f / (float)pieces;
-        const int all_heads = a.heads[0] + a.heads[1];
-        const float by_heads = 1.f / (float)all_heads;
-        const int n = rows * all_heads * pieces;
+        const int turned = some / (HALF ? V : kPairs), pieces = turned + (a.copy && p0 + some == pairs ? (a.head_dim - a.rot_dim) / V : 0);
+        const int all_heads = a.heads[0] + a.heads[1], n = rows * all_heads * pieces;
+        const float by_pieces = 1.f / (float)pieces, by_heads = 1.f / (float)all_heads;
         for (int i = threadIdx.x; i < n; i += kBlock) {
             // (quotients by a product: exact below 2^20, which n is held to)
             const int unit = (int)(((float)i + 0.5f) * by_pieces), piece = i - unit * pieces;
@@ -77,42 +75,36 @@ void sddmm_rotary_kernel(const RotaryArgs a)
             const int which = head_at >= a.heads[0], head = which ? head_at - a.heads[0] : head_at;
             const T *x = (const T *)a.x[which] + (row0 + r) * a.x_row[which] + head * a.x_head[which];
             T *y = (T *)a.y[which] + (row0 + r) * a.y_row[which] + head * a.y_head[which];
-            const float2 *cs = &table[r * some + piece * (HALF ? V : kPairs)];
-            if constexpr (V == 1) {
-                const int at = HALF ? p0 + piece : 2 * (p0 + piece), other = at + (HALF ? pairs : 1);
-                const float f = (float)x[at], g = (float)x[other];
-                y[at] = (T)(f * cs[0].x - g * cs[0].y), y[other] = (T)(f * cs[0].y + g * cs[0].x);
-            } else if constexpr (HALF) {
-                const int at = p0 + piece * V;
-                Vec u = *(const Vec *)(x + at), v = *(const Vec *)(x + at + pairs);
+            // (pieces to turn and to copy lie in one wave: loads and stores are common to both)
+            const bool turn = piece < turned;
+            const int at = !turn ? a.rot_dim + (piece - turned) * V : HALF ? p0 + piece * V : 2 * p0 + piece * (V > 1 ? V : 2);
+            const int other = !turn ? at : HALF ? at + pairs : V > 1 ? at : at + 1;
+            Vec u = *(const Vec *)(x + at), v = u;
+            if constexpr (HALF || V == 1) v = *(const Vec *)(x + other);
+            if (turn) {
+                const float2 *cs = &table[r * some + piece * (HALF ? V : kPairs)];
+                if constexpr (V == 1) {
+                    const float f = (float)u, g = (float)v;
+                    u = (T)(f * cs[0].x - g * cs[0].y), v = (T)(f * cs[0].y + g * cs[0].x);
+                } else if constexpr (HALF) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float f = (float)u[j], g = (float)v[j];
-                    u[j] = (T)(f * cs[j].x - g * cs[j].y), v[j] = (T)(f * cs[j].y + g * cs[j].x);
-                }
-                *(Vec *)(y + at) = u, *(Vec *)(y + at + pairs) = v;
-            } else {
-                const int at = 2 * p0 + piece * V;
-                Vec u = *(const Vec *)(x + at);
+                    for (int j = 0; j < V; ++j) {
+                        const float f = (float)u[j], g = (float)v[j];
+                        u[j] = (T)(f * cs[j].x - g * cs[j].y), v[j] = (T)(f * cs[j].y + g * cs[j].x);
+                    }
+                } else {
 #pragma unroll
-                for (int j = 0; j < V / 2; ++j) {
-                    const float f = (float)u[2 * j], g = (float)u[2 * j + 1];
-                    u[2 * j] = (T)(f * cs[j].x - g * cs[j].y), u[2 * j + 1] = (T)(f * cs[j].y + g * cs[j].x);
+                    for (int j = 0; j < kPairs; ++j) {
+                        const float f = (float)u[2 * j], g = (float)u[2 * j + 1];
+                        u[2 * j] = (T)(f * cs[j].x - g * cs[j].y), u[2 * j + 1] = (T)(f * cs[j].y + g * cs[j].x);
+                    }
                 }
-                *(Vec *)(y + at) = u;
+            }
+            *(Vec *)(y + at) = u;
+            if constexpr (HALF || V == 1) {
+                if (turn) *(Vec *)(y + other) = v;
             }
         }
-    }
-    if (!a.copy) return;
-    const int pieces = (a.head_dim - a.rot_dim) / V, all_heads = a.heads[0] + a.heads[1], n = rows * all_heads * pieces;
-    const float by_pieces = 1.f / (float)pieces, by_heads = 1.f / (float)all_heads;
-    for (int i = threadIdx.x; i < n; i += kBlock) {
-        const int unit = (int)(((float)i + 0.5f) * by_pieces), at = a.rot_dim + (i - unit * pieces) * V;
-        const int r = (int)(((float)unit + 0.5f) * by_heads), head_at = unit - r * all_heads;
-        const int which = head_at >= a.heads[0], head = which ? head_at - a.heads[0] : head_at;
-        const T *x = (const T *)a.x[which] + (row0 + r) * a.x_row[which] + head * a.x_head[which];
-        T *y = (T *)a.y[which] + (row0 + r) * a.y_row[which] + head * a.y_head[which];
-        *(Vec *)(y + at) = *(const Vec *)(x + at);
     }
 }
 
@@ -192,10 +184,11 @@ int sddmm_rotary(const sddmm_rotary_desc *desc, const int32_t *d_positions, cons
     int v = 16 / size;
     while (v > 1 && bits % v) v /= 2;
     const bool half = d.layout == SDDMM_ROTARY_HALF;
-    // Rows of a workgroup: one where there are few (1024 workgroups fill the card), else as many as fill a table; products of whole numbers below 2^20.
+    // Rows of a workgroup: one, two where there are many (16,384 rows of 32 + 8 heads of 128, in halves / interleaved: 1, 2, 4 and 8 rows 80 / 76, 80 / 77, 81 / 80
+    // and 87 / 86 us; two or four pieces of a thread under way together 91 to 126: fewer waves).
     const int64_t pieces = d.rot_dim / (half || v == 1 ? 2 * v : v) + (d.head_dim - d.rot_dim) / v + 1, row_work = pieces * (d.n_heads + d.n_kv_heads);
     if (row_work > (1 << 20)) return fail(SDDMM_ERR_RANGE, "%s: a row of all heads is too long", who);
-    a.per_row = (int)std::max<int64_t>(1, std::min({d.n_rows / 1024, (int64_t)kTable / (d.rot_dim / 2), ((int64_t)1 << 20) / row_work, (int64_t)4}));
+    a.per_row = (int)std::max<int64_t>(1, std::min({d.n_rows / 1024, (int64_t)kTable / (d.rot_dim / 2), ((int64_t)1 << 20) / row_work, (int64_t)2}));
     const int64_t grid = (d.n_rows + a.per_row - 1) / a.per_row;
     if (grid > INT32_MAX) return fail(SDDMM_ERR_RANGE, "%s: too many rows for one launch", who);
     const hipStream_t st = (hipStream_t)stream;
