@@ -15,6 +15,9 @@ constexpr int64_t kMostRows = INT32_MAX;
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// head_dim as the kernels are made for (fp32, whose matrix instructions are a sixteenth as fast, by 32)
+int64_t padded_dim(const sddmm_attention_desc &d) { return d.head_dim <= 32 && d.type == SDDMM_TYPE_F32 ? 32 : d.head_dim <= 64 ? 64 : 128; }
+
 int element(int type) { return type == SDDMM_TYPE_F32 ? 4 : 2; }
 
 bool strides_fit(const sddmm_attention_desc &d, int64_t seq, int64_t row, int64_t head, bool packed)
@@ -155,7 +158,8 @@ DealBack deal_back(const sddmm_attention_desc &d)
         const int64_t places = d.type == SDDMM_TYPE_F32 && d.head_dim > 64 ? kFill / 2 : kFill, tiles = div_up(r.key_rows, tile) * d.n_kv_heads;
         const double share = rows * tiles / places;
         if (most > 2.5 * share) {
-            r.chunk = std::max<int64_t>((int64_t)std::sqrt(1300. * share), 256);
+            const bool slow = d.type == SDDMM_TYPE_F32;  // (its rows take sixteen times as long, its parts no longer)
+            r.chunk = std::max<int64_t>((int64_t)std::sqrt((slow ? 100. : 1300.) * share), slow ? 64 : 256);
             r.splits = std::max<int64_t>(1, std::min<int64_t>(div_up(most, r.chunk), 32));
         }
         r.chunk = std::max(r.chunk, div_up(most, r.splits));
@@ -163,7 +167,7 @@ DealBack deal_back(const sddmm_attention_desc &d)
     }
     r.delta_at = padded(r.rows * d.n_heads * 4);
     r.parts_at = 2 * r.delta_at;
-    r.slopes_at = r.parts_at + (r.splits > 1 ? r.kv_grid * tile * (d.head_dim <= 64 ? 64 : 128) * 8 : 0);
+    r.slopes_at = r.parts_at + (r.splits > 1 ? r.kv_grid * tile * padded_dim(d) * 8 : 0);
     r.bytes = r.slopes_at + (d.slopes ? padded(r.slope_parts * d.n_heads * 8) : 0);
     return r;
 }

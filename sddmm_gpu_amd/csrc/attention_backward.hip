@@ -123,7 +123,7 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
     typedef Tile<T, DP, kKeys> Values;
     typedef typename Elem<T>::Vec8 Vec8;
     // (registers: 128 for the sums, 32 for k, 32 for a tile's scores; v would be 32 more than two waves to a SIMD leave)
-    constexpr bool kKeepV = sizeof(T) == 4 || DP == 64;
+    constexpr bool kKeepV = sizeof(T) == 4 || DP <= 64;
     __shared__ __align__(1024) char lds[2][2][Rows::kBytes];
     __shared__ __align__(1024) char values[kKeepV ? 16 : Values::kBytes];
     __shared__ __align__(16) float stat[2][2][64];
@@ -628,6 +628,9 @@ hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, 
 template <class T>
 hipError_t launch_dims(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, unsigned q_grid, int q_rows, hipStream_t st)
 {
+    if constexpr (sizeof(T) == 4) {
+        if (a.head_dim <= 32) return launch_typed<T, 32>(a, b, kv_grid, q_grid, q_rows, st);
+    }
     return a.head_dim <= 64 ? launch_typed<T, 64>(a, b, kv_grid, q_grid, q_rows, st) : launch_typed<T, 128>(a, b, kv_grid, q_grid, q_rows, st);
 }
 

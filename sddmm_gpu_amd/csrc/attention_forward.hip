@@ -27,6 +27,9 @@ template <class T>
 hipError_t launch_typed(const AttnArgs &a, int rows, int tile, unsigned grid, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
+    if constexpr (sizeof(T) == 4) {
+        if (a.head_dim <= 32) return mod ? launch_rows<T, 32, true>(a, rows, tile, grid, st) : launch_rows<T, 32, false>(a, rows, tile, grid, st);
+    }
     if (a.head_dim <= 64) return mod ? launch_rows<T, 64, true>(a, rows, tile, grid, st) : launch_rows<T, 64, false>(a, rows, tile, grid, st);
     return mod ? launch_rows<T, 128, true>(a, rows, tile, grid, st) : launch_rows<T, 128, false>(a, rows, tile, grid, st);
 }

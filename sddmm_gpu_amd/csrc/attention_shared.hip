@@ -31,6 +31,9 @@ template <class T>
 hipError_t launch_dims(const AttnArgs &a, const AttnArgs &own, int tile, unsigned n_shared, unsigned n_own, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
+    if constexpr (sizeof(T) == 4) {
+        if (a.head_dim <= 32) return mod ? launch_typed<T, 32, true>(a, own, tile, n_shared, n_own, st) : launch_typed<T, 32, false>(a, own, tile, n_shared, n_own, st);
+    }
     if (a.head_dim <= 64) return mod ? launch_typed<T, 64, true>(a, own, tile, n_shared, n_own, st) : launch_typed<T, 64, false>(a, own, tile, n_shared, n_own, st);
     return mod ? launch_typed<T, 128, true>(a, own, tile, n_shared, n_own, st) : launch_typed<T, 128, false>(a, own, tile, n_shared, n_own, st);
 }

@@ -98,6 +98,7 @@ hipError_t join_dims(const AttnArgs &a, hipStream_t st)
 hipError_t launch_attention_token(const AttnArgs &a, int type, unsigned grid, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
+    if (a.head_dim <= 32 && type == SDDMM_TYPE_F32) return launch_typed<float, 32>(a, mod, grid, st);
     if (a.head_dim <= 64)
         return type == SDDMM_TYPE_F32 ? launch_typed<float, 64>(a, mod, grid, st)
              : type == SDDMM_TYPE_F16 ? launch_typed<_Float16, 64>(a, mod, grid, st) : launch_typed<__bf16, 64>(a, mod, grid, st);
