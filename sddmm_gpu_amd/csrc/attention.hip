@@ -120,14 +120,14 @@ Deal deal(const sddmm_attention_desc &d)
 // The same for the backward pass.
 struct DealBack {
     int64_t rows = 0, key_rows = 0, q_slots = 0, q_tiles = 0, kv_slots = 0, kv_tiles = 0, q_grid = 0, kv_grid = 0, splits = 1, chunk = 1, slope_parts = 0;
-    int q_rows = 128;  // of a dq workgroup
+    int q_rows = 128, keys = 128;  // of a dq and a dk, dv workgroup
     int64_t lse_at = 0, delta_at = 0, parts_at = 0, slopes_at = 0, bytes = 0;  // places in the workspace
 };
 
 DealBack deal_back(const sddmm_attention_desc &d)
 {
     DealBack r;
-    const int64_t tile = attention_backward_keys(), group = d.n_heads / d.n_kv_heads;
+    const int64_t group = d.n_heads / d.n_kv_heads;
     r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
     r.key_rows = d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k;
     if (r.rows > 0) {
@@ -143,20 +143,30 @@ DealBack deal_back(const sddmm_attention_desc &d)
         }
     }
     if (r.key_rows > 0) {
-        r.kv_tiles = div_up(d.max_k, tile);
-        r.kv_slots = d.k_ptr ? r.key_rows / tile + d.n_seq : r.kv_tiles;
-        const int64_t workgroups = r.kv_slots * (d.k_ptr ? 1 : d.n_seq) * d.n_kv_heads;
+        // Tiles of 128 keys, or of 32 where all their rows together are so few that most waves would have none (us of forward and backward with 128 and 32:
+        // 3 sequences, 148 tokens in all, 16 heads over 2 of 96, fp32 125 and 100; 228 tokens, 8 over 2 of 128, fp16 53 and 44; 4370 tokens in a window
+        // of 410, 6 over 3 of 64, bf16 85 and 78; but 2898 tokens, 8 over 1 of 128 228 and 280).
         const bool window = d.window_left >= 0 && d.window_right >= 0 && !d.prefix;
-        const int64_t most = group * (window ? std::min<int64_t>(d.max_q, (int64_t)d.window_left + d.window_right + tile) : d.max_q);
-        // A tile of keys that most rows see is cut where it would take more than 2.5 equal shares of all work.  The work of uneven sequences is
-        // not known here: between the mean and the longest length.  A piece costs the time of some 650 rows, written and read, so
-        // pieces of c rows cost 650 work / c and save half of c at the end: c = sqrt(1300 share).  us of the backward pass, bf16, causal, with
+        int64_t workgroups = 0, most = 0;
+        double work = 0.;
+        for (int64_t keys : {128, 32}) {
+            r.keys = (int)keys;
+            r.kv_tiles = div_up(d.max_k, keys);
+            r.kv_slots = d.k_ptr ? r.key_rows / keys + d.n_seq : r.kv_tiles;
+            workgroups = r.kv_slots * (d.k_ptr ? 1 : d.n_seq) * d.n_kv_heads;
+            // Rows of all heads that see a tile, at most, and those of all tiles.  The work of uneven sequences is not known here: between the mean and
+            // the longest length.
+            most = group * (window ? std::min<int64_t>(d.max_q, (int64_t)d.window_left + d.window_right + keys) : d.max_q);
+            const double mean = d.k_ptr ? (double)r.key_rows / d.n_seq : d.max_k;
+            work = most * std::min(1., std::sqrt(mean / std::max(d.max_k, 1))) * (d.window_right == 0 && !window ? 0.5 : 1.) * div_up(r.key_rows, keys) * d.n_kv_heads;
+            if (work >= 32768.) break;
+        }
+        // A tile of keys that most rows see is cut where it would take more than 2.5 equal shares of all work.  A piece costs the time of some 650 rows, written
+        // and read, so pieces of c rows cost 650 work / c and save half of c at the end: c = sqrt(1300 share).  us of the backward pass, bf16, causal, with
         // this and whole tiles: 8192 tokens, 16 heads over 4 of 128 1150 and 1853, 13 documents of 22 to 2281 tokens in all 8192 386 and
         // 590; 4096, 16 over 2 390 and 1537; 2048, 16 over 4 of 64 104 and 300; where whole tiles stay: 8192, 16 over 16 1020, in pieces of 3600 1076.
-        const double mean = d.k_ptr ? (double)r.key_rows / d.n_seq : d.max_k;
-        const double rows = most * std::min(1., std::sqrt(mean / std::max(d.max_k, 1))) * (d.window_right == 0 && !window ? 0.5 : 1.);
-        const int64_t places = d.type == SDDMM_TYPE_F32 && d.head_dim > 64 ? kFill / 2 : kFill, tiles = div_up(r.key_rows, tile) * d.n_kv_heads;
-        const double share = rows * tiles / places;
+        const int64_t places = r.keys == 32 || (d.type == SDDMM_TYPE_F32 && d.head_dim > 64) ? kFill / 2 : kFill;
+        const double share = work / places;
         if (most > 2.5 * share) {
             const bool slow = d.type == SDDMM_TYPE_F32;  // (its rows take sixteen times as long, its parts no longer)
             r.chunk = std::max<int64_t>((int64_t)std::sqrt((slow ? 100. : 1300.) * share), slow ? 64 : 256);
@@ -167,7 +177,7 @@ DealBack deal_back(const sddmm_attention_desc &d)
     }
     r.delta_at = padded(r.rows * d.n_heads * 4);
     r.parts_at = 2 * r.delta_at;
-    r.slopes_at = r.parts_at + (r.splits > 1 ? r.kv_grid * tile * padded_dim(d) * 8 : 0);
+    r.slopes_at = r.parts_at + (r.splits > 1 ? r.kv_grid * r.keys * padded_dim(d) * 8 : 0);
     r.bytes = r.slopes_at + (d.slopes ? padded(r.slope_parts * d.n_heads * 8) : 0);
     return r;
 }
@@ -290,7 +300,7 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
     AttnArgs b = a;
     a.n_slots = (int)r.kv_slots, a.max_tiles = (int)r.kv_tiles, a.n_split = (int)r.splits, a.chunk = (int)std::min<int64_t>(r.chunk, INT32_MAX);
     b.n_slots = (int)r.q_slots, b.max_tiles = (int)r.q_tiles, b.n_split = 1;
-    const hipError_t e = launch_attention_backward(a, b, d.type, (unsigned)r.kv_grid, (unsigned)r.q_grid, r.q_rows, (hipStream_t)stream);
+    const hipError_t e = launch_attention_backward(a, b, d.type, (unsigned)r.kv_grid, r.keys, (unsigned)r.q_grid, r.q_rows, (hipStream_t)stream);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;
 }

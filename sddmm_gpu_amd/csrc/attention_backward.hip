@@ -15,6 +15,7 @@ namespace sddmm {
 namespace {
 
 constexpr int kKeys = 128, kWaves = 4;  // keys of a workgroup of the dk, dv kernel, 32 to a wave
+constexpr int kFewKeys = 32;             // of the one for few keys
 
 // stats[head][row] = (lse in powers of two, dout . out).  A row that saw nothing gets +infinity, so that 2^(s - lse) is 0.
 template <class T, int DP>
@@ -84,42 +85,137 @@ __device__ __forceinline__ int end_row(const AttnArgs &a, int j, int shift, int 
     return a.left < 0 ? n_rows : min(n_rows, max(0, min(j, INT32_MAX / 2) + min(a.left, INT32_MAX / 2) + 1 - shift));
 }
 
-// The keys of a workgroup, and how the rows that see them are cut into pieces (a.n_split at most, of about a.chunk rows of all heads): a
-// key tile early in a long sequence has many times the rows of others.
+// The keys of a workgroup (KEYS of them), and how the rows that see them are cut into pieces (a.n_split at most, of about a.chunk rows of all
+// heads): a key tile early in a long sequence has many times the rows of others.
 struct KeyTile {
     Seq e;
     int s, kv, tile, shift, prefix, any_lo, any_hi, pieces;
 };
+template <int KEYS>
 __device__ __forceinline__ bool key_tile(const AttnArgs &a, int b, KeyTile &k)
 {
     k.kv = b % a.n_kv_heads;
     b /= a.n_kv_heads;
     if (a.k_ptr) {
-        k.s = slot_sequence<true>(a.k_ptr, a.n_seq, 1, kKeys, a.max_tiles, a.n_slots, b, k.tile);
+        k.s = slot_sequence<true>(a.k_ptr, a.n_seq, 1, KEYS, a.max_tiles, a.n_slots, b, k.tile);
         if (k.s < 0) return false;
     } else {
         k.s = b % a.n_seq, k.tile = b / a.n_seq;
     }
     k.e = sequence(a, k.s);
-    if (k.tile * kKeys >= k.e.nk) return false;
+    if (k.tile * KEYS >= k.e.nk) return false;
     k.shift = k.e.nk - k.e.nq, k.prefix = a.prefix ? a.prefix[k.s] : 0;
-    k.any_lo = first_row(a, k.tile * kKeys, k.prefix, k.shift);
-    k.any_hi = end_row(a, min(k.e.nk, k.tile * kKeys + kKeys) - 1, k.shift, k.e.nq);
+    k.any_lo = first_row(a, k.tile * KEYS, k.prefix, k.shift);
+    k.any_hi = end_row(a, min(k.e.nk, k.tile * KEYS + KEYS) - 1, k.shift, k.e.nq);
     const int64_t rows = (int64_t)max(0, k.any_hi - k.any_lo) * a.group;
     k.pieces = (int)max((int64_t)1, min((int64_t)a.n_split, (rows + a.chunk - 1) / a.chunk));
     return true;
 }
 
-// dk and dv.  A wave holds 32 keys: k and v as operands, the sums of dk and dv turned (element of the head by key).  Per tile of rows, q and
-// do of which the four waves share in LDS with their statistics: S = Q K^T and dP = dO V^T, a lane holding one key's; P and dS are
-// operands of dV^T += dO^T P and dK^T += Q^T dS as they lie, q and do being read a second time, in the transposing way.  The query heads that share a key
-// head follow each other in the same sums.
+// 32 keys of a wave: k as an operand, the sums of dk and dv turned (element of the head by key).  Per tile of 32 rows, q and do of which are in LDS
+// with their statistics: S = Q K^T and dP = dO V^T, a lane holding one key's; P and dS are operands of dV^T += dO^T P and dK^T += Q^T dS as
+// they lie, q and do being read a second time, in the transposing way.
+template <class T, int DP, bool MOD>
+struct DkvKeys {
+    static constexpr int DB = DP / 32;
+    typedef typename Elem<T>::Vec8 Vec8;
+    typedef Tile<T, DP, 32> Rows;
+    Vec8 kf[DP / 16];
+    floatx16 dk[DB], dv[DB];
+    float unit;
+    Bend bend;
+    bool bias, there;
+    int key, lo, hi, wave_lo, wave_hi, full_lo, full_hi, shift, h;
+
+    __device__ __forceinline__ void init(const AttnArgs &a, const KeyTile &t, int first, int lane)
+    {
+        h = lane >> 5, key = first + (lane & 31), shift = t.shift;
+        there = key < t.e.nk;
+        lo = first_row(a, key, t.prefix, shift), hi = there ? end_row(a, key, shift, t.e.nq) : 0;
+        const int last = min(t.e.nk, first + 32) - 1;
+        wave_lo = first_row(a, first, t.prefix, shift), wave_hi = last < first ? 0 : end_row(a, last, shift, t.e.nq);
+        full_lo = first_row(a, max(last, 0), t.prefix, shift), full_hi = last < first + 31 ? 0 : end_row(a, first, shift, t.e.nq);
+        const T *k = k_base<T>(a, a.k, t.e, t.s, t.kv) + key * a.k_row;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) kf[c] = global_operand<T>(k, there, 16 * c + 8 * h, a.head_dim);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
+        unit = a.scale * kLog2e, bias = a.slopes != nullptr;
+        if constexpr (MOD) bend.init(a.scale, a.cap);
+    }
+    __device__ __forceinline__ bool sees(int row) const { return row + 32 > wave_lo && row < wave_hi; }
+    // rows `row` on: their tiles, log-sum-exps and deltas; v(c): 16 elements of v as an operand
+    template <class V> __device__ __forceinline__ void add(const char *qt, const char *dot, const float *lse, const float *delta, int row, float slope, int l, V v)
+    {
+        floatx16 x = zero16(), y = zero16(), back;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) x = Elem<T>::mma(Rows::row_operand(qt, 0, c, l), kf[c], x);
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) y = Elem<T>::mma(Rows::row_operand(dot, 0, c, l), v(c), y);
+        scores<MOD>(x, back, bend, unit, bias, slope, (float)(row + 4 * h + shift - key), 1.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const floatx4 m = *(const floatx4 *)(lse + 8 * i + 4 * h), d = *(const floatx4 *)(delta + 8 * i + 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[4 * i + j] = __builtin_amdgcn_exp2f(x[4 * i + j] - m[j]);
+                y[4 * i + j] -= d[j];
+            }
+        }
+        if (row < full_lo || row + 32 > full_hi) {
+            const int at = row + 4 * h - lo;
+            const uint32_t span = hi > lo ? hi - lo : 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool seen = (uint32_t)(at + 8 * (r >> 2) + (r & 3)) < span;
+                x[r] = seen ? x[r] : 0.f;
+                y[r] = seen ? y[r] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            y[r] *= x[r];
+            if constexpr (MOD) y[r] *= back[r];
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const Vec8 p = operand<T>(x, c), ds = operand<T>(y, c);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                dv[d] = Elem<T>::mma(Rows::column_operand(dot, d, c, l), p, dv[d]);
+                dk[d] = Elem<T>::mma(Rows::column_operand(qt, d, c, l), ds, dk[d]);
+            }
+        }
+    }
+    // calls f(i, four elements) for the pieces i = 0 .. 8 DB - 1 of a lane's sums: dk, then dv
+    template <class F> __device__ __forceinline__ void pieces(F f) const
+    {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f(4 * d + i, floatx4{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]});
+                f(4 * (DB + d) + i, floatx4{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]});
+            }
+    }
+    static __device__ __forceinline__ void store(const AttnArgs &a, const KeyTile &t, int key, int i, int h, floatx4 y)
+    {
+        typedef typename Elem<T>::Vec4 Vec4;
+        const int col = 8 * (i % (4 * DB)) + 4 * h;
+        if (col >= a.head_dim) return;
+        if (i < 4 * DB) y *= a.scale;
+        T *to = i < 4 * DB ? (T *)k_base<T>(a, a.dk, t.e, t.s, t.kv) + key * a.k_row : (T *)v_base<T>(a, a.dv, t.e, t.s, t.kv) + key * a.v_row;
+        *(Vec4 *)(to + col) = __builtin_convertvector(y, Vec4);
+    }
+};
+
+// dk and dv of 128 keys; the four waves share the tiles of rows.  The query heads that share a key head follow each other in the same sums.
 template <class T, int DP, bool MOD>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : 2)
 void sddmm_attention_dkv_kernel(const AttnArgs a)
 {
-    constexpr int QT = 32, DB = DP / 32;
-    typedef Tile<T, DP, QT> Rows;
+    typedef DkvKeys<T, DP, MOD> Keys;
+    typedef typename Keys::Rows Rows;
     typedef Tile<T, DP, kKeys> Values;
     typedef typename Elem<T>::Vec8 Vec8;
     // (registers: 128 for the sums, 32 for k, 32 for a tile's scores; v would be 32 more than two waves to a SIMD leave)
@@ -129,152 +225,141 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
     __shared__ __align__(16) float stat[2][2][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
 
-    KeyTile at_keys;
+    KeyTile at;
     // (pieces outermost: next to each other they would go to different dies, the later ones, of which there are fewer, always to the same)
     const int groups = gridDim.x / a.n_split, split = blockIdx.x / groups;
-    if (!key_tile(a, blockIdx.x - split * groups, at_keys) || split >= at_keys.pieces) return;
-    const auto [e, s, kv, tile, shift, prefix, any_lo, any_hi, pieces] = at_keys;
-    const int key = tile * kKeys + wave * 32 + n;
-    const bool there = key < e.nk;
-    const int lo = first_row(a, key, prefix, shift), hi = there ? end_row(a, key, shift, e.nq) : 0;
-    const int k0 = tile * kKeys, w0 = k0 + wave * 32, w1 = min(e.nk, w0 + 32) - 1;
-    const int wave_lo = first_row(a, w0, prefix, shift), wave_hi = w1 < w0 ? 0 : end_row(a, w1, shift, e.nq);
-    const int full_lo = first_row(a, max(w1, 0), prefix, shift), full_hi = w1 < w0 + 31 ? 0 : end_row(a, w0, shift, e.nq);
-
-    const int row_bytes = a.head_dim * (int)sizeof(T);
-    Vec8 kf[DP / 16], vf[kKeepV ? DP / 16 : 1];
+    if (!key_tile<kKeys>(a, blockIdx.x - split * groups, at) || split >= at.pieces) return;
+    const int row_bytes = a.head_dim * (int)sizeof(T), k0 = at.tile * kKeys;
+    Keys keys;
+    keys.init(a, at, k0 + 32 * wave, lane);
+    Vec8 vf[kKeepV ? DP / 16 : 1];
     {
-        const T *k = k_base<T>(a, a.k, e, s, kv) + key * a.k_row, *v = v_base<T>(a, a.v, e, s, kv);
-#pragma unroll
-        for (int c = 0; c < DP / 16; ++c) kf[c] = global_operand<T>(k, there, 16 * c + 8 * h, a.head_dim);
+        const T *v = v_base<T>(a, a.v, at.e, at.s, at.kv);
         if constexpr (kKeepV) {
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) vf[c] = global_operand<T>(v + key * a.v_row, there, 16 * c + 8 * h, a.head_dim);
+            for (int c = 0; c < DP / 16; ++c) vf[c] = global_operand<T>(v + keys.key * a.v_row, keys.there, 16 * c + 8 * h, a.head_dim);
         } else {
-            Values::template request<kWaves>(values, (const char *)(v + k0 * a.v_row), (uint32_t)(a.v_row * sizeof(T)), e.nk - k0, row_bytes, wave, lane);
+            Values::template request<kWaves>(values, (const char *)(v + k0 * a.v_row), (uint32_t)(a.v_row * sizeof(T)), at.e.nk - k0, row_bytes, wave, lane);
         }
     }
-    floatx16 dk[DB], dv[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) dk[d] = dv[d] = zero16();
-
-    const float scale = a.scale, unit = scale * kLog2e;
-    Bend bend;
-    if constexpr (MOD) bend.init(scale, a.cap);
-    const int tiles = any_hi > any_lo ? (any_hi - any_lo + QT - 1) / QT : 0, all = tiles * a.group;
-    const int each = (all + pieces - 1) / pieces, first = split * each, last = min(all, first + each);
+    const int tiles = at.any_hi > at.any_lo ? (at.any_hi - at.any_lo + 31) / 32 : 0, all = tiles * a.group;
+    const int each = (all + at.pieces - 1) / at.pieces, first = split * each, last = min(all, first + each);
     const uint32_t q_stride = (uint32_t)(a.q_row * sizeof(T)), o_stride = (uint32_t)(a.o_row * sizeof(T));
     auto request = [&](int t) {
-        const int head = kv * a.group + t / tiles, row = any_lo + t % tiles * QT;
+        const int head = at.kv * a.group + t / tiles, row = at.any_lo + t % tiles * 32;
         char *to = lds[t & 1][0];
-        Rows::template request<kWaves>(to, (const char *)(q_base<T>(a, a.q, e, s, head) + row * a.q_row), q_stride, e.nq - row, row_bytes, wave, lane);
-        Rows::template request<kWaves>(to + Rows::kBytes, (const char *)(o_base<T>(a, a.dout, e, s, head) + row * a.o_row), o_stride, e.nq - row, row_bytes, wave, lane);
-        if (wave < 2) request_floats<QT>(stat[t & 1][wave], (wave ? a.stat_delta : a.stat_lse) + head * a.rows + e.lse0 + row, e.nq - row, lane);
+        Rows::template request<kWaves>(to, (const char *)(q_base<T>(a, a.q, at.e, at.s, head) + row * a.q_row), q_stride, at.e.nq - row, row_bytes, wave, lane);
+        Rows::template request<kWaves>(to + Rows::kBytes, (const char *)(o_base<T>(a, a.dout, at.e, at.s, head) + row * a.o_row), o_stride, at.e.nq - row, row_bytes, wave, lane);
+        if (wave < 2) request_floats<32>(stat[t & 1][wave], (wave ? a.stat_delta : a.stat_lse) + head * a.rows + at.e.lse0 + row, at.e.nq - row, lane);
     };
     if (first < last) request(first);
     for (int t = first; t < last; ++t) {
         tiles_arrived();
         if (t + 1 < last) request(t + 1);
-        const char *qt = lds[t & 1][0], *dot = lds[t & 1][1];
-        const float slope = MOD && a.slopes ? a.slopes[kv * a.group + t / tiles] * kLog2e : 0.f;
-#pragma unroll 1
-        for (int u = 0; u < QT / 32; ++u) {
-            const int row = any_lo + t % tiles * QT + 32 * u;
-            if (row + 32 <= wave_lo || row >= wave_hi) continue;
-            int l = lane;  // (places in LDS made anew in every tile: kept, they would not fit the registers)
-            asm volatile("" : "+v"(l));
-            floatx16 x = zero16(), y = zero16(), back;
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) x = Elem<T>::mma(Rows::row_operand(qt, 32 * u, c, l), kf[c], x);
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) y = Elem<T>::mma(Rows::row_operand(dot, 32 * u, c, l), kKeepV ? vf[kKeepV ? c : 0] : Values::row_operand(values, 32 * wave, c, l), y);
-            scores<MOD>(x, back, bend, unit, a.slopes != nullptr, slope, (float)(row + 4 * h + shift - key), 1.f);
-            const bool masked = row < full_lo || row + 32 > full_hi;
-            const int at = row + 4 * h - lo;
-            const uint32_t span = hi > lo ? hi - lo : 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const floatx4 lse = *(const floatx4 *)&stat[t & 1][0][32 * u + 8 * i + 4 * h], delta = *(const floatx4 *)&stat[t & 1][1][32 * u + 8 * i + 4 * h];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = 4 * i + j;
-                    x[r] = __builtin_amdgcn_exp2f(x[r] - lse[j]);
-                    y[r] -= delta[j];
-                }
-            }
-            if (masked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool seen = (uint32_t)(at + 8 * (r >> 2) + (r & 3)) < span;
-                    x[r] = seen ? x[r] : 0.f;
-                    y[r] = seen ? y[r] : 0.f;
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                y[r] *= x[r];
-                if constexpr (MOD) y[r] *= back[r];
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const Vec8 p = operand<T>(x, c), ds = operand<T>(y, c);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    dv[d] = Elem<T>::mma(Rows::column_operand(dot, d, 2 * u + c, l), p, dv[d]);
-                    dk[d] = Elem<T>::mma(Rows::column_operand(qt, d, 2 * u + c, l), ds, dk[d]);
-                }
-            }
-        }
+        const float slope = MOD && a.slopes ? a.slopes[at.kv * a.group + t / tiles] * kLog2e : 0.f;
+        const int row = at.any_lo + t % tiles * 32;
+        if (!keys.sees(row)) continue;
+        int l = lane;  // (places in LDS made anew in every tile: kept, they would not fit the registers)
+        asm volatile("" : "+v"(l));
+        keys.add(lds[t & 1][0], lds[t & 1][1], stat[t & 1][0], stat[t & 1][1], row, slope, l,
+                 [&](int c) { if constexpr (kKeepV) return vf[c]; else return Values::row_operand(values, 32 * wave, c, l); });
     }
-#pragma unroll
-    for (int d = 0; d < DB; ++d) dk[d] *= scale;
-    if (pieces > 1) {
-        // parts of dk and dv as they lie in the registers: [part][workgroup][wave][element of the lane / 4][lane] of 16 bytes
-        floatx4 *to = (floatx4 *)a.part_o + ((int64_t)blockIdx.x * kWaves + wave) * (8 * DB * 64) + lane;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                to[(4 * d + i) * 64] = floatx4{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]};
-                to[(4 * (DB + d) + i) * 64] = floatx4{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]};
-            }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // (where there were no rows v may still be under way to LDS)
+    if (at.pieces > 1) {
+        // parts of dk and dv as they lie in the registers: [part][workgroup][wave][piece][lane] of 16 bytes
+        floatx4 *to = (floatx4 *)a.part_o + ((int64_t)blockIdx.x * kWaves + wave) * (8 * Keys::DB * 64) + lane;
+        keys.pieces([&](int i, floatx4 y) { to[i * 64] = y; });
         return;
     }
-    if (!there) return;
-    typedef typename Elem<T>::Vec4 Vec4;
-    T *to = (T *)k_base<T>(a, a.dk, e, s, kv) + key * a.k_row, *to_v = (T *)v_base<T>(a, a.dv, e, s, kv) + key * a.v_row;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int col = 32 * d + 8 * i + 4 * h;
-            if (col >= a.head_dim) continue;
-            *(Vec4 *)(to + col) = __builtin_convertvector((floatx4{dk[d][4 * i], dk[d][4 * i + 1], dk[d][4 * i + 2], dk[d][4 * i + 3]}), Vec4);
-            *(Vec4 *)(to_v + col) = __builtin_convertvector((floatx4{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]}), Vec4);
-        }
+    if (!keys.there) return;
+    keys.pieces([&](int i, floatx4 y) { Keys::store(a, at, k0 + 32 * wave + n, i, h, y); });
 }
 
-// The sum of the parts of dk and dv of the keys whose rows were cut: a workgroup for the keys of a wave.
-template <class T, int DP>
+// The same where workgroups of 128 keys would leave most compute units without work: 32 keys to a workgroup, each wave on every NW-th tile of rows, in LDS of
+// its own and without a barrier; sums are joined at the end.
+template <class T, int DP, bool MOD, int NW>
+__global__ __launch_bounds__(64 * NW, 1)
+void sddmm_attention_dkv_few_kernel(const AttnArgs a)
+{
+    typedef DkvKeys<T, DP, MOD> Keys;
+    typedef typename Keys::Rows Rows;
+    typedef typename Elem<T>::Vec8 Vec8;
+    constexpr int kLoads = 2 * Rows::kBytes / 1024 + 2;
+    __shared__ __align__(1024) char lds[NW][2][2][Rows::kBytes];
+    __shared__ __align__(16) float stat[NW][2][2][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+    KeyTile at;
+    const int groups = gridDim.x / a.n_split, split = blockIdx.x / groups;
+    if (!key_tile<kFewKeys>(a, blockIdx.x - split * groups, at) || split >= at.pieces) return;
+    const int row_bytes = a.head_dim * (int)sizeof(T), k0 = at.tile * kFewKeys;
+    const int tiles = at.any_hi > at.any_lo ? (at.any_hi - at.any_lo + 31) / 32 : 0, all = tiles * a.group;
+    const int each = (all + at.pieces - 1) / at.pieces, first = split * each, last = min(all, first + each);
+    const uint32_t q_stride = (uint32_t)(a.q_row * sizeof(T)), o_stride = (uint32_t)(a.o_row * sizeof(T));
+    // (behind the last tile nothing is read, but the requests are made, so that the waits count the same)
+    auto request = [&](int t, int turn) {
+        const bool more = t < last;
+        const int head = more ? at.kv * a.group + t / tiles : 0, row = more ? at.any_lo + t % tiles * 32 : 0, valid = more ? at.e.nq - row : 0;
+        const int64_t stats = head * a.rows + at.e.lse0 + row;
+        Rows::template request<1>(lds[wave][turn][0], (const char *)(q_base<T>(a, a.q, at.e, at.s, head) + row * a.q_row), q_stride, valid, row_bytes, 0, lane);
+        Rows::template request<1>(lds[wave][turn][1], (const char *)(o_base<T>(a, a.dout, at.e, at.s, head) + row * a.o_row), o_stride, valid, row_bytes, 0, lane);
+        request_floats<32>(stat[wave][turn][0], a.stat_lse + stats, valid, lane);
+        request_floats<32>(stat[wave][turn][1], a.stat_delta + stats, valid, lane);
+    };
+    request(first + wave, 0);
+    Keys keys;
+    keys.init(a, at, k0, lane);
+    Vec8 vf[DP / 16];
+    const T *v = v_base<T>(a, a.v, at.e, at.s, at.kv) + keys.key * a.v_row;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) vf[c] = global_operand<T>(v, keys.there, 16 * c + 8 * h, a.head_dim);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // the first tile and the keys: from here on only tiles are under way
+    for (int t = first + wave, turn = 0; t < last; t += NW, turn ^= 1) {
+        request(t + NW, turn ^ 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+        const float slope = MOD && a.slopes ? a.slopes[at.kv * a.group + t / tiles] * kLog2e : 0.f;
+        const int row = at.any_lo + t % tiles * 32;
+        if (!keys.sees(row)) continue;
+        keys.add(lds[wave][turn][0], lds[wave][turn][1], stat[wave][turn][0], stat[wave][turn][1], row, slope, lane, [&](int c) { return vf[c]; });
+#pragma unroll
+        for (int d = 0; d < Keys::DB; ++d) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(keys.dk[d]), "+v"(keys.dv[d]) :: "memory");
+    }
+    // join the waves: [piece][lane] of 16 bytes for each
+    static_assert(4 * Rows::kBytes >= 256 * DP);
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    floatx4 *mine = (floatx4 *)lds[wave][0][0];
+    keys.pieces([&](int i, floatx4 y) { mine[i * 64 + lane] = y; });
+    __syncthreads();
+    floatx4 *part = (floatx4 *)a.part_o + (int64_t)blockIdx.x * (8 * Keys::DB * 64) + lane;
+#pragma unroll
+    for (int j = 0; j < 8 * Keys::DB / NW; ++j) {
+        const int i = wave * (8 * Keys::DB / NW) + j;
+        floatx4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) y += ((const floatx4 *)lds[w][0][0])[i * 64 + lane];
+        if (at.pieces > 1) part[i * 64] = y;
+        else if (keys.there) Keys::store(a, at, k0 + n, i, h, y);
+    }
+}
+
+// The sum of the parts of dk and dv of the keys whose rows were cut: a workgroup for 32 keys.
+template <class T, int DP, int KEYS>
 __global__ __launch_bounds__(256)
 void sddmm_attention_dkv_sum_kernel(const AttnArgs a)
 {
-    constexpr int DB = DP / 32;
+    typedef DkvKeys<T, DP, false> Keys;
     KeyTile at;
-    if (!key_tile(a, blockIdx.x / kWaves, at) || at.pieces == 1) return;
-    const int wave = blockIdx.x % kWaves, lane = threadIdx.x & 63, key = at.tile * kKeys + wave * 32 + (lane & 31);
+    if (!key_tile<KEYS>(a, blockIdx.x / (KEYS / 32), at) || at.pieces == 1) return;
+    const int lane = threadIdx.x & 63, key = at.tile * KEYS + blockIdx.x % (KEYS / 32) * 32 + (lane & 31);
     if (key >= at.e.nk) return;
-    const int64_t part = (int64_t)gridDim.x * (8 * DB * 64);
-    T *to = (T *)k_base<T>(a, a.dk, at.e, at.s, at.kv) + key * a.k_row, *to_v = (T *)v_base<T>(a, a.dv, at.e, at.s, at.kv) + key * a.v_row;
+    const int64_t part = (int64_t)gridDim.x * (8 * Keys::DB * 64);
 #pragma unroll
-    for (int j = 0; j < 2 * DB; ++j) {
-        const int i = j * 4 + (threadIdx.x >> 6), col = 8 * (i % (4 * DB)) + 4 * (lane >> 5);
-        const floatx4 *from = (const floatx4 *)a.part_o + ((int64_t)blockIdx.x * (8 * DB) + i) * 64 + lane;
+    for (int j = 0; j < 2 * Keys::DB; ++j) {
+        const int i = j * 4 + (threadIdx.x >> 6);
+        const floatx4 *from = (const floatx4 *)a.part_o + ((int64_t)blockIdx.x * (8 * Keys::DB) + i) * 64 + lane;
         floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int p = 0; p < at.pieces; ++p) x += from[p * part];
-        typedef typename Elem<T>::Vec4 Vec4;
-        if (col < a.head_dim) *(Vec4 *)((i < 4 * DB ? to : to_v) + col) = __builtin_convertvector(x, Vec4);
+        Keys::store(a, at, key, i, lane >> 5, x);
     }
 }
 
@@ -607,41 +692,40 @@ void sddmm_attention_dslopes_kernel(const AttnArgs a)
 }
 
 template <class T, int DP>
-hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, unsigned q_grid, int q_rows, hipStream_t st)
+hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, int keys, unsigned q_grid, int q_rows, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
     constexpr int kPer = 256 / (DP / 8), NW = sizeof(T) == 4 && DP == 128 ? 2 : 4;
     const auto dkv = mod ? sddmm_attention_dkv_kernel<T, DP, true> : sddmm_attention_dkv_kernel<T, DP, false>;
+    const auto dkv_few = mod ? sddmm_attention_dkv_few_kernel<T, DP, true, NW> : sddmm_attention_dkv_few_kernel<T, DP, false, NW>;
+    const auto sum = keys == kKeys ? sddmm_attention_dkv_sum_kernel<T, DP, kKeys> : sddmm_attention_dkv_sum_kernel<T, DP, kFewKeys>;
     const auto dq = q_rows == 64 ? (mod ? sddmm_attention_dq_kernel<T, DP, true, 2> : sddmm_attention_dq_kernel<T, DP, false, 2>)
                                  : (mod ? sddmm_attention_dq_kernel<T, DP, true, 4> : sddmm_attention_dq_kernel<T, DP, false, 4>);
     const auto dq_few = mod ? sddmm_attention_dq_few_kernel<T, DP, true, NW> : sddmm_attention_dq_few_kernel<T, DP, false, NW>;
     hipError_t e = hipSuccess;
     if (q_grid) e = launch(sddmm_attention_stats_kernel<T, DP>, dim3((unsigned)((a.rows * a.n_heads + kPer - 1) / kPer)), dim3(256), 0, st, a);
-    if (e == hipSuccess && kv_grid) e = launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a);
-    if (e == hipSuccess && kv_grid && a.n_split > 1)
-        e = launch(sddmm_attention_dkv_sum_kernel<T, DP>, dim3(kv_grid / a.n_split * kWaves), dim3(256), 0, st, a);
+    if (e == hipSuccess && kv_grid) e = keys == kKeys ? launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a) : launch(dkv_few, dim3(kv_grid), dim3(64 * NW), 0, st, a);
+    if (e == hipSuccess && kv_grid && a.n_split > 1) e = launch(sum, dim3(kv_grid / a.n_split * (keys / 32)), dim3(256), 0, st, a);
     if (e == hipSuccess && q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * NW), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
     if (e == hipSuccess && a.dslopes) e = launch(sddmm_attention_dslopes_kernel, dim3((unsigned)a.n_heads), dim3(256), 0, st, b);
     return e;
 }
 
 template <class T>
-hipError_t launch_dims(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, unsigned q_grid, int q_rows, hipStream_t st)
+hipError_t launch_dims(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, int keys, unsigned q_grid, int q_rows, hipStream_t st)
 {
     if constexpr (sizeof(T) == 4) {
-        if (a.head_dim <= 32) return launch_typed<T, 32>(a, b, kv_grid, q_grid, q_rows, st);
+        if (a.head_dim <= 32) return launch_typed<T, 32>(a, b, kv_grid, keys, q_grid, q_rows, st);
     }
-    return a.head_dim <= 64 ? launch_typed<T, 64>(a, b, kv_grid, q_grid, q_rows, st) : launch_typed<T, 128>(a, b, kv_grid, q_grid, q_rows, st);
+    return a.head_dim <= 64 ? launch_typed<T, 64>(a, b, kv_grid, keys, q_grid, q_rows, st) : launch_typed<T, 128>(a, b, kv_grid, keys, q_grid, q_rows, st);
 }
 
 }  // namespace
 
-int attention_backward_keys() { return kKeys; }
-
-hipError_t launch_attention_backward(const AttnArgs &a, const AttnArgs &b, int type, unsigned kv_grid, unsigned q_grid, int q_rows, hipStream_t st)
+hipError_t launch_attention_backward(const AttnArgs &a, const AttnArgs &b, int type, unsigned kv_grid, int keys, unsigned q_grid, int q_rows, hipStream_t st)
 {
-    return type == SDDMM_TYPE_F32 ? launch_dims<float>(a, b, kv_grid, q_grid, q_rows, st)
-         : type == SDDMM_TYPE_F16 ? launch_dims<_Float16>(a, b, kv_grid, q_grid, q_rows, st) : launch_dims<__bf16>(a, b, kv_grid, q_grid, q_rows, st);
+    return type == SDDMM_TYPE_F32 ? launch_dims<float>(a, b, kv_grid, keys, q_grid, q_rows, st)
+         : type == SDDMM_TYPE_F16 ? launch_dims<_Float16>(a, b, kv_grid, keys, q_grid, q_rows, st) : launch_dims<__bf16>(a, b, kv_grid, keys, q_grid, q_rows, st);
 }
 
 }  // namespace sddmm
