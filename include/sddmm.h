@@ -533,8 +533,10 @@ int sddmm_csr_noalloc(int64_t n_rows, int64_t n_cols, int64_t nnz, const int32_t
  * written.  lse: fp32, n_heads to a row, rows in the order of q_ptr or s * max_q + i.
  *
  * Operands: n_heads a multiple of n_kv_heads; head_dim a multiple of 8 up to 128;
- * every pointer and stride a multiple of 16 bytes; a row's stride at least its
- * length and below 2^23 bytes; scale finite and above 0, cap finite.  Products are
+ * every pointer to rows and every stride a multiple of 16 bytes; a row's stride at
+ * least its length and below 2^23 bytes; scale finite and above 0, cap finite, neither
+ * 10^30 times the other.  Heads and sequences of operands may share memory (a stride of
+ * 0); of results they may not, and no result may lie in an operand's place.  Products are
  * summed in fp32, statistics kept in fp32; 16-bit operands: the probabilities (and,
  * backwards, their gradients) are rounded to the operands' type before they are
  * multiplied, as results are; fp32 operands: no rounding below fp32.  Infinities and
@@ -544,7 +546,8 @@ int sddmm_csr_noalloc(int64_t n_rows, int64_t n_cols, int64_t nnz, const int32_t
  * and k_ptr must rise from 0 and end at q_rows and k_rows at most; q_len and k_len
  * are taken as 0 .. max_q and 0 .. max_k.
  *
- * Calls allocate nothing, launch on `stream` only and may be captured into a graph.
+ * Calls allocate nothing, launch on `stream` only (a stream of the current device) and
+ * may be captured into a graph.
  * d_workspace: sddmm_attention_workspace_bytes of device memory, 256-byte aligned, for
  * the time of the call; calls that overlap in time need one each, and a graph keeps
  * using the one that it was captured with.                                       */
@@ -587,7 +590,7 @@ int sddmm_attention_shared(const sddmm_attention_desc *desc, const void *d_q, co
 /* Gradients of sum(out * d_out) by q, k and v (each laid out as its operand, d_dout as out), and by the slopes (d_dslopes, [n_heads] fp32;
  * NULL: not wanted).  d_out and d_lse are what sddmm_attention_forward left for the same description and operands.  They are
  * overwritten, not added to; a key head's are the sums over the query heads that share it, keys that no row sees get 0.
- * No atomics: the same bits on every call.  No gradient may lie in an operand's place.  */
+ * No atomics: the same bits on every call.  */
 int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, const void *d_k, const void *d_v, const void *d_out,
                              const float *d_lse, const void *d_dout, void *d_dq, void *d_dk, void *d_dv, float *d_dslopes,
                              void *d_workspace, int64_t workspace_bytes, void *stream);

@@ -27,6 +27,21 @@ bool strides_fit(const sddmm_attention_desc &d, int64_t seq, int64_t row, int64_
            head >= 0 && (packed || seq >= 0);
 }
 
+// Whether no two rows of an array that is written lie in each other's place (broadcast operands have strides of 0).
+bool apart(const sddmm_attention_desc &d, int64_t seq, int64_t row, int64_t head, int64_t n_seq, int64_t n_rows, int64_t n_heads)
+{
+    std::pair<int64_t, int64_t> dims[3] = {{row, n_rows}, {head, n_heads}, {seq, n_seq}};
+    if (n_seq == 0 || n_rows == 0) return true;
+    std::sort(dims, dims + 3);
+    int64_t extent = d.head_dim;
+    for (const auto &[stride, n] : dims) {
+        if (n <= 1) continue;
+        if (stride < extent) return false;
+        extent += (n - 1) * stride;
+    }
+    return true;
+}
+
 int check_desc(const char *who, const sddmm_attention_desc *p)
 {
     if (!p) return fail(SDDMM_ERR_ARG, "%s: NULL description", who);
@@ -40,10 +55,13 @@ int check_desc(const char *who, const sddmm_attention_desc *p)
     if (d.window_left < -1 || d.window_right < -1) return fail(SDDMM_ERR_ARG, "%s: a window below -1", who);
     if (!std::isfinite(d.scale) || !(d.scale > 0.f)) return fail(SDDMM_ERR_ARG, "%s: scale must be finite and above 0", who);
     if (!std::isfinite(d.cap) || d.cap < 0.f) return fail(SDDMM_ERR_ARG, "%s: cap must be finite and not negative", who);
+    if (d.cap > 0.f && !(d.scale / d.cap > 1e-30f && d.scale / d.cap < 1e30f && d.cap < 1e30f)) return fail(SDDMM_ERR_ARG, "%s: cap and scale are too far apart", who);
     if ((d.q_ptr && d.q_len) || (d.k_ptr && d.k_len)) return fail(SDDMM_ERR_ARG, "%s: lengths beside the pointers of packed sequences", who);
     if (!strides_fit(d, d.q_seq, d.q_row, d.q_head, d.q_ptr) || !strides_fit(d, d.k_seq, d.k_row, d.k_head, d.k_ptr) ||
         !strides_fit(d, d.v_seq, d.v_row, d.v_head, d.k_ptr) || !strides_fit(d, d.o_seq, d.o_row, d.o_head, d.q_ptr))
         return fail(SDDMM_ERR_ARG, "%s: strides must be multiples of 16 bytes, a row's from head_dim to 2^23 bytes", who);
+    for (const void *p : {(const void *)d.q_ptr, (const void *)d.k_ptr, (const void *)d.q_len, (const void *)d.k_len, (const void *)d.prefix, (const void *)d.slopes})
+        if ((uintptr_t)p & 3u) return fail(SDDMM_ERR_ARG, "%s: arrays of the description must be aligned to their elements", who);
     const int64_t rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
     if (rows > kMostRows || d.k_rows > kMostRows || (int64_t)d.shared_len + d.max_k > kMostRows / 2 || d.max_q > kMostRows / 2)
         return fail(SDDMM_ERR_RANGE, "%s: sizes beyond 32-bit positions", who);
@@ -191,7 +209,8 @@ AttnArgs arguments(const sddmm_attention_desc &d)
     a.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
     a.key_rows = d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k;
     a.head_dim = d.head_dim, a.n_heads = d.n_heads, a.n_kv_heads = d.n_kv_heads, a.group = d.n_heads / d.n_kv_heads;
-    a.n_seq = d.n_seq, a.max_q = d.max_q, a.max_k = d.max_k, a.left = d.window_left, a.right = d.window_right, a.shared_len = d.shared_len;
+    a.n_seq = d.n_seq, a.max_q = d.max_q, a.max_k = d.max_k, a.left = std::min(d.window_left, 1 << 30), a.right = std::min(d.window_right, 1 << 30),  // (positions are below)
+    a.shared_len = d.shared_len;
     a.scale = d.scale, a.cap = d.cap;
     return a;
 }
@@ -211,6 +230,8 @@ int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d
     if (r.rows == 0 || d.n_seq == 0) return SDDMM_OK;
     const bool keys = d.k_ptr ? d.k_rows > 0 : d.max_k > 0;
     if (!d_q || !d_out || (keys && (!d_k || !d_v)) || (d.shared_len && (!d_shared_k || !d_shared_v))) return fail(SDDMM_ERR_ARG, "%s: NULL device pointer", who);
+    if (!apart(d, d.o_seq, d.o_row, d.o_head, d.q_ptr ? 1 : d.n_seq, d.q_ptr ? d.q_rows : d.max_q, d.n_heads)) return fail(SDDMM_ERR_ARG, "%s: rows of the result overlap", who);
+    if ((uintptr_t)d_lse & 3u) return fail(SDDMM_ERR_ARG, "%s: lse must be aligned to its elements", who);
     if (!aligned({d_q, d_k, d_v, d_out, d_shared_k, d_shared_v})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
@@ -286,6 +307,11 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
     if (d.n_seq == 0 || (r.rows == 0 && r.key_rows == 0 && !d_dslopes)) return SDDMM_OK;
     if ((r.rows > 0 && (!d_q || !d_out || !d_lse || !d_dout || !d_dq)) || (r.key_rows > 0 && (!d_k || !d_v || !d_dk || !d_dv)))
         return fail(SDDMM_ERR_ARG, "%s: NULL device pointer", who);
+    const int64_t q_seqs = d.q_ptr ? 1 : d.n_seq, k_seqs = d.k_ptr ? 1 : d.n_seq, q_rows = d.q_ptr ? d.q_rows : d.max_q, k_rows = d.k_ptr ? d.k_rows : d.max_k;
+    if (!apart(d, d.q_seq, d.q_row, d.q_head, q_seqs, q_rows, d.n_heads) || !apart(d, d.k_seq, d.k_row, d.k_head, k_seqs, k_rows, d.n_kv_heads) ||
+        !apart(d, d.v_seq, d.v_row, d.v_head, k_seqs, k_rows, d.n_kv_heads))
+        return fail(SDDMM_ERR_ARG, "%s: rows of a gradient overlap", who);
+    if (((uintptr_t)d_lse | (uintptr_t)d_dslopes) & 3u) return fail(SDDMM_ERR_ARG, "%s: lse and d_dslopes must be aligned to their elements", who);
     if (!aligned({d_q, d_k, d_v, d_out, d_dout, d_dq, d_dk, d_dv})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);

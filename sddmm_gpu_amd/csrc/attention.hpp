@@ -305,21 +305,20 @@ __device__ __forceinline__ int end_key(const AttnArgs &a, int pos, int prefix, i
 }
 
 // The bound of scores: cap tanh(t / cap), t = scale * product, of N results in registers, in powers of two (BACK: and 1 - tanh^2 of each).
-// Where all of the wave's |t / cap| are 0.25 at most, which they mostly are, by powers: x (C0 + C1 x^2 + ...), six instructions where 1 - 2 / (1 + e^2y) takes
+// Where all of the wave's |t / cap| are 0.25 at most, which they mostly are, by powers, seven instructions where 1 - 2 / (1 + e^2y) takes
 // two of the slow kind and as many others, and to the last place, since that difference loses 24 bits below 1 (the next term is 1e-8 of the result).
 struct Bend {
-    float limit, c0, c1, c2, c3, c4, twice, to, cap;
+    float limit, by, twice, to, cap;
     __device__ __forceinline__ void init(float scale, float cap_)
     {
         cap = cap_;
-        const float by = cap > 0.f ? scale / cap : 0.f, s = by * by;
+        by = cap > 0.f ? scale / cap : 0.f;
         to = cap * kLog2e, twice = by * (2.f * kLog2e), limit = cap > 0.f ? 0.25f / by : 0.f;
-        c0 = by, c1 = c0 * s * -0.33333334f, c2 = c0 * s * s * 0.13333334f, c3 = c0 * s * s * s * -0.053968254f, c4 = c0 * s * s * s * s * 0.021869489f;
     }
     __device__ __forceinline__ float near(float x) const
     {
-        const float s = x * x;
-        return x * fmaf(s, fmaf(s, fmaf(s, fmaf(s, c4, c3), c2), c1), c0);
+        const float y = x * by, s = y * y;
+        return y * fmaf(s, fmaf(s, fmaf(s, fmaf(s, 0.021869489f, -0.053968254f), 0.13333334f), -0.33333334f), 1.f);
     }
     template <int N, bool BACK>
     __device__ __forceinline__ void apply(floatx16 (&x)[N], floatx16 (&back)[N]) const

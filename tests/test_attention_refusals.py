@@ -6,6 +6,9 @@ from sddmm_gpu_amd import capi
 A = 1 << 20  # an address: aligned, never read
 
 
+HUGE = dict(q_row=64, q_head=1 << 18, q_seq=1 << 34, o_row=64, o_head=1 << 18, o_seq=1 << 34)  # of 2^18 sequences of 2^12 rows of 65536 heads
+
+
 def desc(**kw):
     d = dict(type=capi.TYPE_BF16, n_seq=2, n_heads=4, n_kv_heads=2, head_dim=64, max_q=100, max_k=100)
     d.update(kw)
@@ -24,6 +27,8 @@ BAD = [
     (dict(window_left=-2), "window"), (dict(window_right=-7), "window"),
     (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(cap=-1.0), "cap"), (dict(cap=float("inf")), "cap"), (dict(cap=float("nan")), "cap"),
+    (dict(cap=1e-31, scale=1.0), "too far apart"), (dict(cap=1e31, scale=1.0), "too far apart"), (dict(cap=1.0, scale=1e-31), "too far apart"),
+    (dict(q_ptr=A + 2, q_rows=200), "aligned"), (dict(k_len=A + 1), "aligned"), (dict(slopes=A + 2), "aligned"), (dict(prefix=A + 3), "aligned"),
     (dict(q_ptr=A, q_len=A), "lengths beside"), (dict(k_ptr=A, k_len=A), "lengths beside"),
     (dict(q_row=60), "strides"), (dict(k_row=63 * 4 + 1), "strides"), (dict(v_head=12), "strides"), (dict(o_row=1 << 23), "strides"),
     (dict(k_seq=4), "strides"), (dict(q_head=-64), "strides"), (dict(q_seq=-1024), "strides"),
@@ -44,7 +49,7 @@ def test_sizes_beyond_positions():
             forward(desc(**kw))
         assert e.value.code == capi.ERR_RANGE
     with pytest.raises(capi.SddmmError, match="one launch") as e:
-        forward(desc(n_seq=1 << 18, max_q=1 << 12, n_heads=65536, n_kv_heads=1, q_seq=64, o_seq=64, q_row=64, o_row=64))
+        forward(desc(n_seq=1 << 18, max_q=1 << 12, n_heads=65536, n_kv_heads=1, **HUGE))
     assert e.value.code == capi.ERR_RANGE
 
 
@@ -57,6 +62,19 @@ def test_pointers():
             forward(desc(), **kw)
     with pytest.raises(capi.SddmmError, match="NULL description"):
         capi.check(capi.lib().sddmm_attention_forward(None, A, A, A, A, None, None, 0, None))
+
+
+def test_results_must_not_overlap():
+    for kw in (dict(o_head=0), dict(o_seq=0), dict(o_row=64), dict(o_seq=64), dict(o_head=32), dict(q_ptr=A, q_rows=200, o_head=0)):
+        with pytest.raises(capi.SddmmError, match="overlap"):
+            forward(desc(**kw))
+    for kw in (dict(q_head=0), dict(k_seq=0), dict(v_head=0), dict(k_row=64), dict(q_seq=64)):
+        with pytest.raises(capi.SddmmError, match="rows of a gradient overlap"):
+            backward(desc(**kw))
+    with pytest.raises(capi.SddmmError, match="lse"):
+        forward(desc(), lse=A + 2)
+    with pytest.raises(capi.SddmmError, match="lse"):
+        backward(desc(), lse=A + 1)
 
 
 def test_workspace():
@@ -111,6 +129,6 @@ def test_backward():
         with pytest.raises(capi.SddmmError, match="workspace"):
             backward(desc(), **kw)
     with pytest.raises(capi.SddmmError, match="one launch"):
-        backward(desc(n_seq=1 << 18, max_q=1 << 12, n_heads=65536, n_kv_heads=1, q_seq=64, o_seq=64, q_row=64, o_row=64), n=1 << 62)
+        backward(desc(n_seq=1 << 18, max_q=1 << 12, n_heads=65536, n_kv_heads=1, **HUGE), n=1 << 62)
     backward(desc(n_seq=0), *[0] * 9)
     backward(desc(max_q=0, max_k=0), *[0] * 9)

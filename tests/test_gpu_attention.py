@@ -185,3 +185,90 @@ def test_packed_pairs(dtype, lens, heads, kv, dim, left):
 ])
 def test_shared(dtype, lens, shared, heads, kv, dim, left, cap, bias, prefix):
     Case(dtype, lens, heads, kv, dim, left, 0, cap=cap, bias=bias, prefix=prefix, packed=False, shared=shared).run().check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_of_any_size(dtype):
+    """Scores that rise and fall by hundreds along the keys (the running maximum is raised again and again, and never), and a row that one key
+    decides: probabilities of 2^-100 beside it."""
+    for order in (1, -1):
+        c = Case(dtype, [(140, 500)], 2, 1, 64, -1, 0, scale=1.0)
+        c.k[:500] = (c.k[:500].float() * torch.linspace(0.1, 6, 500).flip(0 if order < 0 else ())[:, None, None]).to(dtype) if order < 0 else (
+            c.k[:500].float() * torch.linspace(0.1, 6, 500)[:, None, None]).to(dtype)
+        c.run().check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinities_and_nans(dtype):
+    """Keys that a row does not see may hold anything; a NaN in a key that it sees makes its row NaN and no other."""
+    c = Case(dtype, [(200, 200)], 1, 1, 64, -1, 0)
+    c.k[150], c.k[160], c.k[199] = math.nan, math.inf, -math.inf
+    c.run()
+    good = Case(dtype, [(200, 200)], 1, 1, 64, -1, 0).run()
+    assert torch.equal(c.out[:150], good.out[:150])
+    assert torch.isnan(c.out[150:200]).all()
+    # one token: what lies before its window or behind its cache is not read
+    for left in (-1, 20):
+        c = Case(dtype, [(1, 100)], 2, 1, 64, left, 0, packed=False)
+        if left >= 0:
+            c.k[0, :100 - 1 - left], c.v[0, :100 - 1 - left] = math.nan, math.inf
+        c.run()
+        assert torch.isfinite(c.out).all()
+
+
+def test_broadcast_operands_and_orders():
+    """Heads-first arrays, keys of one sequence for all (a stride of 0), one head of q for all."""
+    n, mq, mk, heads, kv, dim = 3, 70, 90, 4, 2, 64
+    q, k, v = normal(1, n, heads, mq, dim, dtype=BF16), normal(2, kv, mk, dim, dtype=BF16), normal(3, kv, mk, dim, dtype=BF16)
+    qd, kd, vd = (x.to(DEV) for x in (q, k, v))
+    for one_head in (False, True):
+        out = torch.full((n, mq, heads, dim), 5.0, dtype=BF16, device=DEV)
+        d = capi.AttentionDesc.packed(capi.TYPE_BF16, n, heads, kv, dim, max_q=mq, max_k=mk, window_right=0, q_seq=heads * mq * dim, q_head=0 if one_head else mq * dim,
+                                      q_row=dim, k_seq=0, k_head=mk * dim, k_row=dim, v_seq=0, v_head=mk * dim, v_row=dim)
+        ws = torch.empty(capi.attention_workspace_bytes(d)[0] + 256, dtype=torch.uint8, device=DEV)
+        capi.attention_forward(d, qd.data_ptr(), kd.data_ptr(), vd.data_ptr(), out.data_ptr(), 0, ws.data_ptr(), ws.numel())
+        torch.cuda.synchronize()
+        for s in range(n):
+            for h in range(heads):
+                r = ref.head(q[s, 0 if one_head else h], k[h // 2], v[h // 2], -1, 0, 0, dim ** -0.5, 0.0, 0.0)
+                assert ((out[s, :, h].cpu().double() - r["out"]).abs() <= r["out_tol"]).all()
+
+
+def test_offsets_beyond_32_bits():
+    """A cache whose second sequence begins behind 2^32 bytes and 2^31 elements, rows of it 4 MB apart."""
+    heads, kv, dim, keys, row = 4, 2, 64, 600, 1 << 21
+    k = torch.zeros(2 * keys * row, dtype=BF16, device=DEV)
+    some = normal(4, 2, keys, kv, 2, dim, dtype=BF16)
+    at = torch.arange(2 * keys, device=DEV).view(2, keys, 1, 1, 1) * row + torch.arange(kv, device=DEV).view(kv, 1, 1) * 2 * dim + torch.arange(2, device=DEV).view(2, 1) * dim + torch.arange(dim, device=DEV)
+    k[at.view(-1)] = some.to(DEV).view(-1)
+    for mq in (1, 150):
+        q = normal(5, 2, mq, heads, dim, dtype=BF16)
+        qd, out = q.to(DEV), torch.empty(2, mq, heads, dim, dtype=BF16, device=DEV)
+        d = capi.AttentionDesc.packed(capi.TYPE_BF16, 2, heads, kv, dim, max_q=mq, max_k=keys, window_right=0, k_seq=keys * row, k_row=row, k_head=2 * dim, v_seq=keys * row,
+                                      v_row=row, v_head=2 * dim)
+        ws = torch.empty(capi.attention_workspace_bytes(d)[0] + 256, dtype=torch.uint8, device=DEV)
+        capi.attention_forward(d, qd.data_ptr(), k.data_ptr(), k.data_ptr() + 2 * dim, out.data_ptr(), 0, ws.data_ptr(), ws.numel())
+        torch.cuda.synchronize()
+        for s in range(2):
+            for h in range(heads):
+                r = ref.head(q[s, :, h], some[s, :, h // 2, 0], some[s, :, h // 2, 1], -1, 0, 0, dim ** -0.5, 0.0, 0.0)
+                assert ((out[s, :, h].cpu().double() - r["out"]).abs() <= r["out_tol"]).all()
+
+
+def test_two_streams_at_once():
+    """Calls that overlap in time, a workspace each: the bits of calls one after the other."""
+    cases = [Case(BF16, [(1, 3000 + 100 * i), (1, 500)], 8, 2, 128, -1, 0, packed=False, seed=10 * i) for i in range(4)]
+    want = [c.run().out.clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    held = []
+    for c in cases:
+        q, k, v = (x.to(DEV) for x in (c.q, c.k, c.v))
+        n = capi.attention_workspace_bytes(c.desc)[0]
+        held.append((q, k, v, torch.full_like(q, c.MARK), torch.empty(n, dtype=torch.uint8, device=DEV), n))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, s, (q, k, v, out, ws, n) in zip(cases, streams, held):
+            capi.attention_forward(c.desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, ws.data_ptr(), n, s.cuda_stream)
+    torch.cuda.synchronize()
+    for w, h in zip(want, held):
+        assert torch.equal(w, h[3])
