@@ -535,7 +535,7 @@ int sddmm_csr_noalloc(int64_t n_rows, int64_t n_cols, int64_t nnz, const int32_t
  * Operands: n_heads a multiple of n_kv_heads; head_dim a multiple of 8 up to 128;
  * every pointer to rows and every stride a multiple of 16 bytes; a row's stride at
  * least its length and below 2^23 bytes; scale finite and above 0, cap finite, neither
- * 10^30 times the other.  Heads and sequences of operands may share memory (a stride of
+ * 10^15 times the other.  Heads and sequences of operands may share memory (a stride of
  * 0); of results they may not, and no result may lie in an operand's place.  Products are
  * summed in fp32, statistics kept in fp32; 16-bit operands: the probabilities (and,
  * backwards, their gradients) are rounded to the operands' type before they are

@@ -55,7 +55,7 @@ int check_desc(const char *who, const sddmm_attention_desc *p)
     if (d.window_left < -1 || d.window_right < -1) return fail(SDDMM_ERR_ARG, "%s: a window below -1", who);
     if (!std::isfinite(d.scale) || !(d.scale > 0.f)) return fail(SDDMM_ERR_ARG, "%s: scale must be finite and above 0", who);
     if (!std::isfinite(d.cap) || d.cap < 0.f) return fail(SDDMM_ERR_ARG, "%s: cap must be finite and not negative", who);
-    if (d.cap > 0.f && !(d.scale / d.cap > 1e-30f && d.scale / d.cap < 1e30f && d.cap < 1e30f)) return fail(SDDMM_ERR_ARG, "%s: cap and scale are too far apart", who);
+    if (d.cap > 0.f && !(d.scale / d.cap > 1e-15f && d.scale / d.cap < 1e15f && d.cap < 1e30f)) return fail(SDDMM_ERR_ARG, "%s: cap and scale are too far apart", who);
     if ((d.q_ptr && d.q_len) || (d.k_ptr && d.k_len)) return fail(SDDMM_ERR_ARG, "%s: lengths beside the pointers of packed sequences", who);
     if (!strides_fit(d, d.q_seq, d.q_row, d.q_head, d.q_ptr) || !strides_fit(d, d.k_seq, d.k_row, d.k_head, d.k_ptr) ||
         !strides_fit(d, d.v_seq, d.v_row, d.v_head, d.k_ptr) || !strides_fit(d, d.o_seq, d.o_row, d.o_head, d.q_ptr))
@@ -115,7 +115,7 @@ Deal deal(const sddmm_attention_desc &d)
         // Few workgroups: pieces of 256 keys, two for each wave (one user, 1501 keys, 32 heads over 8: with 64 / 128 / 256 / 512 12.1 / 11.4 / 11.7 / 13.1 us).
         // Where each workgroup has a cache of its own four times as many even out their lengths (64 users of 284 to 8192 keys: 512 / 1024 / 2048 / 4096
         // workgroups 232 / 221 / 210 / 214 us), which short ones do not pay for with a second launch.
-        r.splits = r.max_tiles == 1 && r.grid >= kFill ? pieces(r.grid, keys, 1024, 4 * kFill) : pieces(r.grid, keys, 256, kFill);
+        r.splits = r.max_tiles == 1 && r.grid >= kFill ? pieces(r.grid, keys, 1024, 4 * kFill) : pieces(r.grid, keys, 256, d.shared_len > 0 ? kFill / 2 : kFill);
         r.grid *= r.splits;
     }
     r.parts = r.splits;

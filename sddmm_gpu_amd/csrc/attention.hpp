@@ -305,20 +305,24 @@ __device__ __forceinline__ int end_key(const AttnArgs &a, int pos, int prefix, i
 }
 
 // The bound of scores: cap tanh(t / cap), t = scale * product, of N results in registers, in powers of two (BACK: and 1 - tanh^2 of each).
-// Where all of the wave's |t / cap| are 0.25 at most, which they mostly are, by powers, seven instructions where 1 - 2 / (1 + e^2y) takes
-// two of the slow kind and as many others, and to the last place, since that difference loses 24 bits below 1 (the next term is 1e-8 of the result).
+// Where all of the wave's |y|, y = t / cap, are 0.25 at most, which they mostly are, by powers of y^2 with everything else in their factors: six
+// instructions, where 1 - 2 / (1 + e^2y) takes two of the slow kind and as many others, and to the last place, since that difference loses 24 bits
+// below 1.  What the powers leave out is 8.5e-9 of the result; with 16-bit operands, whose probabilities are rounded to 2^-9 or 2^-12, the
+// last of them is left out too (3.4e-7).
+template <class T>
 struct Bend {
-    float limit, by, twice, to, cap;
+    float limit, by2, twice, to, cap, c0, c1, c2, c3, c4;
     __device__ __forceinline__ void init(float scale, float cap_)
     {
         cap = cap_;
-        by = cap > 0.f ? scale / cap : 0.f;
-        to = cap * kLog2e, twice = by * (2.f * kLog2e), limit = cap > 0.f ? 0.25f / by : 0.f;
+        const float by = cap > 0.f ? scale / cap : 0.f;
+        to = cap * kLog2e, twice = by * (2.f * kLog2e), limit = cap > 0.f ? 0.25f / by : 0.f, by2 = by * by;
+        c0 = scale * kLog2e, c1 = c0 * -0.33333334f, c2 = c0 * 0.13333334f, c3 = c0 * -0.053968254f, c4 = c0 * 0.021869489f;
     }
     __device__ __forceinline__ float near(float x) const
     {
-        const float y = x * by, s = y * y;
-        return y * fmaf(s, fmaf(s, fmaf(s, fmaf(s, 0.021869489f, -0.053968254f), 0.13333334f), -0.33333334f), 1.f);
+        const float s = x * x * by2, last = sizeof(T) == 4 ? fmaf(s, c4, c3) : c3;
+        return x * fmaf(s, fmaf(s, fmaf(s, last, c2), c1), c0);
     }
     template <int N, bool BACK>
     __device__ __forceinline__ void apply(floatx16 (&x)[N], floatx16 (&back)[N]) const
@@ -333,7 +337,7 @@ struct Bend {
             for (int i = 0; i < N; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const float away = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[i][r] * twice)), 1.f);
+                    const float away = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[i][r] * twice)), 1.f) * to;
                     x[i][r] = fabsf(x[i][r]) <= limit ? near(x[i][r]) : away;
                 }
         } else {
@@ -342,13 +346,16 @@ struct Bend {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[i][r] = near(x[i][r]);
         }
+        if constexpr (BACK) {
+            const float from = 1.f / to;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                if constexpr (BACK) back[i][r] = fmaf(-x[i][r], x[i][r], 1.f);
-                x[i][r] *= to;
-            }
+                for (int r = 0; r < 16; ++r) {
+                    const float y = x[i][r] * from;
+                    back[i][r] = fmaf(-y, y, 1.f);
+                }
+        }
     }
 };
 

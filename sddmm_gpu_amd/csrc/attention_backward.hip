@@ -53,13 +53,13 @@ void sddmm_attention_stats_kernel(const AttnArgs a)
 }
 
 // scores in powers of two from products, and what their gradients have to be multiplied by on the way back
-template <bool MOD>
-__device__ __forceinline__ void scores(floatx16 &x, floatx16 &back, const Bend &bend, float unit, bool bias, float slope, float at, float step)
+template <bool MOD, class T>
+__device__ __forceinline__ void scores(floatx16 &x, floatx16 &back, const Bend<T> &bend, float unit, bool bias, float slope, float at, float step)
 {
     if constexpr (MOD) {
         if (bend.cap > 0.f) {
             floatx16 y[1] = {x}, z[1];
-            bend.apply<1, true>(y, z);
+            bend.template apply<1, true>(y, z);
             x = y[0], back = z[0];
         } else {
 #pragma unroll
@@ -123,7 +123,7 @@ struct DkvKeys {
     Vec8 kf[DP / 16];
     floatx16 dk[DB], dv[DB];
     float unit;
-    Bend bend;
+    Bend<T> bend;
     bool bias, there;
     int key, lo, hi, wave_lo, wave_hi, full_lo, full_hi, shift, h;
 
@@ -152,7 +152,7 @@ struct DkvKeys {
         for (int c = 0; c < DP / 16; ++c) x = Elem<T>::mma(Rows::row_operand(qt, 0, c, l), kf[c], x);
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) y = Elem<T>::mma(Rows::row_operand(dot, 0, c, l), v(c), y);
-        scores<MOD>(x, back, bend, unit, bias, slope, (float)(row + 4 * h + shift - key), 1.f);
+        scores<MOD, T>(x, back, bend, unit, bias, slope, (float)(row + 4 * h + shift - key), 1.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const floatx4 m = *(const floatx4 *)(lse + 8 * i + 4 * h), d = *(const floatx4 *)(delta + 8 * i + 4 * h);
@@ -376,7 +376,7 @@ struct DqRows {
     Vec8 qf[DP / 16], of[DP / 16];
     floatx16 dq[DB];
     float lse, delta, unit, slope;
-    Bend bend;
+    Bend<T> bend;
     bool bias, slopes_too, there;
     int pos, lo, hi, h;
     double far_ds, far_p, sum_ds, sum_p;
@@ -413,7 +413,7 @@ struct DqRows {
     {
         floatx16 back;
         const float away = (float)(pos - key - 4 * h);
-        scores<MOD>(x, back, bend, unit, bias, slope, away, -1.f);
+        scores<MOD, T>(x, back, bend, unit, bias, slope, away, -1.f);
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r] - lse);
         if (masked) {

@@ -120,7 +120,7 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
     const float scale = a.scale;
-    Bend bend;
+    Bend<T> bend;
     if constexpr (MOD) bend.init(scale, a.cap);
     const float unit = MOD ? 1.f : scale * kLog2e;  // scores in registers to powers of two
     const float raise = 8.f / unit;
@@ -158,7 +158,7 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
 
         if constexpr (MOD) {
             if (bend.cap > 0.f) {
-                bend.apply<KB, false>(x, x);
+                bend.template apply<KB, false>(x, x);
             } else {
 #pragma unroll
                 for (int i = 0; i < KB; ++i)

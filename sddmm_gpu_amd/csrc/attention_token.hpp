@@ -56,7 +56,7 @@ __device__ __forceinline__ void TokenTile<T, DP, MOD, NW>::run(const AttnArgs &a
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = zero16();
     const float scale = a.scale;
-    Bend bend;
+    Bend<T> bend;
     if constexpr (MOD) bend.init(scale, a.cap);
     const float unit = MOD ? 1.f : scale * kLog2e;
     const float slope = MOD && a.slopes && there ? a.slopes[head] * kLog2e : 0.f;
@@ -95,7 +95,7 @@ __device__ __forceinline__ void TokenTile<T, DP, MOD, NW>::run(const AttnArgs &a
         if constexpr (MOD) {
             if (bend.cap > 0.f) {
                 floatx16 y[1] = {x};
-                bend.apply<1, false>(y, y);
+                bend.template apply<1, false>(y, y);
                 x = y[0];
             } else {
 #pragma unroll

@@ -27,7 +27,7 @@ BAD = [
     (dict(window_left=-2), "window"), (dict(window_right=-7), "window"),
     (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(cap=-1.0), "cap"), (dict(cap=float("inf")), "cap"), (dict(cap=float("nan")), "cap"),
-    (dict(cap=1e-31, scale=1.0), "too far apart"), (dict(cap=1e31, scale=1.0), "too far apart"), (dict(cap=1.0, scale=1e-31), "too far apart"),
+    (dict(cap=1e-16, scale=1.0), "too far apart"), (dict(cap=1e31, scale=1e20), "too far apart"), (dict(cap=1e16, scale=1.0), "too far apart"),
     (dict(q_ptr=A + 2, q_rows=200), "aligned"), (dict(k_len=A + 1), "aligned"), (dict(slopes=A + 2), "aligned"), (dict(prefix=A + 3), "aligned"),
     (dict(q_ptr=A, q_len=A), "lengths beside"), (dict(k_ptr=A, k_len=A), "lengths beside"),
     (dict(q_row=60), "strides"), (dict(k_row=63 * 4 + 1), "strides"), (dict(v_head=12), "strides"), (dict(o_row=1 << 23), "strides"),
