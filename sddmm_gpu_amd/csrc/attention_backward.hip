@@ -223,7 +223,7 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
     __shared__ __align__(1024) char lds[2][2][Rows::kBytes];
     __shared__ __align__(1024) char values[kKeepV ? 16 : Values::kBytes];
     __shared__ __align__(16) float stat[2][2][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
 
     KeyTile at;
     // (pieces outermost: next to each other they would go to different dies, the later ones, of which there are fewer, always to the same)
@@ -271,8 +271,14 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
         keys.pieces([&](int i, floatx4 y) { to[i * 64] = y; });
         return;
     }
-    if (!keys.there) return;
-    keys.pieces([&](int i, floatx4 y) { Keys::store(a, at, k0 + 32 * wave + n, i, h, y); });
+    if constexpr (sizeof(T) == 2) __syncthreads();  // (the tiles have been read by all)
+    char *mine = (char *)lds + wave * 64 * DP;
+    static_assert(sizeof(T) == 4 || kWaves * 64 * DP <= (int)sizeof lds);
+    const int key0 = k0 + 32 * wave;
+    store_turned<T, DP>(mine, keys.dk, a.scale, a.head_dim, lane,
+                        [&](int r) { return key0 + r < at.e.nk ? (T *)k_base<T>(a, a.dk, at.e, at.s, at.kv) + (key0 + r) * a.k_row : nullptr; });
+    store_turned<T, DP>(mine, keys.dv, 1.f, a.head_dim, lane,
+                        [&](int r) { return key0 + r < at.e.nk ? (T *)v_base<T>(a, a.dv, at.e, at.s, at.kv) + (key0 + r) * a.v_row : nullptr; });
 }
 
 // The same where workgroups of 128 keys would leave most compute units without work: 32 keys to a workgroup, each wave on every NW-th tile of rows, in LDS of
@@ -570,13 +576,14 @@ void sddmm_attention_dq_kernel(const AttnArgs a)
         __syncthreads();
         if (threadIdx.x == 0) *slope_part = parts[0] + parts[1] + parts[2] + parts[3];
     }
-    if (half || !rows.there) return;
-    T *to = (T *)q_base<T>(a, a.dq, e, s, head) + row * a.q_row;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            store_dq(a, to, 32 * d + 8 * i + 4 * h, floatx4{rows.dq[d][4 * i], rows.dq[d][4 * i + 1], rows.dq[d][4 * i + 2], rows.dq[d][4 * i + 3]});
+    if (half) return;
+    if constexpr (sizeof(T) == 2) {
+        static_assert(RW * 128 * DP + RW * 1024 + RW * 64 * DP <= (int)sizeof lds || RW == kWaves);
+        if constexpr (RW == kWaves) __syncthreads();  // (the tiles have been read by all)
+    }
+    const int row0 = tile * kRows + row_wave * 32;
+    store_turned<T, DP>((char *)lds + (RW == kWaves ? 0 : RW * 128 * DP + RW * 1024) + row_wave * 64 * DP, rows.dq, a.scale, a.head_dim, lane,
+                        [&](int r) { return row0 + r < e.nq ? (T *)q_base<T>(a, a.dq, e, s, head) + (row0 + r) * a.q_row : nullptr; });
 }
 
 // dq where workgroups of 128 rows would leave compute units without work: 32 rows to a workgroup, each wave on every NW-th tile of keys, in LDS of its

@@ -7,7 +7,7 @@ namespace sddmm {
 namespace {
 
 template <class T, int DP, bool MOD, int ROWS, int RW>
-__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : 2)
+__global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : sizeof(T) == 2 && DP == 64 && !MOD ? 4 : 2)
 void sddmm_attention_forward_kernel(const AttnArgs a)
 {
     typedef ForwardTile<T, DP, MOD, ROWS, RW> Body;

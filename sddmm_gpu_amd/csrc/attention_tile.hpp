@@ -49,7 +49,10 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
         head = kv * a.group + b % a.group;
         b /= a.group;
     }
-    if (a.n_split > 1) { split = b % a.n_split; b /= a.n_split; }
+    if constexpr (ROWS == kRowsShared) {
+        split = b % a.n_split;
+        b /= a.n_split;
+    }
     if (ROWS != kRowsShared && a.q_ptr) {
         s = slot_sequence<false>(a.q_ptr, a.n_seq, 1, kRows, a.max_tiles, a.n_slots, b, tile);
         if (s < 0) return;
@@ -128,7 +131,7 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
     float m = -INFINITY, sum = 0.f;
 
     const int n_tiles = any_hi > any_lo ? (any_hi - any_lo + KT - 1) / KT : 0;
-    const int each = (n_tiles + a.n_split - 1) / a.n_split;
+    const int each = ROWS == kRowsShared ? (n_tiles + a.n_split - 1) / a.n_split : n_tiles;
     const int first = split * each, last = min(n_tiles, first + each);
     const int row_bytes = a.head_dim * (int)sizeof(T);
     const uint32_t k_stride = (uint32_t)(a.k_row * sizeof(T)), v_stride = (uint32_t)(a.v_row * sizeof(T));
@@ -242,9 +245,9 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
                 for (int j = 0; j < 4; ++j) o[d][4 * i + j] = o[d][4 * i + j] * w + y[j] * u;
             }
     }
-    if (!there) return;
     const int64_t at = (e.lse0 + token) * a.n_heads + my_head;
-    if (a.n_part > 1) {
+    if constexpr (ROWS == kRowsShared) {
+        if (!there) return;
         const int64_t all = a.rows * a.n_heads, part = a.part0 + split;
         float *to = a.part_o + (part * all + at) * a.head_dim;
 #pragma unroll
@@ -255,19 +258,24 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
                 if (col < a.head_dim) *(floatx4 *)(to + col) = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
             }
         if (h == 0) a.part_ml[part * all + at] = make_float2(m, sum);
-        return;
-    }
-    const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    T *to = (T *)o_base<T>(a, a.out, e, s, my_head) + (int64_t)token * a.o_row;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int col = 32 * d + 8 * i + 4 * h;
-            const floatx4 y = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * by;
-            if (col < a.head_dim) *(typename Elem<T>::Vec4 *)(to + col) = __builtin_convertvector(y, typename Elem<T>::Vec4);
+    } else {
+        if (there && a.lse && h == 0) a.lse[at] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+        const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        if constexpr (sizeof(T) == 2) {
+            static_assert(RW * 128 * DP + RW * 256 + RW * 64 * DP <= kLds || RW == kWaves);
+            if constexpr (RW == kWaves) __syncthreads();  // (the tiles have been read by all)
         }
-    if (a.lse && h == 0) a.lse[at] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+        const int row0 = tile * kRows + row_wave * 32;
+        store_turned<T, DP>(memory + (RW == kWaves ? 0 : RW * 128 * DP + RW * 256) + row_wave * 64 * DP, o, by, a.head_dim, lane, [&](int r) -> T * {
+            const int at_row = row0 + r;
+            if constexpr (ROWS == kRowsOfHead) {
+                return at_row < e.nq ? (T *)o_base<T>(a, a.out, e, s, my_head) + (int64_t)at_row * a.o_row : nullptr;
+            } else {  // (few: a quotient each)
+                const int t = at_row / a.group;
+                return at_row < e.nq * a.group ? (T *)o_base<T>(a, a.out, e, s, head + at_row % a.group) + (int64_t)t * a.o_row : nullptr;
+            }
+        });
+    }
 }
 
 }  // namespace sddmm
