@@ -112,10 +112,11 @@ Deal deal(const sddmm_attention_desc &d)
         r.max_tiles = div_up(packed, few);
         r.slots = r.max_tiles == 1 ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
         r.grid = r.slots * d.n_kv_heads;
-        // Few workgroups: pieces of 256 keys, two for each wave (one user, 1501 keys, 32 heads over 8: with 64 / 128 / 256 / 512 12.1 / 11.4 / 11.7 / 13.1 us).
+        // Few workgroups: pieces of 256 keys, two for each wave (one user, 1501 keys, 32 heads over 8: with 64 / 128 / 256 / 512 12.1 / 11.4 / 11.7 / 13.1 us); up to
+        // 768 keys a second launch costs more than it saves.
         // Where each workgroup has a cache of its own four times as many even out their lengths (64 users of 284 to 8192 keys: 512 / 1024 / 2048 / 4096
         // workgroups 232 / 221 / 210 / 214 us), which short ones do not pay for with a second launch.
-        r.splits = r.max_tiles == 1 && r.grid >= kFill ? pieces(r.grid, keys, 1024, 4 * kFill) : pieces(r.grid, keys, 256, d.shared_len > 0 ? kFill / 2 : kFill);
+        r.splits = r.max_tiles == 1 && r.grid >= kFill ? pieces(r.grid, keys, 1024, 4 * kFill) : keys <= 768 ? 1 : pieces(r.grid, keys, 256, d.shared_len > 0 ? kFill / 2 : kFill);
         r.grid *= r.splits;
     }
     r.parts = r.splits;
@@ -187,7 +188,7 @@ DealBack deal_back(const sddmm_attention_desc &d)
         const double share = work / places;
         if (most > 2.5 * share) {
             const bool slow = d.type == SDDMM_TYPE_F32;  // (its rows take sixteen times as long, its parts no longer)
-            r.chunk = std::max<int64_t>((int64_t)std::sqrt((slow ? 100. : 1300.) * share), slow ? 64 : 256);
+            r.chunk = std::max<int64_t>((int64_t)std::sqrt((slow ? 100. : 1300.) * share), (slow ? 64 : 256) * (r.keys == 32 ? 4 : 1));  // (four waves share the rows of 32 keys)
             r.splits = std::max<int64_t>(1, std::min<int64_t>(div_up(most, r.chunk), 32));
         }
         r.chunk = std::max(r.chunk, div_up(most, r.splits));

@@ -3,9 +3,10 @@
 //   p_ij = exp(s_ij - lse_i);  dv_j = sum_i p_ij do_i;  ds_ij = p_ij (do_i . v_j - delta_i),  delta_i = do_i . o_i
 //   dt_ij = ds_ij (1 - tanh^2);  dq_i = scale sum_j dt_ij k_j;  dk_j = scale sum_i dt_ij q_i
 //
-// Scores are computed again from q and k: nothing but lse comes from the forward pass.  Two kernels, one that keeps rows of keys and
-// walks the rows that see them (dk, dv), and one that keeps rows of queries and walks their keys (dq), compute them twice: seven
-// products where five would do with atomic additions, but each result is summed by one wave in a fixed order.
+// Scores are computed again from q and k: nothing but lse comes from the forward pass.  Two kernels, one that keeps rows of queries and
+// walks their keys (dq), and one that keeps rows of keys and walks the rows that see them (dk, dv), compute them twice: seven
+// products where five would do with atomic additions, but each result is summed in a fixed order.  The first leaves every row's
+// statistics (lse in powers of two, delta; [n_heads][rows]) for the second.
 #include "attention.hpp"
 #include "attention_launch.hpp"
 #include "launch.hpp"
@@ -16,41 +17,6 @@ namespace {
 
 constexpr int kKeys = 128, kWaves = 4;  // keys of a workgroup of the dk, dv kernel, 32 to a wave
 constexpr int kFewKeys = 32;             // of the one for few keys
-
-// stats[head][row] = (lse in powers of two, dout . out).  A row that saw nothing gets +infinity, so that 2^(s - lse) is 0.
-template <class T, int DP>
-__global__ __launch_bounds__(256)
-void sddmm_attention_stats_kernel(const AttnArgs a)
-{
-    constexpr int kLanes = DP / 8, kPer = 256 / kLanes;
-    const int lane = threadIdx.x % kLanes;
-    const int64_t at = (int64_t)blockIdx.x * kPer + threadIdx.x / kLanes;
-    if (at >= a.rows * a.n_heads) return;
-    const int head = (int)(at % a.n_heads);
-    const int64_t row = at / a.n_heads;
-    int64_t off;
-    if (a.q_ptr) {
-        if (row < a.q_ptr[0] || row >= a.q_ptr[a.n_seq]) return;
-        off = row * a.o_row;
-    } else {
-        const int s = (int)(row / a.max_q), i = (int)(row % a.max_q);
-        if (a.q_len && i >= min(a.q_len[s], a.max_q)) return;
-        off = s * a.o_seq + i * a.o_row;
-    }
-    off += head * a.o_head;
-    const auto x = __builtin_convertvector(global_operand<T>((const T *)a.out + off, true, 8 * lane, a.head_dim), floatx8);
-    const auto y = __builtin_convertvector(global_operand<T>((const T *)a.dout + off, true, 8 * lane, a.head_dim), floatx8);
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf(x[j], y[j], sum);
-#pragma unroll
-    for (int d = 1; d < kLanes; d *= 2) sum += __shfl_xor(sum, d);
-    const float lse = a.lse[at];
-    if (lane == 0) {
-        a.stat_lse[head * a.rows + row] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-        a.stat_delta[head * a.rows + row] = sum;
-    }
-}
 
 // scores in powers of two from products, and what their gradients have to be multiplied by on the way back
 template <bool MOD, class T>
@@ -282,7 +248,8 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
 }
 
 // The same where workgroups of 128 keys would leave most compute units without work: 32 keys to a workgroup, each wave on every NW-th tile of rows, in LDS of
-// its own and without a barrier; sums are joined at the end.
+// its own and without a barrier; sums are joined at the end.  fp32 heads of more than 64: one tile at a time, since a tile's products take eight
+// times as long as its way to LDS, and v in LDS.
 template <class T, int DP, bool MOD, int NW>
 __global__ __launch_bounds__(64 * NW, 1)
 void sddmm_attention_dkv_few_kernel(const AttnArgs a)
@@ -291,8 +258,11 @@ void sddmm_attention_dkv_few_kernel(const AttnArgs a)
     typedef typename Keys::Rows Rows;
     typedef typename Elem<T>::Vec8 Vec8;
     constexpr int kLoads = 2 * Rows::kBytes / 1024 + 2;
-    __shared__ __align__(1024) char lds[NW][2][2][Rows::kBytes];
-    __shared__ __align__(16) float stat[NW][2][2][64];
+    constexpr bool kLarge = sizeof(T) == 4 && DP == 128;
+    constexpr int kTurns = kLarge ? 1 : 2;
+    __shared__ __align__(1024) char lds[NW][kTurns][2][Rows::kBytes];
+    __shared__ __align__(1024) char values[kLarge ? Rows::kBytes : 16];
+    __shared__ __align__(16) float stat[NW][kTurns][2][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
     KeyTile at;
     const int groups = gridDim.x / a.n_split, split = blockIdx.x / groups;
@@ -314,23 +284,31 @@ void sddmm_attention_dkv_few_kernel(const AttnArgs a)
     request(first + wave, 0);
     Keys keys;
     keys.init(a, at, k0, lane);
-    Vec8 vf[DP / 16];
-    const T *v = v_base<T>(a, a.v, at.e, at.s, at.kv) + keys.key * a.v_row;
+    Vec8 vf[kLarge ? 1 : DP / 16];
+    const T *v = v_base<T>(a, a.v, at.e, at.s, at.kv);
+    if constexpr (kLarge) {
+        Rows::template request<NW>(values, (const char *)(v + k0 * a.v_row), (uint32_t)(a.v_row * sizeof(T)), at.e.nk - k0, row_bytes, wave, lane);
+        tiles_arrived();
+    } else {
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) vf[c] = global_operand<T>(v, keys.there, 16 * c + 8 * h, a.head_dim);
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // the first tile and the keys: from here on only tiles are under way
-    for (int t = first + wave, turn = 0; t < last; t += NW, turn ^= 1) {
-        request(t + NW, turn ^ 1);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+        for (int c = 0; c < DP / 16; ++c) vf[c] = global_operand<T>(v + keys.key * a.v_row, keys.there, 16 * c + 8 * h, a.head_dim);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // the first tile and the keys: from here on only tiles are under way
+    }
+    for (int t = first + wave, turn = 0; t < last; t += NW, turn = (turn + 1) % kTurns) {
+        if constexpr (!kLarge) request(t + NW, turn ^ 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLarge ? 0 : kLoads) : "memory");
         const float slope = MOD && a.slopes ? a.slopes[at.kv * a.group + t / tiles] * kLog2e : 0.f;
         const int row = at.any_lo + t % tiles * 32;
-        if (!keys.sees(row)) continue;
-        keys.add(lds[wave][turn][0], lds[wave][turn][1], stat[wave][turn][0], stat[wave][turn][1], row, slope, lane, [&](int c) { return vf[c]; });
+        if (keys.sees(row)) {
+            keys.add(lds[wave][turn][0], lds[wave][turn][1], stat[wave][turn][0], stat[wave][turn][1], row, slope, lane,
+                     [&](int c) { if constexpr (kLarge) return Rows::row_operand(values, 0, c, lane); else return vf[c]; });
 #pragma unroll
-        for (int d = 0; d < Keys::DB; ++d) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(keys.dk[d]), "+v"(keys.dv[d]) :: "memory");
+            for (int d = 0; d < Keys::DB; ++d) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(keys.dk[d]), "+v"(keys.dv[d]) :: "memory");
+        }
+        if constexpr (kLarge) request(t + NW, 0);
     }
     // join the waves: [piece][lane] of 16 bytes for each
-    static_assert(4 * Rows::kBytes >= 256 * DP);
+    static_assert(2 * kTurns * Rows::kBytes >= 256 * DP);
     __builtin_amdgcn_s_waitcnt(0x0070);
     floatx4 *mine = (floatx4 *)lds[wave][0][0];
     keys.pieces([&](int i, floatx4 y) { mine[i * 64 + lane] = y; });
@@ -387,7 +365,7 @@ struct DqRows {
     int pos, lo, hi, h;
     double far_ds, far_p, sum_ds, sum_p;
 
-    __device__ __forceinline__ void init(const AttnArgs &a, const Seq &e, int s, int head, int row, int prefix, bool want_slopes, int lane)
+    __device__ __forceinline__ void init(const AttnArgs &a, const Seq &e, int s, int head, int row, int prefix, bool want_slopes, bool write_stats, int lane)
     {
         h = lane >> 5;
         there = row < e.nq;
@@ -397,8 +375,22 @@ struct DqRows {
         for (int c = 0; c < DP / 16; ++c) qf[c] = global_operand<T>(q, there, 16 * c + 8 * h, a.head_dim);
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) of[c] = global_operand<T>(dout, there, 16 * c + 8 * h, a.head_dim);
-        const int64_t at = (int64_t)head * a.rows + e.lse0 + row;
-        lse = there ? a.stat_lse[at] : INFINITY, delta = there ? a.stat_delta[at] : 0.f;
+        const T *out = o_base<T>(a, a.out, e, s, head) + row * a.o_row;
+        delta = 0.f;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            const floatx8 x = __builtin_convertvector(of[c], floatx8), y = __builtin_convertvector(global_operand<T>(out, there, 16 * c + 8 * h, a.head_dim), floatx8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) delta = fmaf(x[j], y[j], delta);
+        }
+        delta = halves_sum(delta);
+        // (a row that saw nothing gets +infinity, so that 2^(s - lse) is 0)
+        const float m = there ? a.lse[(e.lse0 + row) * a.n_heads + head] : -INFINITY;
+        lse = m == -INFINITY ? INFINITY : m * kLog2e;
+        if (there && h == 0 && write_stats) {
+            const int64_t at = (int64_t)head * a.rows + e.lse0 + row;
+            a.stat_lse[at] = lse, a.stat_delta[at] = delta;
+        }
 #pragma unroll
         for (int d = 0; d < DB; ++d) dq[d] = zero16();
         unit = a.scale * kLog2e;
@@ -513,7 +505,7 @@ void sddmm_attention_dq_kernel(const AttnArgs a)
     const int wave_lo = first_key(a, w0 + shift), wave_hi = w1 < w0 ? 0 : end_key(a, w1 + shift, prefix, e.nk);
     const int full_lo = first_key(a, w1 + shift), full_hi = w1 < w0 + 31 ? 0 : end_key(a, w0 + shift, prefix, e.nk);
     DqRows<T, DP, MOD> rows;
-    rows.init(a, e, s, head, row, prefix, slope_part != nullptr, lane);
+    rows.init(a, e, s, head, row, prefix, slope_part != nullptr, half == 0, lane);
     const T *k = k_base<T>(a, a.k, e, s, kv), *v = v_base<T>(a, a.v, e, s, kv);
 
     const int last = any_hi > any_lo ? (any_hi - any_lo + KT - 1) / KT : 0;
@@ -587,7 +579,8 @@ void sddmm_attention_dq_kernel(const AttnArgs a)
 }
 
 // dq where workgroups of 128 rows would leave compute units without work: 32 rows to a workgroup, each wave on every NW-th tile of keys, in LDS of its
-// own (keys twice, since they are needed to the end of a tile's work) and without a barrier; sums are joined at the end.
+// own (keys twice, since they are needed to the end of a tile's work; not fp32 heads of more than 64, see above) and without a barrier; sums
+// are joined at the end.
 constexpr int kFewRows = 32;
 template <class T, int DP, bool MOD, int NW>
 __global__ __launch_bounds__(64 * NW, 1)
@@ -596,7 +589,9 @@ void sddmm_attention_dq_few_kernel(const AttnArgs a)
     constexpr int KT = 32, DB = DP / 32;
     typedef Tile<T, DP, KT> Keys;
     constexpr int kLoads = Keys::kBytes / 1024;
-    __shared__ __align__(1024) char lds[NW][3][Keys::kBytes];
+    constexpr bool kLarge = sizeof(T) == 4 && DP == 128;
+    constexpr int kTurns = kLarge ? 1 : 2;
+    __shared__ __align__(1024) char lds[NW][kTurns + 1][Keys::kBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
     int b = blockIdx.x, s = 0, tile;
     const int head = b % a.n_heads, kv = head / a.group;
@@ -617,7 +612,7 @@ void sddmm_attention_dq_few_kernel(const AttnArgs a)
     const int any_lo = first_key(a, w0 + shift), any_hi = end_key(a, w1 + shift, prefix, e.nk);
     const int full_lo = first_key(a, w1 + shift), full_hi = w1 < w0 + 31 ? 0 : end_key(a, w0 + shift, prefix, e.nk);
     DqRows<T, DP, MOD> rows;
-    rows.init(a, e, s, head, row, prefix, slope_part != nullptr, lane);
+    rows.init(a, e, s, head, row, prefix, slope_part != nullptr, wave == 0, lane);
     const T *k = k_base<T>(a, a.k, e, s, kv), *v = v_base<T>(a, a.v, e, s, kv);
 
     const int last = any_hi > any_lo ? (any_hi - any_lo + KT - 1) / KT : 0;
@@ -629,17 +624,17 @@ void sddmm_attention_dq_few_kernel(const AttnArgs a)
         const bool more = t < last;
         Keys::template request<1>(to, (const char *)(base + (more ? key : 0) * step), stride, more ? e.nk - key : 0, row_bytes, 0, lane);
     };
-    char *vt = lds[wave][2];
+    char *vt = lds[wave][kTurns];
     __builtin_amdgcn_s_waitcnt(0x0f70);  // the rows: from here on only tiles are under way
     request(lds[wave][0], k, a.k_row, k_stride, wave);
     request(vt, v, a.v_row, v_stride, wave);
-    for (int t = wave, turn = 0; t < last; t += NW, turn ^= 1) {
+    for (int t = wave, turn = 0; t < last; t += NW, turn = (turn + 1) % kTurns) {
         const int key = any_lo + t * KT;
         const char *kt = lds[wave][turn];
-        request(lds[wave][turn ^ 1], k, a.k_row, k_stride, t + NW);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
+        if constexpr (!kLarge) request(lds[wave][turn ^ 1], k, a.k_row, k_stride, t + NW);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLarge ? 0 : 2 * kLoads) : "memory");
         floatx16 x = rows.template product<Keys>(kt, 0, rows.qf, lane);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLarge ? 0 : kLoads) : "memory");
         floatx16 y = rows.template product<Keys>(vt, 0, rows.of, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x), "+v"(y) :: "memory");  // (all of the values have been read)
         request(vt, v, a.v_row, v_stride, t + NW);
@@ -647,9 +642,10 @@ void sddmm_attention_dq_few_kernel(const AttnArgs a)
         rows.template add<Keys>(kt, 0, y, lane);
 #pragma unroll
         for (int d = 0; d < DB; ++d) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(rows.dq[d]) :: "memory");
+        if constexpr (kLarge) request(lds[wave][0], k, a.k_row, k_stride, t + NW);
     }
     // join the waves: [element of the lane / 4][lane] of 16 bytes for each wave
-    static_assert(3 * Keys::kBytes >= 128 * DP);
+    static_assert((kTurns + 1) * Keys::kBytes >= 128 * DP);
     __builtin_amdgcn_s_waitcnt(0x0070);
     floatx4 *mine = (floatx4 *)lds[wave][0];
 #pragma unroll
@@ -702,7 +698,7 @@ template <class T, int DP>
 hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, int keys, unsigned q_grid, int q_rows, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
-    constexpr int kPer = 256 / (DP / 8), NW = sizeof(T) == 4 && DP == 128 ? 2 : 4;
+    constexpr int NW = 4;
     const auto dkv = mod ? sddmm_attention_dkv_kernel<T, DP, true> : sddmm_attention_dkv_kernel<T, DP, false>;
     const auto dkv_few = mod ? sddmm_attention_dkv_few_kernel<T, DP, true, NW> : sddmm_attention_dkv_few_kernel<T, DP, false, NW>;
     const auto sum = keys == kKeys ? sddmm_attention_dkv_sum_kernel<T, DP, kKeys> : sddmm_attention_dkv_sum_kernel<T, DP, kFewKeys>;
@@ -710,10 +706,9 @@ hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, 
                                  : (mod ? sddmm_attention_dq_kernel<T, DP, true, 4> : sddmm_attention_dq_kernel<T, DP, false, 4>);
     const auto dq_few = mod ? sddmm_attention_dq_few_kernel<T, DP, true, NW> : sddmm_attention_dq_few_kernel<T, DP, false, NW>;
     hipError_t e = hipSuccess;
-    if (q_grid) e = launch(sddmm_attention_stats_kernel<T, DP>, dim3((unsigned)((a.rows * a.n_heads + kPer - 1) / kPer)), dim3(256), 0, st, a);
+    if (q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * NW), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
     if (e == hipSuccess && kv_grid) e = keys == kKeys ? launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a) : launch(dkv_few, dim3(kv_grid), dim3(64 * NW), 0, st, a);
     if (e == hipSuccess && kv_grid && a.n_split > 1) e = launch(sum, dim3(kv_grid / a.n_split * (keys / 32)), dim3(256), 0, st, a);
-    if (e == hipSuccess && q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * NW), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
     if (e == hipSuccess && a.dslopes) e = launch(sddmm_attention_dslopes_kernel, dim3((unsigned)a.n_heads), dim3(256), 0, st, b);
     return e;
 }

@@ -74,7 +74,7 @@ void sddmm_attention_join_kernel(const AttnArgs a, const int per_row)
 template <class T, int DP>
 hipError_t launch_typed(const AttnArgs &a, bool mod, unsigned grid, hipStream_t st)
 {
-    constexpr int NW = sizeof(T) == 4 && DP == 128 ? 2 : 4;
+    constexpr int NW = 4;
     return launch(mod ? sddmm_attention_token_kernel<T, DP, true, NW> : sddmm_attention_token_kernel<T, DP, false, NW>, dim3(grid), dim3(64 * NW), 0, st, a);
 }
 
