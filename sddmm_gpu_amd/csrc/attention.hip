@@ -316,7 +316,7 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
     if (!aligned({d_q, d_k, d_v, d_out, d_dout, d_dq, d_dk, d_dv})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (r.q_grid > INT32_MAX || r.kv_grid > INT32_MAX / 4 || r.rows * d.n_heads / 16 > INT32_MAX || r.key_rows * d.n_kv_heads > INT32_MAX)
+    if (r.q_grid > INT32_MAX || r.kv_grid > INT32_MAX / 32 || r.rows * d.n_heads / 16 > INT32_MAX || r.key_rows * d.n_kv_heads > INT32_MAX)
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
 
     AttnArgs a = arguments(d);

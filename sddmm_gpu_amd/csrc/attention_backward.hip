@@ -325,26 +325,29 @@ void sddmm_attention_dkv_few_kernel(const AttnArgs a)
     }
 }
 
-// The sum of the parts of dk and dv of the keys whose rows were cut: a workgroup for 32 keys.
+// The sum of the parts of dk and dv of the keys whose rows were cut: pieces of four elements, one to a thread where there are few keys (us, 148 tokens, 16
+// heads over 2 of 96, fp32 9 with eight and 5 with one), two where there are many, whose workgroups would spend their time on finding their sequence.
+template <int KEYS> constexpr int kSumPieces = KEYS == kKeys ? 2 : 1;
 template <class T, int DP, int KEYS>
 __global__ __launch_bounds__(256)
 void sddmm_attention_dkv_sum_kernel(const AttnArgs a)
 {
     typedef DkvKeys<T, DP, false> Keys;
+    constexpr int kEach = 2 * Keys::DB / kSumPieces<KEYS>;  // workgroups to 32 keys
     KeyTile at;
-    if (!key_tile<KEYS>(a, blockIdx.x / (KEYS / 32), at) || at.pieces == 1) return;
-    const int lane = threadIdx.x & 63, key = at.tile * KEYS + blockIdx.x % (KEYS / 32) * 32 + (lane & 31);
+    const int unit = blockIdx.x / kEach;
+    if (!key_tile<KEYS>(a, unit / (KEYS / 32), at) || at.pieces == 1) return;
+    const int lane = threadIdx.x & 63, key = at.tile * KEYS + unit % (KEYS / 32) * 32 + (lane & 31), i0 = blockIdx.x % kEach * 4 + (threadIdx.x >> 6);
     if (key >= at.e.nk) return;
-    const int64_t part = (int64_t)gridDim.x * (8 * Keys::DB * 64);
+    const int64_t part = (int64_t)(gridDim.x / kEach) * (8 * Keys::DB * 64);
+    const floatx4 *from = (const floatx4 *)a.part_o + (int64_t)unit * (8 * Keys::DB * 64) + lane;
+    floatx4 x[kSumPieces<KEYS>] = {};
+#pragma unroll 8 / kSumPieces<KEYS>
+    for (int p = 0; p < at.pieces; ++p)
 #pragma unroll
-    for (int j = 0; j < 2 * Keys::DB; ++j) {
-        const int i = j * 4 + (threadIdx.x >> 6);
-        const floatx4 *from = (const floatx4 *)a.part_o + ((int64_t)blockIdx.x * (8 * Keys::DB) + i) * 64 + lane;
-        floatx4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int p = 0; p < at.pieces; ++p) x += from[p * part];
-        Keys::store(a, at, key, i, lane >> 5, x);
-    }
+        for (int j = 0; j < kSumPieces<KEYS>; ++j) x[j] += from[p * part + (i0 + 4 * kEach * j) * 64];
+#pragma unroll
+    for (int j = 0; j < kSumPieces<KEYS>; ++j) Keys::store(a, at, key, i0 + 4 * kEach * j, lane >> 5, x[j]);
 }
 
 // dq.  A wave holds 32 rows: q and do as operands, the sums of dq turned.  Per tile of 32 keys in LDS: S^T = K Q^T, dP^T = V dO^T, then
@@ -708,7 +711,7 @@ hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, 
     hipError_t e = hipSuccess;
     if (q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * NW), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
     if (e == hipSuccess && kv_grid) e = keys == kKeys ? launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a) : launch(dkv_few, dim3(kv_grid), dim3(64 * NW), 0, st, a);
-    if (e == hipSuccess && kv_grid && a.n_split > 1) e = launch(sum, dim3(kv_grid / a.n_split * (keys / 32)), dim3(256), 0, st, a);
+    if (e == hipSuccess && kv_grid && a.n_split > 1) e = launch(sum, dim3(kv_grid / a.n_split * (keys / 32) * (DP / 16) / (keys == kKeys ? kSumPieces<kKeys> : 1)), dim3(256), 0, st, a);
     if (e == hipSuccess && a.dslopes) e = launch(sddmm_attention_dslopes_kernel, dim3((unsigned)a.n_heads), dim3(256), 0, st, b);
     return e;
 }

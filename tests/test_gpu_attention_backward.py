@@ -138,3 +138,12 @@ def test_against_differences(cap, bias, left):
         want = (sums[0] - sums[1]) / 2e-2
         got = float((base.ds.cpu().double() * base.slopes.double()).sum())
         assert abs(got - want) <= 2e-2 * float((base.ds.cpu().double() ** 2).sum().sqrt() + 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [24, 64, 104])
+@pytest.mark.parametrize("packed", [True, False])
+def test_keys_whose_rows_are_cut(dtype, dim, packed):
+    # 16 heads' rows to each of some tiles of 128 keys, and of 32
+    check(backward(Case(dtype, [(720, 720), (33, 33)], 16, 1, dim, -1, 0, packed=packed)))
+    check(backward(Case(dtype, [(210, 210), (5, 5)], 16, 1, dim, -1, 0, packed=packed)))
