@@ -543,8 +543,10 @@ int sddmm_csr_noalloc(int64_t n_rows, int64_t n_cols, int64_t nnz, const int32_t
  * NaNs in keys that a row does not see do not reach it; in values (backwards, in rows
  * of q, out and d_out) they may where a row of the same 64 keys or 128 rows meets them.
  * Lengths and pointers of sequences live on the device and are not validated: q_ptr
- * and k_ptr must rise from 0 and end at q_rows and k_rows at most; q_len and k_len
- * are taken as 0 .. max_q and 0 .. max_k.
+ * and k_ptr must rise, end at q_rows and k_rows at most, and give no sequence more than
+ * max_q and max_k; others are held to these bounds, so that results are wrong but
+ * nothing outside the arrays is touched.  q_len and k_len are taken as 0 .. max_q and
+ * 0 .. max_k.
  *
  * Calls allocate nothing, launch on `stream` only (a stream of the current device) and
  * may be captured into a graph.

@@ -68,6 +68,10 @@ int check_desc(const char *who, const sddmm_attention_desc *p)
     return SDDMM_OK;
 }
 
+// Rows and keys of all sequences (0 where none can have any, whatever the arrays hold).
+int64_t rows_of(const sddmm_attention_desc &d) { return d.n_seq == 0 || d.max_q == 0 ? 0 : d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q; }
+int64_t key_rows_of(const sddmm_attention_desc &d) { return d.n_seq == 0 || d.max_k == 0 ? 0 : d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k; }
+
 // How a call's rows are dealt out.
 struct Deal {
     int64_t rows = 0;          // of all sequences
@@ -91,7 +95,7 @@ Deal deal(const sddmm_attention_desc &d)
 {
     Deal r;
     const int64_t group = d.n_heads / d.n_kv_heads, tile = 128, few = kTokenRows;
-    r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
+    r.rows = rows_of(d);
     // keys that a tile's rows can see
     const int64_t span = d.window_left >= 0 && d.window_right >= 0 && !d.prefix ? (int64_t)d.window_left + d.window_right + std::min<int64_t>(d.max_q, tile) : d.max_k;
     const int64_t keys = std::min<int64_t>(d.max_k, span), seqs = d.q_ptr ? 1 : d.n_seq, packed = d.max_q * group;
@@ -147,8 +151,8 @@ DealBack deal_back(const sddmm_attention_desc &d)
 {
     DealBack r;
     const int64_t group = d.n_heads / d.n_kv_heads;
-    r.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
-    r.key_rows = d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k;
+    r.rows = rows_of(d);
+    r.key_rows = key_rows_of(d);
     if (r.rows > 0) {
         // (dq: us of the backward pass with 128, 64 and 32 rows: 4096 tokens, 16 heads of 128 358 / 343 / 411; 16 sequences of 512 163 / 174 / 175;
         // 2048 tokens, 4 heads 107 / 83 / 72)
@@ -207,8 +211,7 @@ AttnArgs arguments(const sddmm_attention_desc &d)
     a.q_seq = d.q_seq, a.q_row = d.q_row, a.q_head = d.q_head, a.k_seq = d.k_seq, a.k_row = d.k_row, a.k_head = d.k_head;
     a.v_seq = d.v_seq, a.v_row = d.v_row, a.v_head = d.v_head, a.o_seq = d.o_seq, a.o_row = d.o_row, a.o_head = d.o_head;
     a.q_ptr = d.q_ptr, a.k_ptr = d.k_ptr, a.q_len = d.q_len, a.k_len = d.k_len, a.prefix = d.prefix, a.slopes = d.slopes;
-    a.rows = d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q;
-    a.key_rows = d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k;
+    a.rows = rows_of(d), a.key_rows = key_rows_of(d);
     a.head_dim = d.head_dim, a.n_heads = d.n_heads, a.n_kv_heads = d.n_kv_heads, a.group = d.n_heads / d.n_kv_heads;
     a.n_seq = d.n_seq, a.max_q = d.max_q, a.max_k = d.max_k, a.left = std::min(d.window_left, 1 << 30), a.right = std::min(d.window_right, 1 << 30),  // (positions are below)
     a.shared_len = d.shared_len;
@@ -223,13 +226,22 @@ bool aligned(std::initializer_list<const void *> pointers)
     return true;
 }
 
+// Whether a result begins where an operand does (workgroups that are still to come read operands).
+bool in_place_of(std::initializer_list<const void *> results, std::initializer_list<const void *> operands)
+{
+    for (const void *r : results)
+        for (const void *o : operands)
+            if (r && r == o) return true;
+    return false;
+}
+
 int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d_q, const void *d_shared_k, const void *d_shared_v, const void *d_k,
                 const void *d_v, void *d_out, float *d_lse, void *d_workspace, int64_t workspace_bytes, void *stream)
 {
     const sddmm_attention_desc &d = *desc;
     const Deal r = deal(d);
-    if (r.rows == 0 || d.n_seq == 0) return SDDMM_OK;
-    const bool keys = d.k_ptr ? d.k_rows > 0 : d.max_k > 0;
+    if (r.rows == 0) return SDDMM_OK;
+    const bool keys = key_rows_of(d) > 0;
     if (!d_q || !d_out || (keys && (!d_k || !d_v)) || (d.shared_len && (!d_shared_k || !d_shared_v))) return fail(SDDMM_ERR_ARG, "%s: NULL device pointer", who);
     if (!apart(d, d.o_seq, d.o_row, d.o_head, d.q_ptr ? 1 : d.n_seq, d.q_ptr ? d.q_rows : d.max_q, d.n_heads)) return fail(SDDMM_ERR_ARG, "%s: rows of the result overlap", who);
     if ((uintptr_t)d_lse & 3u) return fail(SDDMM_ERR_ARG, "%s: lse must be aligned to its elements", who);
@@ -238,6 +250,7 @@ int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
     if (r.grid + r.shared_grid > INT32_MAX || (r.parts > 1 && r.rows * d.n_heads > INT32_MAX))
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
+    if (in_place_of({d_out}, {d_q, d_k, d_v, d_shared_k, d_shared_v})) return fail(SDDMM_ERR_ARG, "%s: the result is in an operand's place", who);
 
     AttnArgs a = arguments(d);
     a.q = d_q, a.k = d_k, a.v = d_v, a.out = d_out, a.lse = d_lse, a.shared_k = d_shared_k, a.shared_v = d_shared_v;
@@ -305,7 +318,7 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
     if (d.shared_len) return fail(SDDMM_ERR_ARG, "%s: shared_len is for sddmm_attention_shared", who);
     if (d_dslopes && !d.slopes) return fail(SDDMM_ERR_ARG, "%s: gradients of slopes that are not there", who);
     const DealBack r = deal_back(d);
-    if (d.n_seq == 0 || (r.rows == 0 && r.key_rows == 0 && !d_dslopes)) return SDDMM_OK;
+    if (r.rows == 0 && r.key_rows == 0 && !d_dslopes) return SDDMM_OK;
     if ((r.rows > 0 && (!d_q || !d_out || !d_lse || !d_dout || !d_dq)) || (r.key_rows > 0 && (!d_k || !d_v || !d_dk || !d_dv)))
         return fail(SDDMM_ERR_ARG, "%s: NULL device pointer", who);
     const int64_t q_seqs = d.q_ptr ? 1 : d.n_seq, k_seqs = d.k_ptr ? 1 : d.n_seq, q_rows = d.q_ptr ? d.q_rows : d.max_q, k_rows = d.k_ptr ? d.k_rows : d.max_k;
@@ -316,8 +329,10 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
     if (!aligned({d_q, d_k, d_v, d_out, d_dout, d_dq, d_dk, d_dv})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (r.q_grid > INT32_MAX || r.kv_grid > INT32_MAX / 32 || r.rows * d.n_heads / 16 > INT32_MAX || r.key_rows * d.n_kv_heads > INT32_MAX)
+    if (r.q_grid > INT32_MAX || r.kv_grid > INT32_MAX / 32)
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
+    if (in_place_of({d_dq, d_dk, d_dv}, {d_q, d_k, d_v, d_out, d_dout, d_lse}) || in_place_of({d_dq}, {d_dk, d_dv}) || in_place_of({d_dk}, {d_dv}))
+        return fail(SDDMM_ERR_ARG, "%s: a gradient is in an operand's or another gradient's place", who);
 
     AttnArgs a = arguments(d);
     char *ws = (char *)d_workspace;

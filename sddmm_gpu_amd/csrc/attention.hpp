@@ -255,7 +255,7 @@ __device__ __forceinline__ typename Elem<T>::Vec8 global_operand(const T *row, b
     return x;
 }
 
-// A sequence: where its rows and keys begin and how many there are.  Lengths from the device are held to their bounds.
+// A sequence: where its rows and keys begin and how many there are.  Lengths and places from the device are held to their bounds.
 struct Seq {
     int64_t q0, k0;  // first row and key, in rows of q_row and k_row (0 where sequences have strides of their own)
     int64_t lse0;    // first row in lse
@@ -265,16 +265,18 @@ __device__ __forceinline__ Seq sequence(const AttnArgs &a, int s)
 {
     Seq r;
     if (a.q_ptr) {
-        r.q0 = r.lse0 = a.q_ptr[s];
-        r.nq = max(0, a.q_ptr[s + 1] - a.q_ptr[s]);
+        const int first = min(max(0, a.q_ptr[s]), (int)a.rows);
+        r.q0 = r.lse0 = first;
+        r.nq = min(max(0, min(a.q_ptr[s + 1], (int)a.rows) - first), a.max_q);
     } else {
         r.q0 = 0;
         r.lse0 = (int64_t)s * a.max_q;
         r.nq = a.q_len ? min(max(0, a.q_len[s]), a.max_q) : a.max_q;
     }
     if (a.k_ptr) {
-        r.k0 = a.k_ptr[s];
-        r.nk = max(0, a.k_ptr[s + 1] - a.k_ptr[s]);
+        const int first = min(max(0, a.k_ptr[s]), (int)a.key_rows);
+        r.k0 = first;
+        r.nk = min(max(0, min(a.k_ptr[s + 1], (int)a.key_rows) - first), a.max_k);
     } else {
         r.k0 = 0;
         r.nk = a.k_len ? min(max(0, a.k_len[s]), a.max_k) : a.max_k;
@@ -310,7 +312,7 @@ __device__ __forceinline__ int slot_sequence(const int32_t *ptr, int n_seq, int 
     if (n_seq <= 64 && max_tiles <= 64) {
         const int lane = threadIdx.x & 63;
         int tiles = 0;
-        if (lane < n_seq) tiles = (max(0, ptr[lane + 1] - ptr[lane]) * per + size - 1) / size;
+        if (lane < n_seq) tiles = (int)min((max((int64_t)0, (int64_t)ptr[lane + 1] - ptr[lane]) * per + size - 1) / size, (int64_t)max_tiles);
         for (int r = max_tiles - 1; r >= 0; --r) {
             uint64_t some = __ballot(tiles > r);
             const int n = __builtin_popcountll(some);
@@ -328,10 +330,10 @@ __device__ __forceinline__ int slot_sequence(const int32_t *ptr, int n_seq, int 
     int lo = 0, hi = n_seq;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if ((int64_t)ptr[mid] * per / size + mid <= slot) lo = mid; else hi = mid;
+        if ((int64_t)max(0, ptr[mid]) * per / size + mid <= slot) lo = mid; else hi = mid;
     }
-    tile = slot - (int)((int64_t)ptr[lo] * per / size + lo);
-    return lo;
+    tile = slot - (int)min((int64_t)max(0, ptr[lo]) * per / size + lo, (int64_t)INT32_MAX);
+    return tile < 0 ? -1 : lo;
 }
 
 // The keys that a row at position pos sees: [lo, hi).

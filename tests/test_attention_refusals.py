@@ -132,3 +132,15 @@ def test_backward():
         backward(desc(n_seq=1 << 18, max_q=1 << 12, n_heads=65536, n_kv_heads=1, **HUGE), n=1 << 62)
     backward(desc(n_seq=0), *[0] * 9)
     backward(desc(max_q=0, max_k=0), *[0] * 9)
+
+
+def test_results_in_the_place_of_operands():
+    for name in ("q", "k", "v"):
+        with pytest.raises(capi.SddmmError, match="in an operand's place"):
+            forward(desc(), **dict(dict(q=A, k=A, v=A, out=4 * A), **{name: 4 * A}))
+    good = dict(q=A, k=2 * A, v=3 * A, out=4 * A, lse=5 * A, dout=6 * A, dq=7 * A, dk=8 * A, dv=9 * A)
+    for result in ("dq", "dk", "dv"):
+        for other in good:
+            if other != result:
+                with pytest.raises(capi.SddmmError, match="gradient's place"):
+                    backward(desc(), **dict(good, **{result: good[other]}))

@@ -147,3 +147,35 @@ def test_keys_whose_rows_are_cut(dtype, dim, packed):
     # 16 heads' rows to each of some tiles of 128 keys, and of 32
     check(backward(Case(dtype, [(720, 720), (33, 33)], 16, 1, dim, -1, 0, packed=packed)))
     check(backward(Case(dtype, [(210, 210), (5, 5)], 16, 1, dim, -1, 0, packed=packed)))
+
+
+@pytest.mark.parametrize("n", [3, 70])
+def test_packed_rows_that_begin_later(n):
+    for lens, heads in (([(5, 9)] * 3 + [(40, 40)] * n, 2), ([(300, 200)] + [(70, 90)] * n, 4)):
+        c = Case(BF16, lens, heads, 1, 64, -1, 0)
+        c.desc.q_ptr, c.desc.k_ptr, c.desc.n_seq = c.desc.q_ptr + 4, c.desc.k_ptr + 4, c.desc.n_seq - 1
+        c.lens, c.where, c.prefix = c.lens[1:], c.where[1:], c.prefix[1:]
+        backward(c)
+        c.check()
+        check(c)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [0, 66])
+def test_pointers_out_of_order_touch_nothing_outside(dtype, n):
+    c = Case(dtype, [(40, 40)] * (8 + n), 4, 2, 64, -1, 0)
+    c.keep["q_ptr"].copy_(torch.tensor(c.keep["q_ptr"].tolist()[:-8] + [30, 10 ** 9, -5, 2 ** 31 - 1, 200, -2 ** 31, 100, 10 ** 6]))
+    c.keep["k_ptr"].copy_(torch.tensor(c.keep["k_ptr"].tolist()[:-8] + [-2 ** 31, 2 ** 31 - 1, -7, 10 ** 9, 90, 50, 10 ** 6, 11]))
+    backward(c)
+    end = 40 * (8 + n)
+    for x in (c.out, c.dq, c.dk, c.dv):
+        assert (x[end:] == c.MARK).all()
+
+
+def test_no_sequences_leave_no_gradient_of_slopes():
+    c = Case(BF16, [(4, 4)], 4, 2, 64, bias=True)
+    c.desc.n_seq = 0
+    ds = torch.full((4,), 5.0, device=DEV)
+    assert capi.attention_workspace_bytes(c.desc)[1] == 0
+    capi.attention_backward(c.desc, 0, 0, 0, 0, 0, 0, 0, 0, 0, ds.data_ptr(), 0, 0)
+    assert (ds == 0).all()
