@@ -166,24 +166,23 @@ DealBack deal_back(const sddmm_attention_desc &d)
         }
     }
     if (r.key_rows > 0) {
-        // Tiles of 128 keys, or of 32 where all their rows together are so few that most waves would have none (us of forward and backward with 128 and 32:
-        // 3 sequences, 148 tokens in all, 16 heads over 2 of 96, fp32 125 and 100; 228 tokens, 8 over 2 of 128, fp16 53 and 44; 4370 tokens in a window
-        // of 410, 6 over 3 of 64, bf16 85 and 78; but 2898 tokens, 8 over 1 of 128 228 and 280).
+        // Work: rows of all heads that see a tile of 128 keys, of all tiles, at most.  That of uneven sequences is not known here: between the mean and the
+        // longest length.
         const bool window = d.window_left >= 0 && d.window_right >= 0 && !d.prefix;
-        int64_t workgroups = 0, most = 0;
-        double work = 0.;
-        for (int64_t keys : {128, 32}) {
-            r.keys = (int)keys;
-            r.kv_tiles = div_up(d.max_k, keys);
-            r.kv_slots = d.k_ptr ? r.key_rows / keys + d.n_seq : r.kv_tiles;
-            workgroups = r.kv_slots * (d.k_ptr ? 1 : d.n_seq) * d.n_kv_heads;
-            // Rows of all heads that see a tile, at most, and those of all tiles.  The work of uneven sequences is not known here: between the mean and
-            // the longest length.
-            most = group * (window ? std::min<int64_t>(d.max_q, (int64_t)d.window_left + d.window_right + keys) : d.max_q);
-            const double mean = d.k_ptr ? (double)r.key_rows / d.n_seq : d.max_k;
-            work = most * std::min(1., std::sqrt(mean / std::max(d.max_k, 1))) * (d.window_right == 0 && !window ? 0.5 : 1.) * div_up(r.key_rows, keys) * d.n_kv_heads;
-            if (work >= 32768.) break;
-        }
+        const double mean = d.k_ptr ? (double)r.key_rows / d.n_seq : d.max_k, uneven = std::min(1., std::sqrt(mean / std::max(d.max_k, 1))) * (d.window_right == 0 && !window ? 0.5 : 1.);
+        auto rows_that_see = [&](int64_t keys) { return group * (window ? std::min<int64_t>(d.max_q, (int64_t)d.window_left + d.window_right + keys) : d.max_q); };
+        double work = rows_that_see(128) * uneven * div_up(r.key_rows, 128) * d.n_kv_heads;
+        // Tiles of 128 keys; of 64, the waves of which share the rows, where the work of 128 is little (heads up to 64, since two workgroups' tiles of longer
+        // ones do not fit a compute unit); of 32 where it is so little that most waves would have none.  us of forward and backward, causal, bf16, heads of 64,
+        // with 128, 64 and 32: 2 sequences of 512, 12 heads (work 24,000) 40 / 37 / 32; 2 of 1024, 8 heads (65,000) 53 / 51 / 43, 8 over 2 56 / 55 / 54, capped
+        // 69 / 66 / 77; 4 of 1024, 12 heads (200,000) 83 / 70 / 85; 5999 tokens in 3, 12 heads (700,000) 239 / 211 / 233; 16,000 in 8 (1.7 million) 436 / 478 / 538.
+        // Heads of 128: 148 tokens in 3, 16 over 2, fp32 125 with 128 and 100 with 32; 228, 8 over 2, fp16 53 and 44; 2898, 8 over 1, bf16 228 and 280.
+        const double few = group == 1 ? 98304. : 32768.;
+        r.keys = work < few ? 32 : work < 1048576. && d.head_dim <= 64 ? 64 : 128;
+        r.kv_tiles = div_up(d.max_k, r.keys);
+        r.kv_slots = d.k_ptr ? r.key_rows / r.keys + d.n_seq : r.kv_tiles;
+        const int64_t workgroups = r.kv_slots * (d.k_ptr ? 1 : d.n_seq) * d.n_kv_heads, most = rows_that_see(r.keys);
+        work = most * uneven * div_up(r.key_rows, r.keys) * d.n_kv_heads;
         // A tile of keys that most rows see is cut where it would take more than 2.5 equal shares of all work.  A piece costs the time of some 650 rows, written
         // and read, so pieces of c rows cost 650 work / c and save half of c at the end: c = sqrt(1300 share).  us of the backward pass, bf16, causal, with
         // this and whole tiles: 8192 tokens, 16 heads over 4 of 128 1150 and 1853, 13 documents of 22 to 2281 tokens in all 8192 386 and

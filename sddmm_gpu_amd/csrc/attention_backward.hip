@@ -15,8 +15,7 @@ namespace sddmm {
 
 namespace {
 
-constexpr int kKeys = 128, kWaves = 4;  // keys of a workgroup of the dk, dv kernel, 32 to a wave
-constexpr int kFewKeys = 32;             // of the one for few keys
+constexpr int kWaves = 4, kFewKeys = 32;  // keys of a workgroup of the dk, dv kernel for few
 
 // scores in powers of two from products, and what their gradients have to be multiplied by on the way back
 template <bool MOD, class T>
@@ -164,6 +163,17 @@ struct DkvKeys {
                 f(4 * (DB + d) + i, floatx4{dv[d][4 * i], dv[d][4 * i + 1], dv[d][4 * i + 2], dv[d][4 * i + 3]});
             }
     }
+    template <class F> __device__ __forceinline__ void join(F f)
+    {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const floatx4 y = f(4 * d + i), z = f(4 * (DB + d) + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dk[d][4 * i + j] += y[j], dv[d][4 * i + j] += z[j];
+            }
+    }
     static __device__ __forceinline__ void store(const AttnArgs &a, const KeyTile &t, int key, int i, int h, floatx4 y)
     {
         typedef typename Elem<T>::Vec4 Vec4;
@@ -175,21 +185,24 @@ struct DkvKeys {
     }
 };
 
-// dk and dv of 128 keys; the four waves share the tiles of rows.  The query heads that share a key head follow each other in the same sums.
-template <class T, int DP, bool MOD>
+// dk and dv of 32 keys to each of KW waves, which share the tiles of rows.  The query heads that share a key head follow each other in the same sums.
+// With two such waves the other two take every second tile of rows, and the sums are joined at the end: twice the workgroups, of half the length.
+template <class T, int DP, bool MOD, int KW>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : 2)
 void sddmm_attention_dkv_kernel(const AttnArgs a)
 {
     typedef DkvKeys<T, DP, MOD> Keys;
     typedef typename Keys::Rows Rows;
+    constexpr int kKeys = 32 * KW, kTiles = kWaves / KW;  // tiles of rows in LDS together
     typedef Tile<T, DP, kKeys> Values;
     typedef typename Elem<T>::Vec8 Vec8;
     // (registers: 128 for the sums, 32 for k, 32 for a tile's scores; v would be 32 more than two waves to a SIMD leave)
     constexpr bool kKeepV = sizeof(T) == 4 || DP <= 64;
-    __shared__ __align__(1024) char lds[2][2][Rows::kBytes];
+    __shared__ __align__(1024) char lds[2][kTiles][2][Rows::kBytes];
     __shared__ __align__(1024) char values[kKeepV ? 16 : Values::kBytes];
-    __shared__ __align__(16) float stat[2][2][64];
+    __shared__ __align__(16) float stat[2][kTiles][2][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+    const int key_wave = wave % KW, part = wave / KW;
 
     KeyTile at;
     // (pieces outermost: next to each other they would go to different dies, the later ones, of which there are fewer, always to the same)
@@ -197,7 +210,7 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
     if (!key_tile<kKeys>(a, blockIdx.x - split * groups, at) || split >= at.pieces) return;
     const int row_bytes = a.head_dim * (int)sizeof(T), k0 = at.tile * kKeys;
     Keys keys;
-    keys.init(a, at, k0 + 32 * wave, lane);
+    keys.init(a, at, k0 + 32 * key_wave, lane);
     Vec8 vf[kKeepV ? DP / 16 : 1];
     {
         const T *v = v_base<T>(a, a.v, at.e, at.s, at.kv);
@@ -211,36 +224,52 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
     const int tiles = at.any_hi > at.any_lo ? (at.any_hi - at.any_lo + 31) / 32 : 0, all = tiles * a.group;
     const int each = (all + at.pieces - 1) / at.pieces, first = split * each, last = min(all, first + each);
     const uint32_t q_stride = (uint32_t)(a.q_row * sizeof(T)), o_stride = (uint32_t)(a.o_row * sizeof(T));
-    auto request = [&](int t) {
-        const int head = at.kv * a.group + t / tiles, row = at.any_lo + t % tiles * 32;
-        char *to = lds[t & 1][0];
-        Rows::template request<kWaves>(to, (const char *)(q_base<T>(a, a.q, at.e, at.s, head) + row * a.q_row), q_stride, at.e.nq - row, row_bytes, wave, lane);
-        Rows::template request<kWaves>(to + Rows::kBytes, (const char *)(o_base<T>(a, a.dout, at.e, at.s, head) + row * a.o_row), o_stride, at.e.nq - row, row_bytes, wave, lane);
-        if (wave < 2) request_floats<32>(stat[t & 1][wave], (wave ? a.stat_delta : a.stat_lse) + head * a.rows + at.e.lse0 + row, at.e.nq - row, lane);
+    auto request = [&](int t, int turn) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            if (t + i >= last) break;
+            const int head = at.kv * a.group + (t + i) / tiles, row = at.any_lo + (t + i) % tiles * 32;
+            char *to = lds[turn][i][0];
+            Rows::template request<kWaves>(to, (const char *)(q_base<T>(a, a.q, at.e, at.s, head) + row * a.q_row), q_stride, at.e.nq - row, row_bytes, wave, lane);
+            Rows::template request<kWaves>(to + Rows::kBytes, (const char *)(o_base<T>(a, a.dout, at.e, at.s, head) + row * a.o_row), o_stride, at.e.nq - row, row_bytes, wave, lane);
+            if (wave / 2 == i % 2) request_floats<32>(stat[turn][i][wave & 1], (wave & 1 ? a.stat_delta : a.stat_lse) + head * a.rows + at.e.lse0 + row, at.e.nq - row, lane);
+        }
     };
-    if (first < last) request(first);
-    for (int t = first; t < last; ++t) {
+    request(first, 0);
+    for (int t = first, turn = 0; t < last; t += kTiles, turn ^= 1) {
         tiles_arrived();
-        if (t + 1 < last) request(t + 1);
-        const float slope = MOD && a.slopes ? a.slopes[at.kv * a.group + t / tiles] * kLog2e : 0.f;
-        const int row = at.any_lo + t % tiles * 32;
+        request(t + kTiles, turn ^ 1);
+        const int mine = t + part;
+        if (kTiles > 1 && mine >= last) continue;
+        const float slope = MOD && a.slopes ? a.slopes[at.kv * a.group + mine / tiles] * kLog2e : 0.f;
+        const int row = at.any_lo + mine % tiles * 32;
         if (!keys.sees(row)) continue;
         int l = lane;  // (places in LDS made anew in every tile: kept, they would not fit the registers)
         asm volatile("" : "+v"(l));
-        keys.add(lds[t & 1][0], lds[t & 1][1], stat[t & 1][0], stat[t & 1][1], row, slope, l,
-                 [&](int c) { if constexpr (kKeepV) return vf[c]; else return Values::row_operand(values, 32 * wave, c, l); });
+        keys.add(lds[turn][part][0], lds[turn][part][1], stat[turn][part][0], stat[turn][part][1], row, slope, l,
+                 [&](int c) { if constexpr (kKeepV) return vf[c]; else return Values::row_operand(values, 32 * key_wave, c, l); });
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);  // (where there were no rows v may still be under way to LDS)
+    constexpr int kPart = 8 * Keys::DB * 64;  // pieces of 16 bytes of a wave's sums
+    if constexpr (KW < kWaves) {
+        static_assert(kTiles == 2 && KW * kPart * 16 <= (int)sizeof lds);
+        __syncthreads();
+        floatx4 *other = (floatx4 *)lds + key_wave * kPart + lane;
+        if (part) keys.pieces([&](int i, floatx4 y) { other[i * 64] = y; });
+        __syncthreads();
+        if (part) return;
+        keys.join([&](int i) { return other[i * 64]; });
+    }
     if (at.pieces > 1) {
         // parts of dk and dv as they lie in the registers: [part][workgroup][wave][piece][lane] of 16 bytes
-        floatx4 *to = (floatx4 *)a.part_o + ((int64_t)blockIdx.x * kWaves + wave) * (8 * Keys::DB * 64) + lane;
+        floatx4 *to = (floatx4 *)a.part_o + ((int64_t)blockIdx.x * KW + key_wave) * kPart + lane;
         keys.pieces([&](int i, floatx4 y) { to[i * 64] = y; });
         return;
     }
-    if constexpr (sizeof(T) == 2) __syncthreads();  // (the tiles have been read by all)
-    char *mine = (char *)lds + wave * 64 * DP;
+    if constexpr (sizeof(T) == 2 && KW == kWaves) __syncthreads();  // (the tiles have been read by all)
+    char *mine = (char *)lds + key_wave * (KW == kWaves ? 64 * DP : kPart * 16);
     static_assert(sizeof(T) == 4 || kWaves * 64 * DP <= (int)sizeof lds);
-    const int key0 = k0 + 32 * wave;
+    const int key0 = k0 + 32 * key_wave;
     store_turned<T, DP>(mine, keys.dk, a.scale, a.head_dim, lane,
                         [&](int r) { return key0 + r < at.e.nk ? (T *)k_base<T>(a, a.dk, at.e, at.s, at.kv) + (key0 + r) * a.k_row : nullptr; });
     store_turned<T, DP>(mine, keys.dv, 1.f, a.head_dim, lane,
@@ -327,7 +356,7 @@ void sddmm_attention_dkv_few_kernel(const AttnArgs a)
 
 // The sum of the parts of dk and dv of the keys whose rows were cut: pieces of four elements, one to a thread where there are few keys (us, 148 tokens, 16
 // heads over 2 of 96, fp32 9 with eight and 5 with one), two where there are many, whose workgroups would spend their time on finding their sequence.
-template <int KEYS> constexpr int kSumPieces = KEYS == kKeys ? 2 : 1;
+template <int KEYS> constexpr int kSumPieces = KEYS == kFewKeys ? 1 : 2;
 template <class T, int DP, int KEYS>
 __global__ __launch_bounds__(256)
 void sddmm_attention_dkv_sum_kernel(const AttnArgs a)
@@ -702,16 +731,19 @@ hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, 
 {
     const bool mod = a.cap > 0.f || a.slopes;
     constexpr int NW = 4;
-    const auto dkv = mod ? sddmm_attention_dkv_kernel<T, DP, true> : sddmm_attention_dkv_kernel<T, DP, false>;
     const auto dkv_few = mod ? sddmm_attention_dkv_few_kernel<T, DP, true, NW> : sddmm_attention_dkv_few_kernel<T, DP, false, NW>;
-    const auto sum = keys == kKeys ? sddmm_attention_dkv_sum_kernel<T, DP, kKeys> : sddmm_attention_dkv_sum_kernel<T, DP, kFewKeys>;
+    auto dkv = mod ? sddmm_attention_dkv_kernel<T, DP, true, 4> : sddmm_attention_dkv_kernel<T, DP, false, 4>;
+    auto sum = keys == kFewKeys ? sddmm_attention_dkv_sum_kernel<T, DP, kFewKeys> : sddmm_attention_dkv_sum_kernel<T, DP, 128>;
+    if constexpr (DP <= 64) {
+        if (keys == 64) dkv = mod ? sddmm_attention_dkv_kernel<T, DP, true, 2> : sddmm_attention_dkv_kernel<T, DP, false, 2>, sum = sddmm_attention_dkv_sum_kernel<T, DP, 64>;
+    }
     const auto dq = q_rows == 64 ? (mod ? sddmm_attention_dq_kernel<T, DP, true, 2> : sddmm_attention_dq_kernel<T, DP, false, 2>)
                                  : (mod ? sddmm_attention_dq_kernel<T, DP, true, 4> : sddmm_attention_dq_kernel<T, DP, false, 4>);
     const auto dq_few = mod ? sddmm_attention_dq_few_kernel<T, DP, true, NW> : sddmm_attention_dq_few_kernel<T, DP, false, NW>;
     hipError_t e = hipSuccess;
     if (q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * NW), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
-    if (e == hipSuccess && kv_grid) e = keys == kKeys ? launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a) : launch(dkv_few, dim3(kv_grid), dim3(64 * NW), 0, st, a);
-    if (e == hipSuccess && kv_grid && a.n_split > 1) e = launch(sum, dim3(kv_grid / a.n_split * (keys / 32) * (DP / 16) / (keys == kKeys ? kSumPieces<kKeys> : 1)), dim3(256), 0, st, a);
+    if (e == hipSuccess && kv_grid) e = keys == kFewKeys ? launch(dkv_few, dim3(kv_grid), dim3(64 * NW), 0, st, a) : launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a);
+    if (e == hipSuccess && kv_grid && a.n_split > 1) e = launch(sum, dim3(kv_grid / a.n_split * (keys / 32) * (DP / 16) / (keys == kFewKeys ? 1 : kSumPieces<128>)), dim3(256), 0, st, a);
     if (e == hipSuccess && a.dslopes) e = launch(sddmm_attention_dslopes_kernel, dim3((unsigned)a.n_heads), dim3(256), 0, st, b);
     return e;
 }
