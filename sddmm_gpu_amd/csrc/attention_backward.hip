@@ -701,8 +701,7 @@ void sddmm_attention_dq_few_kernel(const AttnArgs a)
     if (!rows.there) return;
     T *to = (T *)q_base<T>(a, a.dq, e, s, head) + row * a.q_row;
 #pragma unroll
-    for (int j = 0; j < 4 * DB / NW; ++j) {
-        const int piece = wave * (4 * DB / NW) + j;
+    for (int piece = wave; piece < 4 * DB; piece += NW) {
         floatx4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NW; ++i) y += ((const floatx4 *)lds[i][0])[piece * 64 + lane];
@@ -730,8 +729,16 @@ template <class T, int DP>
 hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, int keys, unsigned q_grid, int q_rows, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
-    constexpr int NW = 4;
-    const auto dkv_few = mod ? sddmm_attention_dkv_few_kernel<T, DP, true, NW> : sddmm_attention_dkv_few_kernel<T, DP, false, NW>;
+    // Waves of the kernels for few: 4, which share a compute unit with another workgroup's, or 8 where that is not to be had anyway, for 16-bit heads up to
+    // 64, whose tiles fit (us of forward and backward, causal, bf16, heads of 64, with 4 and 8: 1000 tokens, 8 heads over 2 55 and 48; 1013 in 2, 4 over 2,
+    // capped and biased 46 and 39; but 8 sequences of 512, 8 heads 50 and 61; fp32, heads of 32 50 and 48, 86 and 96).
+    constexpr int kMore = sizeof(T) == 2 && DP == 64 ? 8 : 4;
+    constexpr unsigned kUnits = 512;  // (workgroups that can be there together)
+    const int kv_waves = kv_grid <= kUnits ? kMore : 4, q_waves = q_grid <= kUnits ? kMore : 4;
+    const auto dkv_few = kv_waves == 4 ? (mod ? sddmm_attention_dkv_few_kernel<T, DP, true, 4> : sddmm_attention_dkv_few_kernel<T, DP, false, 4>)
+                                       : (mod ? sddmm_attention_dkv_few_kernel<T, DP, true, kMore> : sddmm_attention_dkv_few_kernel<T, DP, false, kMore>);
+    const auto dq_few = q_waves == 4 ? (mod ? sddmm_attention_dq_few_kernel<T, DP, true, 4> : sddmm_attention_dq_few_kernel<T, DP, false, 4>)
+                                     : (mod ? sddmm_attention_dq_few_kernel<T, DP, true, kMore> : sddmm_attention_dq_few_kernel<T, DP, false, kMore>);
     auto dkv = mod ? sddmm_attention_dkv_kernel<T, DP, true, 4> : sddmm_attention_dkv_kernel<T, DP, false, 4>;
     auto sum = keys == kFewKeys ? sddmm_attention_dkv_sum_kernel<T, DP, kFewKeys> : sddmm_attention_dkv_sum_kernel<T, DP, 128>;
     if constexpr (DP <= 64) {
@@ -739,10 +746,9 @@ hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, 
     }
     const auto dq = q_rows == 64 ? (mod ? sddmm_attention_dq_kernel<T, DP, true, 2> : sddmm_attention_dq_kernel<T, DP, false, 2>)
                                  : (mod ? sddmm_attention_dq_kernel<T, DP, true, 4> : sddmm_attention_dq_kernel<T, DP, false, 4>);
-    const auto dq_few = mod ? sddmm_attention_dq_few_kernel<T, DP, true, NW> : sddmm_attention_dq_few_kernel<T, DP, false, NW>;
     hipError_t e = hipSuccess;
-    if (q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * NW), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
-    if (e == hipSuccess && kv_grid) e = keys == kFewKeys ? launch(dkv_few, dim3(kv_grid), dim3(64 * NW), 0, st, a) : launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a);
+    if (q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * q_waves), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
+    if (e == hipSuccess && kv_grid) e = keys == kFewKeys ? launch(dkv_few, dim3(kv_grid), dim3(64 * kv_waves), 0, st, a) : launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a);
     if (e == hipSuccess && kv_grid && a.n_split > 1) e = launch(sum, dim3(kv_grid / a.n_split * (keys / 32) * (DP / 16) / (keys == kFewKeys ? 1 : kSumPieces<128>)), dim3(256), 0, st, a);
     if (e == hipSuccess && a.dslopes) e = launch(sddmm_attention_dslopes_kernel, dim3((unsigned)a.n_heads), dim3(256), 0, st, b);
     return e;
