@@ -354,21 +354,42 @@ void sddmm_attention_dkv_few_kernel(const AttnArgs a)
     }
 }
 
+// The slopes' gradients: a head's parts in a fixed order.  A kernel of their own, or further workgroups of the one below, whose launch they then share.
+__device__ __forceinline__ void sum_slopes(const AttnArgs &a, int head)
+{
+    __shared__ double sums[256];
+    double x = 0.;
+    for (int p = threadIdx.x; p < a.slope_parts; p += 256) x += a.slope_part[(int64_t)head * a.slope_parts + p];
+    sums[threadIdx.x] = x;
+    __syncthreads();
+    for (int d = 128; d > 0; d /= 2) {
+        if ((int)threadIdx.x < d) sums[threadIdx.x] += sums[threadIdx.x + d];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) a.dslopes[head] = (float)sums[0];
+}
+__global__ __launch_bounds__(256)
+void sddmm_attention_dslopes_kernel(const AttnArgs a) { sum_slopes(a, blockIdx.x); }
+
 // The sum of the parts of dk and dv of the keys whose rows were cut: pieces of four elements, one to a thread where there are few keys (us, 148 tokens, 16
 // heads over 2 of 96, fp32 9 with eight and 5 with one), two where there are many, whose workgroups would spend their time on finding their sequence.
 template <int KEYS> constexpr int kSumPieces = KEYS == kFewKeys ? 1 : 2;
 template <class T, int DP, int KEYS>
 __global__ __launch_bounds__(256)
-void sddmm_attention_dkv_sum_kernel(const AttnArgs a)
+void sddmm_attention_dkv_sum_kernel(const AttnArgs a, const int n_sum)
 {
     typedef DkvKeys<T, DP, false> Keys;
+    if ((int)blockIdx.x >= n_sum) {
+        sum_slopes(a, blockIdx.x - n_sum);
+        return;
+    }
     constexpr int kEach = 2 * Keys::DB / kSumPieces<KEYS>;  // workgroups to 32 keys
     KeyTile at;
     const int unit = blockIdx.x / kEach;
     if (!key_tile<KEYS>(a, unit / (KEYS / 32), at) || at.pieces == 1) return;
     const int lane = threadIdx.x & 63, key = at.tile * KEYS + unit % (KEYS / 32) * 32 + (lane & 31), i0 = blockIdx.x % kEach * 4 + (threadIdx.x >> 6);
     if (key >= at.e.nk) return;
-    const int64_t part = (int64_t)(gridDim.x / kEach) * (8 * Keys::DB * 64);
+    const int64_t part = (int64_t)(n_sum / kEach) * (8 * Keys::DB * 64);
     const floatx4 *from = (const floatx4 *)a.part_o + (int64_t)unit * (8 * Keys::DB * 64) + lane;
     floatx4 x[kSumPieces<KEYS>] = {};
 #pragma unroll 8 / kSumPieces<KEYS>
@@ -709,22 +730,6 @@ void sddmm_attention_dq_few_kernel(const AttnArgs a)
     }
 }
 
-// The slopes' gradients: a head's parts in a fixed order.
-__global__ __launch_bounds__(256)
-void sddmm_attention_dslopes_kernel(const AttnArgs a)
-{
-    __shared__ double sums[256];
-    double x = 0.;
-    for (int p = threadIdx.x; p < a.slope_parts; p += 256) x += a.slope_part[(int64_t)blockIdx.x * a.slope_parts + p];
-    sums[threadIdx.x] = x;
-    __syncthreads();
-    for (int d = 128; d > 0; d /= 2) {
-        if ((int)threadIdx.x < d) sums[threadIdx.x] += sums[threadIdx.x + d];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) a.dslopes[blockIdx.x] = (float)sums[0];
-}
-
 template <class T, int DP>
 hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, int keys, unsigned q_grid, int q_rows, hipStream_t st)
 {
@@ -749,8 +754,10 @@ hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, 
     hipError_t e = hipSuccess;
     if (q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * q_waves), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
     if (e == hipSuccess && kv_grid) e = keys == kFewKeys ? launch(dkv_few, dim3(kv_grid), dim3(64 * kv_waves), 0, st, a) : launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a);
-    if (e == hipSuccess && kv_grid && a.n_split > 1) e = launch(sum, dim3(kv_grid / a.n_split * (keys / 32) * (DP / 16) / (keys == kFewKeys ? 1 : kSumPieces<128>)), dim3(256), 0, st, a);
-    if (e == hipSuccess && a.dslopes) e = launch(sddmm_attention_dslopes_kernel, dim3((unsigned)a.n_heads), dim3(256), 0, st, b);
+    const unsigned n_sum = kv_grid && a.n_split > 1 ? kv_grid / a.n_split * (keys / 32) * (DP / 16) / (keys == kFewKeys ? 1 : kSumPieces<128>) : 0;
+    const unsigned n_slopes = a.dslopes ? a.n_heads : 0;
+    if (e == hipSuccess && n_sum) e = launch(sum, dim3(n_sum + n_slopes), dim3(256), 0, st, a, (int)n_sum);
+    else if (e == hipSuccess && n_slopes) e = launch(sddmm_attention_dslopes_kernel, dim3(n_slopes), dim3(256), 0, st, a);
     return e;
 }
 
