@@ -100,7 +100,7 @@ Deal deal(const sddmm_attention_desc &d)
     const int64_t span = d.window_left >= 0 && d.window_right >= 0 && !d.prefix ? (int64_t)d.window_left + d.window_right + std::min<int64_t>(d.max_q, tile) : d.max_k;
     const int64_t keys = std::min<int64_t>(d.max_k, span), seqs = d.q_ptr ? 1 : d.n_seq, packed = d.max_q * group;
     // Tiles of 128 rows where that makes 1024 workgroups, else of 64 (us of the forward pass, causal, with 128, 64 and 32: 4096 tokens, 16 heads of 128,
-    // bf16 98 / 93 / 114; 16 sequences of 512 44 / 57 / 88; 2048 tokens, 16 heads of 64 34 / 26 / 21, fp32 155 / 108 / 88; 2048, 4 of 128 43 / 30 / 23),
+    // bf16 111 / 102 / 123; 16 sequences of 512 40 / 51 / 88; 2048 tokens, 16 heads of 64 38 / 25 / 21, fp32 156 / 109 / 89; 2048, 4 of 128 42 / 29 / 23),
     // of one head or of pairs of few tokens and the heads that share a key head (not in packed sequences);
     for (int64_t tile : {128, 64}) {
         r.tile = (int)tile;
@@ -116,17 +116,17 @@ Deal deal(const sddmm_attention_desc &d)
         r.max_tiles = div_up(packed, few);
         r.slots = r.max_tiles == 1 ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
         r.grid = r.slots * d.n_kv_heads;
-        // Few workgroups: pieces of 256 keys, two for each wave (one user, 1501 keys, 32 heads over 8: with 64 / 128 / 256 / 512 12.1 / 11.4 / 11.7 / 13.1 us); up to
+        // Few workgroups: pieces of 256 keys, two for each wave (one user, 1501 keys, 32 heads over 8: with 64 / 128 / 256 / 512 12.9 / 13.3 / 12.6 / 12.9 us, most of it two launches); up to
         // 768 keys a second launch costs more than it saves.
         // Where each workgroup has a cache of its own four times as many even out their lengths (64 users of 284 to 8192 keys: 512 / 1024 / 2048 / 4096
-        // workgroups 232 / 221 / 210 / 214 us), which short ones do not pay for with a second launch.
+        // workgroups 232 / 218 / 207 / 214 us), which short ones do not pay for with a second launch.
         r.splits = r.max_tiles == 1 && r.grid >= kFill ? pieces(r.grid, keys, 1024, 4 * kFill) : keys <= 768 ? 1 : pieces(r.grid, keys, 256, d.shared_len > 0 ? kFill / 2 : kFill);
         r.grid *= r.splits;
     }
     r.parts = r.splits;
     if (d.shared_len > 0) {
         // Tiles of 64 rows up to 256 rows of a key head, and one workgroup of them for each compute unit beside the others' (48 users behind 16,000 keys: 128, 256, 512
-        // of them 50, 43 and 47 us).
+        // of them 49, 38 to 46 and 46 us).
         r.shared_tile = r.rows * group <= 256 ? 64 : 128;
         r.shared_slots = div_up(r.rows * group, r.shared_tile);
         r.shared_splits = pieces(r.shared_slots * d.n_kv_heads, d.shared_len, 256, kFill / 2);
@@ -154,8 +154,8 @@ DealBack deal_back(const sddmm_attention_desc &d)
     r.rows = rows_of(d);
     r.key_rows = key_rows_of(d);
     if (r.rows > 0) {
-        // (dq: us of the backward pass with 128, 64 and 32 rows: 4096 tokens, 16 heads of 128 358 / 343 / 411; 16 sequences of 512 163 / 174 / 175;
-        // 2048 tokens, 4 heads 107 / 83 / 72)
+        // (dq: us of the backward pass with 128, 64 and 32 rows: 4096 tokens, 16 heads of 128 351 / 341 / 402; 16 sequences of 512 123 / 142 / 228;
+        // 2048 tokens, 4 heads 101 / 82 / 66)
         for (int64_t rows : {128, 64, 32}) {
             r.q_rows = (int)rows;
             r.q_tiles = div_up(d.max_q, rows);
@@ -174,9 +174,9 @@ DealBack deal_back(const sddmm_attention_desc &d)
         double work = rows_that_see(128) * uneven * div_up(r.key_rows, 128) * d.n_kv_heads;
         // Tiles of 128 keys; of 64, the waves of which share the rows, where the work of 128 is little (heads up to 64, since two workgroups' tiles of longer
         // ones do not fit a compute unit); of 32 where it is so little that most waves would have none.  us of forward and backward, causal, bf16, heads of 64,
-        // with 128, 64 and 32: 2 sequences of 512, 12 heads (work 24,000) 40 / 37 / 32; 2 of 1024, 8 heads (65,000) 53 / 51 / 43, 8 over 2 56 / 55 / 54, capped
-        // 69 / 66 / 77; 4 of 1024, 12 heads (200,000) 83 / 70 / 85; 5999 tokens in 3, 12 heads (700,000) 239 / 211 / 233; 16,000 in 8 (1.7 million) 436 / 478 / 538.
-        // Heads of 128: 148 tokens in 3, 16 over 2, fp32 125 with 128 and 100 with 32; 228, 8 over 2, fp16 53 and 44; 2898, 8 over 1, bf16 228 and 280.
+        // with 128, 64 and 32: 2 sequences of 512, 12 heads (work 24,000) 45 / 43 / 42; 2 of 1024, 8 heads (65,000) 53 / 51 / 43, 8 over 2 55 / 53 / 54, capped
+        // 68 / 66 / 76; 4 of 1024, 12 heads (200,000) 83 / 69 / 84; 5999 tokens in 3, 12 heads (700,000) 218 / 209 / 226; 16,000 in 8 (1.7 million) 442 / 475 / 538.
+        // Heads of 128, with 128 and 32: 148 tokens in 3, 16 over 2, fp32 112 and 62; 228, 8 over 2, fp16 46 and 48; 2898, 8 over 1, bf16 220 and 276.
         const double few = group == 1 ? 98304. : 32768.;
         r.keys = work < few ? 32 : work < 1048576. && d.head_dim <= 64 ? 64 : 128;
         r.kv_tiles = div_up(d.max_k, r.keys);
@@ -185,8 +185,8 @@ DealBack deal_back(const sddmm_attention_desc &d)
         work = most * uneven * div_up(r.key_rows, r.keys) * d.n_kv_heads;
         // A tile of keys that most rows see is cut where it would take more than 2.5 equal shares of all work.  A piece costs the time of some 650 rows, written
         // and read, so pieces of c rows cost 650 work / c and save half of c at the end: c = sqrt(1300 share).  us of the backward pass, bf16, causal, with
-        // this and whole tiles: 8192 tokens, 16 heads over 4 of 128 1150 and 1853, 13 documents of 22 to 2281 tokens in all 8192 386 and
-        // 590; 4096, 16 over 2 390 and 1537; 2048, 16 over 4 of 64 104 and 300; where whole tiles stay: 8192, 16 over 16 1020, in pieces of 3600 1076.
+        // this and whole tiles: 8192 tokens, 16 heads over 4 of 128 1130 and 1850; 4096, 16 over 2 390 and 1550; 2048, 16 over 4 of 64 80 and 186; forward and
+        // backward of 13 documents of 22 to 2281 tokens in all 8192 345 and 574; where whole tiles stay: 8192, 16 over 16 1015, in pieces 1090.
         const int64_t places = r.keys == 32 || (d.type == SDDMM_TYPE_F32 && d.head_dim > 64) ? kFill / 2 : kFill;
         const double share = work / places;
         if (most > 2.5 * share) {
