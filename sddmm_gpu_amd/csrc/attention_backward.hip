@@ -9,7 +9,7 @@
 // statistics (lse in powers of two, delta; [n_heads][rows]) for the second.
 //
 // Roundings with 16-bit operands: P and dt to the element type, as operands; delta comes from the rounded output.  With bf16 dq and dk are off by 0.0025
-// of their size where rounding the results alone makes 0.0017 (fp32 operands: 3e-7).  A second operand for what dt loses would be two of nine products more.
+// of their size where rounding the results alone makes 0.0017 (fp32 operands: 3e-7).  A second operand for what dt loses would be two products beside seven.
 //
 // 8192 tokens, causal, 16 heads of 128, bf16: dq 0.45 ms and dk, dv 0.61 ms, 0.92 and 0.90 PFLOP/s of their products (a large library product 1.17);
 // fp32, 4096 tokens, 16 heads of 64 1.2 ms, 98 TFLOP/s (154): matrix and vector instructions of a SIMD, which alternate, bound both.
@@ -741,16 +741,17 @@ template <class T, int DP>
 hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, int keys, unsigned q_grid, int q_rows, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
-    // Waves of the kernels for few: 4, which share a compute unit with another workgroup's, or 8 where that is not to be had anyway, for 16-bit heads up to
-    // 64, whose tiles fit (us of forward and backward, causal, bf16, heads of 64, with 4 and 8: 1000 tokens, 8 heads over 2 55 and 48; 1013 in 2, 4 over 2,
-    // capped and biased 46 and 39; but 8 sequences of 512, 8 heads 50 and 61; fp32, heads of 32 50 and 48, 86 and 96).
-    constexpr int kMore = sizeof(T) == 2 && DP == 64 ? 8 : 4;
+    // Waves of the kernels for few: 4, which share a compute unit with another workgroup's, or 8 where that is not to be had anyway and their tiles fit: 16-bit
+    // heads up to 64 (us of forward and backward, causal, bf16, heads of 64, with 4 and 8: 1000 tokens, 8 heads over 2 55 and 48; 1013 in 2, 4 over 2, capped and
+    // biased 46 and 39; but 8 sequences of 512, 8 heads, which fill the card, 50 and 61), and dq of fp32 heads up to 32 (the second of these 72 and 66; with
+    // dk and dv as well 73, and 1000 tokens, 8 over 2 86 and 96).
+    constexpr int kMore = sizeof(T) == 2 && DP == 64 ? 8 : 4, kMoreQ = sizeof(T) * DP <= 128 ? 8 : 4;
     constexpr unsigned kUnits = 512;  // (workgroups that can be there together)
-    const int kv_waves = kv_grid <= kUnits ? kMore : 4, q_waves = q_grid <= kUnits ? kMore : 4;
+    const int kv_waves = kv_grid <= kUnits ? kMore : 4, q_waves = q_grid <= kUnits ? kMoreQ : 4;
     const auto dkv_few = kv_waves == 4 ? (mod ? sddmm_attention_dkv_few_kernel<T, DP, true, 4> : sddmm_attention_dkv_few_kernel<T, DP, false, 4>)
                                        : (mod ? sddmm_attention_dkv_few_kernel<T, DP, true, kMore> : sddmm_attention_dkv_few_kernel<T, DP, false, kMore>);
     const auto dq_few = q_waves == 4 ? (mod ? sddmm_attention_dq_few_kernel<T, DP, true, 4> : sddmm_attention_dq_few_kernel<T, DP, false, 4>)
-                                     : (mod ? sddmm_attention_dq_few_kernel<T, DP, true, kMore> : sddmm_attention_dq_few_kernel<T, DP, false, kMore>);
+                                     : (mod ? sddmm_attention_dq_few_kernel<T, DP, true, kMoreQ> : sddmm_attention_dq_few_kernel<T, DP, false, kMoreQ>);
     auto dkv = mod ? sddmm_attention_dkv_kernel<T, DP, true, 4> : sddmm_attention_dkv_kernel<T, DP, false, 4>;
     auto sum = keys == kFewKeys ? sddmm_attention_dkv_sum_kernel<T, DP, kFewKeys> : sddmm_attention_dkv_sum_kernel<T, DP, 128>;
     if constexpr (DP <= 64) {

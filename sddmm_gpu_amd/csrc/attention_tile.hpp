@@ -13,7 +13,7 @@ constexpr int kWaves = 4;  // of a workgroup, 32 rows to each
 // two halves of the wave; the probabilities are the second operand of O^T += V^T P^T as they lie.  The maximum is raised only
 // when a row's exceeds it by more than 2^8: the sums stay far inside fp32, and the sums of o are rarely scaled.
 // P is rounded to the element type (bf16: half a step is 2^-9 of the step's upper end, as for the output itself), its sum is not: the output is off by
-// 0.0020 of its size where rounding it alone makes 0.0016; a second operand for what P loses would be a third of all products more.
+// 0.0020 of its size where rounding it alone makes 0.0016; a second operand for what P loses would be a third product beside two.
 //
 // What bounds it: matrix and vector instructions about alike, each half of the time on long prompts, with the clock at 1.9 GHz under the power limit.
 // 16,384 tokens, causal, 16 heads over 2 of 128, bf16: 1.03 ms = 1.06 PFLOP/s, where a large library product reaches 1.17; 8192 tokens, 16 heads of 128
