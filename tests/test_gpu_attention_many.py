@@ -87,7 +87,7 @@ def test_shared_keys(dtype, dim, mod, n):
 
 
 @kinds
-@pytest.mark.parametrize("n,length", [(20, 128), (3, 50)])
+@pytest.mark.parametrize("n,length", [(20, 128), (28, 128), (3, 50)])
 def test_few_rows_and_keys(dtype, dim, mod, n, length):
     some(backward(Case(dtype, lengths(n, length, seed=1), 8, 8, dim, -1, 0, prefix=[30] * n, **scores(mod))))
 
