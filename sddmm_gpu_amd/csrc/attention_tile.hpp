@@ -37,6 +37,10 @@ template <class T, int DP, bool MOD, int ROWS, int RW>
 __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const AttnArgs &a, int b, char (&memory)[kLds])
 {
     constexpr int KB = KT / 32 / (kWaves / RW), DB = DP / 32, kRows = 32 * RW;
+    // A wave that is at its softmax goes before another one of its SIMD that is at its products, so that one's vector instructions run beside the other's products; its
+    // second products too, where scores are not bent (us, causal: 8192 tokens, 16 heads of 128, bf16 305 without, 289 and 286; 16,384, 16 over 2 1010, 998 and
+    // 991; 4096, 16 over 4, capped 122, 108 and 112; 4096, 16 of 64, fp32 312, 288 and 288; but 16 sequences of 512 39, 40 and 41, and heads of 64, fp16 175, 194 and 181).
+    constexpr bool kSoftFirst = MOD || sizeof(T) == 4 || DP == 128, kProductToo = !MOD && sizeof(T) == 2;
     typedef typename Elem<T>::Vec8 Vec8;
     auto &lds = *(char (*)[2][2][Keys::kBytes])memory;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
@@ -164,6 +168,7 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
 #pragma unroll
             for (int i = 0; i < KB; ++i) x[i] = Elem<T>::mma(Keys::row_operand(kt, 32 * (half * KB + i), c, l), qf[c], x[i]);
 
+        if constexpr (kSoftFirst) __builtin_amdgcn_s_setprio(1);
         if constexpr (MOD) {
             if (bend.cap > 0.f) {
                 bend.template apply<KB, false>(x, x);
@@ -211,6 +216,7 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
                 x[i][r] = __builtin_amdgcn_exp2f(fmaf(x[i][r], unit, -base));
                 sum += x[i][r];
             }
+        if constexpr (kSoftFirst && !kProductToo) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int i = 0; i < KB; ++i)
 #pragma unroll
@@ -219,6 +225,7 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
 #pragma unroll
                 for (int d = 0; d < DB; ++d) o[d] = Elem<T>::mma(Keys::column_operand(vt, d, 2 * (half * KB + i) + c, l), p, o[d]);
             }
+        if constexpr (kSoftFirst && kProductToo) __builtin_amdgcn_s_setprio(0);
     }
 
     sum = halves_sum(sum);
