@@ -26,7 +26,7 @@ struct AttnArgs {
     void *dq, *dk, *dv;
     float *part_o;              // partial results of split keys: [part][row of all heads][head_dim]
     float2 *part_ml;            // [part][row of all heads]: maximum (in powers of two) and sum
-    float *stat_lse, *stat_delta;  // backward: [n_heads][all rows] log-sum-exp in powers of two, sum of dout * out
+    float *stat_lse, *stat_delta;  // backward: [n_heads][all rows] log-sum-exp in powers of two, - sum of dout * out
     double *slope_part;         // backward: [n_heads][slope_parts] parts of the slopes' gradients, or null
     float *dslopes;
     int64_t q_seq, q_row, q_head, k_seq, k_row, k_head, v_seq, v_row, v_head, o_seq, o_row, o_head;

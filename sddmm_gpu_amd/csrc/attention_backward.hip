@@ -121,10 +121,20 @@ struct DkvKeys {
         if constexpr (MOD) bend.init(a.scale, a.cap);
     }
     __device__ __forceinline__ bool sees(int row) const { return row + 32 > wave_lo && row < wave_hi; }
-    // rows `row` on: their tiles, log-sum-exps and deltas; v(c): 16 elements of v as an operand
-    template <class V> __device__ __forceinline__ void add(const char *qt, const char *dot, const float *lse, const float *delta, int row, float slope, int l, V v)
+    // EARLY: dP begins at - delta, a subtraction less for each score, where registers are left (300 tokens, 16 heads over 4 of 128, bf16 40 and 38 us; in the kernel of
+    // whole tiles they are not: 960 and 1060 us).
+    // rows `row` on: their tiles, log-sum-exps and - deltas; v(c): 16 elements of v as an operand
+    template <bool EARLY, class V> __device__ __forceinline__ void add(const char *qt, const char *dot, const float *lse, const float *minus_delta, int row, float slope, int l, V v)
     {
         floatx16 x = zero16(), y = zero16(), back;
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const floatx4 d = *(const floatx4 *)(minus_delta + 8 * i + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[4 * i + j] = d[j];
+            }
+        }
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) x = Elem<T>::mma(Rows::row_operand(qt, 0, c, l), kf[c], x);
 #pragma unroll
@@ -133,11 +143,13 @@ struct DkvKeys {
         scores<MOD, T>(x, back, bend, unit, bias, slope, (float)(row + 4 * h + shift - key), 1.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const floatx4 m = *(const floatx4 *)(lse + 8 * i + 4 * h), d = *(const floatx4 *)(delta + 8 * i + 4 * h);
+            const floatx4 m = *(const floatx4 *)(lse + 8 * i + 4 * h);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[4 * i + j] = __builtin_amdgcn_exp2f(x[4 * i + j] - m[j]);
-                y[4 * i + j] -= d[j];
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = __builtin_amdgcn_exp2f(x[4 * i + j] - m[j]);
+            if constexpr (!EARLY) {
+                const floatx4 d = *(const floatx4 *)(minus_delta + 8 * i + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[4 * i + j] += d[j];
             }
         }
         if (row < full_lo || row + 32 > full_hi) {
@@ -262,7 +274,7 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
         if (!keys.sees(row)) continue;
         int l = lane;  // (places in LDS made anew in every tile: kept, they would not fit the registers)
         asm volatile("" : "+v"(l));
-        keys.add(lds[turn][part][0], lds[turn][part][1], stat[turn][part][0], stat[turn][part][1], row, slope, l,
+        keys.template add<false>(lds[turn][part][0], lds[turn][part][1], stat[turn][part][0], stat[turn][part][1], row, slope, l,
                  [&](int c) { if constexpr (kKeepV) return vf[c]; else return Values::row_operand(values, 32 * key_wave, c, l); });
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);  // (where there were no rows v may still be under way to LDS)
@@ -345,7 +357,7 @@ void sddmm_attention_dkv_few_kernel(const AttnArgs a)
         const float slope = MOD && a.slopes ? a.slopes[at.kv * a.group + t / tiles] * kLog2e : 0.f;
         const int row = at.any_lo + t % tiles * 32;
         if (keys.sees(row)) {
-            keys.add(lds[wave][turn][0], lds[wave][turn][1], stat[wave][turn][0], stat[wave][turn][1], row, slope, lane,
+            keys.template add<true>(lds[wave][turn][0], lds[wave][turn][1], stat[wave][turn][0], stat[wave][turn][1], row, slope, lane,
                      [&](int c) { if constexpr (kLarge) return Rows::row_operand(values, 0, c, lane); else return vf[c]; });
 #pragma unroll
             for (int d = 0; d < Keys::DB; ++d) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(keys.dk[d]), "+v"(keys.dv[d]) :: "memory");
@@ -458,7 +470,7 @@ struct DqRows {
         lse = m == -INFINITY ? INFINITY : m * kLog2e;
         if (there && h == 0 && write_stats) {
             const int64_t at = (int64_t)head * a.rows + e.lse0 + row;
-            a.stat_lse[at] = lse, a.stat_delta[at] = delta;
+            a.stat_lse[at] = lse, a.stat_delta[at] = -delta;
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d) dq[d] = zero16();
