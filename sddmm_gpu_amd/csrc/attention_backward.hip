@@ -11,7 +11,7 @@
 // Roundings with 16-bit operands: P and dt to the element type, as operands; delta comes from the rounded output.  With bf16 dq and dk are off by 0.0025
 // of their size where rounding the results alone makes 0.0017 (fp32 operands: 3e-7).  A second operand for what dt loses would be two products beside seven.
 //
-// 8192 tokens, causal, 16 heads of 128, bf16: dq 0.45 ms and dk, dv 0.61 ms, 0.92 and 0.90 PFLOP/s of their products (a large library product 1.17);
+// 8192 tokens, causal, 16 heads of 128, bf16: dq 0.42 ms and dk, dv 0.61 ms, 0.98 and 0.90 PFLOP/s of their products (a large library product 1.17);
 // fp32, 4096 tokens, 16 heads of 64 1.2 ms, 98 TFLOP/s (154): matrix and vector instructions of a SIMD, which alternate, bound both.
 #include "attention.hpp"
 #include "attention_launch.hpp"
@@ -213,7 +213,7 @@ struct DkvKeys {
 };
 
 // dk and dv of 32 keys to each of KW waves, which share the tiles of rows.  The query heads that share a key head follow each other in the same sums.
-// 13 documents of 22 to 2281 tokens, 8192 in all, 16 heads over 4 of 128, bf16: 173 us, and 23 to sum the parts: a compute unit has work for 70 % of it.
+// 13 documents of 22 to 2281 tokens, 8192 in all, 16 heads over 4 of 128, bf16: 175 us, and 23 to sum the parts: a compute unit has work for 70 % of it.
 // With two such waves the other two take every second tile of rows, and the sums are joined at the end: twice the workgroups, of half the length.
 template <class T, int DP, bool MOD, int KW>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : 2)
@@ -306,7 +306,7 @@ void sddmm_attention_dkv_kernel(const AttnArgs a)
 
 // The same where workgroups of 128 keys would leave most compute units without work: 32 keys to a workgroup, each wave on every NW-th tile of rows, in LDS of
 // its own and without a barrier; sums are joined at the end.  fp32 heads of more than 64: one tile at a time, since a tile's products take eight
-// times as long as its way to LDS, and v in LDS.  300 tokens, 16 heads over 4 of 128, bf16 25 us, fp32 31: latency of loads and of chains of products.
+// times as long as its way to LDS, and v in LDS.  300 tokens, 16 heads over 4 of 128, bf16 24 us, fp32 31: latency of loads and of chains of products.
 template <class T, int DP, bool MOD, int NW>
 __global__ __launch_bounds__(64 * NW, 1)
 void sddmm_attention_dkv_few_kernel(const AttnArgs a)

@@ -16,8 +16,8 @@ constexpr int kWaves = 4;  // of a workgroup, 32 rows to each
 // 0.0020 of its size where rounding it alone makes 0.0016; a second operand for what P loses would be a third product beside two.
 //
 // What bounds it: matrix and vector instructions about alike, each half of the time on long prompts, with the clock at 1.9 GHz under the power limit.
-// 16,384 tokens, causal, 16 heads over 2 of 128, bf16: 1.03 ms = 1.06 PFLOP/s, where a large library product reaches 1.17; 8192 tokens, 16 heads of 128
-// 0.34 ms (0.81; capped 0.40), of 64, fp16 0.18 ms (0.76); fp32, 4096 tokens, 16 heads of 64 0.30 ms = 113 TFLOP/s of 154.  LDS is read without conflicts.
+// 16,384 tokens, causal, 16 heads over 2 of 128, bf16: 1.00 ms = 1.10 PFLOP/s, where a large library product reaches 1.17; 8192 tokens, 16 heads of 128
+// 0.29 to 0.33 ms by card (0.95; capped 0.36), of 64, fp16 0.18 ms (0.76); fp32, 4096 tokens, 16 heads of 64 0.29 ms = 118 TFLOP/s of 154.  LDS is read without conflicts.
 //
 // What the rows of a workgroup are: the rows of one query head (kRowsOfHead); the (token, head) pairs of the query heads that share
 // a key head, for few tokens (kRowsPacked); the same pairs of all sequences, against the keys that all of them begin with
