@@ -23,11 +23,12 @@ namespace {
 
 constexpr int kWaves = 4, kFewKeys = 32;  // keys of a workgroup of the dk, dv kernel for few
 
-// 16-bit heads of more than 64: a wave that is past its first products goes before another one of its SIMD that is at them, so that one's vector instructions
-// run beside the other's products; of scores that are not bent the second products too (8192 tokens, 16 heads of 128, bf16, causal 1020 and 959 us; 4096,
-// 16 over 4, capped 405 and 386; but heads of 64, fp16 596 and 628, fp32 1212 and 1245).
-template <class T, int DP> __device__ __forceinline__ void raise_priority() { if constexpr (sizeof(T) == 2 && DP == 128) __builtin_amdgcn_s_setprio(1); }
-template <class T, int DP> __device__ __forceinline__ void lower_priority() { if constexpr (sizeof(T) == 2 && DP == 128) __builtin_amdgcn_s_setprio(0); }
+// 16-bit operands, heads of more than 64 or scores that are bent or biased: a wave that is past its first products goes before another one of its SIMD that is at them, so
+// that one's vector instructions run beside the other's products; of plain scores the second products too (us without and with, causal: 8192 tokens, 16 heads of
+// 128, bf16 1020 and 959; 4096, 16 over 4, capped 405 and 386; 8192, 16 of 64, capped 900 and 819, 2048 in 3 sequences, 12 of 64, capped 187 and 189; but
+// plain scores of heads of 64, fp16 596 and 628, fp32 1212 and 1245).
+template <class T, int DP, bool MOD> __device__ __forceinline__ void raise_priority() { if constexpr (sizeof(T) == 2 && (DP == 128 || MOD)) __builtin_amdgcn_s_setprio(1); }
+template <class T, int DP, bool MOD> __device__ __forceinline__ void lower_priority() { if constexpr (sizeof(T) == 2 && (DP == 128 || MOD)) __builtin_amdgcn_s_setprio(0); }
 
 // scores in powers of two from products, and what their gradients have to be multiplied by on the way back
 template <bool MOD, class T>
@@ -139,7 +140,7 @@ struct DkvKeys {
         for (int c = 0; c < DP / 16; ++c) x = Elem<T>::mma(Rows::row_operand(qt, 0, c, l), kf[c], x);
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) y = Elem<T>::mma(Rows::row_operand(dot, 0, c, l), v(c), y);
-        raise_priority<T, DP>();
+        raise_priority<T, DP, MOD>();
         scores<MOD, T>(x, back, bend, unit, bias, slope, (float)(row + 4 * h + shift - key), 1.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -167,7 +168,7 @@ struct DkvKeys {
             y[r] *= x[r];
             if constexpr (MOD) y[r] *= back[r];
         }
-        if constexpr (MOD) lower_priority<T, DP>();
+        if constexpr (MOD) lower_priority<T, DP, MOD>();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const Vec8 p = operand<T>(x, c), ds = operand<T>(y, c);
@@ -177,7 +178,7 @@ struct DkvKeys {
                 dk[d] = Elem<T>::mma(Rows::column_operand(qt, d, c, l), ds, dk[d]);
             }
         }
-        if constexpr (!MOD) lower_priority<T, DP>();
+        if constexpr (!MOD) lower_priority<T, DP, MOD>();
     }
     // calls f(i, four elements) for the pieces i = 0 .. 8 DB - 1 of a lane's sums: dk, then dv
     template <class F> __device__ __forceinline__ void pieces(F f) const
@@ -610,11 +611,11 @@ void sddmm_attention_dq_kernel(const AttnArgs a)
             int l = lane;  // (places in LDS made anew in every tile: kept, they would not fit the registers)
             asm volatile("" : "+v"(l));
             floatx16 x = rows.template product<Keys>(kt, 32 * u, rows.qf, l), y = rows.template product<Keys>(vt, 32 * u, rows.of, l);
-            raise_priority<T, DP>();
+            raise_priority<T, DP, MOD>();
             rows.gradients(x, y, key, key < full_lo || key + 32 > full_hi);
-            if constexpr (MOD) lower_priority<T, DP>();
+            if constexpr (MOD) lower_priority<T, DP, MOD>();
             rows.template add<Keys>(kt, 32 * u, y, l);
-            if constexpr (!MOD) lower_priority<T, DP>();
+            if constexpr (!MOD) lower_priority<T, DP, MOD>();
         }
     }
     if constexpr (RW < kWaves) {  // the halves of the keys
