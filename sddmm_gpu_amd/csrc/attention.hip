@@ -120,7 +120,13 @@ Deal deal(const sddmm_attention_desc &d)
         // 768 keys a second launch costs more than it saves.
         // Where each workgroup has a cache of its own four times as many even out their lengths (64 users of 284 to 8192 keys: 512 / 1024 / 2048 / 4096
         // workgroups 232 / 218 / 207 / 214 us), which short ones do not pay for with a second launch.
-        r.splits = r.max_tiles == 1 && r.grid >= kFill ? pieces(r.grid, keys, 1024, 4 * kFill) : keys <= 768 ? 1 : pieces(r.grid, keys, 256, d.shared_len > 0 ? kFill / 2 : kFill);
+        // fp32 products take 16 times as long: shorter pieces, as many as there are compute units (two workgroups' tiles of long heads do not fit one), where half of those
+        // would have none (us with the rule for 16 bits and this: one token, 16 heads over 4 of 128, 700 keys 34 and 16; 6 sequences of 362, 6 over 3 of 96 20 and 15; a
+        // prompt of 400, 4 of 128 25 and 18; where half of them have work: 38 tokens behind 3014, 32 over 4 of 96 84 and 116).
+        const bool few_slow = d.type == SDDMM_TYPE_F32 && d.shared_len == 0 && r.grid < kFill / 4;
+        if (r.max_tiles == 1 && r.grid >= kFill) r.splits = pieces(r.grid, keys, 1024, 4 * kFill);
+        else if (few_slow) r.splits = keys <= 256 ? 1 : pieces(r.grid, keys, 128, d.head_dim > 64 ? kFill / 2 - r.grid + 1 : kFill);
+        else r.splits = keys <= 768 ? 1 : pieces(r.grid, keys, 256, d.shared_len > 0 ? kFill / 2 : kFill);
         r.grid *= r.splits;
     }
     r.parts = r.splits;
@@ -129,7 +135,8 @@ Deal deal(const sddmm_attention_desc &d)
         // of them 49, 38 to 46 and 46 us).
         r.shared_tile = r.rows * group <= 256 ? 64 : 128;
         r.shared_slots = div_up(r.rows * group, r.shared_tile);
-        r.shared_splits = pieces(r.shared_slots * d.n_kv_heads, d.shared_len, 256, kFill / 2);
+        // Pieces of 256 keys, fp32 of 64 (5 sequences of 4 tokens behind 294 keys, 32 over 8 heads of 96 25 and 16; 4 behind 1000, 16 over 4 of 64 19 and 12).
+        r.shared_splits = pieces(r.shared_slots * d.n_kv_heads, d.shared_len, d.type == SDDMM_TYPE_F32 ? 64 : 256, kFill / 2);
         r.shared_grid = r.shared_slots * d.n_kv_heads * r.shared_splits;
         r.parts += r.shared_splits;
     }
