@@ -198,7 +198,10 @@ DealBack deal_back(const sddmm_attention_desc &d)
         const double share = work / places;
         if (most > 2.5 * share) {
             const bool slow = d.type == SDDMM_TYPE_F32;  // (its rows take sixteen times as long, its parts no longer)
-            r.chunk = std::max<int64_t>((int64_t)std::sqrt((slow ? 100. : 1300.) * share), (slow ? 64 : 256) * (r.keys == 32 ? 4 : 1));  // (four waves share the rows of 32 keys)
+            // At least 256 rows, fp32 64; four times as many where four waves share the rows of 32 keys, fp32 down to half of that where there is room for more workgroups
+            // (us: 253 tokens, 2 heads over 1 of 128 79 and 69; 245, 12 over 3 78 and 72; everywhere: 500, 8 over 8 98 and 107, 1013 in 2, 4 over 2 of 32 67 and 71).
+            const int64_t least = r.keys != 32 ? (slow ? 64 : 256) : slow ? std::min<int64_t>(256, std::max<int64_t>(128, most * workgroups / places)) : 1024;
+            r.chunk = std::max<int64_t>((int64_t)std::sqrt((slow ? 100. : 1300.) * share), least);
             r.splits = std::max<int64_t>(1, std::min<int64_t>(div_up(most, r.chunk), 32));
         }
         r.chunk = std::max(r.chunk, div_up(most, r.splits));
