@@ -38,7 +38,7 @@ __device__ __forceinline__ void near_zero(float t, float &c, float &s)
 // double-precision products and about 25 instructions; made anew for each head they would take as long as the copy), then every thread turns pieces of
 // V elements (16 bytes where sizes and alignment allow it) of the heads of q and k in one launch.  The angle in turns is reduced in
 // 64 bits: at position 10^6 a 32-bit product would be off by 0.06 radians.  Results are rounded once.
-// 16,384 rows of 32 + 8 heads of 128, 96 elements turned, interleaved, bf16: 77 us = 4.4 TB/s read and written (a large copy 5.0); 64 rows 4.4 us.
+// 16,384 rows of 32 + 8 heads of 128, 96 elements turned, interleaved, bf16: 60 us = 5.6 TB/s read and written (a large copy 5.0); 64 rows 4.4 us.
 template <class T, int V, bool HALF>
 __global__ __launch_bounds__(kBlock)
 void sddmm_rotary_kernel(const RotaryArgs a)
@@ -66,44 +66,61 @@ void sddmm_rotary_kernel(const RotaryArgs a)
             table[i] = make_float2(cosine * a.amplitude, sine * a.amplitude * a.sign);
         }
         __syncthreads();
-        const int turned = some / (HALF ? V : kPairs), pieces = turned + (a.copy && p0 + some == pairs ? (a.head_dim - a.rot_dim) / V : 0);
-        const int all_heads = a.heads[0] + a.heads[1], n = rows * all_heads * pieces;
-        const float by_pieces = 1.f / (float)pieces, by_heads = 1.f / (float)all_heads;
+        // Two pieces of a head to a thread where that is possible: the two of pairs in halves, or one and the one half of all pieces on; pieces that are copied likewise
+        // (us, 16,384 rows of 32 + 8 heads of 128, 96 of them turned, interleaved, one and two pieces 78 and 64, 2048 rows 10.1 and 8.4).
+        const int turned = some / (HALF ? V : kPairs), copied = a.copy && p0 + some == pairs ? (a.head_dim - a.rot_dim) / V : 0;
+        const bool two = V > 1 && (HALF ? copied : turned + copied) % 2 == 0;
+        const int items = HALF ? turned + (two ? copied / 2 : copied) : two ? (turned + copied) / 2 : turned + copied;
+        const int all_heads = a.heads[0] + a.heads[1], n = rows * all_heads * items;
+        const float by_items = 1.f / (float)items, by_heads = 1.f / (float)all_heads;
         for (int i = threadIdx.x; i < n; i += kBlock) {
             // (quotients by a product: exact below 2^20, which n is held to)
-            const int unit = (int)(((float)i + 0.5f) * by_pieces), piece = i - unit * pieces;
+            const int unit = (int)(((float)i + 0.5f) * by_items), item = i - unit * items;
             const int r = (int)(((float)unit + 0.5f) * by_heads), head_at = unit - r * all_heads;
             const int which = head_at >= a.heads[0], head = which ? head_at - a.heads[0] : head_at;
             const T *x = (const T *)a.x[which] + (row0 + r) * a.x_row[which] + head * a.x_head[which];
             T *y = (T *)a.y[which] + (row0 + r) * a.y_row[which] + head * a.y_head[which];
-            // (pieces to turn and to copy lie in one wave: loads and stores are common to both)
-            const bool turn = piece < turned;
-            const int at = !turn ? a.rot_dim + (piece - turned) * V : HALF ? p0 + piece * V : 2 * p0 + piece * (V > 1 ? V : 2);
-            const int other = !turn ? at : HALF ? at + pairs : V > 1 ? at : at + 1;
-            Vec u = *(const Vec *)(x + at), v = u;
-            if constexpr (HALF || V == 1) v = *(const Vec *)(x + other);
-            if (turn) {
-                const float2 *cs = &table[r * some + piece * (HALF ? V : kPairs)];
-                if constexpr (V == 1) {
-                    const float f = (float)u, g = (float)v;
-                    u = (T)(f * cs[0].x - g * cs[0].y), v = (T)(f * cs[0].y + g * cs[0].x);
-                } else if constexpr (HALF) {
+            const float2 *angles = &table[r * some];
+            if constexpr (HALF || V == 1) {
+                // (items to turn and to copy lie in one wave: loads and stores are common to both)
+                const bool turn = item < turned, both = turn || two;
+                const int at = !turn ? a.rot_dim + (item - turned) * V : HALF ? p0 + item * V : 2 * (p0 + item);
+                const int other = !turn ? (two ? at + copied / 2 * V : at) : HALF ? at + pairs : at + 1;
+                Vec u = *(const Vec *)(x + at), v = *(const Vec *)(x + other);
+                if (turn) {
+                    const float2 *cs = angles + item * V;
+                    if constexpr (V == 1) {
+                        const float f = (float)u, g = (float)v;
+                        u = (T)(f * cs[0].x - g * cs[0].y), v = (T)(f * cs[0].y + g * cs[0].x);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float f = (float)u[j], g = (float)v[j];
-                        u[j] = (T)(f * cs[j].x - g * cs[j].y), v[j] = (T)(f * cs[j].y + g * cs[j].x);
+                        for (int j = 0; j < V; ++j) {
+                            const float f = (float)u[j], g = (float)v[j];
+                            u[j] = (T)(f * cs[j].x - g * cs[j].y), v[j] = (T)(f * cs[j].y + g * cs[j].x);
+                        }
                     }
-                } else {
+                }
+                *(Vec *)(y + at) = u;
+                if (both) *(Vec *)(y + other) = v;
+            } else {
+                auto place = [&](int k) { return k < turned ? 2 * p0 + k * V : a.rot_dim + (k - turned) * V; };
+                auto turn = [&](Vec &u, int k) {
+                    if (k >= turned) return;
+                    const float2 *cs = angles + k * kPairs;
 #pragma unroll
                     for (int j = 0; j < kPairs; ++j) {
                         const float f = (float)u[2 * j], g = (float)u[2 * j + 1];
                         u[2 * j] = (T)(f * cs[j].x - g * cs[j].y), u[2 * j + 1] = (T)(f * cs[j].y + g * cs[j].x);
                     }
+                };
+                Vec u = *(const Vec *)(x + place(item)), v = u;
+                if (two) v = *(const Vec *)(x + place(item + items));
+                turn(u, item);
+                *(Vec *)(y + place(item)) = u;
+                if (two) {
+                    turn(v, item + items);
+                    *(Vec *)(y + place(item + items)) = v;
                 }
-            }
-            *(Vec *)(y + at) = u;
-            if constexpr (HALF || V == 1) {
-                if (turn) *(Vec *)(y + other) = v;
             }
         }
     }
@@ -185,11 +202,11 @@ int sddmm_rotary(const sddmm_rotary_desc *desc, const int32_t *d_positions, cons
     int v = 16 / size;
     while (v > 1 && bits % v) v /= 2;
     const bool half = d.layout == SDDMM_ROTARY_HALF;
-    // Rows of a workgroup: one, two where there are many (16,384 rows of 32 + 8 heads of 128, in halves / interleaved: 1, 2, 4 and 8 rows 80 / 76, 80 / 77, 81 / 80
-    // and 87 / 86 us; two or four pieces of a thread under way together 91 to 126: fewer waves).
+    // Rows of a workgroup: as many as have one and a half pairs of pieces for each thread, but 1024 workgroups (us, 16,384 rows of 32 + 8 heads of 128, interleaved, one and two
+    // rows 61 and 64; of 8 + 2 heads one, two, four, five and six 28, 21, 18, 17 and 17; of 2 + 2 heads of 64, in halves 14, 9 and, with twelve, 7.5).
     const int64_t pieces = d.rot_dim / (half || v == 1 ? 2 * v : v) + (d.head_dim - d.rot_dim) / v + 1, row_work = pieces * (d.n_heads + d.n_kv_heads);
     if (row_work > (1 << 20)) return fail(SDDMM_ERR_RANGE, "%s: a row of all heads is too long", who);
-    a.per_row = (int)std::max<int64_t>(1, std::min({d.n_rows / 1024, (int64_t)kTable / (d.rot_dim / 2), ((int64_t)1 << 20) / row_work, (int64_t)2}));
+    a.per_row = (int)std::max<int64_t>(1, std::min<int64_t>({d.n_rows / 1024, (int64_t)kTable / (d.rot_dim / 2), ((int64_t)1 << 20) / row_work, 384 / std::max<int64_t>(1, row_work / 2)}));
     const int64_t grid = (d.n_rows + a.per_row - 1) / a.per_row;
     if (grid > INT32_MAX) return fail(SDDMM_ERR_RANGE, "%s: too many rows for one launch", who);
     const hipStream_t st = (hipStream_t)stream;

@@ -49,7 +49,7 @@ def run(desc, pos, freq, q, k, q_out, k_out, stream=0):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("layout", [HALF, INTERLEAVED])
 @pytest.mark.parametrize("rows,heads,kv,dim,rot", [(1, 1, 0, 2, 2), (1, 32, 8, 128, 128), (37, 4, 2, 64, 32), (5000, 3, 1, 128, 96), (70, 2, 1, 80, 40),
-                                                   (9, 2, 2, 50, 50), (33, 3, 1, 41, 26), (4, 2, 1, 12, 4), (3, 1, 1, 4096, 4096), (2, 2, 0, 2100, 2090)])
+                                                   (9, 2, 2, 50, 50), (33, 3, 1, 41, 26), (4, 2, 1, 12, 4), (3, 1, 1, 4096, 4096), (2, 2, 0, 2100, 2090), (6001, 2, 1, 72, 56), (6001, 1, 0, 40, 32), (3333, 1, 1, 16, 8), (2500, 5, 3, 24, 24)])
 def test_rotary(dtype, layout, rows, heads, kv, dim, rot):
     g = torch.Generator().manual_seed(rows)
     pos = torch.randint(0, 1 << 20, (rows,), generator=g)
