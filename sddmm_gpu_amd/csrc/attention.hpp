@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include "../../include/sddmm.h"
+#include "attention_intervals.hpp"
 #include "bf16_parts.hpp"
 
 namespace sddmm {
@@ -336,12 +337,11 @@ __device__ __forceinline__ int slot_sequence(const int32_t *ptr, int n_seq, int 
     return tile < 0 ? -1 : lo;
 }
 
-// The keys that a row at position pos sees: [lo, hi).
-__device__ __forceinline__ int first_key(const AttnArgs &a, int pos) { return a.left < 0 ? 0 : max(0, pos - a.left); }
-__device__ __forceinline__ int end_key(const AttnArgs &a, int pos, int prefix, int n_keys)
-{
-    return a.right < 0 ? n_keys : min(n_keys, max(min(pos, INT32_MAX - 1 - a.right) + a.right + 1, prefix));
-}
+// (attention_intervals.hpp, of a call)
+__device__ __forceinline__ int first_key(const AttnArgs &a, int pos) { return first_key(a.left, pos); }
+__device__ __forceinline__ int end_key(const AttnArgs &a, int pos, int prefix, int n_keys) { return end_key(a.right, pos, prefix, n_keys); }
+__device__ __forceinline__ int first_row(const AttnArgs &a, int j, int prefix, int shift) { return first_row(a.right, j, prefix, shift); }
+__device__ __forceinline__ int end_row(const AttnArgs &a, int j, int shift, int n_rows) { return end_row(a.left, j, shift, n_rows); }
 
 // The bound of scores: cap tanh(t / cap), t = scale * product, of N results in registers, in powers of two (BACK: and 1 - tanh^2 of each).
 // Where all of the wave's |y|, y = t / cap, are 0.25 at most, which they mostly are, by powers of y^2 with everything else in their factors: six

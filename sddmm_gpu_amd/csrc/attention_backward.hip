@@ -53,16 +53,6 @@ __device__ __forceinline__ void scores(floatx16 &x, floatx16 &back, const Bend<T
     }
 }
 
-// The rows that see key j: [first, end).
-__device__ __forceinline__ int first_row(const AttnArgs &a, int j, int prefix, int shift)
-{
-    return a.right < 0 || j < prefix ? 0 : max(0, j - min(a.right, j) - shift);
-}
-__device__ __forceinline__ int end_row(const AttnArgs &a, int j, int shift, int n_rows)
-{
-    return a.left < 0 ? n_rows : min(n_rows, max(0, min(j, INT32_MAX / 2) + min(a.left, INT32_MAX / 2) + 1 - shift));
-}
-
 // The keys of a workgroup (KEYS of them), and how the rows that see them are cut into pieces (a.n_split at most, of about a.chunk rows of all
 // heads): a key tile early in a long sequence has many times the rows of others.
 struct KeyTile {
