@@ -68,6 +68,15 @@ int check_desc(const char *who, const sddmm_attention_desc *p)
     return SDDMM_OK;
 }
 
+// The description with the bounds that packed arrays give: no sequence has more rows or keys than all of them.  Tiles of a sequence then are at most those of the
+// grid, and fit 32 bits as it does, whatever bound the caller names.
+sddmm_attention_desc held(sddmm_attention_desc d)
+{
+    if (d.q_ptr) d.max_q = (int32_t)std::min<int64_t>(d.max_q, d.q_rows);
+    if (d.k_ptr) d.max_k = (int32_t)std::min<int64_t>(d.max_k, d.k_rows);
+    return d;
+}
+
 // Rows and keys of all sequences (0 where none can have any, whatever the arrays hold).
 int64_t rows_of(const sddmm_attention_desc &d) { return d.n_seq == 0 || d.max_q == 0 ? 0 : d.q_ptr ? d.q_rows : (int64_t)d.n_seq * d.max_q; }
 int64_t key_rows_of(const sddmm_attention_desc &d) { return d.n_seq == 0 || d.max_k == 0 ? 0 : d.k_ptr ? d.k_rows : (int64_t)d.n_seq * d.max_k; }
@@ -247,7 +256,7 @@ bool in_place_of(std::initializer_list<const void *> results, std::initializer_l
 int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d_q, const void *d_shared_k, const void *d_shared_v, const void *d_k,
                 const void *d_v, void *d_out, float *d_lse, void *d_workspace, int64_t workspace_bytes, void *stream)
 {
-    const sddmm_attention_desc &d = *desc;
+    const sddmm_attention_desc d = held(*desc);
     const Deal r = deal(d);
     if (r.rows == 0) return SDDMM_OK;
     const bool keys = key_rows_of(d) > 0;
@@ -293,8 +302,9 @@ void sddmm_attention_desc_init(sddmm_attention_desc *desc)
 int sddmm_attention_workspace_bytes(const sddmm_attention_desc *desc, int64_t *forward, int64_t *backward)
 {
     if (int rc = check_desc("sddmm_attention_workspace_bytes", desc)) return rc;
-    if (forward) *forward = deal(*desc).bytes;
-    if (backward) *backward = deal_back(*desc).bytes;
+    const sddmm_attention_desc d = held(*desc);
+    if (forward) *forward = deal(d).bytes;
+    if (backward) *backward = deal_back(d).bytes;
     return SDDMM_OK;
 }
 
@@ -323,7 +333,7 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
 {
     const char *who = "sddmm_attention_backward";
     if (int rc = check_desc(who, desc)) return rc;
-    const sddmm_attention_desc &d = *desc;
+    const sddmm_attention_desc d = held(*desc);
     if (d.shared_len) return fail(SDDMM_ERR_ARG, "%s: shared_len is for sddmm_attention_shared", who);
     if (d_dslopes && !d.slopes) return fail(SDDMM_ERR_ARG, "%s: gradients of slopes that are not there", who);
     const DealBack r = deal_back(d);
