@@ -23,7 +23,7 @@ int element(int type) { return type == SDDMM_TYPE_F32 ? 4 : 2; }
 bool strides_fit(const sddmm_attention_desc &d, int64_t seq, int64_t row, int64_t head, bool packed)
 {
     const int64_t e = element(d.type), piece = 16 / e;
-    return row >= d.head_dim && row * e < ((int64_t)1 << 23) && row % piece == 0 && head % piece == 0 && (packed || seq % piece == 0) &&
+    return row >= d.head_dim && row < ((int64_t)1 << 23) / e && row % piece == 0 && head % piece == 0 && (packed || seq % piece == 0) &&
            head >= 0 && (packed || seq >= 0);
 }
 
