@@ -540,8 +540,10 @@ int sddmm_csr_noalloc(int64_t n_rows, int64_t n_cols, int64_t nnz, const int32_t
  * summed in fp32, statistics kept in fp32; 16-bit operands: the probabilities (and,
  * backwards, their gradients) are rounded to the operands' type before they are
  * multiplied, as results are; fp32 operands: no rounding below fp32.  Infinities and
- * NaNs in keys that a row does not see do not reach it; in values (backwards, in rows
- * of q, out and d_out) they may where a row of the same 64 keys or 128 rows meets them.
+ * NaNs in keys that a row does not see do not reach its out and lse, nor the gradients
+ * of other keys and of slopes, and keys that no row sees get 0 whatever they hold; they may reach
+ * the row's dq, those in values its out, and those in rows of q, out and d_out the dk and dv of keys
+ * that these do not see, where a row of the same 64 keys or 128 rows meets them.
  * Lengths and pointers of sequences live on the device and are not validated: q_ptr
  * and k_ptr must rise, end at q_rows and k_rows at most, and give no sequence more than
  * max_q and max_k; others are held to these bounds, so that results are wrong but

@@ -143,7 +143,12 @@ struct DkvKeys {
                 for (int j = 0; j < 4; ++j) y[4 * i + j] += d[j];
             }
         }
-        if (row < full_lo || row + 32 > full_hi) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            y[r] *= x[r];
+            if constexpr (MOD) y[r] *= back[r];
+        }
+        if (row < full_lo || row + 32 > full_hi) {  // (last: a factor of what is not seen may be NaN)
             const int at = row + 4 * h - lo;
             const uint32_t span = hi > lo ? hi - lo : 0;
 #pragma unroll
@@ -152,11 +157,6 @@ struct DkvKeys {
                 x[r] = seen ? x[r] : 0.f;
                 y[r] = seen ? y[r] : 0.f;
             }
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            y[r] *= x[r];
-            if constexpr (MOD) y[r] *= back[r];
         }
         if constexpr (MOD) lower_priority<T, DP, MOD>();
 #pragma unroll
