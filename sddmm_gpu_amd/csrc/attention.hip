@@ -5,6 +5,7 @@
 #include "internal.hpp"
 #include "attention.hpp"
 #include "attention_launch.hpp"
+#include "launch.hpp"
 
 using namespace sddmm;
 
@@ -197,7 +198,8 @@ DealBack deal_back(const sddmm_attention_desc &d)
         r.keys = work < few ? 32 : work < 1048576. && d.head_dim <= 64 ? 64 : 128;
         r.kv_tiles = div_up(d.max_k, r.keys);
         r.kv_slots = d.k_ptr ? r.key_rows / r.keys + d.n_seq : r.kv_tiles;
-        const int64_t workgroups = r.kv_slots * (d.k_ptr ? 1 : d.n_seq) * d.n_kv_heads, most = rows_that_see(r.keys);
+        // (held to what no launch takes, so that nothing passes 64 bits)
+        const int64_t workgroups = std::min(r.kv_slots * (d.k_ptr ? 1 : d.n_seq), (int64_t)1 << 40) * d.n_kv_heads, most = rows_that_see(r.keys);
         work = most * uneven * div_up(r.key_rows, r.keys) * d.n_kv_heads;
         // A tile of keys that most rows see is cut where it would take more than 2.5 equal shares of all work.  A piece costs the time of some 650 rows, written
         // and read, so pieces of c rows cost 650 work / c and save half of c at the end: c = sqrt(1300 share).  us of the backward pass, bf16, causal, with
@@ -266,7 +268,7 @@ int run_forward(const char *who, const sddmm_attention_desc *desc, const void *d
     if (!aligned({d_q, d_k, d_v, d_out, d_shared_k, d_shared_v})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (r.grid + r.shared_grid > INT32_MAX || (r.parts > 1 && r.rows * d.n_heads > INT32_MAX))
+    if (!launchable(r.grid + r.shared_grid, kAttentionThreads) || (r.parts > 1 && !launchable(attention_join_grid(r.rows * d.n_heads, (int)r.parts, d.head_dim), kAttentionThreads)))
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
     if (in_place_of({d_out}, {d_q, d_k, d_v, d_shared_k, d_shared_v})) return fail(SDDMM_ERR_ARG, "%s: the result is in an operand's place", who);
 
@@ -348,7 +350,8 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
     if (!aligned({d_q, d_k, d_v, d_out, d_dout, d_dq, d_dk, d_dv})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (r.q_grid > INT32_MAX || r.kv_grid > INT32_MAX / 32)
+    if (!launchable(r.q_grid, kAttentionThreads) || !launchable(r.kv_grid, kAttentionThreads) ||
+        !launchable(attention_sum_grid(r.kv_grid, (int)r.splits, r.keys, (int)padded_dim(d), d_dslopes ? d.n_heads : 0), kAttentionThreads))
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
     if (in_place_of({d_dq, d_dk, d_dv}, {d_q, d_k, d_v, d_out, d_dout, d_lse}) || in_place_of({d_dq}, {d_dk, d_dv}) || in_place_of({d_dk}, {d_dv}))
         return fail(SDDMM_ERR_ARG, "%s: a gradient is in an operand's or another gradient's place", who);

@@ -777,8 +777,7 @@ hipError_t launch_typed(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, 
     hipError_t e = hipSuccess;
     if (q_grid) e = q_rows == kFewRows ? launch(dq_few, dim3(q_grid), dim3(64 * q_waves), 0, st, b) : launch(dq, dim3(q_grid), dim3(64 * kWaves), 0, st, b);
     if (e == hipSuccess && kv_grid) e = keys == kFewKeys ? launch(dkv_few, dim3(kv_grid), dim3(64 * kv_waves), 0, st, a) : launch(dkv, dim3(kv_grid), dim3(64 * kWaves), 0, st, a);
-    const unsigned n_sum = kv_grid && a.n_split > 1 ? kv_grid / a.n_split * (keys / 32) * (DP / 16) / (keys == kFewKeys ? 1 : kSumPieces<128>) : 0;
-    const unsigned n_slopes = a.dslopes ? a.n_heads : 0;
+    const unsigned n_slopes = a.dslopes ? a.n_heads : 0, n_sum = (unsigned)attention_sum_grid(kv_grid, a.n_split, keys, DP, 0);
     if (e == hipSuccess && n_sum) e = launch(sum, dim3(n_sum + n_slopes), dim3(256), 0, st, a, (int)n_sum);
     else if (e == hipSuccess && n_slopes) e = launch(sddmm_attention_dslopes_kernel, dim3(n_slopes), dim3(256), 0, st, a);
     return e;
@@ -794,6 +793,11 @@ hipError_t launch_dims(const AttnArgs &a, const AttnArgs &b, unsigned kv_grid, i
 }
 
 }  // namespace
+
+int64_t attention_sum_grid(int64_t kv_grid, int splits, int keys, int padded_dim, int slope_heads)
+{
+    return (splits > 1 ? kv_grid / splits * (keys / 32) * (padded_dim / 16) / (keys == kFewKeys ? 1 : kSumPieces<128>) : 0) + slope_heads;
+}
 
 hipError_t launch_attention_backward(const AttnArgs &a, const AttnArgs &b, int type, unsigned kv_grid, int keys, unsigned q_grid, int q_rows, hipStream_t st)
 {

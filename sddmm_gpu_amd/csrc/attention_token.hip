@@ -79,14 +79,20 @@ hipError_t launch_typed(const AttnArgs &a, bool mod, unsigned grid, hipStream_t 
     return launch(mod ? sddmm_attention_token_kernel<T, DP, true, NW> : sddmm_attention_token_kernel<T, DP, false, NW>, dim3(grid), dim3(64 * NW), 0, st, a);
 }
 
+// lane groups of a workgroup of the kernel above, and how many of them share a row
+int join_groups(int head_dim) { return kJoinBlock / ((head_dim <= 64 ? 64 : 128) / 4); }
+int join_per_row(int n_part, int head_dim)
+{
+    int per_row = 1;
+    while (per_row < join_groups(head_dim) && per_row < n_part) per_row *= 2;
+    return per_row;
+}
+
 template <class T, int DP>
 hipError_t join_typed(const AttnArgs &a, hipStream_t st)
 {
-    constexpr int kGroups = kJoinBlock / (DP / 4);
-    int per_row = 1;
-    while (per_row < kGroups && per_row < a.n_part) per_row *= 2;
-    const int64_t rows = kGroups / per_row, grid = (a.rows * a.n_heads + rows - 1) / rows;
-    return launch(sddmm_attention_join_kernel<T, DP>, dim3((unsigned)grid), dim3(kJoinBlock), 0, st, a, per_row);
+    return launch(sddmm_attention_join_kernel<T, DP>, dim3((unsigned)attention_join_grid(a.rows * a.n_heads, a.n_part, a.head_dim)), dim3(kJoinBlock), 0, st, a,
+                  join_per_row(a.n_part, a.head_dim));
 }
 template <class T>
 hipError_t join_dims(const AttnArgs &a, hipStream_t st)
@@ -95,6 +101,12 @@ hipError_t join_dims(const AttnArgs &a, hipStream_t st)
 }
 
 }  // namespace
+
+int64_t attention_join_grid(int64_t rows_of_heads, int n_part, int head_dim)
+{
+    const int rows = join_groups(head_dim) / join_per_row(n_part, head_dim);
+    return (rows_of_heads + rows - 1) / rows;
+}
 
 hipError_t launch_attention_token(const AttnArgs &a, int type, unsigned grid, hipStream_t st)
 {

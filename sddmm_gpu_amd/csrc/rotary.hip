@@ -208,7 +208,7 @@ int sddmm_rotary(const sddmm_rotary_desc *desc, const int32_t *d_positions, cons
     if (row_work > (1 << 20)) return fail(SDDMM_ERR_RANGE, "%s: a row of all heads is too long", who);
     a.per_row = (int)std::max<int64_t>(1, std::min<int64_t>({d.n_rows / 1024, (int64_t)kTable / (d.rot_dim / 2), ((int64_t)1 << 20) / row_work, 384 / std::max<int64_t>(1, row_work / 2)}));
     const int64_t grid = (d.n_rows + a.per_row - 1) / a.per_row;
-    if (grid > INT32_MAX) return fail(SDDMM_ERR_RANGE, "%s: too many rows for one launch", who);
+    if (!launchable(grid, kBlock)) return fail(SDDMM_ERR_RANGE, "%s: too many rows for one launch", who);
     const hipStream_t st = (hipStream_t)stream;
     const hipError_t e = d.type == SDDMM_TYPE_F32 ? launch_typed<float>(a, v, half, st) : d.type == SDDMM_TYPE_F16 ? launch_typed<_Float16>(a, v, half, st)
                                                                                                                  : launch_typed<__bf16>(a, v, half, st);
