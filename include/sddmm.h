@@ -606,7 +606,8 @@ int sddmm_attention_backward(const sddmm_attention_desc *desc, const void *d_q, 
  * copied.  inverse: with -angle, which is the gradient.  Angles are taken in 64 bits, results of any type rounded once.  Row r
  * of q and k has the position d_positions[r] (device, int32), or first_position + r where d_positions is NULL; d_freq is a
  * device array of rot_dim / 2 doubles, from sddmm_rotary_frequencies or the caller's own.  Strides in elements; d_q_out may
- * be d_q with the same strides (in place), or for instance the rows of a cache; no n_kv_heads: d_k is not looked at.
+ * be d_q with the same strides (in place; d_k_out d_k likewise; no result in any other operand's place), or for instance the rows of
+ * a cache; no n_kv_heads: d_k is not looked at.
  * Any sizes and alignment (the elements' own); pieces of 16 bytes are the fast way.  No counterpart in the reference.  */
 enum { SDDMM_ROTARY_HALF = 0, SDDMM_ROTARY_INTERLEAVED = 1 };
 typedef struct sddmm_rotary_desc {

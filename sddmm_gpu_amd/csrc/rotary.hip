@@ -180,6 +180,10 @@ int sddmm_rotary(const sddmm_rotary_desc *desc, const int32_t *d_positions, cons
     const int size = d.type == SDDMM_TYPE_F32 ? 4 : 2;
     uint64_t low = (uintptr_t)d_q | (uintptr_t)d_q_out | (keys ? (uintptr_t)d_k | (uintptr_t)d_k_out : 0);
     if (low % size || (uintptr_t)d_freq % 8 || (uintptr_t)d_positions % 4) return fail(SDDMM_ERR_ARG, "%s: pointers must be aligned to their elements", who);
+    // (threads of the same and of other workgroups still read what a result in any other place would overwrite)
+    auto moved = [&](int w) { return (d.n_rows > 1 && strides[w][0] != strides[w][2]) || (heads[w] > 1 && strides[w][1] != strides[w][3]); };
+    if ((d_q == d_q_out && moved(0)) || (keys && ((d_k == d_k_out && moved(1)) || d_q_out == d_k || d_k_out == d_q || d_q_out == d_k_out)))
+        return fail(SDDMM_ERR_ARG, "%s: a result is in an operand's or the other result's place (only its own operand's, with the same strides, is taken)", who);
 
     RotaryArgs a{};
     a.positions = d_positions, a.freq = d_freq;
