@@ -437,10 +437,7 @@ class Plan:
             check(rc)
 
     def spmm_form(self):
-        """TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
-ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
-ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BANDS, ROTARY_PARTS = range(5)
-SPMM_CSR, SPMM_TILES or SPMM_WALK: what spmm does behind this plan."""
+        """SPMM_CSR, SPMM_TILES, SPMM_WALK or SPMM_BLOCKS: what spmm does behind this plan."""
         f = c_int32()
         check(lib().sddmm_plan_spmm_form(self.h, byref(f)))
         return f.value
