@@ -571,7 +571,7 @@ typedef struct sddmm_attention_desc {
     int64_t o_seq, o_row, o_head;
     const int32_t *q_ptr, *k_ptr;        /* device, [n_seq + 1], or NULL */
     const int32_t *q_len, *k_len;        /* device, [n_seq], or NULL; not beside q_ptr / k_ptr */
-    const int32_t *prefix;               /* device, [n_seq], or NULL */
+    const int32_t *prefix;               /* device, [n_seq], or NULL; below 0: none */
     const float *slopes;                 /* device, [n_heads], or NULL */
 } sddmm_attention_desc;
 void sddmm_attention_desc_init(sddmm_attention_desc *desc);   /* zeros, windows of -1 */

@@ -111,7 +111,7 @@ __device__ __forceinline__ void ForwardTile<T, DP, MOD, ROWS, RW>::run(const Att
         there = row < n_rows;
         token = PACK ? row / a.group : row;
         if constexpr (PACK) my_head = head + row % a.group;
-        const int shift = e.nk - e.nq, prefix = a.prefix ? max(0, a.prefix[s] - a.shared_len) : 0;
+        const int shift = e.nk - e.nq, prefix = a.prefix ? max(a.prefix[s], a.shared_len) - a.shared_len : 0;
         pos = token + shift;
         lo = first_key(a, pos), hi = end_key(a, pos, prefix, n_keys);
         const int last = min(n_rows, tile * kRows + kRows) - 1, w0 = tile * kRows + row_wave * 32, w1 = min(n_rows, w0 + 32) - 1;

@@ -48,7 +48,7 @@ __device__ __forceinline__ void TokenTile<T, DP, MOD, NW>::run(const AttnArgs &a
     const int row = tile * kTokenRows + n;
     const bool there = row < n_rows;
     const int token = row / a.group, head = kv * a.group + row % a.group;
-    const int shift = e.nk - e.nq, prefix = a.prefix ? max(0, a.prefix[s] - a.shared_len) : 0, pos = token + shift;
+    const int shift = e.nk - e.nq, prefix = a.prefix ? max(a.prefix[s], a.shared_len) - a.shared_len : 0, pos = token + shift;
     const int lo = first_key(a, pos), hi = end_key(a, pos, prefix, n_keys);
     const int t0 = tile * kTokenRows / a.group, t1 = (min(n_rows, tile * kTokenRows + kTokenRows) - 1) / a.group;
     const int any_lo = first_key(a, t0 + shift), any_hi = end_key(a, t1 + shift, prefix, n_keys);
