@@ -132,7 +132,9 @@ Deal deal(const sddmm_attention_desc &d)
         // workgroups 232 / 218 / 207 / 214 us), which short ones do not pay for with a second launch.
         // fp32 products take 16 times as long: shorter pieces, as many as there are compute units (two workgroups' tiles of long heads do not fit one), where half of those
         // would have none (us with the rule for 16 bits and this: one token, 16 heads over 4 of 128, 700 keys 34 and 16; 6 sequences of 362, 6 over 3 of 96 20 and 15; a
-        // prompt of 400, 4 of 128 25 and 18; where half of them have work: 38 tokens behind 3014, 32 over 4 of 96 84 and 116).
+        // prompt of 400, 4 of 128 25 and 18; where half of them have work: 38 tokens behind 3014, 32 over 4 of 96 84 and 116).  On either side of that border, one token of 32 heads
+        // over 8: 120 workgroups, heads of 128, 700 keys 35 and 28, 1500 63 and 42, 4000 126 and 90, of 64 14 (400 keys) and 14, 19 and 24, 31 and 31; 136 workgroups, heads of 128 36 and
+        // 36, 67 and 62, 142 and 152, of 64 14 and 18, 20 and 25, 34 and 33 (heads of 64 gain up to some 96: 64 workgroups 19 and 15, 96 19 and 20).
         const bool few_slow = d.type == SDDMM_TYPE_F32 && d.shared_len == 0 && r.grid < kFill / 4;
         if (r.max_tiles == 1 && r.grid >= kFill) r.splits = pieces(r.grid, keys, 1024, 4 * kFill);
         else if (few_slow) r.splits = keys <= 256 ? 1 : pieces(r.grid, keys, 128, d.head_dim > 64 ? kFill / 2 - r.grid + 1 : kFill);

@@ -11,7 +11,7 @@
 // Roundings with 16-bit operands: P and dt to the element type, as operands; delta comes from the rounded output.  With bf16 dq and dk are off by 0.0025
 // of their size where rounding the results alone makes 0.0017 (fp32 operands: 3e-7).  A second operand for what dt loses would be two products beside seven.
 //
-// 8192 tokens, causal, 16 heads of 128, bf16: dq 0.42 ms and dk, dv 0.61 ms, 0.98 and 0.90 PFLOP/s of their products (a large library product 1.17);
+// 8192 tokens, causal, 16 heads of 128, bf16: dq 0.40 ms and dk, dv 0.56 ms, 1.03 and 0.97 PFLOP/s of their products (a large library product 1.17);
 // fp32, 4096 tokens, 16 heads of 64 1.2 ms, 98 TFLOP/s (154): matrix and vector instructions of a SIMD, which alternate, bound both.
 #include "attention.hpp"
 #include "attention_launch.hpp"
@@ -204,7 +204,7 @@ struct DkvKeys {
 };
 
 // dk and dv of 32 keys to each of KW waves, which share the tiles of rows.  The query heads that share a key head follow each other in the same sums.
-// 13 documents of 22 to 2281 tokens, 8192 in all, 16 heads over 4 of 128, bf16: 175 us, and 23 to sum the parts: a compute unit has work for 70 % of it.
+// 13 documents of 22 to 2281 tokens, 8192 in all, 16 heads over 4 of 128, bf16: 151 us, and 21 to sum the parts: a compute unit has work for 70 % of it.
 // With two such waves the other two take every second tile of rows, and the sums are joined at the end: twice the workgroups, of half the length.
 template <class T, int DP, bool MOD, int KW>
 __global__ __launch_bounds__(64 * kWaves, sizeof(T) == 4 && DP == 128 ? 1 : 2)

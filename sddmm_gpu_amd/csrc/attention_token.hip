@@ -17,7 +17,8 @@ void sddmm_attention_token_kernel(const AttnArgs a)
 
 // The partial results of a row: weights 2^(m - largest m), sums of both.  Groups of head_dim / 4 lanes take the parts of a row in turn,
 // as many groups to a row as it has parts (up to the workgroup's), with all requests under way together, and meet in LDS.  4 to 6 us: latency of a launch
-// and of two dependent loads.  (Its own launch, since the last workgroup to finish would have to be known by a counter that every call finds at 0.)
+// and of two dependent loads.  (Its own launch: the last workgroup to finish would have to be known by a counter that every call finds at 0, which the workspace,
+// anyone's between calls, does not hold.)
 constexpr int kJoinBlock = 256;
 template <class T, int DP>
 __global__ __launch_bounds__(kJoinBlock)
