@@ -550,6 +550,9 @@ int sddmm_csr_noalloc(int64_t n_rows, int64_t n_cols, int64_t nnz, const int32_t
  * nothing outside the arrays is touched.  q_len and k_len are taken as 0 .. max_q and
  * 0 .. max_k.
  *
+ * Calls that would take more workgroups than a launch holds, some 16 million (tiles of rows of all
+ * heads, or of keys), are refused with SDDMM_ERR_RANGE.
+ *
  * Calls allocate nothing, launch on `stream` only (a stream of the current device) and
  * may be captured into a graph.
  * d_workspace: sddmm_attention_workspace_bytes of device memory, 256-byte aligned, for
