@@ -208,11 +208,11 @@ def _keep(s):
     more = dict(max_k=s["longest"], k_len=s["len"].data_ptr(), max_q=s["most_new"], window_right=0)
     if not c["tokens"]:
         more.update(q_ptr=s["ptr"].data_ptr(), q_rows=s["rows"])
+    if c["op"] == "append":
+        more.update(k_seq=c["tokens"] * c["kv_heads"] * c["dim"], v_seq=c["tokens"] * c["kv_heads"] * c["dim"])
     if c["op"] == "attend":
         more.update(window_left=c["left"], cap=c["cap"], scale=s["scale"], slopes=s["slopes"].data_ptr() if c["bias"] else 0)
     s["desc"] = capi.AttentionDesc.packed(t, c["n_seq"], c["heads"], c["kv_heads"], c["dim"], **more)
-    if not c["tokens"]:
-        s["desc"].q_seq = s["desc"].o_seq = 0
     s["cache"] = capi.CacheDesc.packed(
         {"own": t, "i8": capi.TYPE_I8, "e4m3": capi.TYPE_E4M3}[c["held"]], s["n_pages"], c["page"], c["kv_heads"], c["dim"],
         by_token=c["order"] == "token", block_len=c["block"], table=s["table"].data_ptr(), table_row=s["table"].shape[1],
