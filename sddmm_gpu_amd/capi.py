@@ -20,6 +20,7 @@ KERNEL_AUTO, KERNEL_ROW_GATHER, KERNEL_LDS_TILE, KERNEL_PANEL, KERNEL_HYBRID, KE
 EPILOGUE_SCALE, EPILOGUE_RESIDUAL = 0, 1
 FORM_SOFTMAX = 0x100
 TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+TYPE_I8, TYPE_E4M3 = 3, 4  # of a cache
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BANDS, ROTARY_PARTS = range(5)
 SPMM_CSR, SPMM_TILES, SPMM_WALK, SPMM_BLOCKS = 0, 1, 2, 3
@@ -120,6 +121,32 @@ class RotaryDesc(C.Structure):
                             **{**d, **kw})
 
 
+class CacheDesc(C.Structure):
+    """sddmm_cache_desc; CacheDesc.defaults(**fields) starts from sddmm_cache_desc_init (pointers as integers)."""
+    _fields_ = [(n, c_int32) for n in ("type", "page_len", "block_len", "rot_dim", "rot_layout")] + [("rot_amplitude", c_float)] + [(n, c_int64) for n in (
+        "n_pages", "k_page", "k_row", "k_head", "v_page", "v_row", "v_head", "table_row")] + [
+        (n, c_void_p) for n in ("k", "v", "k_scale", "v_scale", "table", "rot_freq")]
+
+    @classmethod
+    def defaults(cls, **kw):
+        d = cls()
+        lib().sddmm_cache_desc_init(byref(d))
+        for k, v in kw.items():
+            if k not in dict(cls._fields_):
+                raise KeyError(k)
+            setattr(d, k, (v or None) if k in ("k", "v", "k_scale", "v_scale", "table", "rot_freq") else v)
+        return d
+
+    @classmethod
+    def packed(cls, type, n_pages, page_len, n_kv_heads, head_dim, by_token=False, **kw):
+        """The strides of contiguous arrays k and v [n_pages, n_kv_heads, page_len, head_dim] (by_token: [n_pages, page_len, n_kv_heads, head_dim])."""
+        d = {}
+        for n in "kv":
+            d[n + "_page"] = page_len * n_kv_heads * head_dim
+            d[n + "_row"], d[n + "_head"] = (n_kv_heads * head_dim, head_dim) if by_token else (head_dim, page_len * head_dim)
+        return cls.defaults(type=type, n_pages=n_pages, page_len=page_len, **{**d, **kw})
+
+
 class LaunchProfile(C.Structure):
     _fields_ = [("kernel", c_int32), ("lanes_per_nnz", c_int32), ("k_slice", c_int32), ("n_kernel_launches", c_int32),
                 ("nnz", c_int64), ("rows", c_int64), ("stream_positions", c_int64), ("ms", c_float)]
@@ -189,6 +216,10 @@ SIGNATURES = {
     "sddmm_attention_forward": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 6 + [c_int64, c_void_p]),
     "sddmm_attention_shared": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 8 + [c_int64, c_void_p]),
     "sddmm_attention_backward": (c_int, [POINTER(AttentionDesc)] + [c_void_p] * 11 + [c_int64, c_void_p]),
+    "sddmm_cache_desc_init": (None, [POINTER(CacheDesc)]),
+    "sddmm_cache_append": (c_int, [POINTER(AttentionDesc), POINTER(CacheDesc)] + [c_void_p] * 5),
+    "sddmm_attention_paged_workspace_bytes": (c_int, [POINTER(AttentionDesc), POINTER(CacheDesc), POINTER(c_int64)]),
+    "sddmm_attention_paged": (c_int, [POINTER(AttentionDesc), POINTER(CacheDesc)] + [c_void_p] * 4 + [c_int64, c_void_p]),
     "sddmm_rotary_desc_init": (None, [POINTER(RotaryDesc)]),
     "sddmm_rotary": (c_int, [POINTER(RotaryDesc)] + [c_void_p] * 7),
     "sddmm_rotary_frequencies": (c_int, [c_int32, c_double, c_int32, c_double, c_int64, c_double, c_double, c_void_p, POINTER(c_double)]),
@@ -535,6 +566,27 @@ def attention_backward(desc, d_q, d_k, d_v, d_out, d_lse, d_dout, d_dq, d_dk, d_
     """sddmm_attention_backward: the gradients of attention_forward's operands (and of the slopes)."""
     rc = lib().sddmm_attention_backward(byref(desc), d_q or None, d_k or None, d_v or None, d_out or None, d_lse or None, d_dout or None, d_dq or None,
                                         d_dk or None, d_dv or None, d_dslopes or None, d_workspace or None, workspace_bytes, stream or None)
+    if rc:
+        check(rc)
+
+
+def cache_append(desc, cache, d_q, d_q_out, d_k, d_v, stream=0):
+    """sddmm_cache_append: new tokens' keys, turned by their positions, and values into a paged cache (CacheDesc); their queries turned (d_q 0: none)."""
+    rc = lib().sddmm_cache_append(byref(desc), byref(cache), d_q or None, d_q_out or None, d_k or None, d_v or None, stream or None)
+    if rc:
+        check(rc)
+
+
+def attention_paged_workspace_bytes(desc, cache):
+    """Bytes of workspace that attention_paged needs."""
+    n = c_int64()
+    check(lib().sddmm_attention_paged_workspace_bytes(byref(desc), byref(cache), byref(n)))
+    return n.value
+
+
+def attention_paged(desc, cache, d_q, d_out, d_lse=0, d_workspace=0, workspace_bytes=0, stream=0):
+    """sddmm_attention_paged: attention_forward over a paged cache, of the operands' type or in 8 bits (cache: CacheDesc)."""
+    rc = lib().sddmm_attention_paged(byref(desc), byref(cache), d_q or None, d_out or None, d_lse or None, d_workspace or None, workspace_bytes, stream or None)
     if rc:
         check(rc)
 

@@ -1,0 +1,97 @@
+// Entry points of the attention over a cache in pages: what they check, which kernels they launch, and how large a workspace is.
+#include <hip/hip_runtime.h>
+#include <cmath>
+#include "attention_launch.hpp"
+#include "attention_paged_launch.hpp"
+#include "cache.hpp"
+#include "launch.hpp"
+
+using namespace sddmm;
+
+namespace {
+
+// How a call's rows and keys are dealt out.
+struct Deal {
+    int64_t rows = 0;  // of all sequences
+    int tiles = 1;     // of 16 rows to a workgroup
+    int64_t slots = 0, max_tiles = 0, grid = 0, splits = 1, chunk = 1;
+    int64_t part_bytes = 0, bytes = 0;
+};
+
+Deal deal(const sddmm_attention_desc &d)
+{
+    Deal r;
+    const int64_t group = d.n_heads / d.n_kv_heads, packed = d.max_q * group;
+    r.rows = rows_of(d);
+    if (r.rows == 0) return r;
+    r.tiles = packed <= 16 ? 1 : 2;
+    const int64_t few = 16 * r.tiles;
+    r.max_tiles = div_up(packed, few);
+    r.slots = r.max_tiles == 1 ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
+    const int64_t workgroups = r.slots * d.n_kv_heads;
+    // keys that a tile's rows can see, in tiles of 32
+    const int64_t span = d.window_left >= 0 && d.window_right >= 0 && !d.prefix ? (int64_t)d.window_left + d.window_right + std::min<int64_t>(d.max_q, few) : d.max_k;
+    const int64_t key_tiles = std::max<int64_t>(1, std::min<int64_t>(div_up(d.max_k, 32), span / 32 + 2));
+    r.splits = std::max<int64_t>(1, std::min(std::min(div_up(2048, workgroups), div_up(key_tiles, 8)), (int64_t)256));
+    r.chunk = div_up(key_tiles, r.splits);
+    r.splits = div_up(key_tiles, r.chunk);
+    r.grid = workgroups * r.splits;
+    if (r.splits > 1) {
+        r.part_bytes = padded(r.splits * r.rows * d.n_heads * d.head_dim * (int64_t)sizeof(float));
+        r.bytes = r.part_bytes + padded(r.splits * r.rows * d.n_heads * (int64_t)sizeof(float2));
+    }
+    return r;
+}
+
+int check(const char *who, const sddmm_attention_desc *desc, const sddmm_cache_desc *cache)
+{
+    if (!desc) return fail(SDDMM_ERR_ARG, "%s: NULL description", who);
+    sddmm_attention_desc d = *desc;  // (keys are the cache's)
+    d.k_seq = d.v_seq = d.k_head = d.v_head = d.k_rows = 0, d.k_row = d.v_row = 128;
+    if (int rc = check_desc(who, &d)) return rc;
+    return check_cache(who, d, cache);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sddmm_attention_paged_workspace_bytes(const sddmm_attention_desc *desc, const sddmm_cache_desc *cache, int64_t *bytes)
+{
+    if (int rc = check("sddmm_attention_paged_workspace_bytes", desc, cache)) return rc;
+    if (bytes) *bytes = deal(held(*desc)).bytes;
+    return SDDMM_OK;
+}
+
+int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_desc *cache, const void *d_q, void *d_out, float *d_lse,
+                          void *d_workspace, int64_t workspace_bytes, void *stream)
+{
+    const char *who = "sddmm_attention_paged";
+    if (int rc = check(who, desc, cache)) return rc;
+    const sddmm_attention_desc d = held(*desc);
+    const Deal r = deal(d);
+    if (r.rows == 0) return SDDMM_OK;
+    if (!d_q || !d_out) return fail(SDDMM_ERR_ARG, "%s: NULL device pointer", who);
+    if (!apart(d, d.o_seq, d.o_row, d.o_head, d.q_ptr ? 1 : d.n_seq, d.q_ptr ? d.q_rows : d.max_q, d.n_heads)) return fail(SDDMM_ERR_ARG, "%s: rows of the result overlap", who);
+    if ((uintptr_t)d_lse & 3u) return fail(SDDMM_ERR_ARG, "%s: lse must be aligned to its elements", who);
+    if (!aligned({d_q, d_out})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
+    if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
+        return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
+    if (!launchable(r.grid, kAttentionThreads) || (r.splits > 1 && !launchable(attention_join_grid(r.rows * d.n_heads, (int)r.splits, d.head_dim), kAttentionThreads)))
+        return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
+    if (in_place_of({d_out, d_lse}, {d_q, cache->k, cache->v, cache->k_scale, cache->v_scale}) || (const void *)d_lse == d_out)
+        return fail(SDDMM_ERR_ARG, "%s: a result is in an operand's or the other result's place", who);
+
+    AttnArgs a = arguments(d);
+    a.q = d_q, a.out = d_out, a.lse = d_lse;
+    a.part_o = (float *)d_workspace, a.part_ml = (float2 *)((char *)d_workspace + r.part_bytes);
+    a.n_slots = (int)r.slots, a.max_tiles = (int)r.max_tiles, a.n_split = (int)r.splits, a.n_part = (int)r.splits, a.chunk = (int)r.chunk;
+    const CacheArgs c = cache_arguments(d, *cache);
+    const hipStream_t st = (hipStream_t)stream;
+    hipError_t e = launch_attention_paged_token(a, c, d.type, held_as(d, *cache), r.tiles, (unsigned)r.grid, st);
+    if (e == hipSuccess && r.splits > 1) e = launch_attention_join(a, d.type, st);
+    if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
+    return SDDMM_OK;
+}
+
+}  // extern "C"
