@@ -142,6 +142,21 @@ struct Tile {
         }
     }
 
+    // The part of the tile that begins `block` bytes into it, by one wave: rows of the sixteen from row `group` on, the first of which is at `base`; those from `from` to
+    // `to_row` - 1 of the sixteen exist, all else becomes 0.
+    static __device__ __forceinline__ void request_rows(char *lds, const char *base, uint32_t stride, int to_row, int from, int bytes, int block, int group, int lane)
+    {
+        const uint32_t range = to_row > 0 ? (uint32_t)(min(to_row, 16) - 1) * stride + (uint32_t)bytes : 0u;
+        uint4v src = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)base),
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)((uintptr_t)base >> 32) & 0xffffu)),
+                            (uint32_t)__builtin_amdgcn_readfirstlane((int)range), 0x00020000u};
+        uint32_t to = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)(lds + block));
+        asm volatile("s_nop 4" : "+s"(src), "+s"(to));
+        const int pos = block + lane * 16, row = pos / kRowBytes, piece = (pos % kRowBytes / 16) ^ turn(row), in = row - group;
+        const uint32_t off = piece * 16 < bytes && in >= from ? (uint32_t)in * stride + (uint32_t)piece * 16 : 0x7ffffff0u;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(src) : "memory");
+    }
+
     // elements 16 c + 8 h + j of row block + n
     static __device__ __forceinline__ typename Elem<T>::Vec8 row_operand(const char *lds, int block, int c, int lane)
     {

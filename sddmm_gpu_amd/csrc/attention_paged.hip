@@ -13,7 +13,8 @@ namespace {
 // How a call's rows and keys are dealt out.
 struct Deal {
     int64_t rows = 0;  // of all sequences
-    int tiles = 1;     // of 16 rows to a workgroup
+    bool token = true; // the kernel for few rows
+    int tiles = 1;     // of 16 rows to a workgroup of it
     int64_t slots = 0, max_tiles = 0, grid = 0, splits = 1, chunk = 1;
     int64_t part_bytes = 0, bytes = 0;
 };
@@ -24,17 +25,22 @@ Deal deal(const sddmm_attention_desc &d)
     const int64_t group = d.n_heads / d.n_kv_heads, packed = d.max_q * group;
     r.rows = rows_of(d);
     if (r.rows == 0) return r;
+    r.token = packed <= 64;
     r.tiles = packed <= 16 ? 1 : 2;
-    const int64_t few = 16 * r.tiles;
+    const int64_t few = r.token ? 16 * r.tiles : 128;
     r.max_tiles = div_up(packed, few);
-    r.slots = r.max_tiles == 1 ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
+    r.slots = r.max_tiles == 1 && r.token ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
     const int64_t workgroups = r.slots * d.n_kv_heads;
     // keys that a tile's rows can see, in tiles of 32
     const int64_t span = d.window_left >= 0 && d.window_right >= 0 && !d.prefix ? (int64_t)d.window_left + d.window_right + std::min<int64_t>(d.max_q, few) : d.max_k;
     const int64_t key_tiles = std::max<int64_t>(1, std::min<int64_t>(div_up(d.max_k, 32), span / 32 + 2));
-    r.splits = std::max<int64_t>(1, std::min(std::min(div_up(2048, workgroups), div_up(key_tiles, 8)), (int64_t)256));
-    r.chunk = div_up(key_tiles, r.splits);
-    r.splits = div_up(key_tiles, r.chunk);
+    if (r.token) {
+        r.splits = std::max<int64_t>(1, std::min(std::min(div_up(2048, workgroups), div_up(key_tiles, 8)), (int64_t)256));
+        r.chunk = div_up(key_tiles, r.splits);
+        r.splits = div_up(key_tiles, r.chunk);
+    } else {
+        r.splits = std::max<int64_t>(1, std::min(std::min(div_up(512, workgroups), div_up(key_tiles, 8)), (int64_t)256));
+    }
     r.grid = workgroups * r.splits;
     if (r.splits > 1) {
         r.part_bytes = padded(r.splits * r.rows * d.n_heads * d.head_dim * (int64_t)sizeof(float));
@@ -68,7 +74,7 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
 {
     const char *who = "sddmm_attention_paged";
     if (int rc = check(who, desc, cache)) return rc;
-    const sddmm_attention_desc d = held(*desc);
+    const sddmm_attention_desc d = sddmm::held(*desc);
     const Deal r = deal(d);
     if (r.rows == 0) return SDDMM_OK;
     if (!d_q || !d_out) return fail(SDDMM_ERR_ARG, "%s: NULL device pointer", who);
@@ -88,7 +94,8 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
     a.n_slots = (int)r.slots, a.max_tiles = (int)r.max_tiles, a.n_split = (int)r.splits, a.n_part = (int)r.splits, a.chunk = (int)r.chunk;
     const CacheArgs c = cache_arguments(d, *cache);
     const hipStream_t st = (hipStream_t)stream;
-    hipError_t e = launch_attention_paged_token(a, c, d.type, held_as(d, *cache), r.tiles, (unsigned)r.grid, st);
+    const int held = held_as(d, *cache);
+    hipError_t e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, (unsigned)r.grid, st) : launch_attention_paged_forward(a, c, d.type, held, (unsigned)r.grid, st);
     if (e == hipSuccess && r.splits > 1) e = launch_attention_join(a, d.type, st);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;

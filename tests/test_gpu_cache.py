@@ -233,6 +233,17 @@ def attend(dtype, pages, table, n_new, after, heads, q, packed, left=-1, right=0
     return out, stat
 
 
+def lost(dtype, held, n_keys, v):
+    """What weights that are rounded to fp16 may be off by in all, where that is more than their share of 2^-11: half of the least step, 2^-25, each, times the values.
+    fp16 operands: the largest weight is 1 at least (and scales of values enter it, in units of the largest, a code of up to 16 times the largest value of a key); bf16
+    operands over codes, many rows: the running maximum is at most the largest score, and weights are 2^7 times those below it, so the largest is 2^7 at least.
+    Results in fp16 are off by half of the least step themselves."""
+    if not n_keys or (dtype == BF16 and held == "own") or dtype == F32:
+        return 0.0
+    each = 2.0 ** -25 * 16 if dtype == F16 else 2.0 ** -32
+    return n_keys * each * v.abs().max() + (2.0 ** -25 if dtype == F16 else 0)
+
+
 def check_attend(dtype, held, n_new, after, heads, kv, dim, page, block, by_token=False, packed=True, seed=5, pad=0, spoil=True, lse=True, **mask):
     table, n_pages = tables(after, page, seed)
     pages = Pages(dtype, held, n_pages, page, block, kv, dim, by_token, seed, pad)
@@ -263,10 +274,7 @@ def check_attend(dtype, held, n_new, after, heads, kv, dim, page, block, by_toke
             pre = mask["prefix"][s] if mask.get("prefix") is not None else 0
             r = ref.head(q[at: at + n, h], k[:, c], v[:, c], mask.get("left", -1), mask.get("right", 0), pre, scale, mask.get("cap", 0.0),
                          float(mask["slopes"][h]) if mask.get("slopes") is not None else 0.0)
-            tol = r["out_tol"]
-            if dtype == F16 and held != "own" and m:
-                # weights below fp16's normal range, in units of the largest scale: half a step 2^-25 each, times a code; the largest weight is 1
-                tol = tol + m * 2.0 ** -25 * (v[:, c].abs().max() * 16)
+            tol = r["out_tol"] + lost(dtype, held, m, v[:, c])
             bad = (out[at: at + n, h].double() - r["out"]).abs() > tol
             assert not bad.any(), (s, h, bad.nonzero()[:4], out[at: at + n, h][bad][:4], r["out"][bad][:4], tol[bad][:4])
             assert not out[at: at + n, h].isnan().any()
@@ -318,3 +326,50 @@ def test_attend_many_rows(dtype, held):
     check_attend(dtype, held, [150, 1, 90, 1, 17], [600, 400, 90, 33, 100], 8, 2, 64, 64, 16)
     check_attend(dtype, held, [130], [390], 4, 4, 128, 32, 1, by_token=True, packed=False)
     check_attend(dtype, held, [65, 64], [65, 300], 2, 1, 128, 16, 16, left=30, cap=10.0)
+
+
+@pytest.mark.parametrize("held", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n_new,after", [([1, 2], [90, 300]), ([70, 3], [200, 130])])
+def test_attend_scales(dtype, held, n_new, after):
+    """Scales that are no powers of two, as calibrated ones, some of them far from the others, and far from 1."""
+    for low, high, extra in ((0.01, 0.02, 0), (1e-3, 1.0, 0), (2e-9, 4e-9, 0), (0.01, 0.02, 1), (300.0, 400.0, 0)):
+        seed = 31
+        table, n_pages = tables(after, 32, seed)
+        pages = Pages(dtype, held, n_pages, 32, 4, 2, 64, False, seed)
+        for i, name in enumerate("kv"):
+            g = torch.Generator().manual_seed(seed + 40 + i)
+            sc = low * (high / low) ** torch.rand(pages.scales[name].shape, generator=g)
+            if extra:
+                sc[torch.rand(sc.shape, generator=g) < 0.3] = 0.015625
+                if name == "v":
+                    sc[torch.rand(sc.shape, generator=g) < 0.1] = 0.0
+            pages.scales[name].copy_(sc)
+            pages.cpu[name] = (pages.cpu[name][0], sc.float())
+        q = normal(seed + 3, sum(n_new), 4, 64).to(dtype)
+        scale = 0.125 * 0.015 / high
+        out, stat = attend(dtype, pages, table, n_new, after, 4, q, True, scale=scale)
+        at = 0
+        for s, (n, m) in enumerate(zip(n_new, after)):
+            k, v = (cref.gathered(pages.cpu[name], s, m, table, 32, 4, held) for name in "kv")
+            for h in range(4):
+                r = ref.head(q[at: at + n, h], k[:, h // 2], v[:, h // 2], -1, 0, 0, scale, 0.0, 0.0)
+                tol = r["out_tol"] + lost(dtype, held, m, v)
+                assert ((out[at: at + n, h].double() - r["out"]).abs() <= tol).all(), (low, high, s, h)
+            at += n
+
+
+@pytest.mark.parametrize("held", ["i8", "e4m3"])
+def test_attend_query_ranges(held):
+    """bf16 queries of any size, which meet codes in fp16."""
+    for size in (1e-30, 1e-4, 1e4, 1e30):
+        table, n_pages = tables([150], 16, 3)
+        pages = Pages(BF16, held, n_pages, 16, 16, 1, 64, False, 4)
+        for n in (2, 130):
+            q = (normal(5, n, 2, 64) * size * torch.exp(2 * normal(6, n, 2, 64))).to(BF16)
+            q[0, 0] = 0
+            out, stat = attend(BF16, pages, table, [n], [150], 2, q, True, scale=min(0.125 / size, 3e38))
+            k, v = (cref.gathered(pages.cpu[name], 0, 150, table, 16, 16, held) for name in "kv")
+            for h in range(2):
+                r = ref.head(q[:, h], k[:, 0], v[:, 0], -1, 0, 0, min(0.125 / size, 3e38), 0.0, 0.0)
+                assert ((out[:, h].double() - r["out"]).abs() <= r["out_tol"] + lost(BF16, held, 150, v)).all(), (size, n, h)
