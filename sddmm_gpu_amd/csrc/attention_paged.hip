@@ -1,7 +1,6 @@
 // Entry points of the attention over a cache in pages: what they check, which kernels they launch, and how large a workspace is.
 #include <hip/hip_runtime.h>
 #include <cmath>
-#include "attention_launch.hpp"
 #include "attention_paged_launch.hpp"
 #include "cache.hpp"
 #include "launch.hpp"
@@ -83,7 +82,7 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
     if (!aligned({d_q, d_out})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (!launchable(r.grid, kAttentionThreads) || (r.splits > 1 && !launchable(attention_join_grid(r.rows * d.n_heads, (int)r.splits, d.head_dim), kAttentionThreads)))
+    if (!launchable(r.grid, 256) || r.slots > 65535 * 256 || (r.splits > 1 && !launchable(attention_paged_join_grid(r.rows * d.n_heads, (int)r.splits, d.head_dim), 512)))
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
     if (in_place_of({d_out, d_lse}, {d_q, cache->k, cache->v, cache->k_scale, cache->v_scale}) || (const void *)d_lse == d_out)
         return fail(SDDMM_ERR_ARG, "%s: a result is in an operand's or the other result's place", who);
@@ -95,8 +94,8 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
     const CacheArgs c = cache_arguments(d, *cache);
     const hipStream_t st = (hipStream_t)stream;
     const int held = held_as(d, *cache);
-    hipError_t e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, (unsigned)r.grid, st) : launch_attention_paged_forward(a, c, d.type, held, (unsigned)r.grid, st);
-    if (e == hipSuccess && r.splits > 1) e = launch_attention_join(a, d.type, st);
+    hipError_t e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, st) : launch_attention_paged_forward(a, c, d.type, held, (unsigned)r.grid, st);
+    if (e == hipSuccess && r.splits > 1) e = launch_attention_paged_join(a, d.type, st);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;
 }

@@ -15,7 +15,7 @@ namespace {
 // The next keys are requested when the scores are done, the next values when the products are; waves have statistics and sums of their own, which
 // are joined at the end.
 template <class T, int HELD, int DP, bool MOD, int R, int NW>
-__global__ __launch_bounds__(64 * NW)
+__global__ __launch_bounds__(64 * NW, 2)
 void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
 {
     typedef typename Elem<T>::Vec8 Vec8;
@@ -30,17 +30,26 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
     __shared__ float2 ml[NW][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
 
-    int b = blockIdx.x;
-    const int kv = b % a.n_kv_heads;
-    b /= a.n_kv_heads;
-    const int split = b % a.n_split;
-    b /= a.n_split;
+    const int kv = blockIdx.x, split = blockIdx.y, b = blockIdx.z;
     int s, tile;
     if (a.q_ptr && a.max_tiles > 1) {
         s = slot_sequence<false>(a.q_ptr, a.n_seq, a.group, kRows, a.max_tiles, a.n_slots, b, tile);
         if (s < 0) return;
+    } else if (a.max_tiles == 1) {
+        s = b, tile = 0;
     } else {
         s = b % a.n_seq, tile = a.max_tiles - 1 - b / a.n_seq;
+    }
+    // The pages that this piece begins with if its rows see the first keys, and any scales: requested before the lengths are known, since each of them is a chain of
+    // misses by itself (one token behind 1501: 11.8 and 7.9 us).
+    const int table_end = (a.max_k - 1) >> c.page_shift;
+    int pages0 = min((split * a.chunk * KT) >> c.page_shift, table_end);
+    uint32_t pages = 0;
+    float scale_raw = 0.f;  // of the key of token `lane`, of the value of token `lane` - 32
+    const float *scale_base = lane < 32 ? c.k_scale : c.v_scale;
+    if (c.n_pages > 0 && a.max_k > 0) {
+        pages = c.page(s, min(pages0 + lane, table_end));
+        if constexpr (HELD != kHeldOwn) scale_raw = *scale_base;
     }
     const Seq e = sequence(a, s);
     const int n_rows = e.nq * a.group, n_keys = c.n_pages > 0 ? e.nk : 0;
@@ -82,113 +91,109 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
     Bend<T> bend;
     if constexpr (MOD) bend.init(scale, a.cap);
 
-    // places: the page of a half tile is the same for all lanes, a lane's place in it fits 32 bits
-    uint32_t pages = 0;
-    int pages0 = INT32_MIN / 2, page[2] = {0, 0};  // (of the tile whose keys, and then values, are requested)
-    auto page_of = [&](int key) {
-        const int i = min(key, n_keys - 1) >> c.page_shift;
-        if (i - pages0 >= 64) {
-            pages0 = i;
-            pages = c.page(s, min(i + lane, (n_keys - 1) >> c.page_shift));
-        }
-        return __builtin_amdgcn_readlane((int)pages, i - pages0);
-    };
-    const int in_page = (1 << c.page_shift) - 1;
-    const bool whole = a.head_dim == DP;
-    uint32_t k_off[S * 8 * kSize / kPiece];
-    bool k_there[S * 8 * kSize / kPiece];
+    // Places: the page of a half tile is the same for all lanes, a lane's place in it fits 32 bits.  What a half tile lacks -- rows behind the last key, all of a tile behind the
+    // wave's last one, elements behind the head's end -- lies outside the range that its loads are given: it becomes 0 and is not read, and the requests are the same in every
+    // tile, so that the waits for them are.
+    constexpr int kLoads = S * 8 * kSize / kPiece;
+    const int in_page = (1 << c.page_shift) - 1, row_bytes = a.head_dim * kSize;
+    uint32_t k_off[kLoads], v_off[4];
 #pragma unroll
-    for (int i = 0; i < S * 8 * kSize / kPiece; ++i) {
-        const int at = (kPiece == 16 && kSize == 1 ? 64 : 32) * i * kSize + kPiece * g;  // bytes
-        k_there[i] = at < a.head_dim * kSize;
-        k_off[i] = (uint32_t)(n * c.k_row) + (k_there[i] ? at : 0);
+    for (int i = 0; i < kLoads; ++i) {
+        const int at = (kPiece == 16 && kSize == 1 ? 64 : 32 * kSize) * i + kPiece * g;
+        k_off[i] = at < row_bytes ? (uint32_t)(n * (int)c.k_row) + at : 0x7ffffff0u;
     }
-    const uint32_t v_off = (uint32_t)(4 * g * c.v_row) + (E * n < a.head_dim ? kValueBytes * n : 0);
-
-    uint32_t k_raw[2][kKeyWords], v_raw[8][kValueWords];
-    float ks[2][4], vs[2][4];
-    const bool fine = c.block_shift < 2;  // the four tokens of a lane's results have scales of their own
-    auto request_scales = [&](const float *scales, int page, int at, float (&to)[4]) {
-        const float *p = scales + c.scale_at(page, kv, at);
-        if (fine) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[i] = p[((at & ((1 << c.block_shift) - 1)) + 4 * g + i) >> c.block_shift];
-        } else {
-            to[0] = p[((at & ((1 << c.block_shift) - 1)) + 4 * g) >> c.block_shift];
-        }
+    for (int i = 0; i < 4; ++i) v_off[i] = kValueBytes * n < row_bytes ? (uint32_t)((4 * g + i) * (int)c.v_row) + kValueBytes * n : 0x7ffffff0u;
+    const char *k_base = c.k + kv * c.k_head, *v_base = c.v + kv * c.v_head;
+    int page0 = 0, page1 = 0;  // of the halves of the tile whose keys, and then values, are requested (no array: indexed by a lane's number it would be one in memory)
+    uint32_t k_raw[2][kKeyWords], v_raw[8][kValueWords];
+    auto range = [&](const char *base, int at, int64_t row, int key, int t) {
+        const uint64_t begin = (uint64_t)(base + at * row);
+        const int rows = t < last ? min(any_hi - key, 16) : 0;
+        const uint32_t lo32 = __builtin_amdgcn_readfirstlane((int)(uint32_t)begin), hi32 = __builtin_amdgcn_readfirstlane((int)(uint32_t)(begin >> 32));
+        return __builtin_amdgcn_make_buffer_rsrc((void *)((uint64_t)hi32 << 32 | lo32), 0, __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * (int)row + row_bytes : 0), 0x00020000);
     };
     auto request_keys = [&](int t) {
-        if (t >= last) return;
+        const int last_page = (n_keys - 1) >> c.page_shift, i0 = min((key0 + t * KT) >> c.page_shift, last_page), i1 = min((key0 + t * KT + 16) >> c.page_shift, last_page);
+        if (i0 < pages0 || i1 - pages0 >= 64) {
+            pages0 = i0;
+            pages = c.page(s, min(i0 + lane, last_page));
+        }
+        page0 = __builtin_amdgcn_readlane((int)pages, i0 - pages0), page1 = __builtin_amdgcn_readlane((int)pages, i1 - pages0);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int key = key0 + t * KT + 16 * u, at = key & in_page;
-            page[u] = page_of(key);
-            const char *p = c.k + page[u] * c.k_page + kv * c.k_head + at * c.k_row;
+            const int key = key0 + t * KT + 16 * u;
+            const auto src = range(k_base + (u ? page1 : page0) * c.k_page, key & in_page, c.k_row, key, t);
 #pragma unroll
-            for (int i = 0; i < S * 8 * kSize / kPiece; ++i) {
+            for (int j = 0; j < kLoads; ++j) {
                 constexpr int W = kPiece / 4;
                 if constexpr (W == 2) {
-                    const uint2v x = *(const uint2v *)(p + k_off[i]);
-                    k_raw[u][2 * i] = x.x, k_raw[u][2 * i + 1] = x.y;
+                    const uint2v x = __builtin_amdgcn_raw_buffer_load_b64(src, k_off[j], 0, 0);
+                    k_raw[u][2 * j] = x.x, k_raw[u][2 * j + 1] = x.y;
                 } else {
 #pragma unroll
                     for (int w = 0; w < W / 4; ++w) {
-                        const uint4v x = *(const uint4v *)(p + k_off[i] + 16 * w);
+                        const uint4v x = __builtin_amdgcn_raw_buffer_load_b128(src, k_off[j] + 16 * w, 0, 0);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) k_raw[u][W * i + 4 * w + j] = x[j];
+                        for (int k = 0; k < 4; ++k) k_raw[u][W * j + 4 * w + k] = x[k];
                     }
                 }
             }
-            if constexpr (HELD != kHeldOwn) request_scales(c.k_scale, page[u], at, ks[u]);
         }
+        if constexpr (HELD != kHeldOwn) {
+            const int at = (key0 + t * KT + (lane & 31)) & in_page;
+            scale_raw = scale_base[c.scale_at(lane & 16 ? page1 : page0, kv, at)];
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (keys' requests before values' everywhere, or the waits for keys would be for both)
     };
     auto request_values = [&](int t) {
-        if (t >= last) return;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int at = (key0 + t * KT + 16 * u) & in_page;
-            const char *p = c.v + page[u] * c.v_page + kv * c.v_head + at * c.v_row;
+            const int key = key0 + t * KT + 16 * u;
+            const auto src = range(v_base + (u ? page1 : page0) * c.v_page, key & in_page, c.v_row, key, t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const char *row = p + i * c.v_row + v_off;
                 uint32_t (&to)[kValueWords] = v_raw[4 * u + i];
-                if constexpr (kValueBytes == 2) to[0] = *(const uint16_t *)row;
-                else if constexpr (kValueBytes == 4) to[0] = *(const uint32_t *)row;
+                if constexpr (kValueBytes == 2) to[0] = __builtin_amdgcn_raw_buffer_load_b16(src, v_off[i], 0, 0);
+                else if constexpr (kValueBytes == 4) to[0] = __builtin_amdgcn_raw_buffer_load_b32(src, v_off[i], 0, 0);
                 else if constexpr (kValueBytes == 8) {
-                    const uint2v x = *(const uint2v *)row;
+                    const uint2v x = __builtin_amdgcn_raw_buffer_load_b64(src, v_off[i], 0, 0);
                     to[0] = x.x, to[1] = x.y;
                 } else {
 #pragma unroll
                     for (int w = 0; w < kValueWords / 4; ++w) {
-                        const uint4v x = *(const uint4v *)(row + 16 * w);
+                        const uint4v x = __builtin_amdgcn_raw_buffer_load_b128(src, v_off[i] + 16 * w, 0, 0);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) to[4 * w + j] = x[j];
                     }
                 }
             }
-            if constexpr (HELD != kHeldOwn) request_scales(c.v_scale, page[u], at, vs[u]);
         }
     };
 
+    if constexpr (HELD != kHeldOwn) asm volatile("" ::"v"(scale_raw));
     int t = first + wave;
-    request_keys(t);
-    request_values(t);
+    if (t < last) {
+        request_keys(t);
+        request_values(t);
+    }
     for (; t < last; t += NW) {
         const int key = key0 + t * KT;
         floatx4 x[R][2];
+        // (a head of 8 elements more than whole pieces: a piece's second half may be anything)
+        if constexpr (kSize == 1 && kPiece == 16) {
+            if (a.head_dim & 8) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < kKeyWords; ++i)
+                        if (i % 4 >= 2) k_raw[u][i] = 64 * (i / 4) + 16 * g + 8 < a.head_dim ? k_raw[u][i] : 0u;
+            }
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int r = 0; r < R; ++r) x[r][u] = floatx4{0.f, 0.f, 0.f, 0.f};
-            if (!whole) {  // (elements behind the head's end: another element of the row was read)
-#pragma unroll
-                for (int i = 0; i < kKeyWords; ++i) {
-                    const int piece = i * 4 / kPiece;
-                    bool in = k_there[piece];
-                    if constexpr (kSize == 1 && kPiece == 16) in = in && (i % 4 < 2 || 64 * piece + 16 * g + 8 < a.head_dim);
-                    k_raw[u][i] = in ? k_raw[u][i] : 0u;
-                }
-            }
 #pragma unroll
             for (int i = 0; i < S; ++i) {
                 Vec8 k;
@@ -204,10 +209,23 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
                 for (int r = 0; r < R; ++r) x[r][u] = mma16<T>(k, qf[r][i], x[r][u]);
             }
         }
-        float y[R][8], kk[8];
+        float y[R][8], kk[8], vv[8];
         if constexpr (HELD != kHeldOwn) {
+            // the scales of the lane's eight tokens, from the lanes that have them; one for four tokens where blocks are as long
+            if (c.block_shift >= 2) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) kk[j] = fine ? ks[j >> 2][j & 3] : ks[j >> 2][0];
+                for (int u = 0; u < 2; ++u) {
+                    kk[4 * u] = __shfl(scale_raw, 16 * u + 4 * g), vv[4 * u] = __shfl(scale_raw, 32 + 16 * u + 4 * g);
+#pragma unroll
+                    for (int i = 1; i < 4; ++i) kk[4 * u + i] = kk[4 * u], vv[4 * u + i] = vv[4 * u];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int from = 16 * (j >> 2) + 4 * g + (j & 3);
+                    kk[j] = __shfl(scale_raw, from), vv[j] = __shfl(scale_raw, 32 + from);
+                }
+            }
         }
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -261,26 +279,20 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
             }
         }
 
-        // values and scales outside the rows' keys may hold anything
+        // values before the rows' keys may hold anything, and so may scales of what is no key of theirs
         if (key < any_lo || key + KT > any_hi) {
-            const int at = key + 4 * g;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int token = at + 16 * (j >> 2) + (j & 3);
+                const int token = key + 4 * g + 16 * (j >> 2) + (j & 3);
                 const bool in = token >= any_lo && token < any_hi;
 #pragma unroll
                 for (int w = 0; w < kValueWords; ++w) v_raw[j][w] = in ? v_raw[j][w] : 0u;
+                vv[j] = in ? vv[j] : 0.f;
             }
         }
         Vec8 p[R];
         if constexpr (HELD != kHeldOwn) {
-            float w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                w[j] = fine ? vs[j >> 2][j & 3] : vs[j >> 2][0];
-                const int token = key + 4 * g + 16 * (j >> 2) + (j & 3);
-                if (key < any_lo || key + KT > any_hi) w[j] = token >= any_lo && token < any_hi ? w[j] : 0.f;
-            }
+            float (&w)[8] = vv;
             if constexpr (kNorm) {
                 // fp16: scales in units of the largest so far, which keeps their products with probabilities in the type's range
                 float most = w[0];
@@ -399,14 +411,105 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
     }
 }
 
+// The parts of a row: sums and totals in units of 2^(largest maximum).  Groups of DP / 4 lanes take parts in turn, eight at a time with maxima and sums under way together, each
+// with a running maximum of its own, and meet in LDS.
+constexpr int kJoinThreads = 512;
+template <class T, int DP>
+__global__ __launch_bounds__(kJoinThreads)
+void sddmm_attention_paged_join_kernel(const AttnArgs a, const int per_row)
+{
+    constexpr int kLanes = DP / 4, kGroups = kJoinThreads / kLanes;
+    __shared__ floatx4 sums[kGroups][kLanes];
+    __shared__ float2 stats[kGroups];
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, mine = group % per_row, col = lane * 4;
+    const int64_t all = a.rows * a.n_heads, at = (int64_t)blockIdx.x * (kGroups / per_row) + group / per_row;
+    const int head = (int)(at % a.n_heads);
+    const int64_t row = at / a.n_heads;
+    int64_t to_row = 0;
+    bool there = at < all;
+    if (a.q_ptr) {
+        there = there && row >= a.q_ptr[0] && row < a.q_ptr[a.n_seq];
+        to_row = row * a.o_row;
+    } else if (there) {
+        const int s = (int)(row / a.max_q), i = (int)(row % a.max_q);
+        there = !a.q_len || i < min(a.q_len[s], a.max_q);
+        to_row = s * a.o_seq + i * a.o_row;
+    }
+    float top = -INFINITY, total = 0.f;
+    floatx4 y = {0.f, 0.f, 0.f, 0.f};
+    for (int p0 = mine; there && p0 < a.n_part; p0 += 8 * per_row) {
+        float2 ml[8];
+        floatx4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int p = min(p0 + i * per_row, a.n_part - 1);
+            ml[i] = a.part_ml[p * all + at];
+            x[i] = col < a.head_dim ? *(const floatx4 *)(a.part_o + (p * all + at) * a.head_dim + col) : floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+        float most = top;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (p0 + i * per_row >= a.n_part) ml[i] = make_float2(-INFINITY, 0.f);
+            most = fmaxf(most, ml[i].x);
+        }
+        const float by = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - most);
+        y *= by, total *= by, top = most;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (ml[i].x == -INFINITY) continue;  // (no keys: its sums were not written)
+            const float w = __builtin_amdgcn_exp2f(ml[i].x - top);
+            y += x[i] * w;
+            total = fmaf(w, ml[i].y, total);
+        }
+    }
+    if (per_row > 1) {
+        sums[group][lane] = y;
+        if (lane == 0) stats[group] = make_float2(top, total);
+        __syncthreads();
+        if (mine) return;
+        float most = top;
+        for (int g = 1; g < per_row; ++g) most = fmaxf(most, stats[group + g].x);
+        const float by = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - most);
+        y *= by, total *= by, top = most;
+        for (int g = 1; g < per_row; ++g) {
+            const float2 one = stats[group + g];
+            if (one.x == -INFINITY) continue;
+            const float w = __builtin_amdgcn_exp2f(one.x - top);
+            y += sums[group + g][lane] * w;
+            total = fmaf(w, one.y, total);
+        }
+    }
+    if (!there) return;
+    const float by = total > 0.f || total != total ? 1.f / total : 0.f;
+    T *to = (T *)a.out + to_row + head * a.o_head;
+    if (col < a.head_dim) *(typename Elem<T>::Vec4 *)(to + col) = __builtin_convertvector(y * by, typename Elem<T>::Vec4);
+    if (a.lse && lane == 0) a.lse[at] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+// lane groups of a workgroup of the kernel above, and how many of them share a row
+int join_groups(int head_dim) { return kJoinThreads / ((head_dim <= 64 ? 64 : 128) / 4); }
+int join_per_row(int n_part, int head_dim)
+{
+    int per_row = 1;
+    while (per_row < join_groups(head_dim) && per_row * 2 < n_part) per_row *= 2;
+    return per_row;
+}
+template <class T>
+hipError_t launch_join(const AttnArgs &a, hipStream_t st)
+{
+    const dim3 grid((unsigned)attention_paged_join_grid(a.rows * a.n_heads, a.n_part, a.head_dim)), block(kJoinThreads);
+    return a.head_dim <= 64 ? launch(sddmm_attention_paged_join_kernel<T, 64>, grid, block, 0, st, a, join_per_row(a.n_part, a.head_dim))
+                            : launch(sddmm_attention_paged_join_kernel<T, 128>, grid, block, 0, st, a, join_per_row(a.n_part, a.head_dim));
+}
+
 template <class T, int HELD, int DP, int R, int NW>
-hipError_t launch_dim(const AttnArgs &a, const CacheArgs &c, unsigned grid, hipStream_t st)
+hipError_t launch_dim(const AttnArgs &a, const CacheArgs &c, dim3 grid, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
-    return launch(mod ? sddmm_attention_paged_token_kernel<T, HELD, DP, true, R, NW> : sddmm_attention_paged_token_kernel<T, HELD, DP, false, R, NW>, dim3(grid), dim3(64 * NW), 0, st, a, c);
+    return launch(mod ? sddmm_attention_paged_token_kernel<T, HELD, DP, true, R, NW> : sddmm_attention_paged_token_kernel<T, HELD, DP, false, R, NW>, grid, dim3(64 * NW), 0, st, a, c);
 }
 template <class T, int HELD, int R, int NW>
-hipError_t launch_held(const AttnArgs &a, const CacheArgs &c, unsigned grid, hipStream_t st)
+hipError_t launch_held(const AttnArgs &a, const CacheArgs &c, dim3 grid, hipStream_t st)
 {
     if constexpr (sizeof(T) == 4) {
         if (a.head_dim <= 32) return launch_dim<T, HELD, 32, R, NW>(a, c, grid, st);
@@ -414,12 +517,12 @@ hipError_t launch_held(const AttnArgs &a, const CacheArgs &c, unsigned grid, hip
     return a.head_dim <= 64 ? launch_dim<T, HELD, 64, R, NW>(a, c, grid, st) : launch_dim<T, HELD, 128, R, NW>(a, c, grid, st);
 }
 template <class T, int R, int NW>
-hipError_t launch_typed(const AttnArgs &a, const CacheArgs &c, int held, unsigned grid, hipStream_t st)
+hipError_t launch_typed(const AttnArgs &a, const CacheArgs &c, int held, dim3 grid, hipStream_t st)
 {
     return held == kHeldI8 ? launch_held<T, kHeldI8, R, NW>(a, c, grid, st) : held == kHeldE4m3 ? launch_held<T, kHeldE4m3, R, NW>(a, c, grid, st) : launch_held<T, kHeldOwn, R, NW>(a, c, grid, st);
 }
 template <int R, int NW>
-hipError_t launch_rows(const AttnArgs &a, const CacheArgs &c, int type, int held, unsigned grid, hipStream_t st)
+hipError_t launch_rows(const AttnArgs &a, const CacheArgs &c, int type, int held, dim3 grid, hipStream_t st)
 {
     return type == SDDMM_TYPE_F32 ? launch_typed<float, R, NW>(a, c, held, grid, st) : type == SDDMM_TYPE_F16 ? launch_typed<_Float16, R, NW>(a, c, held, grid, st)
                                                                                                              : launch_typed<__bf16, R, NW>(a, c, held, grid, st);
@@ -427,8 +530,20 @@ hipError_t launch_rows(const AttnArgs &a, const CacheArgs &c, int type, int held
 
 }  // namespace
 
-hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, unsigned grid, hipStream_t st)
+int64_t attention_paged_join_grid(int64_t rows_of_heads, int n_part, int head_dim)
 {
+    const int rows = join_groups(head_dim) / join_per_row(n_part, head_dim);
+    return (rows_of_heads + rows - 1) / rows;
+}
+
+hipError_t launch_attention_paged_join(const AttnArgs &a, int type, hipStream_t st)
+{
+    return type == SDDMM_TYPE_F32 ? launch_join<float>(a, st) : type == SDDMM_TYPE_F16 ? launch_join<_Float16>(a, st) : launch_join<__bf16>(a, st);
+}
+
+hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, hipStream_t st)
+{
+    const dim3 grid((unsigned)a.n_kv_heads, (unsigned)a.n_split, (unsigned)a.n_slots);
     return tiles == 1 ? launch_rows<1, 4>(a, c, type, held, grid, st) : launch_rows<2, 4>(a, c, type, held, grid, st);
 }
 
