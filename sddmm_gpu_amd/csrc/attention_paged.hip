@@ -14,6 +14,7 @@ struct Deal {
     int64_t rows = 0;  // of all sequences
     bool token = true; // the kernel for few rows
     int tiles = 1;     // of 16 rows to a workgroup of it
+    int tile = 128;    // rows of a workgroup of the kernel for many
     int64_t slots = 0, max_tiles = 0, grid = 0, splits = 1, chunk = 1;
     int64_t part_bytes = 0, bytes = 0;
 };
@@ -26,7 +27,11 @@ Deal deal(const sddmm_attention_desc &d)
     if (r.rows == 0) return r;
     r.token = packed <= 64;
     r.tiles = packed <= 16 ? 1 : 2;
-    const int64_t few = r.token ? 16 * r.tiles : 128;
+    // Many rows: 256 to a workgroup, which share the codes that it makes operands of, where there are 128 workgroups of them and long heads (us with 256 and 128: 2048 tokens behind
+    // 14,336, 16 heads over 2 of 128, 8 bits 317 and 360; 1024 behind 7168, 32 over 8 167 and 177; a prompt of 4096, 32 over 8, 16 bits 147 and 164; 2048, 16 over 4 62 and 62; 128 behind
+    // 8064 50 and 39; 16 of 300 tokens, heads of 64 54 and 43).
+    if (!r.token && d.type != SDDMM_TYPE_F32 && d.head_dim > 64 && (d.q_ptr ? r.rows * group / 256 + d.n_seq : div_up(packed, 256) * d.n_seq) * d.n_kv_heads >= 128) r.tile = 256;
+    const int64_t few = r.token ? 16 * r.tiles : r.tile;
     r.max_tiles = div_up(packed, few);
     r.slots = r.max_tiles == 1 && r.token ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
     const int64_t workgroups = r.slots * d.n_kv_heads;
@@ -45,7 +50,7 @@ Deal deal(const sddmm_attention_desc &d)
         r.chunk = div_up(key_tiles, r.splits);
         r.splits = div_up(key_tiles, r.chunk);
     } else {
-        r.splits = std::max<int64_t>(1, std::min(std::min(div_up(512, workgroups), div_up(key_tiles, 8)), (int64_t)256));
+        r.splits = std::max<int64_t>(1, std::min(std::min(div_up(r.tile == 256 ? 256 : 512, workgroups), div_up(key_tiles, 8)), (int64_t)256));
     }
     r.grid = workgroups * r.splits;
     if (r.splits > 1) {
@@ -89,7 +94,7 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
     if (!aligned({d_q, d_out})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (!launchable(r.grid, 256) || r.slots > 65535 * 256 || (r.splits > 1 && !launchable(attention_paged_join_grid(r.rows * d.n_heads, (int)r.splits, d.head_dim), 512)))
+    if (!launchable(r.grid, 512) || r.slots > 65535 * 256 || (r.splits > 1 && !launchable(attention_paged_join_grid(r.rows * d.n_heads, (int)r.splits, d.head_dim), 512)))
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
     if (in_place_of({d_out, d_lse}, {d_q, cache->k, cache->v, cache->k_scale, cache->v_scale}) || (const void *)d_lse == d_out)
         return fail(SDDMM_ERR_ARG, "%s: a result is in an operand's or the other result's place", who);
@@ -101,7 +106,7 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
     const CacheArgs c = cache_arguments(d, *cache);
     const hipStream_t st = (hipStream_t)stream;
     const int held = held_as(d, *cache);
-    hipError_t e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, st) : launch_attention_paged_forward(a, c, d.type, held, (unsigned)r.grid, st);
+    hipError_t e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, st) : launch_attention_paged_forward(a, c, d.type, held, r.tile, (unsigned)r.grid, st);
     if (e == hipSuccess && r.splits > 1) e = launch_attention_paged_join(a, d.type, st);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;

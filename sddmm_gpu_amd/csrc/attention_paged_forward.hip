@@ -17,30 +17,33 @@ void sddmm_attention_paged_kernel(const AttnArgs a, const CacheArgs c)
 }
 
 template <class T, int HELD, int DP>
-hipError_t launch_dim(const AttnArgs &a, const CacheArgs &c, unsigned grid, hipStream_t st)
+hipError_t launch_dim(const AttnArgs &a, const CacheArgs &c, int tile, unsigned grid, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
+    if constexpr (sizeof(T) == 2) {
+        if (tile == 256) return launch(mod ? sddmm_attention_paged_kernel<T, HELD, DP, true, 8> : sddmm_attention_paged_kernel<T, HELD, DP, false, 8>, dim3(grid), dim3(512), 0, st, a, c);
+    }
     return launch(mod ? sddmm_attention_paged_kernel<T, HELD, DP, true, 4> : sddmm_attention_paged_kernel<T, HELD, DP, false, 4>, dim3(grid), dim3(256), 0, st, a, c);
 }
 template <class T, int HELD>
-hipError_t launch_held(const AttnArgs &a, const CacheArgs &c, unsigned grid, hipStream_t st)
+hipError_t launch_held(const AttnArgs &a, const CacheArgs &c, int tile, unsigned grid, hipStream_t st)
 {
     if constexpr (sizeof(T) == 4) {
-        if (a.head_dim <= 32) return launch_dim<T, HELD, 32>(a, c, grid, st);
+        if (a.head_dim <= 32) return launch_dim<T, HELD, 32>(a, c, tile, grid, st);
     }
-    return a.head_dim <= 64 ? launch_dim<T, HELD, 64>(a, c, grid, st) : launch_dim<T, HELD, 128>(a, c, grid, st);
+    return a.head_dim <= 64 ? launch_dim<T, HELD, 64>(a, c, tile, grid, st) : launch_dim<T, HELD, 128>(a, c, tile, grid, st);
 }
 template <class T>
-hipError_t launch_typed(const AttnArgs &a, const CacheArgs &c, int held, unsigned grid, hipStream_t st)
+hipError_t launch_typed(const AttnArgs &a, const CacheArgs &c, int held, int tile, unsigned grid, hipStream_t st)
 {
-    return held == kHeldI8 ? launch_held<T, kHeldI8>(a, c, grid, st) : held == kHeldE4m3 ? launch_held<T, kHeldE4m3>(a, c, grid, st) : launch_held<T, kHeldOwn>(a, c, grid, st);
+    return held == kHeldI8 ? launch_held<T, kHeldI8>(a, c, tile, grid, st) : held == kHeldE4m3 ? launch_held<T, kHeldE4m3>(a, c, tile, grid, st) : launch_held<T, kHeldOwn>(a, c, tile, grid, st);
 }
 
 }  // namespace
 
-hipError_t launch_attention_paged_forward(const AttnArgs &a, const CacheArgs &c, int type, int held, unsigned grid, hipStream_t st)
+hipError_t launch_attention_paged_forward(const AttnArgs &a, const CacheArgs &c, int type, int held, int tile, unsigned grid, hipStream_t st)
 {
-    return type == SDDMM_TYPE_F32 ? launch_typed<float>(a, c, held, grid, st) : type == SDDMM_TYPE_F16 ? launch_typed<_Float16>(a, c, held, grid, st) : launch_typed<__bf16>(a, c, held, grid, st);
+    return type == SDDMM_TYPE_F32 ? launch_typed<float>(a, c, held, tile, grid, st) : type == SDDMM_TYPE_F16 ? launch_typed<_Float16>(a, c, held, tile, grid, st) : launch_typed<__bf16>(a, c, held, tile, grid, st);
 }
 
 }  // namespace sddmm

@@ -11,8 +11,8 @@ struct CacheArgs;
 // tiles: of 16 rows to a workgroup, 1 or 2; a.chunk: tiles of 32 keys to a piece
 hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, hipStream_t st);
 
-// 128 rows to a workgroup
-hipError_t launch_attention_paged_forward(const AttnArgs &a, const CacheArgs &c, int type, int held, unsigned grid, hipStream_t st);
+// tile: rows of a workgroup, 128 or 256 (16-bit operands)
+hipError_t launch_attention_paged_forward(const AttnArgs &a, const CacheArgs &c, int type, int held, int tile, unsigned grid, hipStream_t st);
 
 int64_t attention_paged_join_grid(int64_t rows_of_heads, int n_part, int head_dim);  // workgroups of the join, of 512 threads
 hipError_t launch_attention_paged_join(const AttnArgs &a, int type, hipStream_t st);

@@ -1,5 +1,6 @@
 // Attention over a cache in pages (gfx950): a tile of rows against tiles of keys.
 #pragma once
+#include <cfloat>
 #include "attention_paged.hpp"
 
 namespace sddmm {
@@ -47,9 +48,9 @@ template <class U, int HELD> __device__ __forceinline__ float fold(float scale, 
         return scale;
     } else {
         constexpr int kLeast = HELD == kHeldI8 ? -24 : -15, kMost = HELD == kHeldI8 ? 5 : 7;
-        const int e = min(max((int)((__float_as_uint(scale) >> 23) & 255u) - 127, kLeast), kMost);
-        const float by = __uint_as_float((uint32_t)(e + 127) << 23);
-        left = scale * __uint_as_float((uint32_t)(127 - e) << 23);
+        const int e = min(max(__builtin_amdgcn_frexp_expf(scale) - 1, kLeast), kMost);
+        const float by = __uint_as_float((uint32_t)((e << 23) + 0x3f800000));
+        left = __builtin_amdgcn_ldexpf(scale, -e);
         return by;
     }
 }
@@ -65,7 +66,8 @@ struct PagedTile {
     static constexpr int KT = sizeof(U) == 2 ? 64 : 32;
     static constexpr int kRows = 32 * NW;
     typedef Tile<U, DP, KT> Keys;
-    static constexpr int kLds = 4 * Keys::kBytes + (HELD != kHeldOwn ? 2 * (2 * KT + 2 * NW) * 4 : 0);
+    static constexpr int kTiles = 4 * Keys::kBytes;
+    static constexpr int kLds = kTiles + (HELD != kHeldOwn ? 4 * (KT * 4 + 8) : 0);
     static __device__ __forceinline__ void run(const AttnArgs &a, const CacheArgs &c, int b, char (&memory)[kLds]);
 };
 
@@ -76,9 +78,12 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
     constexpr bool kCodes = HELD != kHeldOwn, kHalves = kCodes && sizeof(U) == 2;
     constexpr float kShift = kHalves ? 7.f : 0.f;  // probabilities are up to 2^(8 + this): fp16's small ones lose nothing that counts
     typedef typename Elem<U>::Vec8 Vec8;
-    auto &lds = *(char (*)[2][2][Keys::kBytes])memory;
-    float *left = (float *)(memory + 4 * Keys::kBytes);  // [buffer][keys, values][KT], then [buffer][keys, values][NW]: whether any is not 1
-    int *any_left = (int *)(left + 4 * KT);
+    // tiles of keys and of values, two in turn; for each of them what is left of scales, and whether a wave's rows have any that is not 1
+    auto place_of = [&](int which, int t) { return (t & 1) * 2 + which; };
+    auto tile_at = [&](int which, int t) { return memory + place_of(which, t) * Keys::kBytes; };
+    static_assert(8 % NW == 0);
+    float *left = (float *)(memory + kTiles);
+    uint8_t *any_left = (uint8_t *)(left + 4 * KT);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
 
     int s = 0, tile;
@@ -143,7 +148,7 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
     Bend<T> bend;
     if constexpr (MOD) bend.init(scale, a.cap);
     const float unit = MOD ? 1.f : scale * kLog2e * by_row;  // scores in registers to powers of two
-    const float raise = 8.f / unit;
+    const float raise = fminf(8.f / unit, FLT_MAX);  // (finite: added to a maximum of -infinity)
     const float slope = MOD && a.slopes && there ? a.slopes[head] * kLog2e : 0.f;
     float m = -INFINITY, sum = 0.f, norm = 0.f;
 
@@ -167,7 +172,16 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
     constexpr int kPiece = DP == 32 ? 8 : 16, kLanes = DP / kPiece, RPW = 64 / kLanes, kSteps = (KT + RPW * NW - 1) / (RPW * NW), kWords = kPiece / 4;
     uint32_t raw[kCodes ? kSteps : 1][2][kWords];
     float scales[kCodes ? kSteps : 1][2];
-    const int my_row = lane / kLanes, my_piece = lane % kLanes * kPiece;
+    // (of the lanes that write to LDS together, eight, half are four rows behind the others, whose pieces lie in the other banks)
+    const int my_row = kPiece == 8 ? lane / kLanes : kLanes == 8 ? (lane >> 4) | (lane & 4) : ((lane >> 3) & 3) | (lane & 4) | ((lane >> 2) & 8);
+    const int my_piece = (kPiece == 8 ? lane % kLanes : kLanes == 8 ? (lane & 3) | ((lane >> 1) & 4) : lane & 3) * kPiece;
+    static_assert(kLanes == 8 || kLanes == 4);
+    // (16 rows at most, of which `rows` exist: what lies behind them and behind the head's end becomes 0 and is not read)
+    auto rows_at = [&](const char *base, uint32_t row, int rows) {
+        const uint64_t begin = (uint64_t)base;
+        const uint32_t lo32 = __builtin_amdgcn_readfirstlane((int)(uint32_t)begin), hi32 = __builtin_amdgcn_readfirstlane((int)(uint32_t)(begin >> 32));
+        return __builtin_amdgcn_make_buffer_rsrc((void *)((uint64_t)hi32 << 32 | lo32), 0, __builtin_amdgcn_readfirstlane(rows > 0 ? (min(rows, 16) - 1) * (int)row + a.head_dim : 0), 0x00020000);
+    };
     auto request = [&](int t) {
         const int key = key0 + t * KT;
         hold_pages(key);
@@ -176,36 +190,36 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
             for (int j = 0; j < kSteps; ++j) {
                 const int row0 = (j * NW + wave) * RPW;
                 if (row0 >= KT) break;
-                const int page = page_of(key + row0), place = (key + row0) & in_page, piece = my_piece < a.head_dim ? my_piece : 0;
-                const char *pk = c.k + page * c.k_page + kv * c.k_head + place * c.k_row + (uint32_t)(my_row * (int)c.k_row + piece);
-                const char *pv = c.v + page * c.v_page + kv * c.v_head + place * c.v_row + (uint32_t)(my_row * (int)c.v_row + piece);
+                const int at = key + row0, page = page_of(at), place = at & in_page, r = at + my_row;
+                const uint32_t off = r >= any_lo && my_piece < a.head_dim ? my_piece : 0x7ffffff0u;
+                const auto src_k = rows_at(c.k_at(page, kv, place), c.k_row, any_hi - at), src_v = rows_at(c.v_at(page, kv, place), c.v_row, any_hi - at);
+                const uint32_t off_k = off + (uint32_t)(my_row * (int)c.k_row), off_v = off + (uint32_t)(my_row * (int)c.v_row);
                 if constexpr (kPiece == 16) {
-                    const uint4v x = *(const uint4v *)pk, y = *(const uint4v *)pv;
+                    const uint4v x = __builtin_amdgcn_raw_buffer_load_b128(src_k, off_k, 0, 0), y = __builtin_amdgcn_raw_buffer_load_b128(src_v, off_v, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) raw[j][0][i] = x[i], raw[j][1][i] = y[i];
                 } else {
-                    const uint2v x = *(const uint2v *)pk, y = *(const uint2v *)pv;
+                    const uint2v x = __builtin_amdgcn_raw_buffer_load_b64(src_k, off_k, 0, 0), y = __builtin_amdgcn_raw_buffer_load_b64(src_v, off_v, 0, 0);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) raw[j][0][i] = x[i], raw[j][1][i] = y[i];
                 }
-                const int64_t sc = c.scale_at(page, kv, 0) + ((place + my_row) >> c.block_shift);
-                scales[j][0] = c.k_scale[sc], scales[j][1] = c.v_scale[sc];
+                const int64_t first_scale = c.scale_at(page, kv, 0);
+                const uint32_t mine = (uint32_t)((place + my_row) >> c.block_shift);
+                scales[j][0] = (c.k_scale + first_scale)[mine], scales[j][1] = (c.v_scale + first_scale)[mine];
             }
         } else {
             constexpr int kStep = 1024 / Keys::kRowBytes;  // rows of a request
             static_assert(kStep <= 16);
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
-                const char *cache = which ? c.v : c.k;
-                const int64_t page_stride = which ? c.v_page : c.k_page, row_stride = which ? c.v_row : c.k_row, head_stride = which ? c.v_head : c.k_head;
-                char *to = lds[t & 1][which];
+                char *to = tile_at(which, t);
 #pragma unroll
                 for (int i = 0; i < Keys::kBytes / 1024 / NW; ++i) {
                     const int block = (i * NW + wave) * 1024, row0 = block / Keys::kRowBytes, group = row0 & ~15;
                     // rows from any_lo on, up to any_hi, of the sixteen: others are taken as 0
                     const int at = key + group, place = at & in_page, valid = min(any_hi - at, 16);
-                    const char *base = cache + page_of(at) * page_stride + kv * head_stride + place * row_stride;
-                    Keys::request_rows(to, base, (uint32_t)row_stride, valid, max(any_lo - at, 0), a.head_dim * (int)sizeof(T), block, group, lane);
+                    const int page = page_of(at);
+                    Keys::request_rows(to, which ? c.v_at(page, kv, place) : c.k_at(page, kv, place), which ? c.v_row : c.k_row, valid, max(any_lo - at, 0), a.head_dim * (int)sizeof(T), block, group, lane);
                 }
             }
         }
@@ -220,17 +234,20 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
                 if (row0 >= KT) break;
                 const int r = row0 + my_row, at = key + r;
                 const bool in = at >= any_lo && at < any_hi;
+                if (kPiece == 16 && (a.head_dim & 8)) {  // (a head of 8 elements more than whole pieces: what follows them may be anything)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) raw[j][i & 1][2 + i / 2] = my_piece + 8 < a.head_dim ? raw[j][i & 1][2 + i / 2] : 0u;
+                }
 #pragma unroll
                 for (int which = 0; which < 2; ++which) {
                     float rest;
                     const float by = fold<U, HELD>(in ? scales[j][which] : 1.f, rest);
                     some[which] = some[which] || rest != 1.f;
-                    if (kHalves && lane % kLanes == 0) left[((t & 1) * 2 + which) * KT + r] = rest;
-                    char *to = lds[t & 1][which] + r * Keys::kRowBytes;
+                    if (kHalves && my_piece == 0) left[place_of(which, t) * KT + r] = rest;
+                    char *to = tile_at(which, t) + r * Keys::kRowBytes;
 #pragma unroll
                     for (int i = 0; i < kPiece / 8; ++i) {
-                        const bool here = in && my_piece + 8 * i < a.head_dim;
-                        const Vec8 x = expand_by<U, HELD>(here ? raw[j][which][2 * i] : 0u, here ? raw[j][which][2 * i + 1] : 0u, by);
+                        const Vec8 x = expand_by<U, HELD>(raw[j][which][2 * i], raw[j][which][2 * i + 1], by);
                         const int p = (my_piece + 8 * i) * (int)sizeof(U) / 16;
                         if constexpr (sizeof(U) == 2) {
                             *(Vec8 *)(to + ((p ^ Keys::turn(r)) << 4)) = x;
@@ -243,10 +260,159 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
             }
             if constexpr (kHalves) {
                 const bool k_some = __any(some[0]), v_some = __any(some[1]);
-                if (lane == 0) any_left[((t & 1) * 2 + 0) * NW + wave] = k_some, any_left[((t & 1) * 2 + 1) * NW + wave] = v_some;
+                if (lane < 8 / NW) any_left[place_of(0, t) * 8 + wave * (8 / NW) + lane] = k_some, any_left[place_of(1, t) * 8 + wave * (8 / NW) + lane] = v_some;
             }
         }
     };
+    uint2v some_left[2] = {{0u, 0u}, {0u, 0u}};  // of the tile in hand, read while its keys are multiplied
+    auto any_of = [&](int which) { return __builtin_amdgcn_readfirstlane((int)(some_left[which].x | some_left[which].y)) != 0; };
+    floatx16 x[KB];
+    Vec8 p[2 * KB];
+    // S^T = K Q^T, with operands two steps ahead: LDS answers after as long as four products take
+    auto key_products = [&](int t) {
+        const char *kt = tile_at(0, t);
+        if constexpr (kHalves) {
+#pragma unroll
+            for (int which = 0; which < 2; ++which) some_left[which] = *(const uint2v *)(any_left + place_of(which, t) * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < KB; ++i) x[i] = zero16();
+        constexpr int kAhead = sizeof(U) == 2 ? 2 : 0;
+        Vec8 kx[kAhead + 1][KB];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int k = 0; k < KB; ++k) kx[i][k] = Keys::row_operand(kt, 32 * k, i, lane);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
+                if (i + kAhead < DP / 16) kx[(i + kAhead) % (kAhead + 1)][k] = Keys::row_operand(kt, 32 * k, i + kAhead, lane);
+#pragma unroll
+            for (int k = 0; k < KB; ++k) x[k] = Elem<U>::mma(kx[i % (kAhead + 1)][k], qf[i], x[k]);
+            if constexpr (kAhead > 0) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // scores to probabilities, with the maximum raised where it has to be
+    auto weights = [&](int t) {
+        const int key = key0 + t * KT;
+        if constexpr (kHalves) {
+            if (any_of(0)) {
+                const float *by = left + place_of(0, t) * KT;
+#pragma unroll
+                for (int k = 0; k < KB; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const floatx4 f = *(const floatx4 *)(by + 32 * k + 8 * i + 4 * h);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[k][4 * i + j] *= f[j];
+                    }
+            }
+        }
+        if constexpr (MOD) {
+            if constexpr (!__is_same(T, U)) {
+#pragma unroll
+                for (int k = 0; k < KB; ++k) x[k] *= by_row;
+            }
+            if (bend.cap > 0.f) {
+                bend.template apply<KB, false>(x, x);
+            } else {
+#pragma unroll
+                for (int k = 0; k < KB; ++k)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[k][r] *= scale * kLog2e;
+            }
+            if (a.slopes) {
+                const float at = (float)(pos - key - 4 * h);
+#pragma unroll
+                for (int k = 0; k < KB; ++k)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[k][r] = fmaf(-slope, fabsf(at - (float)(32 * k + 8 * (r >> 2) + (r & 3))), x[k][r]);
+            }
+        }
+        if (key < full_lo || key + KT > full_hi) {
+            const int at = key + 4 * h - lo;
+            const uint32_t span = there && hi > lo ? hi - lo : 0;
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[k][r] = (uint32_t)(at + 32 * k + 8 * (r >> 2) + (r & 3)) < span ? x[k][r] : -INFINITY;
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, x[k][r]);
+        top = halves_max(top);
+        if (__any(top > m + raise)) {
+            const float raised = fmaxf(m, top), by = raised == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - raised) * unit);
+            m = raised;
+            sum *= by;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= by;
+        }
+        const float base = (m == -INFINITY ? 0.f : m * unit) - kShift;
+        float sum_odd = 0.f;
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                x[k][r] = __builtin_amdgcn_exp2f(fmaf(x[k][r], unit, -base));
+                (r & 1 ? sum_odd : sum) += x[k][r];
+            }
+        sum += sum_odd;
+        if constexpr (kHalves) {
+            // factors of values, in units of the largest so far
+            const bool some = any_of(1);
+            const float *by = left + place_of(1, t) * KT;
+            float most = 1.f;
+            if (some) {
+                most = fmaxf(by[n], by[n + 32 < KT ? n + 32 : n]);
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+            }
+            if (most > norm) {
+                const float to = norm / most;
+                norm = most;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] *= to;
+            }
+            if (some || norm != 1.f) {
+                const float in = 1.f / norm;
+#pragma unroll
+                for (int k = 0; k < KB; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const floatx4 f = *(const floatx4 *)(by + 32 * k + 8 * i + 4 * h) * in;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[k][4 * i + j] *= f[j];
+                    }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i) p[i] = operand<U>(x[i / 2], i & 1);
+    };
+    // O^T += V^T P^T, the next step's operands being under way
+    auto value_products = [&](int t) {
+        const char *vt = tile_at(1, t);
+        constexpr int kSet = sizeof(U) == 2 ? 2 : 1;
+        Vec8 vx[kSet][DB];
+        if constexpr (kSet == 2) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) vx[0][d] = Keys::column_operand(vt, d, 0, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                if (kSet == 1) vx[0][d] = Keys::column_operand(vt, d, i, lane);
+                else if (i + 1 < 2 * KB) vx[(i + 1) & 1][d] = Keys::column_operand(vt, d, i + 1, lane);
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] = Elem<U>::mma(vx[kSet == 2 ? i & 1 : 0][d], p[i], o[d]);
+        }
+    };
+    auto seen = [&](int t) { return key0 + t * KT + KT > wave_lo && key0 + t * KT < wave_hi; };
     if (first < last) {
         request(first);
         place_codes(first);
@@ -254,122 +420,11 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
     for (int t = first; t < last; ++t) {
         tiles_arrived();
         if (t + 1 < last) request(t + 1);
-        const int key = key0 + t * KT;
-        if (key + KT > wave_lo && key < wave_hi) {
-            const char *kt = lds[t & 1][0], *vt = lds[t & 1][1];
-            floatx16 x[KB];
-#pragma unroll
-            for (int i = 0; i < KB; ++i) x[i] = zero16();
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-                for (int k = 0; k < KB; ++k) x[k] = Elem<U>::mma(Keys::row_operand(kt, 32 * k, i, lane), qf[i], x[k]);
+        if (seen(t)) {
+            key_products(t);
             __builtin_amdgcn_s_setprio(1);
-            if constexpr (kHalves) {
-                int some = 0;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) some |= any_left[(t & 1) * 2 * NW + w];
-                if (__builtin_amdgcn_readfirstlane(some)) {
-                    const float *by = left + (t & 1) * 2 * KT;
-#pragma unroll
-                    for (int k = 0; k < KB; ++k)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const floatx4 f = *(const floatx4 *)(by + 32 * k + 8 * i + 4 * h);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) x[k][4 * i + j] *= f[j];
-                        }
-                }
-            }
-            if constexpr (MOD) {
-                if constexpr (!__is_same(T, U)) {
-#pragma unroll
-                    for (int k = 0; k < KB; ++k) x[k] *= by_row;
-                }
-                if (bend.cap > 0.f) {
-                    bend.template apply<KB, false>(x, x);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < KB; ++k)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) x[k][r] *= scale * kLog2e;
-                }
-                if (a.slopes) {
-                    const float at = (float)(pos - key - 4 * h);
-#pragma unroll
-                    for (int k = 0; k < KB; ++k)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) x[k][r] = fmaf(-slope, fabsf(at - (float)(32 * k + 8 * (r >> 2) + (r & 3))), x[k][r]);
-                }
-            }
-            if (key < full_lo || key + KT > full_hi) {
-                const int at = key + 4 * h - lo;
-                const uint32_t span = there && hi > lo ? hi - lo : 0;
-#pragma unroll
-                for (int k = 0; k < KB; ++k)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[k][r] = (uint32_t)(at + 32 * k + 8 * (r >> 2) + (r & 3)) < span ? x[k][r] : -INFINITY;
-            }
-            float top = x[0][0];
-#pragma unroll
-            for (int k = 0; k < KB; ++k)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, x[k][r]);
-            top = halves_max(top);
-            if (__any(top > m + raise || (m == -INFINITY && top > m))) {
-                const float raised = fmaxf(m, top), by = raised == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - raised) * unit);
-                m = raised;
-                sum *= by;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] *= by;
-            }
-            const float base = (m == -INFINITY ? 0.f : m * unit) - kShift;
-#pragma unroll
-            for (int k = 0; k < KB; ++k)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    x[k][r] = __builtin_amdgcn_exp2f(fmaf(x[k][r], unit, -base));
-                    sum += x[k][r];
-                }
-            if constexpr (kHalves) {
-                // factors of values, in units of the largest so far
-                int some = 0;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) some |= any_left[((t & 1) * 2 + 1) * NW + w];
-                some = __builtin_amdgcn_readfirstlane(some);
-                const float *by = left + ((t & 1) * 2 + 1) * KT;
-                float most = 1.f;
-                if (some) {
-                    most = fmaxf(by[n], by[n + 32 < KT ? n + 32 : n]);
-#pragma unroll
-                    for (int d = 1; d < 32; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-                }
-                if (most > norm) {
-                    const float to = norm / most;
-                    norm = most;
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) o[d] *= to;
-                }
-                if (some || norm != 1.f) {
-                    const float in = 1.f / norm;
-#pragma unroll
-                    for (int k = 0; k < KB; ++k)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const floatx4 f = *(const floatx4 *)(by + 32 * k + 8 * i + 4 * h) * in;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) x[k][4 * i + j] *= f[j];
-                        }
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < KB; ++k)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const Vec8 p = operand<U>(x[k], i);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) o[d] = Elem<U>::mma(Keys::column_operand(vt, d, 2 * k + i, lane), p, o[d]);
-                }
+            weights(t);
+            value_products(t);
             __builtin_amdgcn_s_setprio(0);
         }
         if (t + 1 < last) place_codes(t + 1);

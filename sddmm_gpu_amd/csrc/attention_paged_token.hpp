@@ -105,11 +105,10 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_off[i] = kValueBytes * n < row_bytes ? (uint32_t)((4 * g + i) * (int)c.v_row) + kValueBytes * n : 0x7ffffff0u;
-    const char *k_base = c.k + kv * c.k_head, *v_base = c.v + kv * c.v_head;
     int page0 = 0, page1 = 0;  // of the halves of the tile whose keys, and then values, are requested (no array: indexed by a lane's number it would be one in memory)
     uint32_t k_raw[2][kKeyWords], v_raw[8][kValueWords];
-    auto range = [&](const char *base, int at, int64_t row, int key, int t) {
-        const uint64_t begin = (uint64_t)(base + at * row);
+    auto range = [&](const char *base, uint32_t row, int key, int t) {
+        const uint64_t begin = (uint64_t)base;
         const int rows = t < last ? min(any_hi - key, 16) : 0;
         const uint32_t lo32 = __builtin_amdgcn_readfirstlane((int)(uint32_t)begin), hi32 = __builtin_amdgcn_readfirstlane((int)(uint32_t)(begin >> 32));
         return __builtin_amdgcn_make_buffer_rsrc((void *)((uint64_t)hi32 << 32 | lo32), 0, __builtin_amdgcn_readfirstlane(rows > 0 ? (rows - 1) * (int)row + row_bytes : 0), 0x00020000);
@@ -124,7 +123,7 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int key = key0 + t * KT + 16 * u;
-            const auto src = range(k_base + (u ? page1 : page0) * c.k_page, key & in_page, c.k_row, key, t);
+            const auto src = range(c.k_at(u ? page1 : page0, kv, key & in_page), c.k_row, key, t);
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
                 constexpr int W = kPiece / 4;
@@ -151,7 +150,7 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int key = key0 + t * KT + 16 * u;
-            const auto src = range(v_base + (u ? page1 : page0) * c.v_page, key & in_page, c.v_row, key, t);
+            const auto src = range(c.v_at(u ? page1 : page0, kv, key & in_page), c.v_row, key, t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 uint32_t (&to)[kValueWords] = v_raw[4 * u + i];

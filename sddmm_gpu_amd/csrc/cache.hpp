@@ -14,8 +14,13 @@ struct CacheArgs {
     char *k, *v;
     float *k_scale, *v_scale;
     const int32_t *table;
-    int64_t k_page, k_row, k_head, v_page, v_row, v_head, table_row;
+    int64_t k_head, v_head, table_row;
+    uint32_t k_page, k_row, v_page, v_row;
     int32_t n_pages, page_shift, block_shift, n_kv_heads;
+
+    // row `at` of a page of one head (a page's rows lie within 2^32 bytes)
+    __device__ __forceinline__ char *k_at(int page, int kv, int at) const { return k + kv * k_head + ((uint64_t)(uint32_t)page * k_page + (uint32_t)at * k_row); }
+    __device__ __forceinline__ char *v_at(int page, int kv, int at) const { return v + kv * v_head + ((uint64_t)(uint32_t)page * v_page + (uint32_t)at * v_row); }
 
     // the entry at `i` of sequence s, held to the pages that exist
     __device__ __forceinline__ int page(int s, int i) const { return min(max(table[s * table_row + i], 0), n_pages - 1); }
@@ -46,7 +51,9 @@ inline int check_cache(const char *who, const sddmm_attention_desc &d, const sdd
     for (int64_t row : {c.k_row, c.v_row})
         if (row < d.head_dim || row >= ((int64_t)1 << 23) / e || row % piece) return fail(SDDMM_ERR_ARG, "%s: rows of the cache must be multiples of 16 bytes apart, from head_dim to 2^23 bytes", who);
     for (int64_t s : {c.k_page, c.v_page, c.k_head, c.v_head})
-        if (s < 0 || s % piece) return fail(SDDMM_ERR_ARG, "%s: strides of pages and heads must be multiples of 16 bytes", who);
+        if (s < 0 || s > ((int64_t)1 << 40) || s % piece) return fail(SDDMM_ERR_ARG, "%s: strides of pages and heads must be multiples of 16 bytes", who);
+    for (int64_t bytes : {c.k_page * e, c.v_page * e, c.k_row * e * c.page_len, c.v_row * e * c.page_len})
+        if (bytes > UINT32_MAX) return fail(SDDMM_ERR_RANGE, "%s: pages 2^32 bytes apart, or rows of a page", who);
     if (c.table_row < div_up(d.max_k, c.page_len)) return fail(SDDMM_ERR_ARG, "%s: table_row = %lld is less than the pages of max_k tokens", who, (long long)c.table_row);
     if (!aligned({c.k, c.v})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (((uintptr_t)c.k_scale | (uintptr_t)c.v_scale | (uintptr_t)c.table) & 3u) return fail(SDDMM_ERR_ARG, "%s: arrays of the description must be aligned to their elements", who);
@@ -59,7 +66,7 @@ inline CacheArgs cache_arguments(const sddmm_attention_desc &d, const sddmm_cach
     const int64_t e = c.type == d.type ? element(d.type) : 1;
     CacheArgs a{};
     a.k = (char *)c.k, a.v = (char *)c.v, a.k_scale = c.k_scale, a.v_scale = c.v_scale, a.table = c.table;
-    a.k_page = c.k_page * e, a.k_row = c.k_row * e, a.k_head = c.k_head * e, a.v_page = c.v_page * e, a.v_row = c.v_row * e, a.v_head = c.v_head * e;
+    a.k_page = (uint32_t)(c.k_page * e), a.k_row = (uint32_t)(c.k_row * e), a.k_head = c.k_head * e, a.v_page = (uint32_t)(c.v_page * e), a.v_row = (uint32_t)(c.v_row * e), a.v_head = c.v_head * e;
     a.table_row = c.table_row;
     a.n_pages = (int32_t)c.n_pages, a.page_shift = log2_of(c.page_len), a.block_shift = c.type == d.type ? 0 : log2_of(c.block_len), a.n_kv_heads = d.n_kv_heads;
     return a;

@@ -217,7 +217,7 @@ void sddmm_cache_append_kernel(const AppendArgs p)
         // (units of a block's earlier tokens too, where blocks are longer than units)
         const bool some = u < n_units && first >= 0 && first < hi && (first + kUnit > lo || 1 << c.block_shift > kUnit) && c.n_pages > 0;
         const int page = some ? c.page(s, first >> c.page_shift) : 0, in_page = first & ((1 << c.page_shift) - 1);
-        char *cache = is_v ? c.v + page * c.v_page + kv * c.v_head + in_page * c.v_row : c.k + page * c.k_page + kv * c.k_head + in_page * c.k_row;
+        char *cache = is_v ? c.v_at(page, kv, in_page) : c.k_at(page, kv, in_page);
         const int64_t cache_row = is_v ? c.v_row : c.k_row;
         const T *rows = is_v ? (const T *)a.v + (a.q_ptr ? e.q0 * a.v_row : s * a.v_seq) + kv * a.v_head : (const T *)a.k + (a.q_ptr ? e.q0 * a.k_row : s * a.k_seq) + kv * a.k_head;
         const int64_t row = is_v ? a.v_row : a.k_row;
