@@ -2,6 +2,7 @@
 // block of tokens and head; and their queries turned on the way.
 #include <hip/hip_runtime.h>
 #include <cstring>
+#include <type_traits>
 #include "cache.hpp"
 #include "internal.hpp"
 #include "launch.hpp"
@@ -17,7 +18,7 @@ struct AppendArgs {
     AttnArgs a;      // q, k, v: the new rows; out: the turned queries
     CacheArgs c;
     const double *freq;
-    int32_t rot_dim, half, chunk_shift, max_chunks, n_slots, heads_per, head_groups, fast;
+    int32_t rot_dim, half, chunk_shift, max_chunks, n_slots, heads_per, head_groups, fast, table;  // table: entries of a chunk's angles
     float amplitude;
 };
 
@@ -55,13 +56,7 @@ __device__ __forceinline__ int find_sequence(const AppendArgs &p, int slot, int 
     return chunk < 0 ? -1 : lo;
 }
 
-template <class T> __device__ __forceinline__ void load8(const T *p, float (&x)[8])
-{
-    typedef T Vec __attribute__((ext_vector_type(8)));
-    const Vec v = *(const Vec *)p;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)v[j];
-}
+template <class T> struct Piece { typedef T Vec __attribute__((ext_vector_type(8))); };
 template <class T> __device__ __forceinline__ void store8(T *p, const float (&x)[8])
 {
     typedef T Vec __attribute__((ext_vector_type(8)));
@@ -101,6 +96,38 @@ template <int HELD> __device__ __forceinline__ uint2 codes_of(const float (&x)[8
     }
     return make_uint2(r[0], r[1]);
 }
+// The same for finite values within the range and a scale whose reciprocal is exact: the integer is the last byte of 1.5 * 2^23 and it.
+template <int HELD> __device__ __forceinline__ uint2 codes_of_scaled(const float (&x)[8], float by)
+{
+    uint32_t r[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        if constexpr (HELD == kHeldI8) {
+            uint32_t y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = __float_as_uint(fmaf(x[4 * w + j], by, 12582912.f));
+            r[w] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0400u), __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400u), 0x05040100u);
+        } else {
+            const int low = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w] * by, x[4 * w + 1] * by, 0, false);
+            r[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2] * by, x[4 * w + 3] * by, low, true);
+        }
+    }
+    return make_uint2(r[0], r[1]);
+}
+
+// The maximum over 2^`levels` lanes in a row: 0 to 6.
+__device__ __forceinline__ float lanes_max(float x, int levels)
+{
+    auto dpp = [](float y, auto ctrl) { return fmaxf(y, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(y), (int)__float_as_uint(y), decltype(ctrl)::value, 0xf, 0xf, false))); };
+    if (levels > 0) x = dpp(x, std::integral_constant<int, 0xB1>());   // lanes 1 apart,
+    if (levels > 1) x = dpp(x, std::integral_constant<int, 0x4E>());   // 2 apart,
+    if (levels > 2) x = dpp(x, std::integral_constant<int, 0x141>());  // eight turned round (fours are alike by now),
+    if (levels > 3) x = dpp(x, std::integral_constant<int, 0x140>());  // sixteen turned round
+    if (levels > 4) x = fmaxf(x, __shfl_xor(x, 16));
+    if (levels > 5) x = halves_max(x);
+    return x;
+}
+
 template <int HELD> __device__ __forceinline__ void values_of(uint2 codes, float (&x)[8])
 {
     const uint32_t r[2] = {codes.x, codes.y};
@@ -132,12 +159,15 @@ __device__ __forceinline__ float least_scale(float top, float most)
 // Turned in 64 bits: a code is a rounding to few bits, whose borders products in 32 bits would cross for one element in 10^5, so that codes depended on the way
 // of computing.
 template <class T, int HELD, int LPR>
-__global__ __launch_bounds__(kBlock)
+__global__ __launch_bounds__(kBlock, sizeof(T) == 4 ? 2 : 3)
 void sddmm_cache_append_kernel(const AppendArgs p)
 {
     constexpr int kRows = 64 / LPR, kPasses = kUnit / kRows;  // of a wave at a time, of a unit
     constexpr float kMost = HELD == kHeldI8 ? 127.f : 448.f;
+    // Cosines and sines in 64 bits for what becomes codes or fp32, in 32 bits for what becomes 16.
+    constexpr bool kCoarse = sizeof(T) == 2, kKeysCoarse = kCoarse && HELD == kHeldOwn;
     extern __shared__ double2 angles[];
+    float2 *const coarse = (float2 *)(angles + (kKeysCoarse ? 0 : p.table));
     __shared__ float tops[4];
     const AttnArgs &a = p.a;
     const CacheArgs &c = p.c;
@@ -155,33 +185,60 @@ void sddmm_cache_append_kernel(const AppendArgs p)
     const int64_t first_of = ((int64_t)(start >> p.chunk_shift) + chunk) << p.chunk_shift;
     if (first_of >= e.nk) return;
     const int p0 = (int)first_of, lo = max(p0, start), hi = min(p0 + (1 << p.chunk_shift), e.nk), n = hi - lo;
-    const int pairs = p.rot_dim / 2;
-    for (int i = threadIdx.x; i < n * pairs; i += kBlock) {
-        const int r = i / pairs, pair = i - r * pairs;
-        double2 cs = cos_sin((double)(lo + r) * p.freq[pair]);
-        cs.x *= p.amplitude, cs.y *= p.amplitude;
-        angles[i] = cs;
-    }
-    if (pairs) __syncthreads();
-
     // the places of this lane's two pieces in a row (or none): pairs that lie in halves, then the rest two by two
     const int hp = p.half && p.fast ? p.rot_dim / 16 : 0, n_pieces = a.head_dim / 8;
     int at[2];
     at[0] = item < hp ? 8 * item : 8 * (2 * hp + 2 * (item - hp));
     at[1] = item < hp ? 8 * (item + hp) : at[0] + 8;
     const bool there[2] = {at[0] < 8 * n_pieces, at[1] < 8 * n_pieces};
+    typedef typename Piece<T>::Vec Vec;
+    auto fetch = [&](const T *row, Vec (&x)[2]) {  // (a lane without a piece takes the row's first)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[i] = *(const Vec *)(row + (there[i] ? at[i] : 0));
+    };
+
+    // keys and values: units of 16 tokens, those of a block next to each other, a wave's first requested before the angles are made
+    const int units_per = 1 << (p.chunk_shift - 4), n_units = n_heads * 2 * units_per;
+    const T *rows = nullptr;
+    int64_t row = 0;
+    Vec raw[kPasses][2];
+    auto request = [&](int u) {
+        const int part = u % units_per, is_v = (u / units_per) & 1, kv = head0 + u / (2 * units_per), first = p0 + kUnit * part;
+        rows = is_v ? (const T *)a.v + (a.q_ptr ? e.q0 * a.v_row : s * a.v_seq) + kv * a.v_head : (const T *)a.k + (a.q_ptr ? e.q0 * a.k_row : s * a.k_seq) + kv * a.k_head;
+        row = is_v ? a.v_row : a.k_row;
+#pragma unroll
+        for (int t = 0; t < kPasses; ++t) fetch(rows + (min(max(first + t * kRows + mine, lo), hi - 1) - start) * row, raw[t]);
+    };
+    if (wave < n_units) request(wave);
+
+    // (element e of a token's pairs at place (e % 8) * eighths + e / 8: the lanes of a row, which take eight pairs each, read next to each other)
+    const int pairs = p.rot_dim / 2, eighths = (pairs + 7) / 8;
+    for (int i = threadIdx.x; i < n * pairs; i += kBlock) {
+        const int r = i / pairs, pair = i - r * pairs, to = (r * 9 + (pair & 7)) * eighths + (pair >> 3);
+        double2 cs = cos_sin((double)(lo + r) * p.freq[pair]);
+        cs.x *= p.amplitude, cs.y *= p.amplitude;
+        if (!kKeysCoarse) angles[to] = cs;
+        if (kCoarse) coarse[to] = make_float2((float)cs.x, (float)cs.y);
+    }
+    if (pairs) __syncthreads();
+
     // a row's two pieces, turned
-    auto load = [&](const T *row, int token, bool turn, float (&x)[2][8]) {
+    auto turned = [&]<bool COARSE>(std::bool_constant<COARSE>, const Vec (&r)[2], const T *row, int token, bool turn, float (&x)[2][8]) {
+        typedef std::conditional_t<COARSE, float, double> F;
+        typedef std::conditional_t<COARSE, float2, double2> F2;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (there[i]) load8(row + at[i], x[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[i][j] = there[i] ? (float)r[i][j] : 0.f;
         if (!turn || at[0] >= p.rot_dim) return;
-        const double2 *cs = angles + (token - lo) * pairs;
+        const F2 *cs;
+        if constexpr (COARSE) cs = coarse; else cs = angles;
+        cs += (token - lo) * 9 * eighths;
         if (hp) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const double2 w = cs[at[0] + j];
-                const double u = x[0][j], v = x[1][j];
+                const F2 w = cs[j * eighths + item];
+                const F u = x[0][j], v = x[1][j];
                 x[0][j] = (float)(u * w.x - v * w.y), x[1][j] = (float)(u * w.y + v * w.x);
             }
         } else if (!p.half) {
@@ -190,8 +247,8 @@ void sddmm_cache_append_kernel(const AppendArgs p)
 #pragma unroll
                 for (int j = 0; j < 8; j += 2)
                     if (at[i] + j < p.rot_dim) {
-                        const double2 w = cs[(at[i] + j) / 2];
-                        const double u = x[i][j], v = x[i][j + 1];
+                        const F2 w = cs[(4 * i + j / 2) * eighths + item];
+                        const F u = x[i][j], v = x[i][j + 1];
                         x[i][j] = (float)(u * w.x - v * w.y), x[i][j + 1] = (float)(u * w.y + v * w.x);
                     }
         } else {
@@ -203,56 +260,63 @@ void sddmm_cache_append_kernel(const AppendArgs p)
                     const int k = at[i] + j;
                     if (k >= p.rot_dim) continue;
                     const bool first = k < pairs;
-                    const double2 w = cs[first ? k : k - pairs];
-                    const double u = x[i][j], v = (float)row[first ? k + pairs : k - pairs];
+                    const int pair = first ? k : k - pairs;
+                    const F2 w = cs[(pair & 7) * eighths + (pair >> 3)];
+                    const F u = x[i][j], v = (float)row[first ? k + pairs : k - pairs];
                     x[i][j] = (float)(first ? u * w.x - v * w.y : v * w.y + u * w.x);
                 }
         }
     };
 
-    // keys and values: units of 16 tokens, those of a block next to each other
-    const int units_per = 1 << (p.chunk_shift - 4), n_units = n_heads * 2 * units_per;
     for (int u0 = 0; u0 < n_units; u0 += 4) {
         const int u = u0 + wave, part = u % units_per, is_v = (u / units_per) & 1, kv = head0 + u / (2 * units_per), first = p0 + kUnit * part;
         // (units of a block's earlier tokens too, where blocks are longer than units)
         const bool some = u < n_units && first >= 0 && first < hi && (first + kUnit > lo || 1 << c.block_shift > kUnit) && c.n_pages > 0;
         const int page = some ? c.page(s, first >> c.page_shift) : 0, in_page = first & ((1 << c.page_shift) - 1);
         char *cache = is_v ? c.v_at(page, kv, in_page) : c.k_at(page, kv, in_page);
-        const int64_t cache_row = is_v ? c.v_row : c.k_row;
-        const T *rows = is_v ? (const T *)a.v + (a.q_ptr ? e.q0 * a.v_row : s * a.v_seq) + kv * a.v_head : (const T *)a.k + (a.q_ptr ? e.q0 * a.k_row : s * a.k_seq) + kv * a.k_head;
-        const int64_t row = is_v ? a.v_row : a.k_row;
+        const uint32_t cache_row = is_v ? c.v_row : c.k_row;
         float x[kPasses][2][8], top[kPasses];
-        bool fresh[kPasses];
+        bool fresh[kPasses], odd = false;
 #pragma unroll
         for (int t = 0; t < kPasses; ++t) {
             const int pos = first + t * kRows + mine;
             fresh[t] = some && pos >= max(lo, 0) && pos < hi;
             top[t] = 0.f;
             if (!fresh[t]) continue;
-            load(rows + (pos - start) * row, pos, !is_v, x[t]);
+            turned(std::bool_constant<kKeysCoarse>(), raw[t], rows + (pos - start) * row, pos, !is_v, x[t]);
             if constexpr (HELD == kHeldOwn) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (there[i]) store8((T *)(cache + (t * kRows + mine) * cache_row) + at[i], x[t][i]);
+                    if (there[i]) store8((T *)(cache + (uint32_t)(t * kRows + mine) * cache_row) + at[i], x[t][i]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float y = fabsf(x[t][i][j]);
-                        if (there[i] && y < INFINITY) top[t] = fmaxf(top[t], y);
+                        top[t] = fmaxf(top[t], fabsf(x[t][i][j]));
+                        if (sizeof(T) == 4) odd = odd || x[t][i][j] != x[t][i][j];  // (a NaN of 16 bits ends in a byte of 0, as its code does)
                     }
+                odd = odd || top[t] == INFINITY;
             }
         }
+        if (u + 4 < n_units) request(u + 4);
         if constexpr (HELD != kHeldOwn) {
-            const int block = 1 << c.block_shift;
+            const bool plain = !__any(odd);
+            if (!plain) {  // the largest finite element
 #pragma unroll
-            for (int t = 0; t < kPasses; ++t) {
+                for (int t = 0; t < kPasses; ++t) {
+                    top[t] = 0.f;
 #pragma unroll
-                for (int d = 1; d < LPR; d *= 2) top[t] = fmaxf(top[t], __shfl_xor(top[t], d));
-                for (int d = 1; d < min(block, kRows); d *= 2) top[t] = fmaxf(top[t], __shfl_xor(top[t], d * LPR));
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (fresh[t] && fabsf(x[t][i][j]) < INFINITY) top[t] = fmaxf(top[t], fabsf(x[t][i][j]));
+                }
             }
+            const int block = 1 << c.block_shift;
             if (kPasses == 2 && block > kRows) top[0] = top[kPasses - 1] = fmaxf(top[0], top[kPasses - 1]);
+#pragma unroll
+            for (int t = 0; t < kPasses; ++t) top[t] = lanes_max(top[t], (LPR == 8 ? 3 : 2) + min(c.block_shift, LPR == 8 ? 3 : 4));
             if (block > kUnit) {
                 __syncthreads();
                 if (lane == 0) tops[wave] = top[0];
@@ -275,15 +339,19 @@ void sddmm_cache_append_kernel(const AppendArgs p)
                 const float old = begin < start ? scales[c.scale_at(page, kv, in_page + place)] : 0.f;
                 scale[t] = old;
                 if (!(old > 0.f && top[t] <= old * kMost)) scale[t] = least_scale(top[t], kMost);
-                char *to = cache + place * cache_row;
-                if (fresh[t]) {
-                    const float by = 1.f / scale[t];
-                    const bool power = (__float_as_uint(scale[t]) & 0x7fffffu) == 0;  // of two: so is its reciprocal
+                char *to = cache + (uint32_t)place * cache_row;
+                const uint32_t bits = __float_as_uint(scale[t]);
+                if (fresh[t] && plain && (bits & 0x7fffffu) == 0 && bits - 0x00800000u < 0x7e000000u) {
+                    const float by = __uint_as_float(0x7f000000u - bits);  // (a power of two's reciprocal)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (there[i]) *(uint2 *)(to + at[i]) = codes_of_scaled<HELD>(x[t][i], by);
+                } else if (fresh[t]) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (!there[i]) continue;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) x[t][i][j] = power ? x[t][i][j] * by : x[t][i][j] / scale[t];
+                        for (int j = 0; j < 8; ++j) x[t][i][j] /= scale[t];
                         *(uint2 *)(to + at[i]) = codes_of<HELD>(x[t][i]);
                     }
                 } else if (pos < start && scale[t] != old) {
@@ -312,15 +380,35 @@ void sddmm_cache_append_kernel(const AppendArgs p)
     const int heads = n_heads * a.group, all = n * heads;
     const T *from = (const T *)a.q + (a.q_ptr ? e.q0 * a.q_row : s * a.q_seq);
     T *to = (T *)a.out + (a.q_ptr ? e.q0 * a.q_row : s * a.q_seq);
-    for (int i = wave * kRows + mine; i < all; i += 4 * kRows) {
-        const int t = i / heads;
-        const int64_t row = (lo + t - start) * a.q_row + (head0 * a.group + i - t * heads) * a.q_head;
-        float x[2][8];
-        load(from + row, lo + t, true, x);
-        __builtin_amdgcn_wave_barrier();  // (in place: partners are read before anything of the row is written)
+    // (token and head of a lane's row, going on by so many of each; kSets rows of a lane under way)
+    constexpr int kSets = sizeof(T) == 2 ? 4 : 2;
+    const int step_tokens = 4 * kRows / heads, step_heads = 4 * kRows % heads;
+    int i = (3 - wave) * kRows + mine, t = i / heads, head = i - t * heads;
+    while (i - mine < all) {
+        Vec set[kSets][2];
+        int64_t place[kSets];
+        int token[kSets];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (there[k]) store8(to + row + at[k], x[k]);
+        for (int k = 0; k < kSets; ++k) {
+            token[k] = lo + t;
+            place[k] = (lo + min(t, n - 1) - start) * a.q_row + (head0 * a.group + head) * a.q_head;
+            if (i - mine + k * 4 * kRows < all) fetch(from + place[k], set[k]);
+            t += step_tokens, head += step_heads;
+            if (head >= heads) head -= heads, ++t;
+        }
+#pragma unroll
+        for (int k = 0; k < kSets; ++k) {
+            if (i + k * 4 * kRows < all) {
+                float x[2][8];
+                turned(std::bool_constant<kCoarse>(), set[k], from + place[k], token[k], true, x);
+                __builtin_amdgcn_wave_barrier();  // (in place: partners are read before anything of the row is written)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    if (there[j]) store8(to + place[k] + at[j], x[j]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        i += kSets * 4 * kRows;
     }
 }
 
@@ -393,12 +481,16 @@ int sddmm_cache_append(const sddmm_attention_desc *desc, const sddmm_cache_desc 
     const int64_t chunk = (int64_t)1 << p.chunk_shift;
     p.max_chunks = (int32_t)((d.max_q + chunk - 2) / chunk + 1);
     const int64_t slots = d.q_ptr ? new_rows / chunk + 2 * (int64_t)d.n_seq : (int64_t)d.n_seq * p.max_chunks;
-    p.head_groups = (int32_t)std::min<int64_t>(d.n_kv_heads, std::max<int64_t>(1, div_up(2048, slots)));
-    p.heads_per = (int32_t)div_up(d.n_kv_heads, p.head_groups);
+    // Key heads of a workgroup: so few that there are 2048 workgroups, but, where there are 512 all the same, as many as make a row for each of 16 groups of lanes (us with 512, 1024, 2048, 4096
+    // workgroups: 16,384 tokens, 32 heads over 8 of 128 96 / 96 / 84 / 88; 5999 tokens, 12 heads of 64 18 / 22 / 26 / 26).
+    const int64_t lane_rows = d.head_dim <= 64 ? 2 + p.a.group : 4 + 2 * (int64_t)p.a.group;  // groups of rows that a wave takes at a time, of a key head
+    const int64_t many = div_up(d.n_kv_heads, std::min<int64_t>(d.n_kv_heads, div_up(512, slots)));
+    p.heads_per = (int32_t)std::max(div_up(d.n_kv_heads, std::min<int64_t>(d.n_kv_heads, div_up(2048, slots))), std::min(many, div_up(16, lane_rows)));
     p.head_groups = (int32_t)div_up(d.n_kv_heads, p.heads_per);
     p.n_slots = (int32_t)std::min<int64_t>(slots, INT32_MAX);
     if (slots > INT32_MAX || !launchable(slots * p.head_groups, kBlock)) return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
-    const size_t lds = (size_t)chunk * (c.rot_dim / 2) * sizeof(double2);
+    p.table = (int32_t)(chunk * div_up(c.rot_dim / 2, 8) * 9);
+    const size_t lds = p.table * (d.type == SDDMM_TYPE_F32 ? sizeof(double2) : held == kHeldOwn ? sizeof(float2) : sizeof(double2) + sizeof(float2));
     const unsigned grid = (unsigned)(slots * p.head_groups);
     const hipStream_t st = (hipStream_t)stream;
     const hipError_t e = d.type == SDDMM_TYPE_F32 ? launch_typed<float>(p, held, grid, lds, st) : d.type == SDDMM_TYPE_F16 ? launch_typed<_Float16>(p, held, grid, lds, st)

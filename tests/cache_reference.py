@@ -40,6 +40,17 @@ def turned(x, pos, freq, rot, layout, amplitude):
     return y
 
 
+def pair_sizes(x, rot, layout, amplitude):
+    """amplitude * (|x| + |y|) of each turned element's pair, 0 for the others."""
+    y = torch.zeros(x.shape, dtype=torch.float64)
+    if rot:
+        half = rot // 2
+        first = torch.arange(half) * (1 if layout == HALF else 2)
+        second = first + (half if layout == HALF else 1)
+        y[..., first] = y[..., second] = abs(amplitude) * (x[..., first].double().abs() + x[..., second].double().abs())
+    return y
+
+
 def append(cache, rows, n_new, after, table, page, block, held, dtype):
     """Puts rows [n, heads, dim] (fp32; of all sequences one behind the other) into cache = (values or codes [page, token, head, dim] in
     64 bits, scales [page, head, blocks of a page])."""

@@ -115,12 +115,20 @@ def check_append(dtype, held, n_new, after, heads, kv, dim, page, block, rot, la
     cache = pages.desc(t, rot_dim=rot, rot_layout=layout, rot_amplitude=amplitude, rot_freq=d_freq.data_ptr() if rot else 0)
     capi.cache_append(desc, cache, dq.data_ptr() if queries else 0, out.data_ptr() if queries else 0, dk.data_ptr(), dv.data_ptr(), stream())
     torch.cuda.synchronize()
+    # What is turned into 16 bits: cosine and sine are rounded to fp32 (2^-24 of at most 1), and so are a product and the sum of it and the other one: 4 * 2^-24 of the pair's
+    # size at most; then the rounding to the type.  What is turned into fp32 or codes: in 64 bits, rounded to fp32.
+    coarse = 0.0 if dtype == F32 else 4 * 2.0 ** -24
+    sizes = {"q": coarse * cref.pair_sizes(q, rot, layout, amplitude), "k": 0.0, "v": 0.0}
+    if held == "own" and coarse:
+        at_cache = torch.zeros_like(pages.cpu["k"][0])
+        cref.append((at_cache, None), (coarse * cref.pair_sizes(k, rot, layout, amplitude) * 1.01).float(), n_new, after, table, page, block, "own", F32)
+        sizes["k"] = at_cache
     for name in "kv":
         got, scale = pages.read(name)
         want, want_scale = pages.cpu[name]
         if held == "own":
-            # rounded to fp32 and then to the type; angles and products in 64 bits
-            tol = (ref.HALF[dtype] + 2.0 ** -23) * want.abs() + 1e-37 + (2.0 ** -24 if dtype == F16 else 0)
+            # (`want` is rounded to the type itself: another half a step)
+            tol = 2 * (ref.HALF[dtype] + 2.0 ** -23) * want.abs() + 1e-37 + (2.0 ** -24 if dtype == F16 else 0) + sizes[name]
             same = (got == want) | (got.isnan() & want.isnan())
             assert (same | ((got - want).abs() <= tol)).all(), (name, (got - want).abs().max())
         else:
@@ -134,7 +142,7 @@ def check_append(dtype, held, n_new, after, heads, kv, dim, page, block, rot, la
                 for s, n in enumerate(n_new):
                     assert (o[s, n:] == 7.0).all()  # rows behind a sequence's new ones
             o = torch.cat([o[s, :n] for s, n in enumerate(n_new)])
-        tol = (ref.HALF[dtype] + 2.0 ** -23) * want_q.abs() + (2.0 ** -24 if dtype == F16 else 1e-37) + 1e-12 * amplitude * q.double().abs().amax(-1, keepdim=True)
+        tol = (ref.HALF[dtype] + 2.0 ** -23) * want_q.abs() + (2.0 ** -24 if dtype == F16 else 1e-37) + 1e-12 * amplitude * q.double().abs().amax(-1, keepdim=True) + sizes["q"]
         assert ((o.double() - want_q).abs() <= tol).all()
 
 
