@@ -40,6 +40,7 @@ struct AttnArgs {
     int32_t n_split;            // pieces that the keys of a tile of rows are cut into
     int32_t part0, n_part;      // first piece of this launch, pieces in all
     int32_t slope_parts;
+    int32_t few_rows;           // pages, sequences of both kinds: those of so many rows (of a key head) at most are the kernel's for few rows, the others the other's; 0: all
     int32_t chunk;              // backward: rows (of all query heads) that a workgroup of keys walks, more being cut into pieces
     float scale, cap;
 };
@@ -283,7 +284,7 @@ __device__ __forceinline__ Seq sequence(const AttnArgs &a, int s)
     if (a.q_ptr) {
         const int first = min(max(0, a.q_ptr[s]), (int)a.rows);
         r.q0 = r.lse0 = first;
-        r.nq = min(max(0, min(a.q_ptr[s + 1], (int)a.rows) - first), a.max_q);
+        r.nq = min(max(0, min(max(0, a.q_ptr[s + 1]), (int)a.rows) - first), a.max_q);
     } else {
         r.q0 = 0;
         r.lse0 = (int64_t)s * a.max_q;
@@ -292,7 +293,7 @@ __device__ __forceinline__ Seq sequence(const AttnArgs &a, int s)
     if (a.k_ptr) {
         const int first = min(max(0, a.k_ptr[s]), (int)a.key_rows);
         r.k0 = first;
-        r.nk = min(max(0, min(a.k_ptr[s + 1], (int)a.key_rows) - first), a.max_k);
+        r.nk = min(max(0, min(max(0, a.k_ptr[s + 1]), (int)a.key_rows) - first), a.max_k);
     } else {
         r.k0 = 0;
         r.nk = a.k_len ? min(max(0, a.k_len[s]), a.max_k) : a.max_k;

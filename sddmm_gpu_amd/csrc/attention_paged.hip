@@ -16,7 +16,8 @@ struct Deal {
     int tiles = 1;     // of 16 rows to a workgroup of it
     int tile = 128;    // rows of a workgroup of the kernel for many
     int64_t slots = 0, max_tiles = 0, grid = 0, splits = 1, chunk = 1;
-    int64_t part_bytes = 0, bytes = 0;
+    int64_t few_rows = 0, few_grid = 0, few_splits = 0;  // sequences of few rows beside others: rows at most, workgroups and pieces
+    int64_t parts = 1, part_bytes = 0, bytes = 0;
 };
 
 Deal deal(const sddmm_attention_desc &d)
@@ -27,10 +28,12 @@ Deal deal(const sddmm_attention_desc &d)
     if (r.rows == 0) return r;
     r.token = packed <= 64;
     r.tiles = packed <= 16 ? 1 : 2;
+    // Sequences of few rows among those of many, as far as numbers tell: packed ones whose longest is four times the mean.
+    const bool mixed = !r.token && d.type != SDDMM_TYPE_F32 && d.q_ptr && group <= 32 && (double)d.max_q * d.n_seq >= 4. * d.q_rows;
     // Many rows: 256 to a workgroup, which share the codes that it makes operands of, where there are 128 workgroups of them and long heads (us with 256 and 128: 2048 tokens behind
     // 14,336, 16 heads over 2 of 128, 8 bits 317 and 360; 1024 behind 7168, 32 over 8 167 and 177; a prompt of 4096, 32 over 8, 16 bits 147 and 164; 2048, 16 over 4 62 and 62; 128 behind
     // 8064 50 and 39; 16 of 300 tokens, heads of 64 54 and 43).
-    if (!r.token && d.type != SDDMM_TYPE_F32 && d.head_dim > 64 && (d.q_ptr ? r.rows * group / 256 + d.n_seq : div_up(packed, 256) * d.n_seq) * d.n_kv_heads >= 128) r.tile = 256;
+    if (!r.token && !mixed && d.type != SDDMM_TYPE_F32 && d.head_dim > 64 && (d.q_ptr ? r.rows * group / 256 + d.n_seq : div_up(packed, 256) * d.n_seq) * d.n_kv_heads >= 128) r.tile = 256;
     const int64_t few = r.token ? 16 * r.tiles : r.tile;
     r.max_tiles = div_up(packed, few);
     r.slots = r.max_tiles == 1 && r.token ? d.n_seq : d.q_ptr ? r.rows * group / few + d.n_seq : r.max_tiles * d.n_seq;
@@ -50,12 +53,26 @@ Deal deal(const sddmm_attention_desc &d)
         r.chunk = div_up(key_tiles, r.splits);
         r.splits = div_up(key_tiles, r.chunk);
     } else {
-        r.splits = std::max<int64_t>(1, std::min(std::min(div_up(r.tile == 256 ? 256 : 512, workgroups), div_up(key_tiles, 8)), (int64_t)256));
+        // As many pieces as fill the card (rows of packed sequences counted without the slots that few of them leave empty where most sequences have few rows: three pieces of prompts beside
+        // 29 tokens, 1053 rows of 32 heads over 8, up to 4096 keys, in whole and in 2, 3 and 4 pieces 153, 111, 126 and 132 us).
+        const int64_t filled = mixed ? std::max<int64_t>(1, r.rows * group / r.tile * d.n_kv_heads) : workgroups;
+        r.splits = std::max<int64_t>(1, std::min(std::min(div_up(r.tile == 256 ? 256 : 512, filled), div_up(key_tiles, 8)), (int64_t)256));
     }
     r.grid = workgroups * r.splits;
-    if (r.splits > 1) {
-        r.part_bytes = padded(r.splits * r.rows * d.n_heads * d.head_dim * (int64_t)sizeof(float));
-        r.bytes = r.part_bytes + padded(r.splits * r.rows * d.n_heads * (int64_t)sizeof(float2));
+    r.parts = r.splits;
+    if (mixed) {
+        r.few_rows = group <= 16 ? 16 : 32;
+        const int64_t caches = (int64_t)d.n_seq * d.n_kv_heads;
+        // (beside the others: a workgroup for each compute unit, pieces of up to 4096 keys; 512 and 1024 workgroups 113 and 120 us where 256 take 111)
+        r.few_splits = std::max<int64_t>(1, std::min(std::min(std::max(div_up(256, caches), div_up(key_tiles, 128)), div_up(key_tiles, 4)), (int64_t)256));
+        r.chunk = div_up(key_tiles, r.few_splits);
+        r.few_splits = div_up(key_tiles, r.chunk);
+        r.few_grid = caches * r.few_splits;
+        r.parts = std::max(r.parts, r.few_splits);
+    }
+    if (r.parts > 1) {
+        r.part_bytes = padded(r.parts * r.rows * d.n_heads * d.head_dim * (int64_t)sizeof(float));
+        r.bytes = r.part_bytes + padded(r.parts * r.rows * d.n_heads * (int64_t)sizeof(float2));
     }
     return r;
 }
@@ -94,7 +111,7 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
     if (!aligned({d_q, d_out})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (!launchable(r.grid, 512) || r.slots > 65535 * 256 || (r.splits > 1 && !launchable(attention_paged_join_grid(r.rows * d.n_heads, (int)r.splits, d.head_dim), 512)))
+    if (!launchable(r.grid + r.few_grid, 512) || r.slots > 65535 * 256 || (r.parts > 1 && !launchable(attention_paged_join_grid(r.rows * d.n_heads, (int)r.parts, d.head_dim), 512)))
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
     if (in_place_of({d_out, d_lse}, {d_q, cache->k, cache->v, cache->k_scale, cache->v_scale}) || (const void *)d_lse == d_out)
         return fail(SDDMM_ERR_ARG, "%s: a result is in an operand's or the other result's place", who);
@@ -102,12 +119,20 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
     AttnArgs a = arguments(d);
     a.q = d_q, a.out = d_out, a.lse = d_lse;
     a.part_o = (float *)d_workspace, a.part_ml = (float2 *)((char *)d_workspace + r.part_bytes);
-    a.n_slots = (int)r.slots, a.max_tiles = (int)r.max_tiles, a.n_split = (int)r.splits, a.n_part = (int)r.splits, a.chunk = (int)r.chunk;
+    a.n_slots = (int)r.slots, a.max_tiles = (int)r.max_tiles, a.n_split = (int)r.splits, a.n_part = (int)r.parts, a.chunk = (int)r.chunk;
+    a.few_rows = (int)r.few_rows;
     const CacheArgs c = cache_arguments(d, *cache);
     const hipStream_t st = (hipStream_t)stream;
     const int held = held_as(d, *cache);
-    hipError_t e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, st) : launch_attention_paged_forward(a, c, d.type, held, r.tile, (unsigned)r.grid, st);
-    if (e == hipSuccess && r.splits > 1) e = launch_attention_paged_join(a, d.type, st);
+    hipError_t e;
+    if (r.few_grid > 0) {
+        AttnArgs few = a;
+        few.n_slots = d.n_seq, few.max_tiles = 1, few.n_split = (int)r.few_splits;
+        e = launch_attention_paged_mixed(a, few, c, d.type, held, (unsigned)r.grid, (unsigned)r.few_grid, st);
+    } else {
+        e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, st) : launch_attention_paged_forward(a, c, d.type, held, r.tile, (unsigned)r.grid, st);
+    }
+    if (e == hipSuccess && r.parts > 1) e = launch_attention_paged_join(a, d.type, st);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;
 }

@@ -5,6 +5,41 @@ namespace sddmm {
 
 namespace {
 
+template <class T, int HELD, int DP, bool MOD, int R, int NW>
+__global__ __launch_bounds__(64 * NW, 2)
+void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
+{
+    typedef PagedToken<T, HELD, DP, MOD, R, NW> Body;
+    __shared__ __align__(16) char lds[Body::kLds];
+    Body::run(a, c, blockIdx.x, blockIdx.y, blockIdx.z, lds);
+}
+
+template <class T, int HELD, int DP, int R, int NW>
+hipError_t launch_dim(const AttnArgs &a, const CacheArgs &c, dim3 grid, hipStream_t st)
+{
+    const bool mod = a.cap > 0.f || a.slopes;
+    return launch(mod ? sddmm_attention_paged_token_kernel<T, HELD, DP, true, R, NW> : sddmm_attention_paged_token_kernel<T, HELD, DP, false, R, NW>, grid, dim3(64 * NW), 0, st, a, c);
+}
+template <class T, int HELD, int R, int NW>
+hipError_t launch_held(const AttnArgs &a, const CacheArgs &c, dim3 grid, hipStream_t st)
+{
+    if constexpr (sizeof(T) == 4) {
+        if (a.head_dim <= 32) return launch_dim<T, HELD, 32, R, NW>(a, c, grid, st);
+    }
+    return a.head_dim <= 64 ? launch_dim<T, HELD, 64, R, NW>(a, c, grid, st) : launch_dim<T, HELD, 128, R, NW>(a, c, grid, st);
+}
+template <class T, int R, int NW>
+hipError_t launch_typed(const AttnArgs &a, const CacheArgs &c, int held, dim3 grid, hipStream_t st)
+{
+    return held == kHeldI8 ? launch_held<T, kHeldI8, R, NW>(a, c, grid, st) : held == kHeldE4m3 ? launch_held<T, kHeldE4m3, R, NW>(a, c, grid, st) : launch_held<T, kHeldOwn, R, NW>(a, c, grid, st);
+}
+template <int R, int NW>
+hipError_t launch_rows(const AttnArgs &a, const CacheArgs &c, int type, int held, dim3 grid, hipStream_t st)
+{
+    return type == SDDMM_TYPE_F32 ? launch_typed<float, R, NW>(a, c, held, grid, st) : type == SDDMM_TYPE_F16 ? launch_typed<_Float16, R, NW>(a, c, held, grid, st)
+                                                                                                             : launch_typed<__bf16, R, NW>(a, c, held, grid, st);
+}
+
 // The parts of a row: sums and totals in units of 2^(largest maximum).  Groups of DP / 4 lanes take parts in turn, eight at a time with maxima and sums under way together, each
 // with a running maximum of its own, and meet in LDS.
 constexpr int kJoinThreads = 512;
@@ -29,6 +64,7 @@ void sddmm_attention_paged_join_kernel(const AttnArgs a, const int per_row)
         there = !a.q_len || i < min(a.q_len[s], a.max_q);
         to_row = s * a.o_seq + i * a.o_row;
     }
+    if (there && a.few_rows && a.part_ml[at].y == kDone) there = false;  // (the kernel for many rows has written its result)
     float top = -INFINITY, total = 0.f;
     floatx4 y = {0.f, 0.f, 0.f, 0.f};
     for (int p0 = mine; there && p0 < a.n_part; p0 += 8 * per_row) {

@@ -6,8 +6,6 @@
 
 namespace sddmm {
 
-namespace {
-
 // The (token, head) pairs that share a key head are the rows, R tiles of 16: they read every key once.  Every wave of a workgroup takes keys of its own,
 // each NW-th tile of 32, from memory to registers without LDS or a barrier: S^T = K Q^T with the keys' rows as they lie -- a lane takes pieces of its token's row, in
 // the order that memory has, and q's elements are in that order too -- and O^T += V^T P^T, the probabilities as they lie, a lane taking DP / 16
@@ -16,8 +14,13 @@ namespace {
 // The next keys are requested when the scores are done, the next values when the products are; waves have statistics and sums of their own, which
 // are joined at the end.
 template <class T, int HELD, int DP, bool MOD, int R, int NW>
-__global__ __launch_bounds__(64 * NW, 2)
-void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
+struct PagedToken {
+    static constexpr int kLds = NW * 16 * (DP + 4) * 4 + NW * 16 * 8;
+    static __device__ __forceinline__ void run(const AttnArgs &a, const CacheArgs &c, int kv, int split, int b, char (&memory)[kLds]);
+};
+
+template <class T, int HELD, int DP, bool MOD, int R, int NW>
+__device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const AttnArgs &a, const CacheArgs &c, int kv, int split, int b, char (&memory)[kLds])
 {
     typedef typename Elem<T>::Vec8 Vec8;
     constexpr int KT = 32, S = DP / 32, E = DP / 16;           // keys of a tile, steps of a product over a head's elements, values' elements of a lane
@@ -27,11 +30,10 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
     constexpr int kValueBytes = E * kSize, kValueWords = (kValueBytes + 3) / 4;
     constexpr bool kNorm = __is_same(T, _Float16) && HELD != kHeldOwn;
     constexpr int kRows = 16 * R;
-    __shared__ __align__(16) float joined[NW][16][DP + 4];
-    __shared__ float2 ml[NW][16];
+    auto &joined = *(float (*)[NW][16][DP + 4])memory;
+    auto &ml = *(float2 (*)[NW][16])(memory + sizeof joined);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
 
-    const int kv = blockIdx.x, split = blockIdx.y, b = blockIdx.z;
     int s, tile;
     if (a.q_ptr && a.max_tiles > 1) {
         s = slot_sequence<false>(a.q_ptr, a.n_seq, a.group, kRows, a.max_tiles, a.n_slots, b, tile);
@@ -54,7 +56,7 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
     }
     const Seq e = sequence(a, s);
     const int n_rows = e.nq * a.group, n_keys = c.n_pages > 0 ? e.nk : 0;
-    if (tile * kRows >= n_rows) return;
+    if (tile * kRows >= n_rows || (a.few_rows && n_rows > a.few_rows)) return;
     const int shift = e.nk - e.nq, prefix = a.prefix ? a.prefix[s] : 0;
     const int t0 = tile * kRows / a.group, t1 = (min(n_rows, tile * kRows + kRows) - 1) / a.group;
     const int any_lo = first_key(a, t0 + shift), any_hi = end_key(a, t1 + shift, prefix, n_keys);
@@ -400,7 +402,13 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
             const int64_t at = (e.lse0 + token) * a.n_heads + head, all = a.rows * a.n_heads;
             if (parts) {
                 if (top != -INFINITY && col < a.head_dim) *(floatx4 *)(a.part_o + (split * all + at) * a.head_dim + col) = z;
-                if (col == 0) a.part_ml[split * all + at] = make_float2(top, total);
+                if (col == 0) {
+                    a.part_ml[split * all + at] = make_float2(top, total);
+                    // (parts that there are of other rows only)
+                    if (split == 0) {
+                        for (int i = a.n_split; i < a.n_part; ++i) a.part_ml[i * all + at] = make_float2(-INFINITY, 0.f);
+                    }
+                }
             } else {
                 z *= total > 0.f || total != total ? 1.f / total : 0.f;
                 T *to = (T *)o_base<T>(a, a.out, e, s, head) + (int64_t)token * a.o_row;
@@ -410,33 +418,5 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
         }
     }
 }
-
-template <class T, int HELD, int DP, int R, int NW>
-hipError_t launch_dim(const AttnArgs &a, const CacheArgs &c, dim3 grid, hipStream_t st)
-{
-    const bool mod = a.cap > 0.f || a.slopes;
-    return launch(mod ? sddmm_attention_paged_token_kernel<T, HELD, DP, true, R, NW> : sddmm_attention_paged_token_kernel<T, HELD, DP, false, R, NW>, grid, dim3(64 * NW), 0, st, a, c);
-}
-template <class T, int HELD, int R, int NW>
-hipError_t launch_held(const AttnArgs &a, const CacheArgs &c, dim3 grid, hipStream_t st)
-{
-    if constexpr (sizeof(T) == 4) {
-        if (a.head_dim <= 32) return launch_dim<T, HELD, 32, R, NW>(a, c, grid, st);
-    }
-    return a.head_dim <= 64 ? launch_dim<T, HELD, 64, R, NW>(a, c, grid, st) : launch_dim<T, HELD, 128, R, NW>(a, c, grid, st);
-}
-template <class T, int R, int NW>
-hipError_t launch_typed(const AttnArgs &a, const CacheArgs &c, int held, dim3 grid, hipStream_t st)
-{
-    return held == kHeldI8 ? launch_held<T, kHeldI8, R, NW>(a, c, grid, st) : held == kHeldE4m3 ? launch_held<T, kHeldE4m3, R, NW>(a, c, grid, st) : launch_held<T, kHeldOwn, R, NW>(a, c, grid, st);
-}
-template <int R, int NW>
-hipError_t launch_rows(const AttnArgs &a, const CacheArgs &c, int type, int held, dim3 grid, hipStream_t st)
-{
-    return type == SDDMM_TYPE_F32 ? launch_typed<float, R, NW>(a, c, held, grid, st) : type == SDDMM_TYPE_F16 ? launch_typed<_Float16, R, NW>(a, c, held, grid, st)
-                                                                                                             : launch_typed<__bf16, R, NW>(a, c, held, grid, st);
-}
-
-}  // namespace
 
 }  // namespace sddmm

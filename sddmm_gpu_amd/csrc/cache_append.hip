@@ -185,6 +185,7 @@ void sddmm_cache_append_kernel(const AppendArgs p)
     const int64_t first_of = ((int64_t)(start >> p.chunk_shift) + chunk) << p.chunk_shift;
     if (first_of >= e.nk) return;
     const int p0 = (int)first_of, lo = max(p0, start), hi = min(p0 + (1 << p.chunk_shift), e.nk), n = hi - lo;
+    if (n <= 0) return;  // (no new rows)
     // the places of this lane's two pieces in a row (or none): pairs that lie in halves, then the rest two by two
     const int hp = p.half && p.fast ? p.rot_dim / 16 : 0, n_pieces = a.head_dim / 8;
     int at[2];

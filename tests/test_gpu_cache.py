@@ -381,3 +381,13 @@ def test_attend_query_ranges(held):
             for h in range(2):
                 r = ref.head(q[:, h], k[:, 0], v[:, 0], -1, 0, 0, min(0.125 / size, 3e38), 0.0, 0.0)
                 assert ((out[:, h].double() - r["out"]).abs() <= r["out_tol"] + lost(BF16, held, 150, v)).all(), (size, n, h)
+
+
+@pytest.mark.parametrize("held", ["i8", "e4m3", "own"])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (20, 1, 128), (40, 1, 64)])
+def test_attend_mixed(dtype, held, heads, kv, dim):
+    """Pieces of prompts beside single tokens, drafts and sequences without new rows."""
+    new = [1, 160, 1, 0, 2, 1, 1, 40, 1, 1, 3, 1, 0, 1]
+    check_attend(dtype, held, new, [700, 300, 1, 50, 90, 33, 1100, 40, 64, 500, 3, 17, 0, 200], heads, kv, dim, 32, 8)
+    check_attend(dtype, held, new, [2000, 1300, 1, 50, 90, 33, 1100, 40, 64, 500, 2, 17, 0, 0], heads, kv, dim, 64, 16, left=300, cap=20.0)
