@@ -111,7 +111,7 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
     if (!aligned({d_q, d_out})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (!launchable(r.grid + r.few_grid, 512) || r.slots > 65535 * 256 || (r.parts > 1 && !launchable(attention_paged_join_grid(r.rows * d.n_heads, (int)r.parts, d.head_dim), 512)))
+    if (!launchable(r.grid + r.few_grid, 512) || (r.parts > 1 && !launchable(attention_paged_join_grid(r.rows * d.n_heads, (int)r.parts, d.head_dim), 512)))
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
     if (in_place_of({d_out, d_lse}, {d_q, cache->k, cache->v, cache->k_scale, cache->v_scale}) || (const void *)d_lse == d_out)
         return fail(SDDMM_ERR_ARG, "%s: a result is in an operand's or the other result's place", who);
@@ -130,7 +130,7 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
         few.n_slots = d.n_seq, few.max_tiles = 1, few.n_split = (int)r.few_splits;
         e = launch_attention_paged_mixed(a, few, c, d.type, held, (unsigned)r.grid, (unsigned)r.few_grid, st);
     } else {
-        e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, st) : launch_attention_paged_forward(a, c, d.type, held, r.tile, (unsigned)r.grid, st);
+        e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, (unsigned)r.grid, st) : launch_attention_paged_forward(a, c, d.type, held, r.tile, (unsigned)r.grid, st);
     }
     if (e == hipSuccess && r.parts > 1) e = launch_attention_paged_join(a, d.type, st);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));

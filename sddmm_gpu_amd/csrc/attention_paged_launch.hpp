@@ -9,7 +9,7 @@ struct AttnArgs;
 struct CacheArgs;
 
 // tiles: of 16 rows to a workgroup, 1 or 2; a.chunk: tiles of 32 keys to a piece
-hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, hipStream_t st);
+hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, unsigned grid, hipStream_t st);
 
 // tile: rows of a workgroup, 128 or 256 (16-bit operands)
 hipError_t launch_attention_paged_forward(const AttnArgs &a, const CacheArgs &c, int type, int held, int tile, unsigned grid, hipStream_t st);

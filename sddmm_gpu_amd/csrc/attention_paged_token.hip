@@ -11,7 +11,8 @@ void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
 {
     typedef PagedToken<T, HELD, DP, MOD, R, NW> Body;
     __shared__ __align__(16) char lds[Body::kLds];
-    Body::run(a, c, blockIdx.x, blockIdx.y, blockIdx.z, lds);
+    const uint32_t b = blockIdx.x / a.n_kv_heads;
+    Body::run(a, c, blockIdx.x - b * a.n_kv_heads, b % a.n_split, b / a.n_split, lds);
 }
 
 template <class T, int HELD, int DP, int R, int NW>
@@ -145,10 +146,9 @@ hipError_t launch_attention_paged_join(const AttnArgs &a, int type, hipStream_t 
     return type == SDDMM_TYPE_F32 ? launch_join<float>(a, st) : type == SDDMM_TYPE_F16 ? launch_join<_Float16>(a, st) : launch_join<__bf16>(a, st);
 }
 
-hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, hipStream_t st)
+hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, unsigned grid, hipStream_t st)
 {
-    const dim3 grid((unsigned)a.n_kv_heads, (unsigned)a.n_split, (unsigned)a.n_slots);
-    return tiles == 1 ? launch_rows<1, 4>(a, c, type, held, grid, st) : launch_rows<2, 4>(a, c, type, held, grid, st);
+    return tiles == 1 ? launch_rows<1, 4>(a, c, type, held, dim3(grid), st) : launch_rows<2, 4>(a, c, type, held, dim3(grid), st);
 }
 
 }  // namespace sddmm

@@ -43,17 +43,10 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
     } else {
         s = b % a.n_seq, tile = a.max_tiles - 1 - b / a.n_seq;
     }
-    // The pages that this piece begins with if its rows see the first keys, and any scales: requested before the lengths are known, since each of them is a chain of
-    // misses by itself (one token behind 1501: 11.8 and 7.9 us).
-    const int table_end = (a.max_k - 1) >> c.page_shift;
-    int pages0 = min((split * a.chunk * KT) >> c.page_shift, table_end);
+    int pages0 = -64;  // the table's entries from here on are in lanes, 64 at a time
     uint32_t pages = 0;
     float scale_raw = 0.f;  // of the key of token `lane`, of the value of token `lane` - 32
     const float *scale_base = lane < 32 ? c.k_scale : c.v_scale;
-    if (c.n_pages > 0 && a.max_k > 0) {
-        pages = c.page(s, min(pages0 + lane, table_end));
-        if constexpr (HELD != kHeldOwn) scale_raw = *scale_base;
-    }
     const Seq e = sequence(a, s);
     const int n_rows = e.nq * a.group, n_keys = c.n_pages > 0 ? e.nk : 0;
     if (tile * kRows >= n_rows || (a.few_rows && n_rows > a.few_rows)) return;
@@ -173,7 +166,6 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
         }
     };
 
-    if constexpr (HELD != kHeldOwn) asm volatile("" ::"v"(scale_raw));
     int t = first + wave;
     if (t < last) {
         request_keys(t);
