@@ -635,18 +635,19 @@ enum { SDDMM_ROTARY_PLAIN = 0, SDDMM_ROTARY_LINEAR = 1, SDDMM_ROTARY_BASE = 2, S
 int sddmm_rotary_frequencies(int32_t rot_dim, double base, int32_t scaling, double factor, int64_t known_len, double low, double high,
                              double *freq, double *amplitude);
 
-/* A cache of keys and values in pages, which sequences take in any order as they grow: no sequence reserves room for its longest
- * length, and sequences that begin alike may share pages.  The tokens page_len * i .. page_len * (i + 1) - 1 of sequence s lie in page
- * table[s * table_row + i]; token t of page p and key head h begins at element p * k_page + (t % page_len) * k_row + h * k_head of k, v likewise.
- * Rows are held in the operands' type, or in 8 bits: codes (SDDMM_TYPE_I8: -127 .. 127; SDDMM_TYPE_E4M3: 4 bits of exponent, 3 of mantissa, the
- * largest 448) that stand for code * scale, with a scale for each block_len tokens of a page and head, in [n_pages][n_kv_heads][page_len / block_len]
- * arrays.  No counterpart in the reference.
+/* A cache of keys and values in pages, which sequences take in any order as they grow: no sequence reserves room for its longest length, and
+ * sequences that begin alike may share pages.  The tokens page_len * i .. page_len * (i + 1) - 1 of sequence s lie in page
+ * table[s * table_row + i]; token t of page p and key head h begins at element p * k_page + (t % page_len) * k_row + h * k_head of k, v
+ * likewise.  Rows are held in the operands' type, or in 8 bits: codes (SDDMM_TYPE_I8: -127 .. 127; SDDMM_TYPE_E4M3: 4 bits of exponent, 3 of mantissa, the largest 448) that
+ * stand for code * scale, with a scale for each block_len tokens of a page and head, in [n_pages][n_kv_heads][page_len / block_len] arrays.  No
+ * counterpart in the reference.
  *
- * Both calls go with a sddmm_attention_desc, which describes the new tokens (type, heads, head_dim, n_seq, max_q, q_ptr or q_len, strides; shared_len
- * 0, no k_ptr) and the lengths: k_len (NULL: max_k for all) counts the new tokens, so that new row i of n_q has the position k_len - n_q + i
- * in either call, and one description serves both.  Strides of pages, rows and heads are multiples of 16 bytes, rows lie in whole pieces of
- * 16 bytes; a row's stride is at least head_dim and below 2^23 bytes, and pages, and the rows of one head in a page, lie within 2^32 bytes.  Entries of the table that a call uses are taken as 0 .. n_pages - 1, lengths as
- * 0 .. max_k: others give wrong results, but nothing outside the arrays is touched.  Calls allocate nothing, launch on `stream` only and may be captured. */
+ * Both calls go with a sddmm_attention_desc, which describes the new tokens (type, heads, head_dim, n_seq, max_q, q_ptr or q_len, strides;
+ * shared_len 0, no k_ptr) and the lengths: k_len (NULL: max_k for all) counts the new tokens, so that new row i of n_q has the position k_len -
+ * n_q + i in either call, and one description serves both.  Strides of pages, rows and heads are multiples of 16 bytes, rows lie in whole pieces
+ * of 16 bytes; a row's stride is at least head_dim and below 2^23 bytes, and pages, and the rows of one head in a page, lie within 2^32 bytes.
+ * Entries of the table that a call uses are taken as 0 .. n_pages - 1, lengths as 0 .. max_k: others give wrong results, but nothing outside the
+ * arrays is touched.  Calls allocate nothing, launch on `stream` only and may be captured. */
 enum { SDDMM_TYPE_I8 = 3, SDDMM_TYPE_E4M3 = 4 };   /* of a cache */
 
 typedef struct sddmm_cache_desc {
@@ -666,19 +667,22 @@ typedef struct sddmm_cache_desc {
 void sddmm_cache_desc_init(sddmm_cache_desc *cache);   /* zeros, block_len 1, rot_amplitude 1 */
 
 /* The new tokens' keys, turned by their positions, and values go into the cache; their queries are turned into d_q_out (laid out as d_q, which it
- * may be), unless d_q is NULL.  d_k and d_v are the new rows, with the description's k_ and v_ strides and the rows' numbering of q (q_ptr, or k_seq for each of max_q).
- * Angles are taken in 64 bits; what becomes fp32 or codes is turned in 64 bits and rounded to fp32, what becomes 16 bits is turned in fp32.  8 bits: a block keeps its scale while the new tokens'
- * largest finite element is at most 127 (448) times that, and gets the least power of two (from 2^-126 on) that is enough otherwise: its earlier tokens' codes are
- * then rounded anew to the larger steps.  A block without earlier tokens begins with that power of two.  Codes are rounded to the nearest, ties to even; infinities
- * become the largest code, NaNs 0 (E4M3: NaN).  What lies behind the new tokens stays as it was; tokens at positions below 0 are not
- * stored.  No two sequences of a call may bring new tokens to one page.  */
+ * may be), unless d_q is NULL.  d_k and d_v are the new rows, with the description's k_ and v_ strides and the rows' numbering of q (q_ptr, or
+ * k_seq for each of max_q).  Angles are taken in 64 bits; what becomes fp32 or codes is turned in 64 bits and rounded to fp32, what becomes 16
+ * bits is turned in fp32.  8 bits: a block keeps its scale while the new tokens' largest finite element is at most 127 (448) times that, and gets
+ * the least power of two (from 2^-126 on) that is enough otherwise: its earlier tokens' codes are then rounded anew to the larger steps.  A block
+ * without earlier tokens begins with that power of two.  Codes are rounded to the nearest, ties to even; infinities become the largest code, NaNs
+ * 0 (E4M3: NaN).  What lies behind the new tokens stays as it was; tokens at positions below 0 are not stored.  New tokens of a call go to pages
+ * that no other sequence of it, and no other part of their own, has (those that are only read may be anyone's). */
 int sddmm_cache_append(const sddmm_attention_desc *desc, const sddmm_cache_desc *cache, const void *d_q, void *d_q_out, const void *d_k,
                        const void *d_v, void *stream);
 
-/* sddmm_attention_forward over the cache: the same masks, bends, biases, rows and results (lse may be NULL; the description's k_ and v_ strides and k_rows are not
- * looked at).  Products with codes are exact and summed in fp32, scales are applied in fp32 to scores and probabilities (or as powers of two, exactly); 16-bit
- * operands: probabilities times scales of values are rounded to the operands' type, or fp16, before they are multiplied, and those below 2^-24 of a row's largest may be lost.  What lies in a sequence's pages behind its end or before its rows' windows does not reach
- * the results, whatever it holds. */
+/* sddmm_attention_forward over the cache: the same masks, bends, biases, rows and results (lse may be NULL; the description's k_ and v_ strides
+ * and k_rows are not looked at).  Products with codes are exact and summed in fp32, scales are applied in fp32 to scores and probabilities (or as
+ * powers of two, exactly); 16-bit operands: probabilities times scales of values are rounded before they are multiplied, to 16 bits or 11 (more
+ * than 64 rows of a key head over a bf16 cache: 8), and those below 2^-24 of a row's largest may be lost.  What lies in a sequence's pages behind
+ * its end or before its rows' windows does not reach the results, whatever it holds; infinities and NaNs in keys that a row does not see do not
+ * reach its out and lse, those in values may reach its out where one of 256 rows beside it sees them. */
 int sddmm_attention_paged_workspace_bytes(const sddmm_attention_desc *desc, const sddmm_cache_desc *cache, int64_t *bytes);
 int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_desc *cache, const void *d_q, void *d_out, float *d_lse,
                           void *d_workspace, int64_t workspace_bytes, void *stream);
