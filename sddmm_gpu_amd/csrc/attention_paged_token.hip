@@ -41,10 +41,10 @@ hipError_t launch_rows(const AttnArgs &a, const CacheArgs &c, int type, int held
                                                                                                              : launch_typed<__bf16, R, NW>(a, c, held, grid, st);
 }
 
-// The parts of a row: sums and totals in units of 2^(largest maximum).  Groups of DP / 4 lanes take parts in turn, eight at a time with maxima and sums under way together, each
+// The parts of a row: sums and totals in units of 2^(largest maximum).  Groups of DP / 4 lanes take parts in turn, N at a time with maxima and sums under way together, each
 // with a running maximum of its own, and meet in LDS.
 constexpr int kJoinThreads = 512;
-template <class T, int DP>
+template <class T, int DP, int N>
 __global__ __launch_bounds__(kJoinThreads)
 void sddmm_attention_paged_join_kernel(const AttnArgs a, const int per_row)
 {
@@ -68,25 +68,25 @@ void sddmm_attention_paged_join_kernel(const AttnArgs a, const int per_row)
     if (there && a.few_rows && a.part_ml[at].y == kDone) there = false;  // (the kernel for many rows has written its result)
     float top = -INFINITY, total = 0.f;
     floatx4 y = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = mine; there && p0 < a.n_part; p0 += 8 * per_row) {
-        float2 ml[8];
-        floatx4 x[8];
+    for (int p0 = mine; there && p0 < a.n_part; p0 += N * per_row) {
+        float2 ml[N];
+        floatx4 x[N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < N; ++i) {
             const int p = min(p0 + i * per_row, a.n_part - 1);
             ml[i] = a.part_ml[p * all + at];
             x[i] = col < a.head_dim ? *(const floatx4 *)(a.part_o + (p * all + at) * a.head_dim + col) : floatx4{0.f, 0.f, 0.f, 0.f};
         }
         float most = top;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < N; ++i) {
             if (p0 + i * per_row >= a.n_part) ml[i] = make_float2(-INFINITY, 0.f);
             most = fmaxf(most, ml[i].x);
         }
         const float by = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - most);
         y *= by, total *= by, top = most;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < N; ++i) {
             if (ml[i].x == -INFINITY) continue;  // (no keys: its sums were not written)
             const float w = __builtin_amdgcn_exp2f(ml[i].x - top);
             y += x[i] * w;
@@ -125,12 +125,20 @@ int join_per_row(int n_part, int head_dim)
     while (per_row < join_groups(head_dim) && per_row * 2 < n_part) per_row *= 2;
     return per_row;
 }
+template <class T, int DP>
+hipError_t launch_join_dim(const AttnArgs &a, hipStream_t st)
+{
+    const int per_row = join_per_row(a.n_part, a.head_dim);
+    const dim3 grid((unsigned)attention_paged_join_grid(a.rows * a.n_heads, a.n_part, a.head_dim)), block(kJoinThreads);
+    // As many at a time as a group has, up to eight (us of the whole call with 2 / 4 / 8: two parts, 2048 rows of 16 heads 309 / - / 312, 1053 of 32 heads 107 / - / 111; 64 parts - / 16.8 / 17.3;
+    // 128 and 256 of one row - / 15.1 and 17.1 / 14.8 and 16.7).
+    auto *fn = a.n_part <= 2 * per_row ? sddmm_attention_paged_join_kernel<T, DP, 2> : a.n_part <= 4 * per_row ? sddmm_attention_paged_join_kernel<T, DP, 4> : sddmm_attention_paged_join_kernel<T, DP, 8>;
+    return launch(fn, grid, block, 0, st, a, per_row);
+}
 template <class T>
 hipError_t launch_join(const AttnArgs &a, hipStream_t st)
 {
-    const dim3 grid((unsigned)attention_paged_join_grid(a.rows * a.n_heads, a.n_part, a.head_dim)), block(kJoinThreads);
-    return a.head_dim <= 64 ? launch(sddmm_attention_paged_join_kernel<T, 64>, grid, block, 0, st, a, join_per_row(a.n_part, a.head_dim))
-                            : launch(sddmm_attention_paged_join_kernel<T, 128>, grid, block, 0, st, a, join_per_row(a.n_part, a.head_dim));
+    return a.head_dim <= 64 ? launch_join_dim<T, 64>(a, st) : launch_join_dim<T, 128>(a, st);
 }
 
 }  // namespace
