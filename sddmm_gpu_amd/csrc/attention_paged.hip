@@ -42,13 +42,15 @@ Deal deal(const sddmm_attention_desc &d)
     const int64_t span = d.window_left >= 0 && d.window_right >= 0 && !d.prefix ? (int64_t)d.window_left + d.window_right + std::min<int64_t>(d.max_q, few) : d.max_k;
     const int64_t key_tiles = std::max<int64_t>(1, std::min<int64_t>(div_up(d.max_k, 32), span / 32 + 2));
     if (r.token) {
-        // Pieces of 128 keys and more, so that there are 512 workgroups, two to a compute unit; where there are as many without pieces, eight times as many, which evens out the
-        // lengths of caches (us with 512 / 1024 / 2048 / 4096: 64 users of up to 8192 keys, 8 key heads of 128 126 / 145 / 129 / 120; 4 of up to 32,768, 2 key heads 18.1 / 19.5 / 23.2 / 23.2;
-        // 16 of a window of 2048, 4 of 64 17.2 / 21.6 / 22.1 / 22.1; pieces of 128 / 256 / 512 keys at least: one user, 1501 keys, 10.5 / 11.2 / 13.1).
+        // Pieces, so that there are 512 workgroups, two to a compute unit; where there are as many without pieces, eight times as many, which evens out the lengths of caches (us with
+        // 512 / 1024 / 4096: 64 users of up to 8192 keys, 8 key heads of 128 126 / 145 / 120; 512 / 1024: 4 of up to 32,768, 2 key heads 16.8 / 18.5; 16 of a window of 2048, 4 of 64
+        // 16.5 / 20.5; 8 of 6000, 8 tokens of 4 heads for each of 4 22 / 33).  Of 256 keys and more, or of 128 while these are so few that the join is short (of 128 and of 256 keys: one
+        // user, 1501 keys, 10.2 / 10.4; 16,384 keys, 8 heads over 2 11.5 / 12.1; 2 users, 4 tokens, 8192 keys 11.9 / 12.6; 32,768 keys 14.8 / 13.1; 16 tokens, 16 heads, 8192 keys 18.6 / 15.9).
         if (workgroups >= 512) {
             r.splits = std::min(div_up(4096, workgroups), div_up(key_tiles, 32));
         } else {
-            r.splits = std::min(std::min(div_up(512, workgroups), div_up(key_tiles, 4)), (int64_t)256);
+            const int64_t fine = std::min(div_up(key_tiles, 4), std::min<int64_t>(128, 8192 / (r.rows * d.n_heads)));
+            r.splits = std::min(std::min(div_up(512, workgroups), std::max(fine, div_up(key_tiles, 8))), (int64_t)256);
         }
         r.chunk = div_up(key_tiles, r.splits);
         r.splits = div_up(key_tiles, r.chunk);
