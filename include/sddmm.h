@@ -679,7 +679,7 @@ int sddmm_cache_append(const sddmm_attention_desc *desc, const sddmm_cache_desc 
 
 /* sddmm_attention_forward over the cache: the same masks, bends, biases, rows and results (lse may be NULL; the description's k_ and v_ strides
  * and k_rows are not looked at).  Products with codes are exact and summed in fp32, scales are applied in fp32 to scores and probabilities (or as
- * powers of two, exactly); 16-bit operands: probabilities times scales of values are rounded before they are multiplied, to 16 bits or 11 (more
+ * powers of two, exactly); 16-bit operands: probabilities times scales of values are rounded before they are multiplied, to 11 bits or more (more
  * than 64 rows of a key head over a bf16 cache: 8), and those below 2^-24 of a row's largest may be lost.  What lies in a sequence's pages behind
  * its end or before its rows' windows does not reach the results, whatever it holds; infinities and NaNs in keys that a row does not see do not
  * reach its out and lse, those in values may reach its out where one of 256 rows beside it sees them. */

@@ -13,6 +13,11 @@ namespace sddmm {
 // within the lane.  Codes are made 16-bit operands in registers (two instructions for two to four of them); scales go to scores and probabilities.
 // The next keys are requested when the scores are done, the next values when the products are; waves have statistics and sums of their own, which
 // are joined at the end.
+//
+// Bound by reading the caches where there are many (64 users of 284 to 8192 keys, 8 key heads of 128, 8 bits: 119 us, 4.6 TB/s; a large copy makes 4.7; vector instructions for 41 % of
+// the time, matrix ones for 9), by chains of loads -- lengths, pages, keys, the next keys -- where there are few (4 users of up to 32,768 keys, 2 key heads: 12.5 us in 512 workgroups of
+// four tiles a wave, compute units busy for 42 %).  Sixteen waves to a workgroup, which need no pieces and no join for one user, are slower: 16.2 us for 1501 keys where both launches
+// take 10.2 (one compute unit's rate).
 template <class T, int HELD, int DP, bool MOD, int R, int NW>
 struct PagedToken {
     static constexpr int kLds = NW * 16 * (DP + 4) * 4 + NW * 16 * 8;
@@ -284,9 +289,9 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
                 vv[j] = in ? vv[j] : 0.f;
             }
         }
-        // Probabilities as operands; bf16: with a second one for what the first, of 8 bits, leaves: an output is then off by its own rounding only (0.0017 of its size, 0.0026 with one
-        // operand and few keys), for 1 % of the time, since products are far from what bounds this kernel (64 users of up to 8192 keys, 122 and 123 us).
-        constexpr bool kRest = __is_same(T, __bf16);
+        // Probabilities as operands; 16 bits: with a second one for what the first, of 8 or 11 bits, leaves: an output is then off by its own rounding only (bf16: 0.0017 of its size, 0.0026
+        // with one operand and few keys), for 1 % of the time, since products are far from what bounds this kernel (64 users of up to 8192 keys, 122 and 123 us).
+        constexpr bool kRest = sizeof(T) == 2;
         Vec8 p[R], rest[kRest ? R : 1];
         auto round = [&](int r, const floatx8 &f) {
             p[r] = __builtin_convertvector(f, Vec8);
