@@ -15,7 +15,7 @@ namespace sddmm {
 // are joined at the end.
 //
 // Bound by reading the caches where there are many (64 users of 284 to 8192 keys, 8 key heads of 128, 8 bits: 119 us, 4.6 TB/s; a large copy makes 4.7; vector instructions for 41 % of
-// the time, matrix ones for 9), by chains of loads -- lengths, pages, keys, the next keys -- where there are few (4 users of up to 32,768 keys, 2 key heads: 12.5 us in 512 workgroups of
+// the time, matrix ones for 9), by chains of loads -- lengths, pages, keys, the next keys -- where there are few (4 users of up to 32,768 keys, 2 key heads: 13.2 us in 512 workgroups of
 // four tiles a wave, compute units busy for 42 %).  Sixteen waves to a workgroup, which need no pieces and no join for one user, are slower: 16.2 us for 1501 keys where both launches
 // take 10.2 (one compute unit's rate).
 template <class T, int HELD, int DP, bool MOD, int R, int NW>
