@@ -5,8 +5,10 @@ namespace sddmm {
 
 namespace {
 
+// Two waves to a SIMD, but one for two tiles of rows over fp32 rows of 128 elements, which do not fit 256 registers (us with two, which spill, and one: 4 tokens of 42 users, 64 heads over 8,
+// up to 1231 keys 166 and 112; 5 of 32, 16 over 4, 3000 108 and 77; 8 of one, 4096 24 and 19).
 template <class T, int HELD, int DP, bool MOD, int R, int NW>
-__global__ __launch_bounds__(64 * NW, 2)
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && HELD == kHeldOwn && DP == 128 && R == 2 ? 1 : 2)
 void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
 {
     typedef PagedToken<T, HELD, DP, MOD, R, NW> Body;
