@@ -172,3 +172,48 @@ def test_bf16_weights_keep_their_bits():
                 bound = 2.0 ** -8 * (r["out"].abs() + r["out_tol"]) + 2.0 ** -16 * 1.02 * pv + r["out_tol"]
                 assert ((out[at: at + n, h].double() - r["out"]).abs() <= bound).all(), (held, s, h)
             at += n
+
+
+@pytest.mark.parametrize("dtype,held", [(BF16, "i8"), (BF16, "own"), (F32, "e4m3")])
+@pytest.mark.parametrize("n_new", [[2, 1], [70, 40], [90, 1, 1, 1, 1, 1, 1]])
+def test_places_beyond_32_bits(dtype, held, n_new):
+    """Keys in pages 2^32 - 16 bytes apart, heads within them 2^31, and values in rows of nearly 2^23: the same bits as a compact cache gives."""
+    page, block, kv, heads, dim = 16, 8, 2, 4, 64
+    after = [n + 9 for n in n_new]
+    table, n_pages = tables(after, page, 3)
+    small = Pages(dtype, held, n_pages, page, block, kv, dim, False, 4)
+    size = small.gpu["k"].element_size()
+    strides = {"k": ((2 ** 32 - 16) // size, 2 ** 31 // size, 256 // size), "v": (2 ** 28 // size, (2 ** 27 + 2 ** 23 - 4096) // size, (2 ** 23 - 16) // size)}  # page, head, row
+    t = torch.tensor(table, dtype=torch.int32, device=DEV)
+    total, most = sum(n_new), max(n_new)
+    length = torch.tensor(after, dtype=torch.int32, device=DEV)
+    ptr = torch.tensor([0] + n_new, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(DEV)
+    q, k, v = (normal(6 + i, total, h, dim).to(dtype).to(DEV) for i, h in enumerate((heads, kv, kv)))
+    desc = capi.AttentionDesc.packed(CODE[dtype], len(n_new), heads, kv, dim, max_q=most, max_k=max(after), k_len=length.data_ptr(), q_ptr=ptr.data_ptr(), q_rows=total, window_right=0)
+    far, views, scales = {}, {}, {}
+    for name in "kv":
+        p, h, r = strides[name]
+        far[name] = torch.empty((n_pages - 1) * p + (kv - 1) * h + page * r, dtype=small.store, device=DEV)
+        views[name] = far[name].as_strided((n_pages, kv, page, dim), (p, h, r, 1))
+        views[name].copy_(small.gpu[name])
+        scales[name] = small.scales[name].clone() if held != "own" else None
+    more = dict(k=far["k"].data_ptr(), v=far["v"].data_ptr())
+    for name in "kv":
+        more[name + "_page"], more[name + "_head"], more[name + "_row"] = strides[name]
+        if held != "own":
+            more[name + "_scale"] = scales[name].data_ptr()
+    outs = []
+    for cache in (small.desc(t), small.desc(t, **more)):
+        capi.cache_append(desc, cache, 0, 0, k.data_ptr(), v.data_ptr(), stream())
+        out = torch.full_like(q, 7.0)
+        n = capi.attention_paged_workspace_bytes(desc, cache)
+        ws = torch.full((max(n, 16),), 255, dtype=torch.uint8, device=DEV)
+        capi.attention_paged(desc, cache, q.data_ptr(), out.data_ptr(), 0, ws.data_ptr(), n, stream())
+        torch.cuda.synchronize()
+        outs.append(out)
+    assert torch.equal(*outs) and not outs[0].isnan().any()
+    for name in "kv":
+        assert torch.equal(views[name].contiguous().view(torch.uint8), small.gpu[name].view(torch.uint8))
+        assert held == "own" or torch.equal(scales[name], small.scales[name])
+    del far, views
+    torch.cuda.empty_cache()
