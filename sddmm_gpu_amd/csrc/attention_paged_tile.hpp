@@ -382,7 +382,7 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
                 for (int d = 0; d < DB; ++d) o[d] *= to;
             }
             if (some || norm != 1.f) {
-                const float in = 1.f / norm;
+                const float in = norm > 0.f ? 1.f / norm : 0.f;  // (0: no factor but 0 so far)
 #pragma unroll
                 for (int k = 0; k < KB; ++k)
 #pragma unroll
