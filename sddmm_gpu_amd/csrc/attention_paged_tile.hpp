@@ -247,6 +247,7 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
                     float rest;
                     const float by = fold<U, HELD>(in ? scales[j][which] : 1.f, rest);
                     some[which] = some[which] || rest != 1.f;
+                    if (!in) rest = 0.f;  // (no key: no factor of its own, where the tile's factors are compared)
                     if (kHalves && my_piece == 0) left[place_of(which, t) * KT + r] = rest;
                     char *to = tile_at(which, t) + r * Keys::kRowBytes;
 #pragma unroll

@@ -71,3 +71,13 @@ def test_scales_of_zero(dtype, held, n_new):
     for length in (128, 150, 400):
         for zero in (lambda j: j >= 0, lambda j: j < 64, lambda j: (j >= 64) & (j < 128), lambda j: j >= 64, lambda j: j < 128, lambda j: j != 5):
             check(dtype, held, n_new, ends(n_new, length), lambda n: torch.where(zero(torch.arange(n)), 0.0, one))
+
+
+@pytest.mark.parametrize("held", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n_new", [FEW, MANY, MIXED, [40], [66]])
+def test_tiny_scales(dtype, held, n_new):
+    """Values of about 2^-e, in caches that end inside a tile of keys."""
+    for length in (40, 64, 66, 130, 150):
+        for e in (15, 24, 38, 44, 48, 60, 100):
+            check(dtype, held, n_new, ends(n_new, length), lambda n: torch.full((n,), 2.0 ** -e), unit=2.0 ** (5 - e), cap=30.0 if e == 48 else 0.0)
