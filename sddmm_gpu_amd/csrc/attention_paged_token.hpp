@@ -1,5 +1,6 @@
 // Attention over a cache in pages for few rows (gfx950): the newest tokens of every sequence.
 #pragma once
+#include <type_traits>
 #include "attention_paged.hpp"
 #include "attention_paged_launch.hpp"
 #include "launch.hpp"
@@ -28,12 +29,15 @@ template <class T, int HELD, int DP, bool MOD, int R, int NW>
 __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const AttnArgs &a, const CacheArgs &c, int kv, int split, int b, char (&memory)[kLds])
 {
     typedef typename Elem<T>::Vec8 Vec8;
+    // What probabilities times scales and values' codes are multiplied in: fp16 rows over codes take bf16, whose range is that of the scales (in fp16 a value of 2^14 times the others,
+    // whatever its probability, would cost the others' weights their bits).
+    typedef std::conditional_t<__is_same(T, _Float16) && HELD != kHeldOwn, __bf16, T> W;
+    typedef typename Elem<W>::Vec8 Weights;
     constexpr int KT = 32, S = DP / 32, E = DP / 16;           // keys of a tile, steps of a product over a head's elements, values' elements of a lane
     constexpr int kSize = HELD == kHeldOwn ? (int)sizeof(T) : 1;
     constexpr int kPiece = HELD != kHeldOwn && S > 1 ? 16 : 8 * kSize;  // bytes of a key's row that a lane takes at a time: of two steps, or of one
     constexpr int kKeyWords = S * 8 * kSize / 4;               // a lane's registers of a key's row
     constexpr int kValueBytes = E * kSize, kValueWords = (kValueBytes + 3) / 4;
-    constexpr bool kNorm = __is_same(T, _Float16) && HELD != kHeldOwn;
     constexpr int kRows = 16 * R;
     auto &joined = *(float (*)[NW][16][DP + 4])memory;
     auto &ml = *(float2 (*)[NW][16])(memory + sizeof joined);
@@ -81,7 +85,7 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
     }
 
     floatx4 o[R][E];
-    float m[R], sum[R], norm = 0.f, by_norm = 0.f;
+    float m[R], sum[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         m[r] = -INFINITY, sum[r] = 0.f;
@@ -292,35 +296,17 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
         // Probabilities as operands; 16 bits: with a second one for what the first, of 8 or 11 bits, leaves: an output is then off by its own rounding only (bf16: 0.0017 of its size, 0.0026
         // with one operand and few keys), for 1 % of the time, since products are far from what bounds this kernel (64 users of up to 8192 keys, 122 and 123 us).
         constexpr bool kRest = sizeof(T) == 2;
-        Vec8 p[R], rest[kRest ? R : 1];
+        Weights p[R], rest[kRest ? R : 1];
         auto round = [&](int r, const floatx8 &f) {
-            p[r] = __builtin_convertvector(f, Vec8);
-            if constexpr (kRest) rest[r] = __builtin_convertvector(f - __builtin_convertvector(p[r], floatx8), Vec8);
+            p[r] = __builtin_convertvector(f, Weights);
+            if constexpr (kRest) rest[r] = __builtin_convertvector(f - __builtin_convertvector(p[r], floatx8), Weights);
         };
         if constexpr (HELD != kHeldOwn) {
-            float (&w)[8] = vv;
-            if constexpr (kNorm) {
-                // fp16: scales in units of the largest so far, which keeps their products with probabilities in the type's range
-                float most = w[0];
-#pragma unroll
-                for (int j = 1; j < 8; ++j) most = fmaxf(most, w[j]);
-                most = groups_max(most);
-                if (__any(most > norm)) {
-                    const float by = norm / most;
-                    norm = most, by_norm = 1.f / most;
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int d = 0; d < E; ++d) o[r][d] *= by;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] *= by_norm;
-            }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 floatx8 f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = y[r][j] * w[j];
+                for (int j = 0; j < 8; ++j) f[j] = y[r][j] * vv[j];
                 round(r, f);
             }
         } else {
@@ -332,9 +318,9 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
                 round(r, f);
             }
         }
-        auto add = [&](const Vec8 &v, int r, int d) {
-            o[r][d] = mma16<T>(v, p[r], o[r][d]);
-            if constexpr (kRest) o[r][d] = mma16<T>(v, rest[r], o[r][d]);
+        auto add = [&](const Weights &v, int r, int d) {
+            o[r][d] = mma16<W>(v, p[r], o[r][d]);
+            if constexpr (kRest) o[r][d] = mma16<W>(v, rest[r], o[r][d]);
         };
         // element d of the lane's elements, of its eight tokens
         if constexpr (HELD != kHeldOwn) {
@@ -347,7 +333,7 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
                 turn4(x1);
 #pragma unroll
                 for (int d = 0; d < (E < 4 ? E : 4); ++d) {
-                    const Vec8 v = expand<T, HELD>(x0[d], x1[d]);
+                    const Weights v = expand<W, HELD>(x0[d], x1[d]);
 #pragma unroll
                     for (int r = 0; r < R; ++r) add(v, r, 4 * q + d);
                 }
@@ -358,14 +344,14 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
                 uint4v w;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[j] = __builtin_amdgcn_perm(v_raw[2 * j + 1][d / 2], v_raw[2 * j][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
-                const Vec8 v = __builtin_bit_cast(Vec8, w);
+                const Weights v = __builtin_bit_cast(Weights, w);
 #pragma unroll
                 for (int r = 0; r < R; ++r) add(v, r, d);
             }
         } else {
 #pragma unroll
             for (int d = 0; d < E; ++d) {
-                Vec8 v;
+                Weights v;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(v_raw[j][d]);
 #pragma unroll
@@ -384,7 +370,7 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int d = 0; d < E; ++d) joined[wave][n][E * (4 * g + i) + d] = kNorm ? o[r][d][i] * norm : o[r][d][i];
+            for (int d = 0; d < E; ++d) joined[wave][n][E * (4 * g + i) + d] = o[r][d][i];
         if (g == 0) ml[wave][n] = make_float2(m[r] == -INFINITY ? m[r] : m[r] * unit, total_of_wave);
         __syncthreads();
         constexpr int kEach = 16 * DP / 4 / (64 * NW);  // pieces of four elements to a thread

@@ -81,3 +81,13 @@ def test_tiny_scales(dtype, held, n_new):
     for length in (40, 64, 66, 130, 150):
         for e in (15, 24, 38, 44, 48, 60, 100):
             check(dtype, held, n_new, ends(n_new, length), lambda n: torch.full((n,), 2.0 ** -e), unit=2.0 ** (5 - e), cap=30.0 if e == 48 else 0.0)
+
+
+@pytest.mark.parametrize("held", ["i8", "e4m3"])
+@pytest.mark.parametrize("n_new", [FEW, MANY, MIXED])
+def test_scales_far_apart_in_fp16(held, n_new):
+    """The same within the range of fp16: one token of values up to 2^15 that rows hardly see, values of about 2^-10 (2^-2) for the rest."""
+    large, small = (2.0 ** 8, 2.0 ** -15) if held == "i8" else (2.0 ** 6, 2.0 ** -17)
+    for length in (96, 150, 700):
+        for j in (0, 5, 60):
+            check(F16, held, n_new, ends(n_new, length), lambda n: torch.where(torch.arange(n) == j, large, small), away=(j,) if j < 40 else (), unit=2.0 ** -5)
