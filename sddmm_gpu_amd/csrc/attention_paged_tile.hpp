@@ -154,7 +154,8 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
     const float unit = MOD ? 1.f : scale * kLog2e * by_row;  // scores in registers to powers of two
     const float raise = fminf(8.f / unit, FLT_MAX);  // (finite: added to a maximum of -infinity)
     const float slope = MOD && a.slopes && there ? a.slopes[head] * kLog2e : 0.f;
-    float m = -INFINITY, sum = 0.f, norm = 0.f;
+    float m = -INFINITY, sum = 0.f;
+    float norm = 1.f, best = 0.f;  // codes in 16 bits: the unit of the row's weights, and the largest of them in units of 2^15 (see `weights`)
 
     // tiles begin at multiples of 16, so that sixteen rows lie in one page
     const int key0 = any_lo & ~15, n_tiles = any_hi > any_lo ? (any_hi - key0 + KT - 1) / KT : 0;
@@ -352,7 +353,7 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
         if (__any(top > m + raise)) {
             const float raised = fmaxf(m, top), by = raised == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - raised) * unit);
             m = raised;
-            sum *= by;
+            sum *= by, best *= by;
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= by;
         }
@@ -367,32 +368,40 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
             }
         sum += sum_odd;
         if constexpr (kHalves) {
-            // factors of values, in units of the largest so far
-            const bool some = any_of(1);
-            const float *by = left + place_of(1, t) * KT;
-            float most = 1.f;
-            if (some) {
-                most = fmaxf(by[n], by[n + 32 < KT ? n + 32 : n]);
-#pragma unroll
-                for (int d = 1; d < 32; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-            }
-            if (most > norm) {
-                const float to = norm / most;
-                norm = most;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] *= to;
-            }
-            if (some || norm != 1.f) {
-                const float in = norm > 0.f ? 1.f / norm : 0.f;  // (0: no factor but 0 so far)
+            // Weights: probabilities times what is left of values' scales, in units of a power of two of the row's own, so that its largest so far is from 2^7 to 2^15 of them
+            // whatever the scales, those of other rows' keys among them (where all are 0 the unit stays).  1, and nothing to do, while no scale leaves anything.
+            // (`largest` without an else: one would cost a hundred spilled registers)
+            float largest = fmaxf(best, __builtin_amdgcn_exp2f(fmaf(top, unit, -base)) * 0x1p-15f);
+            if (any_of(1) || __any(norm != 1.f)) {
+                const float *by = left + place_of(1, t) * KT;
+                float most = 0.f;
 #pragma unroll
                 for (int k = 0; k < KB; ++k)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const floatx4 f = *(const floatx4 *)(by + 32 * k + 8 * i + 4 * h) * in;
+                        const floatx4 f = *(const floatx4 *)(by + 32 * k + 8 * i + 4 * h) * 0x1p-15f;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) x[k][4 * i + j] *= f[j];
+                        for (int j = 0; j < 4; ++j) x[k][4 * i + j] *= f[j], most = fmaxf(most, x[k][4 * i + j]);
                     }
+                best = fmaxf(best, halves_max(most));
+                largest = best;
+                const bool change = best > norm || (best < norm * 0x1p-8f && best > 0.f);
+                if (__any(change)) {
+                    // (2^-111 and more, so that 2^15 of its reciprocals are a number)
+                    const int e = best <= 1.f && best >= 0x1p-8f ? 0 : max(__builtin_amdgcn_frexp_expf(best), -111);
+                    const float to = change ? __uint_as_float((uint32_t)(127 + e) << 23) : norm;
+                    const int up = (int)(__float_as_uint(norm) >> 23) - (int)(__float_as_uint(to) >> 23);
+                    norm = to;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[d][i] = __builtin_amdgcn_ldexpf(o[d][i], up);
+                }
+                const float in = __uint_as_float(0x7f000000u - __float_as_uint(norm)) * 0x1p15f;  // (a power of two's reciprocal)
+#pragma unroll
+                for (int k = 0; k < KB; ++k) x[k] *= in;
             }
+            best = largest;
         }
 #pragma unroll
         for (int i = 0; i < 2 * KB; ++i) p[i] = operand<U>(x[i / 2], i & 1);

@@ -84,6 +84,28 @@ def test_tiny_scales(dtype, held, n_new):
 
 
 @pytest.mark.parametrize("held", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n_new", [FEW, MANY, MIXED])
+def test_scales_far_apart(dtype, held, n_new):
+    """Rows whose values are far smaller than others of the tile: of a token behind them, or of one that they hardly see; scales that rise and fall along the cache."""
+    for length in (96, 150, 700):
+        def last_large(n):
+            return torch.where(torch.arange(n) == n - 1, 2.0 ** 60, 2.0 ** -30)
+
+        def first_large(n):
+            return torch.where(torch.arange(n) == 0, 2.0 ** 60, 2.0 ** -30)
+
+        def rising(n):
+            return torch.ldexp(torch.ones(n), torch.arange(n) * 80 // n - 60)
+
+        check(dtype, held, n_new, ends(n_new, length), last_large, unit=2.0 ** -25)
+        check(dtype, held, n_new, ends(n_new, length), first_large, unit=2.0 ** -25, away=(0,))
+        check(dtype, held, n_new, ends(n_new, length), first_large, unit=2.0 ** -25, away=(0,), cap=400.0)
+        check(dtype, held, n_new, ends(n_new, length), rising, unit=2.0 ** -10)
+        check(dtype, held, n_new, ends(n_new, length), lambda n: rising(n).flip(0), unit=2.0 ** -10)
+
+
+@pytest.mark.parametrize("held", ["i8", "e4m3"])
 @pytest.mark.parametrize("n_new", [FEW, MANY, MIXED])
 def test_scales_far_apart_in_fp16(held, n_new):
     """The same within the range of fp16: one token of values up to 2^15 that rows hardly see, values of about 2^-10 (2^-2) for the rest."""
