@@ -673,7 +673,8 @@ void sddmm_cache_desc_init(sddmm_cache_desc *cache);   /* zeros, block_len 1, ro
  * the least power of two (from 2^-126 on) that is enough otherwise: its earlier tokens' codes are then rounded anew to the larger steps.  A block
  * without earlier tokens begins with that power of two.  Codes are rounded to the nearest, ties to even; infinities become the largest code, NaNs
  * 0 (E4M3: NaN).  What lies behind the new tokens stays as it was; tokens at positions below 0 are not stored.  New tokens of a call go to pages
- * that no other sequence of it, and no other part of their own, has (those that are only read may be anyone's). */
+ * that no other sequence of it, and no other part of their own, has (those that are only read may be anyone's).  Keys' scales and values' are
+ * arrays apart from each other and from all others. */
 int sddmm_cache_append(const sddmm_attention_desc *desc, const sddmm_cache_desc *cache, const void *d_q, void *d_q_out, const void *d_k,
                        const void *d_v, void *stream);
 

@@ -1,6 +1,7 @@
 // New tokens into a paged cache (gfx950): keys turned by their positions and values, in the operands' type or in 8 bits with a scale for each
 // block of tokens and head; and their queries turned on the way.
 #include <hip/hip_runtime.h>
+#include <cstdlib>
 #include <cstring>
 #include <type_traits>
 #include "cache.hpp"
@@ -471,6 +472,12 @@ int sddmm_cache_append(const sddmm_attention_desc *desc, const sddmm_cache_desc 
     sddmm_attention_desc pages = d;
     if (!apart(pages, c.k_page, c.k_row, c.k_head, c.n_pages, c.page_len, d.n_kv_heads) || !apart(pages, c.v_page, c.v_row, c.v_head, c.n_pages, c.page_len, d.n_kv_heads))
         return fail(SDDMM_ERR_ARG, "%s: rows of the cache overlap", who);
+    if (c.type != d.type) {
+        // (keys' scales and values' are read and written by different waves)
+        const int64_t scales = c.n_pages * d.n_kv_heads * (c.page_len / c.block_len) * (int64_t)sizeof(float), between = std::llabs((int64_t)((intptr_t)c.k_scale - (intptr_t)c.v_scale));
+        if (c.k_scale && c.v_scale && (between < scales || in_place_of({c.k_scale, c.v_scale}, {d_q, d_q ? d_q_out : nullptr, d_k, d_v, c.k, c.v})))
+            return fail(SDDMM_ERR_ARG, "%s: scales are in another array's place", who);
+    }
     if (in_place_of({c.k, c.v}, {d_q, d_q_out, d_k, d_v}) || (c.k && c.k == c.v) || (d_q && in_place_of({d_q_out}, {d_k, d_v})))
         return fail(SDDMM_ERR_ARG, "%s: a result is in an operand's or another result's place", who);
 

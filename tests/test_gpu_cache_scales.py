@@ -2,9 +2,10 @@
 import pytest
 import torch
 
+from sddmm_gpu_amd import capi
 from tests import attention_reference as ref
 from tests import cache_reference as cref
-from tests.test_gpu_cache import BF16, F16, F32, Pages, attend, normal, tables
+from tests.test_gpu_cache import BF16, DEV, F16, F32, Pages, attend, normal, stream, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +114,23 @@ def test_scales_far_apart_in_fp16(held, n_new):
     for length in (96, 150, 700):
         for j in (0, 5, 60):
             check(F16, held, n_new, ends(n_new, length), lambda n: torch.where(torch.arange(n) == j, large, small), away=(j,) if j < 40 else (), unit=2.0 ** -5)
+
+
+def test_scales_in_one_array():
+    """Keys' and values' scales one behind the other: as in arrays of their own."""
+    n_new, page, block, heads, kv, dim = [9, 30], 16, 8, 4, 2, 64
+    after = [20, 30]
+    table, n_pages = tables(after, page, 3)
+    results = []
+    for together in (False, True):
+        pages = Pages(BF16, "i8", n_pages, page, block, kv, dim, False, 4)
+        if together:
+            both = torch.stack([pages.scales["k"], pages.scales["v"]])
+            pages.scales = {"k": both[0], "v": both[1]}
+        k, v = (normal(6 + i, sum(n_new), kv, dim).to(BF16).to(DEV) * 40 for i in range(2))
+        t, length, ptr = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (table, after, [0, 9, 39]))
+        desc = capi.AttentionDesc.packed(capi.TYPE_BF16, 2, heads, kv, dim, max_q=30, max_k=30, k_len=length.data_ptr(), q_ptr=ptr.data_ptr(), q_rows=39)
+        capi.cache_append(desc, pages.desc(t), 0, 0, k.data_ptr(), v.data_ptr(), stream())
+        torch.cuda.synchronize()
+        results.append([x.cpu() for name in "kv" for x in (pages.gpu[name], pages.scales[name])])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
