@@ -27,6 +27,7 @@ struct AttnArgs {
     void *dq, *dk, *dv;
     float *part_o;              // partial results of split keys: [part][row of all heads][head_dim]
     float2 *part_ml;            // [part][row of all heads]: maximum (in powers of two) and sum
+    float2 *not_ml;             // pages, few rows beside many: the others' part_ml where they have parts, for rows that have none there
     float *stat_lse, *stat_delta;  // backward: [n_heads][all rows] log-sum-exp in powers of two, - sum of dout * out
     double *slope_part;         // backward: [n_heads][slope_parts] parts of the slopes' gradients, or null
     float *dslopes;
@@ -40,7 +41,8 @@ struct AttnArgs {
     int32_t n_split;            // pieces that the keys of a tile of rows are cut into
     int32_t part0, n_part;      // first piece of this launch, pieces in all
     int32_t slope_parts;
-    int32_t few_rows;           // pages, sequences of both kinds: those of so many rows (of a key head) at most are the kernel's for few rows, the others the other's; 0: all
+    int32_t few_rows;           // pages, sequences of both kinds: those of so many rows (of a key head) at most are the kernel's for few rows, whose parts are by sequence, key head
+                                // and row, the others the other's; 0: all
     int32_t chunk;              // backward: rows (of all query heads) that a workgroup of keys walks, more being cut into pieces
     float scale, cap;
 };

@@ -17,7 +17,7 @@ struct Deal {
     int tile = 128;    // rows of a workgroup of the kernel for many
     int64_t slots = 0, max_tiles = 0, grid = 0, splits = 1, chunk = 1;
     int64_t few_rows = 0, few_grid = 0, few_splits = 0;  // sequences of few rows beside others: rows at most, workgroups and pieces
-    int64_t parts = 1, part_bytes = 0, bytes = 0;
+    int64_t part_o = 0, part_ml = 0, few_o = 0, few_ml = 0, bytes = 0;  // where parts lie in the workspace, and those of sequences of few rows beside others
 };
 
 Deal deal(const sddmm_attention_desc &d)
@@ -61,21 +61,22 @@ Deal deal(const sddmm_attention_desc &d)
         r.splits = std::max<int64_t>(1, std::min(std::min(div_up(r.tile == 256 ? 256 : 512, filled), div_up(key_tiles, 8)), (int64_t)256));
     }
     r.grid = workgroups * r.splits;
-    r.parts = r.splits;
     if (mixed) {
         r.few_rows = group <= 16 ? 16 : 32;
         const int64_t caches = (int64_t)d.n_seq * d.n_kv_heads;
         // (beside the others: a workgroup for each compute unit, pieces of up to 4096 keys; 512 and 1024 workgroups 113 and 120 us where 256 take 111)
-        r.few_splits = std::max<int64_t>(1, std::min(std::min(std::max(div_up(256, caches), div_up(key_tiles, 128)), div_up(key_tiles, 4)), (int64_t)256));
+        // No more than 4096 workgroups, where there are several to a cache: their parts (68 MB for heads of 128) would grow with the longest length that a caller allows for.
+        r.few_splits = std::max<int64_t>(1, std::min(std::min(std::max(div_up(256, caches), std::min(div_up(key_tiles, 128), 4096 / caches)), div_up(key_tiles, 4)), (int64_t)256));
         r.chunk = div_up(key_tiles, r.few_splits);
         r.few_splits = div_up(key_tiles, r.chunk);
         r.few_grid = caches * r.few_splits;
-        r.parts = std::max(r.parts, r.few_splits);
     }
-    if (r.parts > 1) {
-        r.part_bytes = padded(r.parts * r.rows * d.n_heads * d.head_dim * (int64_t)sizeof(float));
-        r.bytes = r.part_bytes + padded(r.parts * r.rows * d.n_heads * (int64_t)sizeof(float2));
-    }
+    auto place = [&](int64_t parts, int64_t rows, int64_t &o, int64_t &ml) {
+        o = r.bytes, ml = o + padded(parts * rows * d.head_dim * (int64_t)sizeof(float));
+        r.bytes = ml + padded(parts * rows * (int64_t)sizeof(float2));
+    };
+    if (r.splits > 1) place(r.splits, r.rows * d.n_heads, r.part_o, r.part_ml);
+    if (r.few_splits > 1) place(r.few_splits, d.n_seq * r.few_rows * d.n_kv_heads, r.few_o, r.few_ml);
     return r;
 }
 
@@ -113,28 +114,32 @@ int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_de
     if (!aligned({d_q, d_out})) return fail(SDDMM_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || ((uintptr_t)d_workspace & 255u)))
         return fail(SDDMM_ERR_ARG, "%s: a workspace of %lld bytes, 256-byte aligned, is needed (got %lld)", who, (long long)r.bytes, (long long)workspace_bytes);
-    if (!launchable(r.grid + r.few_grid, 512) || (r.parts > 1 && !launchable(attention_paged_join_grid(r.rows * d.n_heads, (int)r.parts, d.head_dim), 512)))
+    const int64_t join = (r.splits > 1 ? attention_paged_join_grid(r.rows * d.n_heads, (int)r.splits, d.head_dim) : 0) +
+                         (r.few_splits > 1 ? attention_paged_join_grid(d.n_seq * r.few_rows * d.n_kv_heads, (int)r.few_splits, d.head_dim) : 0);
+    if (!launchable(r.grid + r.few_grid, 512) || !launchable(join, 512))
         return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
     if (in_place_of({d_out, d_lse}, {d_q, cache->k, cache->v, cache->k_scale, cache->v_scale}) || (const void *)d_lse == d_out)
         return fail(SDDMM_ERR_ARG, "%s: a result is in an operand's or the other result's place", who);
 
     AttnArgs a = arguments(d);
     a.q = d_q, a.out = d_out, a.lse = d_lse;
-    a.part_o = (float *)d_workspace, a.part_ml = (float2 *)((char *)d_workspace + r.part_bytes);
-    a.n_slots = (int)r.slots, a.max_tiles = (int)r.max_tiles, a.n_split = (int)r.splits, a.n_part = (int)r.parts, a.chunk = (int)r.chunk;
+    char *const ws = (char *)d_workspace;
+    a.part_o = (float *)(ws + r.part_o), a.part_ml = (float2 *)(ws + r.part_ml);
+    a.n_slots = (int)r.slots, a.max_tiles = (int)r.max_tiles, a.n_split = a.n_part = (int)r.splits, a.chunk = (int)r.chunk;
     a.few_rows = (int)r.few_rows;
     const CacheArgs c = cache_arguments(d, *cache);
     const hipStream_t st = (hipStream_t)stream;
     const int held = held_as(d, *cache);
     hipError_t e;
+    AttnArgs few = a;
     if (r.few_grid > 0) {
-        AttnArgs few = a;
-        few.n_slots = d.n_seq, few.max_tiles = 1, few.n_split = (int)r.few_splits;
+        few.n_slots = d.n_seq, few.max_tiles = 1, few.n_split = few.n_part = (int)r.few_splits;
+        few.part_o = (float *)(ws + r.few_o), few.part_ml = (float2 *)(ws + r.few_ml), few.not_ml = r.splits > 1 ? a.part_ml : nullptr;
         e = launch_attention_paged_mixed(a, few, c, d.type, held, (unsigned)r.grid, (unsigned)r.few_grid, st);
     } else {
         e = r.token ? launch_attention_paged_token(a, c, d.type, held, r.tiles, (unsigned)r.grid, st) : launch_attention_paged_forward(a, c, d.type, held, r.tile, (unsigned)r.grid, st);
     }
-    if (e == hipSuccess && r.parts > 1) e = launch_attention_paged_join(a, d.type, st);
+    if (e == hipSuccess && join > 0) e = launch_attention_paged_join(a, r.few_splits > 1 ? &few : nullptr, d.type, st);
     if (e != hipSuccess) return fail(SDDMM_ERR_HIP, "%s: launch failed: %s", who, hipGetErrorString(e));
     return SDDMM_OK;
 }

@@ -19,8 +19,8 @@ template <> __device__ __forceinline__ floatx4 mma16<float>(floatx8 a, floatx8 b
     return c;
 }
 
-// the sum, in the place of a row's first part, of a row that has no parts
-constexpr float kDone = -1.f;
+// the sum, in the place of a row's first part, of a row that is not the kernel's for many rows
+constexpr float kNone = -1.f;
 
 // Eight codes, four to a register, as an operand: both kinds are exact in 16 bits.
 template <class T, int HELD> __device__ __forceinline__ typename Elem<T>::Vec8 expand(uint32_t lo, uint32_t hi)

@@ -17,6 +17,7 @@ hipError_t launch_attention_paged_forward(const AttnArgs &a, const CacheArgs &c,
 // sequences of many rows (128 to a workgroup) and of few_rows at most (of 16 or 32); 16-bit operands
 hipError_t launch_attention_paged_mixed(const AttnArgs &many, const AttnArgs &few, const CacheArgs &c, int type, int held, unsigned n_many, unsigned n_few, hipStream_t st);
 int64_t attention_paged_join_grid(int64_t rows_of_heads, int n_part, int head_dim);  // workgroups of the join, of 512 threads
-hipError_t launch_attention_paged_join(const AttnArgs &a, int type, hipStream_t st);
+// a's parts, if it has any, and, where not null, those of `few`
+hipError_t launch_attention_paged_join(const AttnArgs &a, const AttnArgs *few, int type, hipStream_t st);
 
 }  // namespace sddmm

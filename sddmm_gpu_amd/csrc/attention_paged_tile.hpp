@@ -461,15 +461,9 @@ __device__ __forceinline__ void PagedTile<T, HELD, DP, MOD, NW>::run(const AttnA
                 const int col = 32 * d + 8 * i + 4 * h;
                 if (col < a.head_dim) *(floatx4 *)(to + col) = floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
             }
-        if (h == 0) {
-            a.part_ml[split * all + at] = make_float2(m, sum);
-            if (split == 0) {  // (parts that there are of other rows only)
-                for (int i = a.n_split; i < a.n_part; ++i) a.part_ml[i * all + at] = make_float2(-INFINITY, 0.f);
-            }
-        }
+        if (h == 0) a.part_ml[split * all + at] = make_float2(m, sum);
         return;
     }
-    if (there && a.n_part > 1 && h == 0) a.part_ml[at] = make_float2(-INFINITY, kDone);
     if (there && a.lse && h == 0) a.lse[at] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
     const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
     __syncthreads();  // (the tiles have been read by all)

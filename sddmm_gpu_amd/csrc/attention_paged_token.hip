@@ -1,4 +1,5 @@
 // Attention over a cache in pages for few rows (gfx950): workgroups of four waves, and the sum of partial results of keys that were cut into pieces.
+#include <algorithm>
 #include "attention_paged_token.hpp"
 
 namespace sddmm {
@@ -44,30 +45,36 @@ hipError_t launch_rows(const AttnArgs &a, const CacheArgs &c, int type, int held
 }
 
 // The parts of a row: sums and totals in units of 2^(largest maximum).  Groups of DP / 4 lanes take parts in turn, N at a time with maxima and sums under way together, each
-// with a running maximum of its own, and meet in LDS.
+// with a running maximum of its own, and meet in LDS.  FEW: the parts of sequences of few rows beside others.
 constexpr int kJoinThreads = 512;
-template <class T, int DP, int N>
-__global__ __launch_bounds__(kJoinThreads)
-void sddmm_attention_paged_join_kernel(const AttnArgs a, const int per_row)
+template <class T, int DP, int N, bool FEW>
+__device__ __forceinline__ void join_parts(const AttnArgs &a, int per_row, int block, floatx4 (&sums)[kJoinThreads / (DP / 4)][DP / 4], float2 (&stats)[kJoinThreads / (DP / 4)])
 {
     constexpr int kLanes = DP / 4, kGroups = kJoinThreads / kLanes;
-    __shared__ floatx4 sums[kGroups][kLanes];
-    __shared__ float2 stats[kGroups];
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, mine = group % per_row, col = lane * 4;
-    const int64_t all = a.rows * a.n_heads, at = (int64_t)blockIdx.x * (kGroups / per_row) + group / per_row;
-    const int head = (int)(at % a.n_heads);
-    const int64_t row = at / a.n_heads;
-    int64_t to_row = 0;
+    const int64_t all = FEW ? (int64_t)a.n_seq * a.n_kv_heads * a.few_rows : a.rows * a.n_heads, at = (int64_t)block * (kGroups / per_row) + group / per_row;
+    int64_t to_row = 0, to_lse = at;
+    int head;
     bool there = at < all;
-    if (a.q_ptr) {
-        there = there && row >= a.q_ptr[0] && row < a.q_ptr[a.n_seq];
-        to_row = row * a.o_row;
-    } else if (there) {
-        const int s = (int)(row / a.max_q), i = (int)(row % a.max_q);
-        there = !a.q_len || i < min(a.q_len[s], a.max_q);
-        to_row = s * a.o_seq + i * a.o_row;
+    if constexpr (FEW) {
+        const int row = (int)(at % a.few_rows), kv = (int)(at / a.few_rows % a.n_kv_heads), s = (int)min(at / a.few_rows / a.n_kv_heads, (int64_t)a.n_seq - 1), token = row / a.group;
+        const Seq e = sequence(a, s);
+        head = kv * a.group + row % a.group;
+        there = there && row < e.nq * a.group && e.nq * a.group <= a.few_rows;
+        to_row = (e.q0 + token) * a.o_row, to_lse = (e.lse0 + token) * a.n_heads + head;
+    } else {
+        head = (int)(at % a.n_heads);
+        const int64_t row = at / a.n_heads;
+        if (a.q_ptr) {
+            there = there && row >= a.q_ptr[0] && row < a.q_ptr[a.n_seq];
+            to_row = row * a.o_row;
+        } else if (there) {
+            const int s = (int)(row / a.max_q), i = (int)(row % a.max_q);
+            there = !a.q_len || i < min(a.q_len[s], a.max_q);
+            to_row = s * a.o_seq + i * a.o_row;
+        }
+        if (there && a.few_rows && a.part_ml[at].y == kNone) there = false;
     }
-    if (there && a.few_rows && a.part_ml[at].y == kDone) there = false;  // (the kernel for many rows has written its result)
     float top = -INFINITY, total = 0.f;
     floatx4 y = {0.f, 0.f, 0.f, 0.f};
     for (int p0 = mine; there && p0 < a.n_part; p0 += N * per_row) {
@@ -116,7 +123,25 @@ void sddmm_attention_paged_join_kernel(const AttnArgs a, const int per_row)
     const float by = total > 0.f || total != total ? 1.f / total : 0.f;
     T *to = (T *)a.out + to_row + head * a.o_head;
     if (col < a.head_dim) *(typename Elem<T>::Vec4 *)(to + col) = __builtin_convertvector(y * by, typename Elem<T>::Vec4);
-    if (a.lse && lane == 0) a.lse[at] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+    if (a.lse && lane == 0) a.lse[to_lse] = (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+template <class T, int DP, int N>
+__global__ __launch_bounds__(kJoinThreads)
+void sddmm_attention_paged_join_kernel(const AttnArgs a, const int per_row)
+{
+    __shared__ floatx4 sums[kJoinThreads / (DP / 4)][DP / 4];
+    __shared__ float2 stats[kJoinThreads / (DP / 4)];
+    join_parts<T, DP, N, false>(a, per_row, blockIdx.x, sums, stats);
+}
+// The first n_first workgroups: a's parts; the others: those of `few`.
+template <class T, int DP, int N>
+__global__ __launch_bounds__(kJoinThreads)
+void sddmm_attention_paged_join_both_kernel(const AttnArgs a, const int per_row, const AttnArgs few, const int per_row_few, const int n_first)
+{
+    __shared__ floatx4 sums[kJoinThreads / (DP / 4)][DP / 4];
+    __shared__ float2 stats[kJoinThreads / (DP / 4)];
+    if ((int)blockIdx.x < n_first) join_parts<T, DP, N, false>(a, per_row, blockIdx.x, sums, stats);
+    else join_parts<T, DP, N, true>(few, per_row_few, blockIdx.x - n_first, sums, stats);
 }
 
 // lane groups of a workgroup of the kernel above, and how many of them share a row
@@ -128,19 +153,27 @@ int join_per_row(int n_part, int head_dim)
     return per_row;
 }
 template <class T, int DP>
-hipError_t launch_join_dim(const AttnArgs &a, hipStream_t st)
+hipError_t launch_join_dim(const AttnArgs &a, const AttnArgs *few, hipStream_t st)
 {
-    const int per_row = join_per_row(a.n_part, a.head_dim);
-    const dim3 grid((unsigned)attention_paged_join_grid(a.rows * a.n_heads, a.n_part, a.head_dim)), block(kJoinThreads);
+    const int per_row = join_per_row(a.n_part, a.head_dim), per_row_few = few ? join_per_row(few->n_part, a.head_dim) : 1;
+    const unsigned first = a.n_part > 1 ? (unsigned)attention_paged_join_grid(a.rows * a.n_heads, a.n_part, a.head_dim) : 0;
     // As many at a time as a group has, up to eight (us of the whole call with 2 / 4 / 8: two parts, 2048 rows of 16 heads 309 / - / 312, 1053 of 32 heads 107 / - / 111; 64 parts - / 16.8 / 17.3;
     // 128 and 256 of one row - / 15.1 and 17.1 / 14.8 and 16.7).
-    auto *fn = a.n_part <= 2 * per_row ? sddmm_attention_paged_join_kernel<T, DP, 2> : a.n_part <= 4 * per_row ? sddmm_attention_paged_join_kernel<T, DP, 4> : sddmm_attention_paged_join_kernel<T, DP, 8>;
-    return launch(fn, grid, block, 0, st, a, per_row);
+    const int most = std::max((a.n_part + per_row - 1) / per_row, few ? (few->n_part + per_row_few - 1) / per_row_few : 0);
+    if constexpr (sizeof(T) == 2) {
+        if (few) {
+            const unsigned second = (unsigned)attention_paged_join_grid((int64_t)few->n_seq * few->n_kv_heads * few->few_rows, few->n_part, a.head_dim);
+            auto *fn = most <= 2 ? sddmm_attention_paged_join_both_kernel<T, DP, 2> : most <= 4 ? sddmm_attention_paged_join_both_kernel<T, DP, 4> : sddmm_attention_paged_join_both_kernel<T, DP, 8>;
+            return launch(fn, dim3(first + second), dim3(kJoinThreads), 0, st, a, per_row, *few, per_row_few, (int)first);
+        }
+    }
+    auto *fn = most <= 2 ? sddmm_attention_paged_join_kernel<T, DP, 2> : most <= 4 ? sddmm_attention_paged_join_kernel<T, DP, 4> : sddmm_attention_paged_join_kernel<T, DP, 8>;
+    return launch(fn, dim3(first), dim3(kJoinThreads), 0, st, a, per_row);
 }
 template <class T>
-hipError_t launch_join(const AttnArgs &a, hipStream_t st)
+hipError_t launch_join(const AttnArgs &a, const AttnArgs *few, hipStream_t st)
 {
-    return a.head_dim <= 64 ? launch_join_dim<T, 64>(a, st) : launch_join_dim<T, 128>(a, st);
+    return a.head_dim <= 64 ? launch_join_dim<T, 64>(a, few, st) : launch_join_dim<T, 128>(a, few, st);
 }
 
 }  // namespace
@@ -151,9 +184,9 @@ int64_t attention_paged_join_grid(int64_t rows_of_heads, int n_part, int head_di
     return (rows_of_heads + rows - 1) / rows;
 }
 
-hipError_t launch_attention_paged_join(const AttnArgs &a, int type, hipStream_t st)
+hipError_t launch_attention_paged_join(const AttnArgs &a, const AttnArgs *few, int type, hipStream_t st)
 {
-    return type == SDDMM_TYPE_F32 ? launch_join<float>(a, st) : type == SDDMM_TYPE_F16 ? launch_join<_Float16>(a, st) : launch_join<__bf16>(a, st);
+    return type == SDDMM_TYPE_F32 ? launch_join<float>(a, few, st) : type == SDDMM_TYPE_F16 ? launch_join<_Float16>(a, few, st) : launch_join<__bf16>(a, few, st);
 }
 
 hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, unsigned grid, hipStream_t st)

@@ -363,6 +363,7 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
 
     // join the waves, 16 rows at a time: a lane holds DP / 4 elements in a row of its row
     const bool parts = a.n_part > 1;
+    const int64_t all = a.few_rows ? (int64_t)a.n_seq * a.n_kv_heads * a.few_rows : a.rows * a.n_heads;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const float total_of_wave = groups_sum(sum[r]);
@@ -393,16 +394,12 @@ __device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const A
                 if (one.x != -INFINITY) z += y * by;
             }
             const int token = row / a.group, head = kv * a.group + row % a.group;
-            const int64_t at = (e.lse0 + token) * a.n_heads + head, all = a.rows * a.n_heads;
+            const int64_t at = (e.lse0 + token) * a.n_heads + head;
+            if (a.not_ml && split == 0 && col == 0) a.not_ml[at] = make_float2(-INFINITY, kNone);
             if (parts) {
-                if (top != -INFINITY && col < a.head_dim) *(floatx4 *)(a.part_o + (split * all + at) * a.head_dim + col) = z;
-                if (col == 0) {
-                    a.part_ml[split * all + at] = make_float2(top, total);
-                    // (parts that there are of other rows only)
-                    if (split == 0) {
-                        for (int i = a.n_split; i < a.n_part; ++i) a.part_ml[i * all + at] = make_float2(-INFINITY, 0.f);
-                    }
-                }
+                const int64_t to = split * all + (a.few_rows ? ((int64_t)s * a.n_kv_heads + kv) * a.few_rows + row : at);
+                if (top != -INFINITY && col < a.head_dim) *(floatx4 *)(a.part_o + to * a.head_dim + col) = z;
+                if (col == 0) a.part_ml[to] = make_float2(top, total);
             } else {
                 z *= total > 0.f || total != total ? 1.f / total : 0.f;
                 T *to = (T *)o_base<T>(a, a.out, e, s, head) + (int64_t)token * a.o_row;
