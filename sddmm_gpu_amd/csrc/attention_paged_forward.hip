@@ -20,7 +20,7 @@ template <class T, int HELD, int DP>
 hipError_t launch_dim(const AttnArgs &a, const CacheArgs &c, int tile, unsigned grid, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2 && DP == 128) {
         if (tile == 256) return launch(mod ? sddmm_attention_paged_kernel<T, HELD, DP, true, 8> : sddmm_attention_paged_kernel<T, HELD, DP, false, 8>, dim3(grid), dim3(512), 0, st, a, c);
     }
     return launch(mod ? sddmm_attention_paged_kernel<T, HELD, DP, true, 4> : sddmm_attention_paged_kernel<T, HELD, DP, false, 4>, dim3(grid), dim3(256), 0, st, a, c);

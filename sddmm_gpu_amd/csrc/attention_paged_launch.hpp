@@ -11,7 +11,7 @@ struct CacheArgs;
 // tiles: of 16 rows to a workgroup, 1 or 2; a.chunk: tiles of 32 keys to a piece
 hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, unsigned grid, hipStream_t st);
 
-// tile: rows of a workgroup, 128 or 256 (16-bit operands)
+// tile: rows of a workgroup, 128 or, of 16-bit heads of more than 64, 256
 hipError_t launch_attention_paged_forward(const AttnArgs &a, const CacheArgs &c, int type, int held, int tile, unsigned grid, hipStream_t st);
 
 // sequences of many rows (128 to a workgroup) and of few_rows at most (of 16 or 32); 16-bit operands

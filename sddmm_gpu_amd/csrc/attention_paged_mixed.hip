@@ -16,7 +16,7 @@ __global__ __launch_bounds__(256, 2)
 void sddmm_attention_paged_mixed_kernel(const AttnArgs many, const AttnArgs few, const CacheArgs c, const int n_many)
 {
     typedef PagedTile<T, HELD, DP, MOD, 4> First;
-    typedef PagedToken<T, HELD, DP, MOD, R, 4> Second;
+    typedef PagedToken<T, HELD, DP, MOD, R> Second;
     __shared__ __align__(1024) char lds[First::kLds > Second::kLds ? First::kLds : Second::kLds];
     if ((int)blockIdx.x < n_many) {
         First::run(many, c, blockIdx.x, *(char (*)[First::kLds])lds);

@@ -8,40 +8,40 @@ namespace {
 
 // Two waves to a SIMD, but one for two tiles of rows over fp32 rows of 128 elements, which do not fit 256 registers (us with two, which spill, and one: 4 tokens of 42 users, 64 heads over 8,
 // up to 1231 keys 166 and 112; 5 of 32, 16 over 4, 3000 108 and 77; 8 of one, 4096 24 and 19).
-template <class T, int HELD, int DP, bool MOD, int R, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 4 && HELD == kHeldOwn && DP == 128 && R == 2 ? 1 : 2)
+template <class T, int HELD, int DP, bool MOD, int R>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && HELD == kHeldOwn && DP == 128 && R == 2 ? 1 : 2)
 void sddmm_attention_paged_token_kernel(const AttnArgs a, const CacheArgs c)
 {
-    typedef PagedToken<T, HELD, DP, MOD, R, NW> Body;
+    typedef PagedToken<T, HELD, DP, MOD, R> Body;
     __shared__ __align__(16) char lds[Body::kLds];
     const uint32_t b = blockIdx.x / a.n_kv_heads;
     Body::run(a, c, blockIdx.x - b * a.n_kv_heads, b % a.n_split, b / a.n_split, lds);
 }
 
-template <class T, int HELD, int DP, int R, int NW>
+template <class T, int HELD, int DP, int R>
 hipError_t launch_dim(const AttnArgs &a, const CacheArgs &c, dim3 grid, hipStream_t st)
 {
     const bool mod = a.cap > 0.f || a.slopes;
-    return launch(mod ? sddmm_attention_paged_token_kernel<T, HELD, DP, true, R, NW> : sddmm_attention_paged_token_kernel<T, HELD, DP, false, R, NW>, grid, dim3(64 * NW), 0, st, a, c);
+    return launch(mod ? sddmm_attention_paged_token_kernel<T, HELD, DP, true, R> : sddmm_attention_paged_token_kernel<T, HELD, DP, false, R>, grid, dim3(256), 0, st, a, c);
 }
-template <class T, int HELD, int R, int NW>
+template <class T, int HELD, int R>
 hipError_t launch_held(const AttnArgs &a, const CacheArgs &c, dim3 grid, hipStream_t st)
 {
     if constexpr (sizeof(T) == 4) {
-        if (a.head_dim <= 32) return launch_dim<T, HELD, 32, R, NW>(a, c, grid, st);
+        if (a.head_dim <= 32) return launch_dim<T, HELD, 32, R>(a, c, grid, st);
     }
-    return a.head_dim <= 64 ? launch_dim<T, HELD, 64, R, NW>(a, c, grid, st) : launch_dim<T, HELD, 128, R, NW>(a, c, grid, st);
+    return a.head_dim <= 64 ? launch_dim<T, HELD, 64, R>(a, c, grid, st) : launch_dim<T, HELD, 128, R>(a, c, grid, st);
 }
-template <class T, int R, int NW>
+template <class T, int R>
 hipError_t launch_typed(const AttnArgs &a, const CacheArgs &c, int held, dim3 grid, hipStream_t st)
 {
-    return held == kHeldI8 ? launch_held<T, kHeldI8, R, NW>(a, c, grid, st) : held == kHeldE4m3 ? launch_held<T, kHeldE4m3, R, NW>(a, c, grid, st) : launch_held<T, kHeldOwn, R, NW>(a, c, grid, st);
+    return held == kHeldI8 ? launch_held<T, kHeldI8, R>(a, c, grid, st) : held == kHeldE4m3 ? launch_held<T, kHeldE4m3, R>(a, c, grid, st) : launch_held<T, kHeldOwn, R>(a, c, grid, st);
 }
-template <int R, int NW>
+template <int R>
 hipError_t launch_rows(const AttnArgs &a, const CacheArgs &c, int type, int held, dim3 grid, hipStream_t st)
 {
-    return type == SDDMM_TYPE_F32 ? launch_typed<float, R, NW>(a, c, held, grid, st) : type == SDDMM_TYPE_F16 ? launch_typed<_Float16, R, NW>(a, c, held, grid, st)
-                                                                                                             : launch_typed<__bf16, R, NW>(a, c, held, grid, st);
+    return type == SDDMM_TYPE_F32 ? launch_typed<float, R>(a, c, held, grid, st) : type == SDDMM_TYPE_F16 ? launch_typed<_Float16, R>(a, c, held, grid, st)
+                                                                                                             : launch_typed<__bf16, R>(a, c, held, grid, st);
 }
 
 // The parts of a row: sums and totals in units of 2^(largest maximum).  Groups of DP / 4 lanes take parts in turn, N at a time with maxima and sums under way together, each
@@ -191,7 +191,7 @@ hipError_t launch_attention_paged_join(const AttnArgs &a, const AttnArgs *few, i
 
 hipError_t launch_attention_paged_token(const AttnArgs &a, const CacheArgs &c, int type, int held, int tiles, unsigned grid, hipStream_t st)
 {
-    return tiles == 1 ? launch_rows<1, 4>(a, c, type, held, dim3(grid), st) : launch_rows<2, 4>(a, c, type, held, dim3(grid), st);
+    return tiles == 1 ? launch_rows<1>(a, c, type, held, dim3(grid), st) : launch_rows<2>(a, c, type, held, dim3(grid), st);
 }
 
 }  // namespace sddmm

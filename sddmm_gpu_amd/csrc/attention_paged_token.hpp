@@ -19,14 +19,15 @@ namespace sddmm {
 // the time, matrix ones for 9), by chains of loads -- lengths, pages, keys, the next keys -- where there are few (4 users of up to 32,768 keys, 2 key heads: 13.2 us in 512 workgroups of
 // four tiles a wave, compute units busy for 42 %).  Sixteen waves to a workgroup, which need no pieces and no join for one user, are slower: 16.2 us for 1501 keys where both launches
 // take 10.2 (one compute unit's rate).
-template <class T, int HELD, int DP, bool MOD, int R, int NW>
+template <class T, int HELD, int DP, bool MOD, int R>
 struct PagedToken {
+    static constexpr int NW = 4;  // waves
     static constexpr int kLds = NW * 16 * (DP + 4) * 4 + NW * 16 * 8;
     static __device__ __forceinline__ void run(const AttnArgs &a, const CacheArgs &c, int kv, int split, int b, char (&memory)[kLds]);
 };
 
-template <class T, int HELD, int DP, bool MOD, int R, int NW>
-__device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R, NW>::run(const AttnArgs &a, const CacheArgs &c, int kv, int split, int b, char (&memory)[kLds])
+template <class T, int HELD, int DP, bool MOD, int R>
+__device__ __forceinline__ void PagedToken<T, HELD, DP, MOD, R>::run(const AttnArgs &a, const CacheArgs &c, int kv, int split, int b, char (&memory)[kLds])
 {
     typedef typename Elem<T>::Vec8 Vec8;
     // What probabilities times scales and values' codes are multiplied in: fp16 rows over codes take bf16, whose range is that of the scales (in fp16 a value of 2^14 times the others,

@@ -19,7 +19,7 @@ struct AppendArgs {
     AttnArgs a;      // q, k, v: the new rows; out: the turned queries
     CacheArgs c;
     const double *freq;
-    int32_t rot_dim, half, chunk_shift, max_chunks, n_slots, heads_per, head_groups, fast, table;  // table: entries of a chunk's angles
+    int32_t rot_dim, half, chunk_shift, max_chunks, heads_per, head_groups, fast, table;  // table: entries of a chunk's angles
     float amplitude;
 };
 
@@ -496,7 +496,6 @@ int sddmm_cache_append(const sddmm_attention_desc *desc, const sddmm_cache_desc 
     const int64_t many = div_up(d.n_kv_heads, std::min<int64_t>(d.n_kv_heads, div_up(512, slots)));
     p.heads_per = (int32_t)std::max(div_up(d.n_kv_heads, std::min<int64_t>(d.n_kv_heads, div_up(2048, slots))), std::min(many, div_up(16, lane_rows)));
     p.head_groups = (int32_t)div_up(d.n_kv_heads, p.heads_per);
-    p.n_slots = (int32_t)std::min<int64_t>(slots, INT32_MAX);
     if (slots > INT32_MAX || !launchable(slots * p.head_groups, kBlock)) return fail(SDDMM_ERR_RANGE, "%s: too many rows and heads for one launch", who);
     p.table = (int32_t)(chunk * div_up(c.rot_dim / 2, 8) * 9);
     const size_t lds = p.table * (d.type == SDDMM_TYPE_F32 ? sizeof(double2) : held == kHeldOwn ? sizeof(float2) : sizeof(double2) + sizeof(float2));
