@@ -57,7 +57,7 @@ Deal deal(const sddmm_attention_desc &d)
     } else {
         // As many pieces as fill the card (rows of packed sequences counted without the slots that few of them leave empty where most sequences have few rows: three pieces of prompts beside
         // 29 tokens, 1053 rows of 32 heads over 8, up to 4096 keys, in whole and in 2, 3 and 4 pieces 153, 111, 126 and 132 us).
-        const int64_t filled = mixed ? std::max<int64_t>(1, r.rows * group / r.tile * d.n_kv_heads) : workgroups;
+        const int64_t filled = mixed ? std::max<int64_t>(1, r.rows * group / r.tile) * d.n_kv_heads : workgroups;
         r.splits = std::max<int64_t>(1, std::min(std::min(div_up(r.tile == 256 ? 256 : 512, filled), div_up(key_tiles, 8)), (int64_t)256));
     }
     r.grid = workgroups * r.splits;

@@ -29,3 +29,11 @@ def test_mixed_batches():
         short = workspace(capi.TYPE_BF16, capi.TYPE_I8, n_seq, heads, kv, 128, max_q, rows, 4096)
         for max_k in (32768, 131072, 1 << 20):
             assert workspace(capi.TYPE_BF16, capi.TYPE_I8, n_seq, heads, kv, 128, max_q, rows, max_k) - short <= 4096 * 32 * 4 * 130 + 1024
+
+
+def test_few_rows_of_many_heads():
+    """Packed batches of fewer rows than a tile holds, whose longest sequence is bounded by nothing but their sum."""
+    for n_seq, heads, kv in ((42, 96, 32), (19, 160, 32), (54, 96, 3), (382, 64, 2), (30, 128, 64)):
+        for max_k in (4096, 131072, 1 << 24):
+            rows, row = n_seq, 4 * (128 + 2)
+            assert workspace(capi.TYPE_BF16, capi.TYPE_I8, n_seq, heads, kv, 128, rows, rows, max_k) <= row * (2 * rows * heads + 4096 * 32 + 512 * 256 + 256), (n_seq, heads, kv, max_k)
