@@ -683,7 +683,9 @@ int sddmm_cache_append(const sddmm_attention_desc *desc, const sddmm_cache_desc 
  * powers of two, exactly); 16-bit operands: probabilities times scales of values are rounded before they are multiplied, to 11 bits or more (more
  * than 64 rows of a key head over a bf16 cache: 8), and those below 2^-24 of a row's largest may be lost.  What lies in a sequence's pages behind
  * its end or before its rows' windows does not reach the results, whatever it holds; infinities and NaNs in keys that a row does not see do not
- * reach its out and lse, those in values may reach its out where one of 256 rows beside it sees them. */
+ * reach its out and lse, those in values may reach its out where one of 256 rows beside it sees them.  Rows of more than 64 to a key head, bf16
+ * over codes: a row's elements below 2^-27 of its largest lose bits.  The workspace holds one part of each row, head_dim + 2
+ * numbers in fp32, and 140 MB (heads of 128) at most, whatever the lengths.  Work is dealt out by max_q and max_k: bounds far above the true lengths cost time. */
 int sddmm_attention_paged_workspace_bytes(const sddmm_attention_desc *desc, const sddmm_cache_desc *cache, int64_t *bytes);
 int sddmm_attention_paged(const sddmm_attention_desc *desc, const sddmm_cache_desc *cache, const void *d_q, void *d_out, float *d_lse,
                           void *d_workspace, int64_t workspace_bytes, void *stream);

@@ -26,9 +26,14 @@ Deal deal(const sddmm_attention_desc &d)
     const int64_t group = d.n_heads / d.n_kv_heads, packed = d.max_q * group;
     r.rows = rows_of(d);
     if (r.rows == 0) return r;
+    // (us with the border at 32 / 64 / 128 rows, 8 key heads of 128: 16 users of up to 3000 keys, 36 and 64 rows over 8 bits 51 / 41 / 42 and 52 / 42 / 42, 96 and 128 rows 53 / 53 / 60 and
+    // 56 / 56 / 77; over 16 bits 36 and 64 rows 44 / 46 / 46 and 44 / 47 / 47, 128 rows 49 / 49 / 88; one user of 8000 keys, 64 and 128 rows over 8 bits 22 / 22 / 22 and 28 / 28 / 25, over 16 bits
+    // 20 / 22 / 22 and 25 / 25 / 25)
     r.token = packed <= 64;
     r.tiles = packed <= 16 ? 1 : 2;
-    // Sequences of few rows among those of many, as far as numbers tell: packed ones whose longest is four times the mean.
+    // Sequences of few rows among those of many, as far as numbers tell: packed ones whose longest is four times the mean (us in one launch and with tiles of rows for all, 32 heads over 8 of 128:
+    // 32 sequences, up to 4000 keys, 2000 rows, the longest 8, 12 and 15 times the mean 218 and 231, 173 and 206, 141 and 158, 1000 rows, 31 times, 147 and 200; 8 sequences, up to 2000 keys, 1000
+    // rows, 3 times 68 and 57, 5 to 8 times, where a few long tiles are most of the work, 82 to 84 and 67 to 74).
     const bool mixed = !r.token && d.type != SDDMM_TYPE_F32 && d.q_ptr && group <= 32 && (double)d.max_q * d.n_seq >= 4. * d.q_rows;
     // Many rows: 256 to a workgroup, which share the codes that it makes operands of, where there are 128 workgroups of them and long heads (us with 256 and 128: 2048 tokens behind
     // 14,336, 16 heads over 2 of 128, 8 bits 317 and 360; 1024 behind 7168, 32 over 8 167 and 177; a prompt of 4096, 32 over 8, 16 bits 147 and 164; 2048, 16 over 4 62 and 62; 128 behind
