@@ -50,3 +50,50 @@ def test_parts_of_both(dtype, held, heads, kv, n_new, after, max_k):
                 x, y = stat[at: at + n, h].double(), r["lse"]
                 assert ((x == y) | ((x - y).abs() <= r["lse_tol"])).all(), (s, h)
             at += n
+
+
+def test_mixed_batches_in_a_graph():
+    """A captured append and attention over a packed batch, replayed with other sequences long, others without rows and other lengths, with eager work between."""
+    n_seq, heads, kv, dim, page, block, most, rows = 9, 8, 2, 64, 32, 8, 120, 160
+    longest = 3000
+    width = -(-longest // page)
+    table = torch.arange(n_seq * width, dtype=torch.int32).view(n_seq, width).flip(1).contiguous().to(DEV)
+    freq = torch.from_numpy(capi.rotary_frequencies(dim)[0]).to(DEV)
+    sides = []
+    for _ in range(2):
+        pages = Pages(BF16, "e4m3", n_seq * width, page, block, kv, dim, False, 5)
+        s = dict(pages=pages, ptr=torch.zeros(n_seq + 1, dtype=torch.int32, device=DEV), len=torch.zeros(n_seq, dtype=torch.int32, device=DEV))
+        s.update({n: torch.zeros(rows, h, dim, dtype=BF16, device=DEV) for n, h in (("q", heads), ("k", kv), ("v", kv), ("out", heads))})
+        s["desc"] = capi.AttentionDesc.packed(capi.TYPE_BF16, n_seq, heads, kv, dim, max_q=most, max_k=longest, k_len=s["len"].data_ptr(), q_ptr=s["ptr"].data_ptr(), q_rows=rows, window_right=0)
+        s["cache"] = pages.desc(table, rot_dim=dim, rot_layout=0, rot_freq=freq.data_ptr())
+        s["size"] = capi.attention_paged_workspace_bytes(s["desc"], s["cache"])
+        s["ws"] = torch.full((s["size"],), 255, dtype=torch.uint8, device=DEV)
+        sides.append(s)
+
+    def calls(s, st):
+        capi.cache_append(s["desc"], s["cache"], s["q"].data_ptr(), s["q"].data_ptr(), s["k"].data_ptr(), s["v"].data_ptr(), st)
+        capi.attention_paged(s["desc"], s["cache"], s["q"].data_ptr(), s["out"].data_ptr(), 0, s["ws"].data_ptr(), s["size"], st)
+
+    assert sides[0]["size"] > 0
+    for s in sides:
+        calls(s, stream())  # (code is loaded outside the capture; no rows)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        calls(sides[0], torch.cuda.current_stream().cuda_stream)
+    for step, (new, after) in enumerate([([100, 1, 1, 0, 1, 1, 3, 1, 1], [100, 2000, 30, 0, 1, 2999, 90, 64, 700]), ([1, 1, 1, 120, 0, 1, 1, 30, 1], [101, 2001, 31, 1200, 1, 3000, 91, 94, 701]),
+                                         ([1] * 9, [102, 2002, 32, 1201, 2, 2500, 92, 95, 702]), ([0, 0, 0, 0, 0, 0, 0, 0, 120], [102, 2002, 32, 1201, 2, 2500, 92, 95, 822])]):
+        q, k, v = (normal(30 * step + i, rows, h, dim).to(BF16) for i, h in enumerate((heads, kv, kv)))
+        for s in sides:
+            s["ptr"].copy_(torch.tensor([0] + new, dtype=torch.int32).cumsum(0, dtype=torch.int32)), s["len"].copy_(torch.tensor(after, dtype=torch.int32))
+            s["q"].copy_(q), s["k"].copy_(k), s["v"].copy_(v), s["out"].fill_(5.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        calls(sides[1], stream())
+        junk = torch.ones(1000, device=DEV).sum()
+        torch.cuda.synchronize()
+        assert float(junk) == 1000.0
+        x, y = sides
+        assert torch.equal(x["out"], y["out"]) and torch.equal(x["q"], y["q"]) and not x["out"].isnan().any() and (x["out"][sum(new):] == 5.0).all()
+        for name in "kv":
+            assert torch.equal(x["pages"].gpu[name].view(torch.uint8), y["pages"].gpu[name].view(torch.uint8)) and torch.equal(x["pages"].scales[name], y["pages"].scales[name])
